@@ -386,6 +386,83 @@ int mlq_hip_attention_decode(int device, const float* q, const float* keys, cons
 int mlq_hip_matmul_f32(int device, const float* a, const float* b, int m, int k, int n, int b_transposed, float* c,
                        void* stream);
 
+/* ---- Paged key/value cache of several sequences ----
+ * The reference keeps one sequence's keys and values in f32, contiguously
+ * (CudaKVCache, include/mini_llama/cuda_kv_cache.h), and attends with one token
+ * at a time (cuda_attention.h:11-31).  Here sequences share a cache of pages,
+ * held in f32 or in the block formats of the weights (quantized along a head's
+ * elements, the bytes per block those of MLQ_Q*_BLOCK_BYTES), and a call serves
+ * any number of new tokens of every sequence.
+ *
+ * A cache holds n_layers x n_pages pages; a page holds page_size positions of
+ * all KV heads.  Which page holds which positions of which sequence is the
+ * caller's business: a sequence's pages are a list of page ids, entry i holding
+ * positions i * page_size .., the same for every layer.  Sequences may share
+ * pages (a common prefix).  page_size: a power of two, 32 to 65536; head_dim: a
+ * multiple of 8, up to 256.  The cache starts out as zeros. */
+typedef struct mlq_kv_cache_s* mlq_kv_cache_t;
+int mlq_hip_kv_cache_create(int device, int type, int n_layers, int n_pages, int page_size, int n_kv_heads,
+                            int head_dim, mlq_kv_cache_t* out);
+/* Its description; any out pointer may be NULL.  bytes: of device memory. */
+int mlq_hip_kv_cache_info(mlq_kv_cache_t cache, int* type, int* n_layers, int* n_pages, int* page_size,
+                          int* n_kv_heads, int* head_dim, size_t* bytes);
+/* Releases the handle; the memory goes with the last of its plans.  The cache's
+ * calls must be done.  NULL is a no-op. */
+int mlq_hip_kv_cache_destroy(mlq_kv_cache_t cache);
+
+/* What a step's calls share for all layers: the query heads and who sees whom,
+ * and, from each set, the batch with its work lists in device memory.
+ * A token at position i sees positions j <= i; with window > 0 only those with
+ * j > i - window or j < sinks (the sequence's first tokens, which stay visible).
+ * scale: of the scores, 0 for 1/sqrt(head_dim).  n_heads: a multiple of the
+ * cache's KV heads (query head h reads KV head h / (n_heads / n_kv_heads)).
+ * max_seqs, max_tokens and max_pages bound a set's sequences, new tokens and
+ * page entries (max_pages * page_size up to 2^30, max_tokens * n_heads up to
+ * 2^30).  A plan holds device memory of its own (about 55 MB at head_dim 128,
+ * for results of work that is split over long contexts): its calls must not
+ * overlap in time (one stream, or events), graph replays included, and one host
+ * thread uses it at a time. */
+typedef struct mlq_kv_plan_s* mlq_kv_plan_t;
+int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
+                           int max_tokens, int max_pages, mlq_kv_plan_t* out);
+/* The batch of the calls that follow: sequence s has kv_len[s] positions, the
+ * last new_tokens[s] of them new (0 is allowed, and so is a length of 0), and
+ * ceil(kv_len[s] / page_size) page ids in `pages`, one sequence's after the
+ * other's.  All host arrays, copied before the call returns.  Lengths, page ids
+ * and capacities are checked here, and no two new tokens may go to one slot; a
+ * refused set leaves the batch as it was.  Asynchronous on `stream`; not under graph capture. */
+int mlq_hip_kv_plan_set(mlq_kv_plan_t plan, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
+                        void* stream);
+int mlq_hip_kv_plan_destroy(mlq_kv_plan_t plan);
+
+/* The three calls below take the batch's tokens in the order of the sequences,
+ * as rows of contiguous f32 device buffers that start 16-byte aligned; rows
+ * after the last new token are neither read nor written.  Asynchronous on
+ * `stream`.  Under graph capture they record launches that serve any batch set
+ * later, so the buffers must hold max_tokens rows (whole sequences read back:
+ * max_pages * page_size). */
+
+/* Writes the new tokens' k and v [tokens][n_kv_heads][head_dim] into their pages
+ * of `layer`.  Quantized blocks are those of mlq_hip_quantize bit for bit, a
+ * head's last block holding what head_dim leaves.  theta > 0 rotates k first
+ * (RoPE at each token's position, pairs as mlq_hip_rope; in 64 bits, rounded to
+ * f32 once) and, unless q is NULL, writes q [tokens][n_heads][head_dim] rotated
+ * to q_out, which may be q.  theta 0: no rotation, q NULL. */
+int mlq_hip_kv_write(mlq_kv_plan_t plan, int layer, const float* k, const float* v, const float* q, float* q_out,
+                     float theta, int neox, void* stream);
+/* Reads back what `layer` holds, as f32 [positions][n_kv_heads][head_dim]: all
+ * positions of the sequences, one sequence after the other, or, with new_only
+ * != 0, the new tokens' alone. */
+int mlq_hip_kv_read(mlq_kv_plan_t plan, int layer, int new_only, float* k, float* v, void* stream);
+/* out [tokens][n_heads][head_dim]: attention of the new tokens' q over the pages
+ * of `layer`, which hold the new tokens too (write first).  f32 throughout: the
+ * products run as pairs of fp16 parts.  A position a token does not see has no
+ * part in its result, whatever it holds.  A 32-element block of a key or value
+ * that holds an element that is not finite (in f32 caches also one of magnitude
+ * 2^110 or more, in quantized ones a scale that is not finite) counts as NaN
+ * for the tokens that see it.  The same call gives the same bits. */
+int mlq_hip_kv_attention(mlq_kv_plan_t plan, int layer, const float* q, float* out, void* stream);
+
 /* Kernel selection introspection: name of the kernel the next call with this
  * shape would launch (for profiles and tests). */
 int mlq_hip_kernel_name(int qtype, int rows, int out_features, int in_features, char* buf,

@@ -1,0 +1,178 @@
+// Batches over the paged key/value cache: checks and work lists (kv_plan.h).
+
+#include "kv_plan.h"
+
+#include <algorithm>
+
+namespace mlq {
+namespace {
+
+// Workgroups of four waves that keep 256 CUs busy: a split makes more of them
+// until there are this many, and no more.
+constexpr int kTargetGroups = 1024;
+// Fewer tiles than this are not split further: the parts' merge would cost more
+// than the tiles (two a wave).
+constexpr int kLeastTiles = 8;
+// From this many workgroups on, many-row sequences run without splits: each wave has
+// rows of its own and a workgroup's waves read the same tiles together.
+constexpr int kEnoughGroups = 512;
+
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Tiles that query rows at positions lo .. hi can see, in the numbering of KvAttnItem.
+struct Seen {
+    int sinks, shift, count;
+};
+
+Seen seen_tiles(const KvPlanShape& s, int lo, int hi) {
+    const int last = hi / kKvTile;
+    const int first = s.window > 0 ? std::max(0, lo - s.window + 1) / kKvTile : 0;
+    // the sinks are first positions: below `first` they are whole tiles of their own
+    const int sinks = s.window > 0 ? std::min(first, ceil_div(s.sinks, kKvTile)) : 0;
+    return Seen{sinks, first - sinks, sinks + last - first + 1};
+}
+
+}  // namespace
+
+KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
+    const int extra = ceil_div(kTargetGroups, s.n_kv_heads);
+    const int64_t rows = static_cast<int64_t>(s.max_tokens) * s.group;
+    const int wide = static_cast<int>(rows / s.wide_rows) + s.max_seqs;
+    KvPlanLimits l;
+    l.items[0] = s.max_seqs + extra;
+    l.items[1] = wide + extra;
+    // Only items beyond an unsplit list's are parts, and a split of n parts adds n - 1
+    // items: at most twice the extra ones.
+    l.slots[0] = l.slots[1] = 2 * extra;
+    return l;
+}
+
+std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
+                          KvBatch* out) {
+    if (n_seqs < 0 || n_seqs > s.max_seqs) {
+        return std::to_string(n_seqs) + " sequences, the plan holds " + std::to_string(s.max_seqs);
+    }
+    if (n_seqs > 0 && (new_tokens == nullptr || kv_len == nullptr)) return "null lengths";
+    int64_t tokens = 0, entries = 0, positions = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+        const std::string who = "sequence " + std::to_string(i);
+        if (new_tokens[i] < 0) return who + ": negative token count";
+        if (kv_len[i] < new_tokens[i]) {
+            return who + ": " + std::to_string(new_tokens[i]) + " new tokens in a length of " + std::to_string(kv_len[i]);
+        }
+        tokens += new_tokens[i];
+        positions += kv_len[i];
+        entries += kv_len[i] / s.page_size + (kv_len[i] % s.page_size != 0);
+    }
+    if (tokens > s.max_tokens) {
+        return std::to_string(tokens) + " new tokens, the plan holds " + std::to_string(s.max_tokens);
+    }
+    if (entries > s.max_pages) {
+        return std::to_string(entries) + " page entries, the plan holds " + std::to_string(s.max_pages);
+    }
+    if (entries > 0 && pages == nullptr) return "null page list";
+    for (int64_t e = 0; e < entries; ++e) {
+        if (pages[e] < 0 || pages[e] >= s.n_pages) {
+            return "page entry " + std::to_string(e) + " is " + std::to_string(pages[e]) + ", the cache has " +
+                   std::to_string(s.n_pages) + " pages";
+        }
+    }
+
+    KvBatch& b = *out;
+    b = KvBatch();
+    b.n_tokens = static_cast<int>(tokens);
+    b.n_positions = static_cast<int>(positions);
+
+    // Pages, tiles, and the slots new tokens go to (page, first and last slot in the page).
+    struct Written {
+        int page, lo, hi;
+    };
+    std::vector<Written> written;
+    std::vector<KvAttnItem> base[2];
+    int token0 = 0, row0 = 0, page0 = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+        const int len = kv_len[i], n = new_tokens[i], start = len - n;
+        for (int p = 0; p < len; p += s.page_size) {
+            b.pages.push_back(KvPage{pages[page0 + p / s.page_size], std::min(s.page_size, len - p), row0 + p});
+        }
+        for (int p = start; p < len;) {
+            const int end = std::min(len, (p / kKvTile + 1) * kKvTile);
+            b.fresh.push_back(KvTileItem{pages[page0 + p / s.page_size], p % s.page_size / kKvTile, p % kKvTile, end - p,
+                                         token0 + p - start, p});
+            p = end;
+        }
+        for (int p = start; p < len;) {
+            const int end = std::min(len, (p / s.page_size + 1) * s.page_size);
+            written.push_back(Written{pages[page0 + p / s.page_size], p % s.page_size, (end - 1) % s.page_size});
+            p = end;
+        }
+        if (n > 0) {
+            const int rows = n * s.group;
+            const int kind = rows <= kKvNarrowRows ? 0 : 1;
+            base[kind].push_back(KvAttnItem{token0, n, len, page0, 0, 0, 0, 0, 0, kKvWaves, 0, 1, 0});
+        }
+        token0 += n;
+        row0 += len;
+        page0 += len / s.page_size + (len % s.page_size != 0);
+    }
+    std::sort(written.begin(), written.end(), [](const Written& x, const Written& y) {
+        return x.page != y.page ? x.page < y.page : x.lo < y.lo;
+    });
+    for (size_t k = 1; k < written.size(); ++k) {
+        if (written[k].page == written[k - 1].page && written[k].lo <= written[k - 1].hi) {
+            return "page " + std::to_string(written[k].page) + " takes two new tokens in slot " + std::to_string(written[k].lo);
+        }
+    }
+
+    for (int kind = 0; kind < 2; ++kind) {
+        const int per = kind == 0 ? kKvNarrowRows : s.wide_rows;
+        int64_t groups = 0;  // workgroups with rows of their own in every wave
+        for (const KvAttnItem& q : base[kind]) groups += ceil_div(q.new_tokens * s.group, per * kKvWaves);
+        const bool together = kind == 1 && groups * s.n_kv_heads >= kEnoughGroups;
+        const int step = together ? per * kKvWaves : per;
+        std::vector<KvAttnItem> whole;
+        int64_t tiles = 0;
+        for (const KvAttnItem& q : base[kind]) {
+            const int rows = q.new_tokens * s.group, start = q.len - q.new_tokens;
+            for (int r = 0; r < rows; r += step) {
+                const Seen t = seen_tiles(s, start + r / s.group, start + (std::min(rows, r + step) - 1) / s.group);
+                KvAttnItem it = q;
+                it.row0 = r;
+                it.count = t.count;
+                it.sinks = t.sinks;
+                it.shift = t.shift;
+                it.stride = together ? 1 : kKvWaves;
+                tiles += t.count;
+                whole.push_back(it);
+            }
+        }
+        std::vector<KvAttnItem>& list = b.items[kind];
+        if (together) {
+            list = std::move(whole);
+        } else {
+            // Parts of at most `most` tiles, as even as they come.
+            const int target = ceil_div(kTargetGroups, s.n_kv_heads);
+            const int most = std::max<int64_t>(kLeastTiles, (tiles + target - 1) / target);
+            int slot = 0;
+            for (const KvAttnItem& w : whole) {
+                const int parts = ceil_div(w.count, most);
+                for (int p = 0; p < parts; ++p) {
+                    KvAttnItem it = w;
+                    it.first = static_cast<int>(static_cast<int64_t>(w.count) * p / parts);
+                    it.count = static_cast<int>(static_cast<int64_t>(w.count) * (p + 1) / parts) - it.first;
+                    it.split = p;
+                    it.nsplit = parts;
+                    it.slot = slot;
+                    list.push_back(it);
+                }
+                if (parts > 1) slot += parts;
+            }
+        }
+        // The longest first: what starts last is short.
+        std::stable_sort(list.begin(), list.end(),
+                         [](const KvAttnItem& x, const KvAttnItem& y) { return x.count > y.count; });
+    }
+    return "";
+}
+
+}  // namespace mlq

@@ -6,6 +6,7 @@
 // replaced by "hip".  Every check runs on the host before any launch, so a
 // malformed call never reaches a kernel.
 
+#include "abi.h"
 #include "decoder.h"
 #include "gguf_index.h"
 #include "mlq_kernels.h"
@@ -469,6 +470,19 @@ int grow_stage(DeviceState& st, size_t bytes) {
 }
 
 }  // namespace
+
+namespace mlq {
+
+int abi_fail(int code, const std::string& msg) { return fail(code, msg); }
+int abi_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+int abi_device(int device) { return ensure_device(device); }
+hipStream_t abi_stream(int device, void* stream) { return resolve_stream(device, stream); }
+bool abi_capturing(hipStream_t s) { return capturing(s); }
+int abi_device_ptr(const void* p, int device, const char* caller, const char* what, size_t bytes) {
+    return check_device_ptr(p, device, caller, what, bytes);
+}
+
+}  // namespace mlq
 
 extern "C" {
 

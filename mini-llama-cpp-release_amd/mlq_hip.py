@@ -143,6 +143,17 @@ _SIGS = {
     "mlq_hip_attention_decode": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp] + [ctypes.c_int] * 7 + [_vp, _vp]),
     "mlq_hip_matmul_f32": (ctypes.c_int, [ctypes.c_int, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int, _vp, _vp]),
+    "mlq_hip_kv_cache_create": (ctypes.c_int, [ctypes.c_int] * 7 + [ctypes.POINTER(_vp)]),
+    "mlq_hip_kv_cache_info": (ctypes.c_int, [_vp] + [ctypes.POINTER(ctypes.c_int)] * 6 +
+                              [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlq_hip_kv_cache_destroy": (ctypes.c_int, [_vp]),
+    "mlq_hip_kv_plan_create": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float] +
+                               [ctypes.c_int] * 3 + [ctypes.POINTER(_vp)]),
+    "mlq_hip_kv_plan_set": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp]),
+    "mlq_hip_kv_plan_destroy": (ctypes.c_int, [_vp]),
+    "mlq_hip_kv_write": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_float, ctypes.c_int, _vp]),
+    "mlq_hip_kv_read": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
+    "mlq_hip_kv_attention": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
     "mlq_hip_kernel_name": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                             ctypes.c_char_p, ctypes.c_size_t]),
 }
@@ -605,6 +616,85 @@ class Decoder:
     def __del__(self):
         try:
             self.close()
+        except Exception:
+            pass
+
+
+def _ptr(b):
+    return b if b is None or isinstance(b, int) else b.ptr
+
+
+class KvCache:
+    """Pages of keys and values that several sequences share (mlq_hip_kv_cache_*)."""
+
+    def __init__(self, qtype: int, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 device: int = 0):
+        h = _vp()
+        _check(load().mlq_hip_kv_cache_create(device, qtype, n_layers, n_pages, page_size, n_kv_heads, head_dim,
+                                              ctypes.byref(h)))
+        self.h = h.value
+
+    def info(self) -> dict:
+        names = ("type", "n_layers", "n_pages", "page_size", "n_kv_heads", "head_dim")
+        v, n = [ctypes.c_int() for _ in names], ctypes.c_size_t()
+        _check(_LIB.mlq_hip_kv_cache_info(self.h, *[ctypes.byref(x) for x in v], ctypes.byref(n)))
+        return {**{k: x.value for k, x in zip(names, v)}, "bytes": n.value}
+
+    def destroy(self) -> None:
+        if getattr(self, "h", None):
+            _LIB.mlq_hip_kv_cache_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+class KvPlan:
+    """A batch over a KvCache and its calls (mlq_hip_kv_plan_*, _write, _read, _attention).
+    Buffers are DeviceBuffers or device pointers; every call is asynchronous."""
+
+    def __init__(self, cache: KvCache, n_heads: int, max_seqs: int, max_tokens: int, max_pages: int, window: int = 0,
+                 sinks: int = 0, scale: float = 0.0):
+        h = _vp()
+        _check(load().mlq_hip_kv_plan_create(cache.h, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages,
+                                             ctypes.byref(h)))
+        self.h = h.value
+        self._page_size = cache.info()["page_size"]
+
+    def set(self, new_tokens, kv_len, pages, stream=None) -> None:
+        """new_tokens and kv_len per sequence; pages: their page ids, one sequence's after the other's."""
+        n = np.ascontiguousarray(new_tokens, np.int32).ravel()
+        t = np.ascontiguousarray(kv_len, np.int32).ravel()
+        p = np.ascontiguousarray(pages, np.int32).ravel()
+        if n.size != t.size:
+            raise ValueError("one length per sequence")
+        need = int(sum(-(-int(x) // self._page_size) for x in t if x > 0))
+        if p.size != need:
+            raise ValueError(f"{p.size} page ids, the lengths need {need}")
+        _check(_LIB.mlq_hip_kv_plan_set(self.h, n.size, n.ctypes.data, t.ctypes.data, p.ctypes.data, stream))
+
+    def write(self, layer: int, k, v, q=None, q_out=None, theta: float = 0.0, neox: bool = False, stream=None) -> None:
+        """k and v into the batch's pages; theta > 0 rotates k, and q into q_out."""
+        _check(_LIB.mlq_hip_kv_write(self.h, layer, _ptr(k), _ptr(v), _ptr(q), _ptr(q_out), theta, int(neox), stream))
+
+    def read(self, layer: int, k, v, new_only: bool = False, stream=None) -> None:
+        """What the cache holds, as f32: all positions, or the new tokens' alone."""
+        _check(_LIB.mlq_hip_kv_read(self.h, layer, int(new_only), _ptr(k), _ptr(v), stream))
+
+    def attention(self, layer: int, q, out, stream=None) -> None:
+        _check(_LIB.mlq_hip_kv_attention(self.h, layer, _ptr(q), _ptr(out), stream))
+
+    def destroy(self) -> None:
+        if getattr(self, "h", None):
+            _LIB.mlq_hip_kv_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.destroy()
         except Exception:
             pass
 
