@@ -1,0 +1,11 @@
+// Attention over pages of Q4_0 keys and values (kv_attention.h).
+
+#include "kv_attention.h"
+
+namespace mlq {
+
+hipError_t launch_kv_attention_q4_0(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
+    return kv::launch<2>(a, kind, count, q, out, s);
+}
+
+}  // namespace mlq
