@@ -1,11 +1,13 @@
-// Attention of a batch's new tokens over the paged cache (kv_layout.h) on MFMA.
+// Attention of a batch's new tokens over the paged cache (kv_layout.h) on MFMA: what its two
+// kernels share, and the one for up to eight query rows a KV head (decode).
 //
 // out = softmax_j(scale q . k_j) v over the positions j that a token at position i
 // sees: j <= i and, with a window of w, j > i - w or j < sinks.
 //
-// A wave walks tiles of 32 positions of one KV head for up to 32 query rows (row =
-// token * group + query head of the group, so grouped heads fill the tile and share
-// what is read).  Per tile, in v_mfma_f32_16x16x32_f16 with operands that come
+// A wave walks tiles of 32 positions of one KV head for up to eight query rows (row =
+// token * group + query head of the group, so grouped heads share what is read), the
+// four waves of a workgroup every fourth tile each, and workgroups parts of a long context; the
+// states are merged in a fixed order, the last workgroup to arrive merging the parts.  Per tile, in v_mfma_f32_16x16x32_f16 with operands that come
 // from memory as they lie there:
 //
 //   S^T = K Q^T   per block b of 32 elements: the codes are whole numbers (exact in
@@ -23,9 +25,8 @@
 // zero takes no digits from the others.  It moves only when t + e passes it by 6, so the
 // accumulators are seldom rescaled.  The sum of the weights is f32 in the same frame.
 //
-// Where few rows share a KV head (up to 8: decode), the hi parts are columns 0 .. 7 of
-// the query operand and the lo parts columns 8 .. 15, of the weights as well: one product
-// where there would be two, the halves added at the end.
+// The hi parts are columns 0 .. 7 of the query operand and the lo parts columns 8 .. 15, of
+// the weights as well: one product where there would be two, the halves added at the end.
 //
 // What a row does not see gets weight 0, and 0 times a scale that is Inf or NaN is 0
 // (v_mul_legacy_f32); codes are finite always.
@@ -153,104 +154,163 @@ __device__ __forceinline__ float inverse_power(uint32_t s) {
 
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-template <int QT, int NB, int ROWS>
-__global__ __launch_bounds__(kThreads) void attention_kernel(KvAttention a, int kind, int count,
-                                                                const float* __restrict__ q, float* __restrict__ out) {
+// A lane's part of a query row (elements 8 g .. of every block), relative to the row's
+// largest, which becomes 2^13 .. 2^14; the blocks' sums; what takes a score to base 2.
+template <int NB>
+__device__ __forceinline__ void load_query(const float* q, int hd, int g, float scale, float (*v)[8], float* sum, float* to_t) {
+    float top = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int e = 32 * b + 8 * g;
+        float4 x = make_float4(0, 0, 0, 0), y = x;
+        if (e < hd) {
+            x = *reinterpret_cast<const float4*>(q + e);
+            y = *reinterpret_cast<const float4*>(q + e + 4);
+        }
+        v[b][0] = x.x, v[b][1] = x.y, v[b][2] = x.z, v[b][3] = x.w;
+        v[b][4] = y.x, v[b][5] = y.y, v[b][6] = y.z, v[b][7] = y.w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[b][j]));
+    }
+    top = max_quarters(top);
+    // exponent, kept where 2^(13 - e) and its inverse are normal
+    const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 127);
+    const float up = ldexpf(1.0f, 13 - e);
+    *to_t = ldexpf(scale, e - 13);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        sum[b] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[b][j] *= up;
+            sum[b] += v[b][j];
+        }
+    }
+}
+
+// The state of a wave's rows (accumulators, running maximum, sum) in memory, for parts
+// of a split that other workgroups merge: written through, read past the caches.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t state_rsrc(float* states, size_t index, int floats) {
+    return __builtin_amdgcn_make_buffer_rsrc(states + index * floats, static_cast<short>(0), floats * 4, 0x00020000);
+}
+template <int NQ, int NB>
+__device__ __forceinline__ void leave_state(__amdgpu_buffer_rsrc_t rs, int lane, const f4_t (*o)[2 * NB], const float* m,
+                                            const float* l) {
+    constexpr int QUADS = NQ * 2 * NB;
+#pragma unroll
+    for (int u = 0; u < NQ; ++u) {
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, o[u][t]), rs, ((u * 2 * NB + t) * 64 + lane) * 16, 0,
+                                                   kCoherent);
+        }
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[u]), rs, (QUADS * 256 + 2 * u * 64 + lane) * 4, 0,
+                                              kCoherent);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[u]), rs,
+                                              (QUADS * 256 + (2 * u + 1) * 64 + lane) * 4, 0, kCoherent);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
+}
+// Takes another state of the same rows into one's own.
+__device__ __forceinline__ void fold(float& m, float& l, float m1, float l1, float* w0, float* w1) {
+    const float to = fmaxf(m, m1);
+    *w0 = __builtin_amdgcn_exp2f(m - to);
+    *w1 = __builtin_amdgcn_exp2f(m1 - to);
+    m = to;
+    l = l * *w0 + l1 * *w1;
+}
+template <int NQ, int NB>
+__device__ __forceinline__ void take_state(__amdgpu_buffer_rsrc_t rs, int lane, f4_t (*o)[2 * NB], float* m, float* l) {
+    constexpr int QUADS = NQ * 2 * NB;
+#pragma unroll
+    for (int u = 0; u < NQ; ++u) {
+        const float m1 = bits<float>(__builtin_amdgcn_raw_buffer_load_b32(rs, (QUADS * 256 + 2 * u * 64 + lane) * 4, 0, kCoherent));
+        const float l1 =
+            bits<float>(__builtin_amdgcn_raw_buffer_load_b32(rs, (QUADS * 256 + (2 * u + 1) * 64 + lane) * 4, 0, kCoherent));
+        f4_t x[2 * NB];
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) {
+            x[t] = __builtin_bit_cast(f4_t,
+                                      __builtin_amdgcn_raw_buffer_load_b128(rs, ((u * 2 * NB + t) * 64 + lane) * 16, 0, kCoherent));
+        }
+        float w0, w1;
+        fold(m[u], l[u], m1, l1, &w0, &w1);
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) o[u][t] = o[u][t] * w0 + x[t] * w1;
+    }
+}
+// One arrival of `parts`: whether it is the last, which leaves the counter at zero.
+__device__ __forceinline__ unsigned arrive(unsigned* counter, int parts) {
+    const unsigned before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before + 1 != static_cast<unsigned>(parts)) return 0u;
+    __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return 1u;
+}
+// A lane's elements of an output row: 4 g .. of every sixteen.
+template <int NB>
+__device__ __forceinline__ void store_row(float* out, int hd, int g, const f4_t* o, float inv) {
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t) {
+        const int d = 16 * t + 4 * g;
+        if (d < hd) *reinterpret_cast<f4_t*>(out + d) = o[t] * inv;
+    }
+}
+
+template <int QT, int NB>
+__global__ __launch_bounds__(kThreads, 2) void attention_kernel(KvAttention a, int count, const float* __restrict__ q,
+                                                                 float* __restrict__ out) {
     using F = KvForm<QT>;
-    constexpr bool STACK = ROWS == kKvNarrowRows;
-    constexpr int NQ = ROWS == 32 ? 2 : 1;  // query tiles of 16 columns
     constexpr int SB = F::kScaleBytes;
     constexpr int KL = F::key_lane(NB), VL = F::value_lane(NB);
     constexpr int KW = KL / 4, VW = VL / 4;
     constexpr int KS = NB * SB, VS = 2 * NB * SB;  // words of a lane's scales: 4 keys a half tile, 8 keys
-    constexpr int QUADS = NQ * 2 * NB;             // accumulators
-    constexpr int STATE = (QUADS * 4 + 2 * NQ) * 64;  // floats of a wave's state
+    constexpr int STATE = (8 * NB + 2) * 64;       // floats of a wave's state
     __shared__ float merge[2 * STATE];
     __shared__ unsigned last;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
+    const bool low = i16 >= 8;  // the lane's column holds low parts
     const int n_kv = a.kv.n_kv, hd = a.kv.head_dim, heads = n_kv * a.group;
     const int page_tiles = a.kv.page_tiles, tile_shift = __builtin_ctz(page_tiles);
-    const int total = (count > 0 ? count : uniform(a.lists.counts + kKvCountNarrow + kind)) * n_kv;
+    const int total = (count > 0 ? count : uniform(a.lists.counts + kKvCountNarrow)) * n_kv;
 
     for (int w = blockIdx.x; w < total; w += gridDim.x) {
         const int head = w % n_kv;
-        const KvAttnItem it = uniform(a.lists.items[kind] + w / n_kv);
-        const bool together = it.stride == 1;
+        const KvAttnItem it = uniform(a.lists.items[0] + w / n_kv);
         const int rows = it.new_tokens * a.group, start = it.len - it.new_tokens;
-        const int row0 = it.row0 + (together ? wave * ROWS : 0);
-        const bool idle = row0 >= rows;
-        const int row1 = min(rows, row0 + ROWS);
-        const int pos_lo = start + min(row0, rows - 1) / a.group, pos_hi = start + (max(row1, 1) - 1) / a.group;
+        const int row1 = min(rows, it.row0 + kKvNarrowRows);
+        const int pos_lo = start + it.row0 / a.group, pos_hi = start + (row1 - 1) / a.group;
+        const int row = min(it.row0 + (i16 & 7), rows - 1);
+        const int pos = start + row / a.group;
+        const size_t out_row =
+            (static_cast<size_t>(it.token0 + row / a.group) * heads + head * a.group + row % a.group) * hd;
 
-        // Queries: row's elements relative to its largest, which becomes 2^13 .. 2^14.
-        h8_t qh[NQ][NB], ql[NQ][NB];
-        float qsum[NQ][NB], to_t[NQ];
-        int pos[NQ];
-        size_t out_row[NQ];
-#pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            const int r = min(row0 + 16 * u + (STACK ? i16 & 7 : i16), rows - 1);
-            const int token = r / a.group;
-            pos[u] = start + token;
-            out_row[u] = (static_cast<size_t>(it.token0 + token) * heads + head * a.group + r % a.group) * hd;
+        h8_t qs[NB];
+        float qsum[NB], to_t;
+        {
             float v[NB][8];
-            float top = 0.0f;
+            load_query<NB>(q + out_row, hd, g, a.scale, v, qsum, &to_t);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const int e = 32 * b + 8 * g;
-                float4 x = make_float4(0, 0, 0, 0), y = x;
-                if (e < hd) {
-                    x = *reinterpret_cast<const float4*>(q + out_row[u] + e);
-                    y = *reinterpret_cast<const float4*>(q + out_row[u] + e + 4);
-                }
-                v[b][0] = x.x, v[b][1] = x.y, v[b][2] = x.z, v[b][3] = x.w;
-                v[b][4] = y.x, v[b][5] = y.y, v[b][6] = y.z, v[b][7] = y.w;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[b][j]));
-            }
-            top = max_quarters(top);
-            // exponent, kept where 2^(13 - e) and its inverse are normal
-            const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 127);
-            const float up = ldexpf(1.0f, 13 - e);
-            to_t[u] = ldexpf(a.scale, e - 13);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[b][j] *= up;
-                    sum += v[b][j];
-                }
                 h8_t hi, lo;
                 split8(v[b], &hi, &lo);
-                qh[u][b] = STACK && i16 >= 8 ? lo : hi;
-                ql[u][b] = lo;
-                if (QT == 3) qsum[u][b] = STACK && i16 >= 8 ? 0.0f : sum_quarters(sum);
+                qs[b] = low ? lo : hi;
+                if (QT == 3) qsum[b] = low ? 0.0f : sum_quarters(qsum[b]);
             }
         }
 
-        f4_t o[NQ][2 * NB];
-        float om[NQ][NB];  // Q4_1: this lane's part of the sum of weights times minima
-        float m[NQ], l[NQ];
         const f4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        f4_t o[1][2 * NB];
+        float om[NB];  // Q4_1: this lane's part of the sum of weights times minima
+        float m = -3.402823466e38f, l = 0.0f;
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            m[u] = -3.402823466e38f;
-            l[u] = 0.0f;
+        for (int t = 0; t < 2 * NB; ++t) o[0][t] = zero;
 #pragma unroll
-            for (int t = 0; t < 2 * NB; ++t) o[u][t] = zero;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) om[u][b] = 0.0f;
-        }
+        for (int b = 0; b < NB; ++b) om[b] = 0.0f;
 
-        // This wave's tiles: every it.stride-th of the item's, those past its last row left out.
-        const int past = pos_hi / kKvTile + 1;  // tiles up to here have something to see
-        int end = it.first + it.count;
-        if (past - it.shift < end) end = max(past - it.shift, it.sinks);
-        if (idle) end = 0;
-        int at = it.first + (together ? 0 : wave);
+        // This wave's tiles: every fourth of the item's.
+        const int end = it.first + it.count;
         auto tile_of = [&](int i) { return i < it.sinks ? i : i + it.shift; };
         auto page_of = [&](int i) { return uniform(&a.lists.pages[it.page0 + (tile_of(i) >> tile_shift)].page); };
         auto base_of = [&](int i, int page) {
@@ -286,28 +346,28 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(KvAttention a, int 
             return static_cast<float>(i % 2 == 0 ? p.x : p.y);
         };
 
+        int at = it.first + wave;
         int next_page = 0;
         if (at < end) {
             const uint8_t* tile = base_of(at, page_of(at));
             load_keys(tile);
             load_values(tile);
-            if (at + it.stride < end) next_page = page_of(at + it.stride);
+            if (at + kKvWaves < end) next_page = page_of(at + kKvWaves);
         }
-        for (; at < end; at += it.stride) {
+        for (; at < end; at += kKvWaves) {
             const int first = tile_of(at) * kKvTile;
-            const bool more = at + it.stride < end;
-            const uint8_t* next = base_of(more ? at + it.stride : at, next_page);
-            if (at + 2 * it.stride < end) next_page = page_of(at + 2 * it.stride);
+            const bool more = at + kKvWaves < end;
+            const uint8_t* next = base_of(more ? at + kKvWaves : at, next_page);
+            if (at + 2 * kKvWaves < end) next_page = page_of(at + 2 * kKvWaves);
 
-            // Scores.
-            f4_t s[NQ][2];
+            // Scores, halves apart.
+            float t[8];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) s[u][h] = zero;
+                f4_t s = zero;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    f4_t acc[NQ];
+                    f4_t acc;
                     if (QT == 0) {
                         h8_t hi, lo;
                         float v[8];
@@ -315,197 +375,140 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(KvAttention a, int 
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(bits<float>(kw[h][8 * b + j]), inv);
                         split8(v, &hi, &lo);
-#pragma unroll
-                        for (int u = 0; u < NQ; ++u) {
-                            acc[u] = mfma(hi, qh[u][b], zero);
-                            if (!STACK) acc[u] = mfma(hi, ql[u][b], acc[u]);
-                            acc[u] = mfma(lo, qh[u][b], acc[u]);
-                        }
+                        acc = mfma(lo, qs[b], mfma(hi, qs[b], zero));
+                    } else if (QT == 1) {
+                        acc = mfma(codes8(kw[h][2 * b], kw[h][2 * b + 1], static_cast<_Float16>(128.0f)), qs[b], zero);
                     } else {
-                        h8_t k;
-                        if (QT == 1) {
-                            k = codes8(kw[h][2 * b], kw[h][2 * b + 1], static_cast<_Float16>(128.0f));
-                        } else {
-                            const uint32_t x = kw[h][b];
-                            k = codes8(x & 0x0f0f0f0fu, (x >> 4) & 0x0f0f0f0fu, static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f));
-                        }
-#pragma unroll
-                        for (int u = 0; u < NQ; ++u) {
-                            acc[u] = mfma(k, qh[u][b], zero);
-                            if (!STACK) acc[u] = mfma(k, ql[u][b], acc[u]);
-                        }
+                        const uint32_t x = kw[h][b];
+                        acc = mfma(codes8(x & 0x0f0f0f0fu, (x >> 4) & 0x0f0f0f0fu, static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f)),
+                                   qs[b], zero);
                     }
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[u][h][i] = fmaf(scale_at(ks[h], 4 * b + i), acc[u][i], s[u][h][i]);
-                            if (QT == 3) s[u][h][i] = fmaf(scale_at(km[h], 4 * b + i), qsum[u][b], s[u][h][i]);
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        s[i] = fmaf(scale_at(ks[h], 4 * b + i), acc[i], s[i]);
+                        if (QT == 3) s[i] = fmaf(scale_at(km[h], 4 * b + i), qsum[b], s[i]);
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[4 * h + i] = s[i];
             }
             if (more) load_keys(next);
 
             // Weights.
-            float e[8];  // log2 of a position's largest value scale, plus a constant
-            {
-                uint32_t top[8];
+            float e[8];  // log2 of a position's largest value scale, nearly, plus a constant
+#pragma unroll
+            for (int j = 0; j < 8; j += QT == 0 ? 1 : 2) {
                 if (QT == 0) {
+                    uint32_t top = vs[j];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        top[j] = vs[j];
-#pragma unroll
-                        for (int b = 1; b < NB; ++b) top[j] = max(top[j], vs[8 * b + j]);
-                        e[j] = static_cast<float>(top[j]) * 0x1p-23f;
-                    }
+                    for (int b = 1; b < NB; ++b) top = max(top, vs[8 * b + j]);
+                    e[j] = static_cast<float>(top) * 0x1p-23f;
                 } else {
+                    us2_t top = bits<us2_t>(vs[j / 2]);
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        us2_t t = bits<us2_t>(vs[j / 2]);
-#pragma unroll
-                        for (int b = 1; b < NB; ++b) t = __builtin_elementwise_max(t, bits<us2_t>(vs[4 * b + j / 2]));
-                        e[j] = static_cast<float>(t.x) * 0x1p-10f;
-                        e[j + 1] = static_cast<float>(t.y) * 0x1p-10f;
-                    }
+                    for (int b = 1; b < NB; ++b) top = __builtin_elementwise_max(top, bits<us2_t>(vs[4 * b + j / 2]));
+                    e[j] = static_cast<float>(top.x) * 0x1p-10f;
+                    e[j + 1] = static_cast<float>(top.y) * 0x1p-10f;
                 }
             }
             constexpr float kBias = (QT == 0 ? 127.0f : 15.0f) + 8.0f;
             const bool full = first + kKvTile - 1 <= pos_lo &&
                               (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
-            float p[NQ][8];
+            float top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float x = s[u][j >> 2][j & 3];
-                    if (STACK) x += other_half(x);
-                    x *= to_t[u];
-                    // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
-                    if (QT >= 2) x = fmaf(x, 0.0f, x);
-                    if (!full) {
-                        const int key = first + (j >> 2) * 16 + 4 * g + (j & 3);
-                        const bool seen = key <= pos[u] && (a.window == 0 || key > pos[u] - a.window || key < a.sinks);
-                        x = seen ? x : -INFINITY;
-                    }
-                    p[u][j] = x;
-                    top = fmaxf(top, x + e[j]);
+            for (int j = 0; j < 8; ++j) {
+                t[j] = (t[j] + other_half(t[j])) * to_t;
+                // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
+                if (QT >= 2) t[j] = fmaf(t[j], 0.0f, t[j]);
+                if (!full) {
+                    const int key = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                    const bool seen = key <= pos && (a.window == 0 || key > pos - a.window || key < a.sinks);
+                    t[j] = seen ? t[j] : -INFINITY;
                 }
-                top = max_quarters(top);
-                if (__any(top > m[u] + kSlack)) {
-                    const float to = top > m[u] + kSlack ? top : m[u];
-                    const float c = __builtin_amdgcn_exp2f(m[u] - to);
-                    m[u] = to;
-                    l[u] *= c;
+                top = fmaxf(top, t[j] + e[j]);
+            }
+            top = max_quarters(top);
+            if (__any(top > m + kSlack)) {
+                const float to = top > m + kSlack ? top : m;
+                const float c = __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= c;
 #pragma unroll
-                    for (int t = 0; t < 2 * NB; ++t) o[u][t] *= c;
-                    if (QT == 3) {
+                for (int x = 0; x < 2 * NB; ++x) o[0][x] *= c;
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) om[u][b] *= c;
-                    }
-                }
-                const float frame = m[u] - kBias;
+                for (int b = 0; b < NB; ++b) om[b] *= c;
+            }
+            const float frame = m - kBias;
+            float p[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    p[u][j] = __builtin_amdgcn_exp2f(p[u][j] - frame);
-                    l[u] += p[u][j];
-                }
+            for (int j = 0; j < 8; ++j) {
+                p[j] = __builtin_amdgcn_exp2f(t[j] - frame);
+                l += p[j];
             }
 
             // Values.
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                h8_t ph[NQ], pl[NQ];
+                float v[8];
+                h8_t hi, lo;
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    float v[8];
+                for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[j], scale_at(vs, 8 * b + j));
+                split8(v, &hi, &lo);
+                const h8_t ps = low ? lo : hi;
+                if (QT == 3) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[u][j], scale_at(vs, 8 * b + j));
-                    h8_t hi, lo;
-                    split8(v, &hi, &lo);
-                    ph[u] = STACK && i16 >= 8 ? lo : hi;
-                    pl[u] = lo;
-                    if (QT == 3) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) om[u][b] += mul_or_zero(p[u][j], scale_at(vm, 8 * b + j));
-                    }
+                    for (int j = 0; j < 8; ++j) om[b] += mul_or_zero(p[j], scale_at(vm, 8 * b + j));
                 }
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    h8_t c, lo;
+                for (int x = 0; x < 2; ++x) {
+                    f4_t& acc = o[0][2 * b + x];
                     if (QT == 0) {
-                        float v[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            v[j] = mul_or_zero(bits<float>(vw[16 * b + 8 * t + j]), inverse_power(vs[8 * b + j]));
+                            v[j] = mul_or_zero(bits<float>(vw[16 * b + 8 * x + j]), inverse_power(vs[8 * b + j]));
                         }
-                        split8(v, &c, &lo);
+                        split8(v, &hi, &lo);
+                        acc = mfma(lo, ps, mfma(hi, ps, acc));
                     } else if (QT == 1) {
-                        c = codes8(vw[4 * b + 2 * t], vw[4 * b + 2 * t + 1], static_cast<_Float16>(128.0f));
+                        acc = mfma(codes8(vw[4 * b + 2 * x], vw[4 * b + 2 * x + 1], static_cast<_Float16>(128.0f)), ps, acc);
                     } else {
-                        const uint32_t x = vw[2 * b], y = vw[2 * b + 1];
-                        c = codes8((t == 0 ? x : x >> 4) & 0x0f0f0f0fu, (t == 0 ? y : y >> 4) & 0x0f0f0f0fu,
-                                   static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f));
-                    }
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u) {
-                        f4_t& acc = o[u][2 * b + t];
-                        acc = mfma(c, ph[u], acc);
-                        if (!STACK) acc = mfma(c, pl[u], acc);
-                        if (QT == 0) acc = mfma(lo, ph[u], acc);
+                        const uint32_t y = vw[2 * b], z = vw[2 * b + 1];
+                        acc = mfma(codes8((x == 0 ? y : y >> 4) & 0x0f0f0f0fu, (x == 0 ? z : z >> 4) & 0x0f0f0f0fu,
+                                          static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f)), ps, acc);
                     }
                 }
             }
             if (more) load_values(next);
         }
 
-        // The lanes' sums, the stacked halves and the minima's part together.
+        // The lanes' sums, the halves and the minima's part together.
+        l = sum_quarters(l);
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            l[u] = sum_quarters(l[u]);
+        for (int b = 0; b < NB; ++b) {
+            const float add = QT == 3 ? sum_quarters(om[b]) : 0.0f;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float add = QT == 3 ? sum_quarters(om[u][b]) : 0.0f;
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = o[u][2 * b + t][i];
-                        if (STACK) x += other_half(x);
-                        o[u][2 * b + t][i] = QT == 3 ? x + add : x;
-                    }
-            }
+                for (int i = 0; i < 4; ++i) {
+                    const float y = o[0][2 * b + x][i];
+                    o[0][2 * b + x][i] = y + other_half(y) + add;
+                }
         }
-        // Takes in another state of the same rows.
-        auto fold = [&](int u, float m1, float l1, float* w0, float* w1) {
-            const float to = fmaxf(m[u], m1);
-            *w0 = __builtin_amdgcn_exp2f(m[u] - to);
-            *w1 = __builtin_amdgcn_exp2f(m1 - to);
-            m[u] = to;
-            l[u] = l[u] * *w0 + l1 * *w1;
-        };
+        // The four waves' states into wave 0, in a fixed order.
         auto leave = [&](float* to) {
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-#pragma unroll
-                for (int t = 0; t < 2 * NB; ++t) *reinterpret_cast<f4_t*>(to + ((u * 2 * NB + t) * 64 + lane) * 4) = o[u][t];
-                to[QUADS * 256 + (2 * u) * 64 + lane] = m[u];
-                to[QUADS * 256 + (2 * u + 1) * 64 + lane] = l[u];
-            }
+            for (int x = 0; x < 2 * NB; ++x) *reinterpret_cast<f4_t*>(to + (x * 64 + lane) * 4) = o[0][x];
+            to[2 * NB * 256 + lane] = m;
+            to[2 * NB * 256 + 64 + lane] = l;
         };
         auto take = [&](const float* from) {
+            float w0, w1;
+            fold(m, l, from[2 * NB * 256 + lane], from[2 * NB * 256 + 64 + lane], &w0, &w1);
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                float w0, w1;
-                fold(u, from[QUADS * 256 + (2 * u) * 64 + lane], from[QUADS * 256 + (2 * u + 1) * 64 + lane], &w0, &w1);
-#pragma unroll
-                for (int t = 0; t < 2 * NB; ++t) {
-                    const f4_t x = *reinterpret_cast<const f4_t*>(from + ((u * 2 * NB + t) * 64 + lane) * 4);
-                    o[u][t] = o[u][t] * w0 + x * w1;
-                }
+            for (int x = 0; x < 2 * NB; ++x) {
+                o[0][x] = o[0][x] * w0 + *reinterpret_cast<const f4_t*>(from + (x * 64 + lane) * 4) * w1;
             }
         };
-        // The four waves' states into wave 0, in a fixed order.
         auto merge_waves = [&] {
             __syncthreads();
             if (wave >= 2) leave(merge + (wave - 2) * STATE);
@@ -516,119 +519,33 @@ __global__ __launch_bounds__(kThreads) void attention_kernel(KvAttention a, int 
             __syncthreads();
             if (wave == 0) take(merge);
         };
-        if (!together) merge_waves();
+        merge_waves();
 
         if (it.nsplit > 1) {
-            // This part's state to memory; the workgroup that arrives last merges all parts.
-            const size_t each = static_cast<size_t>(STATE) * sizeof(float);
-            uint8_t* const parts = reinterpret_cast<uint8_t*>(a.partial);
+            // This part's state to memory; the workgroup that arrives last merges all parts, wave w
+            // taking w, w + 4, ...
             auto rsrc_of = [&](int split) {
-                return __builtin_amdgcn_make_buffer_rsrc(
-                    parts + (static_cast<size_t>(it.slot + split) * n_kv + head) * each, static_cast<short>(0),
-                    static_cast<int>(each), 0x00020000);
+                return state_rsrc(a.partial, static_cast<size_t>(it.slot + split) * n_kv + head, STATE);
             };
             if (wave == 0) {
-                const __amdgpu_buffer_rsrc_t rs = rsrc_of(it.split);
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-#pragma unroll
-                    for (int t = 0; t < 2 * NB; ++t) {
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, o[u][t]), rs,
-                                                               ((u * 2 * NB + t) * 64 + lane) * 16, 0, kCoherent);
-                    }
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[u]), rs,
-                                                          (QUADS * 256 + (2 * u) * 64 + lane) * 4, 0, kCoherent);
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[u]), rs,
-                                                          (QUADS * 256 + (2 * u + 1) * 64 + lane) * 4, 0, kCoherent);
-                }
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
-                if (lane == 0) {
-                    unsigned* const c = a.arrived + static_cast<size_t>(it.slot) * n_kv + head;
-                    const unsigned before = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    last = before + 1 == static_cast<unsigned>(it.nsplit) ? 1u : 0u;
-                    if (last != 0u) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                leave_state<1, NB>(rsrc_of(it.split), lane, o, &m, &l);
+                if (lane == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);
             }
             __syncthreads();
             const bool mine = last != 0u;
             __syncthreads();
             if (!mine) continue;
-            // Wave w takes parts w, w + 4, ...
+            m = -3.402823466e38f;
+            l = 0.0f;
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                m[u] = -3.402823466e38f;
-                l[u] = 0.0f;
-#pragma unroll
-                for (int t = 0; t < 2 * NB; ++t) o[u][t] = zero;
-            }
-            for (int part = wave; part < it.nsplit; part += kKvWaves) {
-                const __amdgpu_buffer_rsrc_t rs = rsrc_of(part);
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    const float m1 = bits<float>(__builtin_amdgcn_raw_buffer_load_b32(rs, (QUADS * 256 + (2 * u) * 64 + lane) * 4, 0, kCoherent));
-                    const float l1 = bits<float>(__builtin_amdgcn_raw_buffer_load_b32(rs, (QUADS * 256 + (2 * u + 1) * 64 + lane) * 4, 0, kCoherent));
-                    f4_t x[2 * NB];
-#pragma unroll
-                    for (int t = 0; t < 2 * NB; ++t) {
-                        x[t] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, ((u * 2 * NB + t) * 64 + lane) * 16, 0, kCoherent));
-                    }
-                    float w0, w1;
-                    fold(u, m1, l1, &w0, &w1);
-#pragma unroll
-                    for (int t = 0; t < 2 * NB; ++t) o[u][t] = o[u][t] * w0 + x[t] * w1;
-                }
-            }
+            for (int x = 0; x < 2 * NB; ++x) o[0][x] = zero;
+            for (int part = wave; part < it.nsplit; part += kKvWaves) take_state<1, NB>(rsrc_of(part), lane, o, &m, &l);
             merge_waves();
         }
 
-        if (!idle && (together || wave == 0)) {
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                if (row0 + 16 * u + i16 >= row1 || (STACK && i16 >= 8)) continue;
-                const float inv = 1.0f / l[u];
-#pragma unroll
-                for (int t = 0; t < 2 * NB; ++t) {
-                    const int d = 16 * t + 4 * g;
-                    if (d < hd) *reinterpret_cast<f4_t*>(out + out_row[u] + d) = o[u][t] * inv;
-                }
-            }
-        }
-    }
-}
-
-template <int QT, int NB, int ROWS>
-hipError_t launch_rows(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
-    // recorded launches walk whatever list is set by then: four workgroups a CU
-    const unsigned grid = count > 0 ? static_cast<unsigned>(count) * a.kv.n_kv : 1024u;
-    attention_kernel<QT, NB, ROWS><<<grid, kThreads, 0, s>>>(a, kind, count, q, out);
-    return hipGetLastError();
-}
-
-template <int QT, int NB>
-hipError_t launch_blocks(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
-    return kind == 0 ? launch_rows<QT, NB, kKvNarrowRows>(a, kind, count, q, out, s)
-                     : launch_rows<QT, NB, NB <= 4 ? 32 : 16>(a, kind, count, q, out, s);
-}
-
-template <int QT>
-hipError_t launch(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
-    switch (a.kv.nb) {
-        case 1: return launch_blocks<QT, 1>(a, kind, count, q, out, s);
-        case 2: return launch_blocks<QT, 2>(a, kind, count, q, out, s);
-        case 3: return launch_blocks<QT, 3>(a, kind, count, q, out, s);
-        case 4: return launch_blocks<QT, 4>(a, kind, count, q, out, s);
-        case 6: return launch_blocks<QT, 6>(a, kind, count, q, out, s);
-        case 8: return launch_blocks<QT, 8>(a, kind, count, q, out, s);
-        default: return hipErrorInvalidValue;
+        if (wave == 0 && !low && it.row0 + i16 < row1) store_row<NB>(out + out_row, hd, g, o[0], 1.0f / l);
     }
 }
 
 }  // namespace kv
-
-// One translation unit a type.
-hipError_t launch_kv_attention_f32(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
-hipError_t launch_kv_attention_q8_0(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
-hipError_t launch_kv_attention_q4_0(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
-hipError_t launch_kv_attention_q4_1(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
-
 }  // namespace mlq

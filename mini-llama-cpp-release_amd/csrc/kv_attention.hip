@@ -1,10 +1,16 @@
 // Attention over the paged cache: which type's kernels a call runs (kv_attention.h).
 
-#include "kv_attention.h"
+#include "kv_layout.h"
 
 namespace mlq {
 
-int kv_wide_rows(int nb) { return nb <= 4 ? 32 : 16; }
+// One translation unit a type.
+hipError_t launch_kv_attention_f32(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+hipError_t launch_kv_attention_q8_0(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+hipError_t launch_kv_attention_q4_0(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+hipError_t launch_kv_attention_q4_1(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+
+int kv_wide_rows(int nb) { return nb <= 4 ? 128 : 64; }
 
 size_t kv_partial_floats(int nb, int kind) {
     return static_cast<size_t>(kind == 0 ? 1 : kv_wide_rows(nb) / 16) * 64 * (8 * nb + 2);

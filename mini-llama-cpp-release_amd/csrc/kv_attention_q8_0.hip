@@ -1,6 +1,6 @@
-// Attention over pages of Q8_0 keys and values (kv_attention.h).
+// Attention over pages of Q8_0 keys and values (kv_attention.h, kv_attention_rows.h).
 
-#include "kv_attention.h"
+#include "kv_attention_rows.h"
 
 namespace mlq {
 

@@ -118,7 +118,7 @@ struct KvAttention {
     float* partial;     // [slot][KV head][kv_partial_floats]
     unsigned* arrived;  // [first slot of a split][KV head], zero between launches
 };
-// Rows per wave of the kernel for many rows, and a part's floats in `partial` by list (0 narrow, 1 wide).
+// Query rows of a workgroup of the kernel for many rows, and a part's floats in `partial` by list (0 narrow, 1 wide).
 int kv_wide_rows(int nb);
 size_t kv_partial_floats(int nb, int kind);
 // count: items of the narrow (kind 0) or wide list, 0 as above.

@@ -7,15 +7,11 @@
 namespace mlq {
 namespace {
 
-// Workgroups of four waves that keep 256 CUs busy: a split makes more of them
-// until there are this many, and no more.
-constexpr int kTargetGroups = 1024;
-// Fewer tiles than this are not split further: the parts' merge would cost more
-// than the tiles (two a wave).
+// A split makes workgroups until there are this many (few rows, many rows: four and
+// two a CU), and no more.
+constexpr int kTargetGroups[2] = {1024, 512};
+// Fewer tiles than this are not split further: the parts' merge would cost more.
 constexpr int kLeastTiles = 8;
-// From this many workgroups on, many-row sequences run without splits: each wave has
-// rows of its own and a workgroup's waves read the same tiles together.
-constexpr int kEnoughGroups = 512;
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -35,15 +31,16 @@ Seen seen_tiles(const KvPlanShape& s, int lo, int hi) {
 }  // namespace
 
 KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
-    const int extra = ceil_div(kTargetGroups, s.n_kv_heads);
     const int64_t rows = static_cast<int64_t>(s.max_tokens) * s.group;
-    const int wide = static_cast<int>(rows / s.wide_rows) + s.max_seqs;
+    const int whole[2] = {s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
     KvPlanLimits l;
-    l.items[0] = s.max_seqs + extra;
-    l.items[1] = wide + extra;
-    // Only items beyond an unsplit list's are parts, and a split of n parts adds n - 1
-    // items: at most twice the extra ones.
-    l.slots[0] = l.slots[1] = 2 * extra;
+    for (int kind = 0; kind < 2; ++kind) {
+        // Only an item of n parts adds to the list, n - 1 items, and all parts take slots: at
+        // most twice what is added.
+        const int extra = ceil_div(kTargetGroups[kind], s.n_kv_heads);
+        l.items[kind] = whole[kind] + extra;
+        l.slots[kind] = 2 * extra;
+    }
     return l;
 }
 
@@ -109,7 +106,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
         if (n > 0) {
             const int rows = n * s.group;
             const int kind = rows <= kKvNarrowRows ? 0 : 1;
-            base[kind].push_back(KvAttnItem{token0, n, len, page0, 0, 0, 0, 0, 0, kKvWaves, 0, 1, 0});
+            base[kind].push_back(KvAttnItem{token0, n, len, page0, 0, 0, 0, 0, 0, 0, 1, 0});
         }
         token0 += n;
         row0 += len;
@@ -125,11 +122,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     }
 
     for (int kind = 0; kind < 2; ++kind) {
-        const int per = kind == 0 ? kKvNarrowRows : s.wide_rows;
-        int64_t groups = 0;  // workgroups with rows of their own in every wave
-        for (const KvAttnItem& q : base[kind]) groups += ceil_div(q.new_tokens * s.group, per * kKvWaves);
-        const bool together = kind == 1 && groups * s.n_kv_heads >= kEnoughGroups;
-        const int step = together ? per * kKvWaves : per;
+        const int step = kind == 0 ? kKvNarrowRows : s.wide_rows;
         std::vector<KvAttnItem> whole;
         int64_t tiles = 0;
         for (const KvAttnItem& q : base[kind]) {
@@ -141,32 +134,27 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
                 it.count = t.count;
                 it.sinks = t.sinks;
                 it.shift = t.shift;
-                it.stride = together ? 1 : kKvWaves;
                 tiles += t.count;
                 whole.push_back(it);
             }
         }
+        // Parts of at most `most` tiles, as even as they come.
         std::vector<KvAttnItem>& list = b.items[kind];
-        if (together) {
-            list = std::move(whole);
-        } else {
-            // Parts of at most `most` tiles, as even as they come.
-            const int target = ceil_div(kTargetGroups, s.n_kv_heads);
-            const int most = std::max<int64_t>(kLeastTiles, (tiles + target - 1) / target);
-            int slot = 0;
-            for (const KvAttnItem& w : whole) {
-                const int parts = ceil_div(w.count, most);
-                for (int p = 0; p < parts; ++p) {
-                    KvAttnItem it = w;
-                    it.first = static_cast<int>(static_cast<int64_t>(w.count) * p / parts);
-                    it.count = static_cast<int>(static_cast<int64_t>(w.count) * (p + 1) / parts) - it.first;
-                    it.split = p;
-                    it.nsplit = parts;
-                    it.slot = slot;
-                    list.push_back(it);
-                }
-                if (parts > 1) slot += parts;
+        const int target = ceil_div(kTargetGroups[kind], s.n_kv_heads);
+        const int most = static_cast<int>(std::max<int64_t>(kLeastTiles, (tiles + target - 1) / target));
+        int slot = 0;
+        for (const KvAttnItem& w : whole) {
+            const int parts = ceil_div(w.count, most);
+            for (int p = 0; p < parts; ++p) {
+                KvAttnItem it = w;
+                it.first = static_cast<int>(static_cast<int64_t>(w.count) * p / parts);
+                it.count = static_cast<int>(static_cast<int64_t>(w.count) * (p + 1) / parts) - it.first;
+                it.split = p;
+                it.nsplit = parts;
+                it.slot = slot;
+                list.push_back(it);
             }
+            if (parts > 1) slot += parts;
         }
         // The longest first: what starts last is short.
         std::stable_sort(list.begin(), list.end(),

@@ -30,20 +30,17 @@ struct KvPage {
 // its tiles.  The tiles a row can see are numbered without the gap between the
 // first tiles that stay visible (`sinks` of them) and the window: tile i is i
 // below `sinks` and i + shift from there.
-// stride 1: every wave takes the rows after the wave before it, over all tiles;
-// stride kKvWaves: the waves share one set of rows and take every fourth tile.
 struct KvAttnItem {
     int token0, new_tokens, len, page0;  // the sequence: first row in q, new tokens, positions, first entry in the page list
     int row0, first, count;
     int sinks, shift;
-    int stride;
     int split, nsplit, slot;  // part `split` of nsplit; the parts' first slot in the partial results
 };
 
 struct KvPlanShape {
     int page_size, n_pages, n_kv_heads;
     int group;      // query heads per KV head
-    int wide_rows;  // query rows per wave of the kernel for many rows
+    int wide_rows;  // query rows of a workgroup of the kernel for many rows
     int window, sinks;
     int max_seqs, max_tokens, max_pages;
 };

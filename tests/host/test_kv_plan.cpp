@@ -39,7 +39,7 @@ void one(std::mt19937& rng, int trial) {
     s.page_size = pick(rng, {32, 64, 256, 4096});
     s.n_kv_heads = pick(rng, {1, 2, 8, 32});
     s.group = pick(rng, {1, 2, 7, 8, 16});
-    s.wide_rows = pick(rng, {16, 32});
+    s.wide_rows = pick(rng, {64, 128});
     s.window = pick(rng, {0, 0, 1, 20, 32, 33, 100, 1000});
     s.sinks = s.window ? pick(rng, {0, 1, 4, 32, 40, 3000}) : 0;
     const int n_seqs = rng() % 6;
@@ -97,15 +97,14 @@ void one(std::mt19937& rng, int trial) {
     std::map<int, std::set<int>> parts;
     for (int kind = 0; kind < 2; ++kind) {
         CHECK(static_cast<int>(b.items[kind].size()) <= lim.items[kind], "trial %d", trial);
-        const int per = kind == 0 ? mlq::kKvNarrowRows : s.wide_rows;
+        const int step = kind == 0 ? mlq::kKvNarrowRows : s.wide_rows;
         for (const KvAttnItem& it : b.items[kind]) {
             CHECK(it.count > 0 && it.first >= 0 && it.split < it.nsplit, "trial %d", trial);
             if (it.nsplit > 1) {
                 CHECK(it.slot >= 0 && it.slot + it.nsplit <= lim.slots[kind], "trial %d: slot %d of %d", trial, it.slot, lim.slots[kind]);
-                CHECK(it.stride == mlq::kKvWaves && parts[2 * it.slot + kind].insert(it.split).second, "trial %d", trial);
+                CHECK(parts[2 * it.slot + kind].insert(it.split).second, "trial %d", trial);
             }
             const int rows = it.new_tokens * s.group;
-            const int step = it.stride == 1 ? per * mlq::kKvWaves : per;
             CHECK(it.row0 < rows && it.row0 % step == 0, "trial %d", trial);
             for (int k = it.first; k < it.first + it.count; ++k) {
                 const int tile = k < it.sinks ? k : k + it.shift;
@@ -142,7 +141,7 @@ void refused(const KvPlanShape& s, std::vector<int> fresh, std::vector<int> len,
 int main() {
     std::mt19937 rng(7);
     for (int t = 0; t < 200; ++t) one(rng, t);
-    const KvPlanShape s{64, 10, 2, 4, 32, 0, 0, 3, 100, 6};
+    const KvPlanShape s{64, 10, 2, 4, 128, 0, 0, 3, 100, 6};
     refused(s, {1, 1, 1, 1}, {1, 1, 1, 1}, {0, 1, 2, 3}, "4 sequences, the plan holds 3");
     refused(s, {-1}, {4}, {0}, "negative token count");
     refused(s, {5}, {4}, {0}, "5 new tokens in a length of 4");
