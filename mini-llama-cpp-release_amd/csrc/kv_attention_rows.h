@@ -22,20 +22,25 @@
 #include "kv_attention.h"
 #include "quant_device.h"
 
+#include <type_traits>
+
 namespace mlq {
 namespace kv {
 
-// Scales of a tile in LDS.
+// Scales of a tile in LDS: what a code (f32: an element) is multiplied by, and, for f32
+// arithmetic on quantized codes, what is added then.
 template <int QT, int NB>
 struct TileScales {
-    // keys, values: what a code (f32: an element) is multiplied by and, quantized, what is added then
-    float scale[2][QT == 0 ? 1 : 2][NB][kKvTile];
-    float key_up[kKvTile];           // 2^ek
-    float value_log[kKvTile];        // ev
-    float value_up[kKvTile];         // 2^ev
-    uint32_t bad[NB];                // positions whose value block is not finite
-    uint32_t any_bad;
+    static constexpr bool kPacked = QT == 1 || QT == 2;  // decoded in packed fp16
+    typename std::conditional<kPacked, _Float16, float>::type scale[2][QT == 3 ? 2 : 1][NB][kKvTile];  // keys, values
+    float key_up[kKvTile];     // 2^ek
+    float value_log[kKvTile];  // ev
+    float value_up[kKvTile];   // 2^ev
+    uint32_t bad[NB];          // positions whose value block is not finite
+    uint32_t flags;            // kBad: any of `bad`; kFar: some power of two is not 1
 };
+constexpr uint32_t kBad = 1, kFar = 2;
+constexpr float kLift = 256.0f;  // operands lie in LDS times this
 
 template <int QT, int NB>
 constexpr int rows_lds_bytes() {
@@ -85,7 +90,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
             pos[u] = start + token;
             out_row[u] = (static_cast<size_t>(it.token0 + token) * heads + head * a.group + r % a.group) * hd;
             float v[NB][8], sum[NB];
-            load_query<NB>(q + out_row[u], hd, g, a.scale, v, sum, &to_t[u]);
+            load_query<NB>(q + out_row[u], hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) split8(v[b], &qh[u][b], &ql[u][b]);
         }
@@ -156,35 +161,33 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
                                           : reinterpret_cast<const uint16_t*>(p + x * F::plane(NB))[at];
                 }
         };
-        // Scales to LDS.  A position's power of two: what brings its largest element to about 2^8.
+        // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position: 1 where the
+        // position's largest element is from 2^-10 to 2^7 (the parts then lose what they do at 1,
+        // 2^-22, and none reaches 2^15), else what brings it to [1, 2).
         auto make_scales = [&](Scales* s) {
             if (wave != 0) return;
-            constexpr float kOff = QT == 1 ? 128.0f : QT == 2 ? 8.0f : 0.0f;  // of a stored code
             float d[NB], add[NB];
             float top = 0.0f;
             bool bad[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                if (QT == 0) {
-                    d[b] = bits<float>(raw_s[0][b]);
-                    add[b] = 0.0f;
-                } else {
-                    d[b] = half_value(static_cast<uint16_t>(raw_s[0][b]));
-                    add[b] = QT == 3 ? half_value(static_cast<uint16_t>(raw_s[F::kPlanes - 1][b])) : -kOff * d[b];
-                }
+                d[b] = QT == 0 ? bits<float>(raw_s[0][b]) : half_value(static_cast<uint16_t>(raw_s[0][b]));
+                add[b] = QT == 3 ? half_value(static_cast<uint16_t>(raw_s[F::kPlanes - 1][b])) : 0.0f;
                 bad[b] = !(fabsf(d[b]) < INFINITY) || !(fabsf(add[b]) < INFINITY);
-                const float most = QT == 0 ? d[b] : QT == 3 ? 16.0f * d[b] + fabsf(add[b]) : kOff * d[b];
+                const float most = QT == 0 ? d[b] : QT == 3 ? fmaf(16.0f, d[b], fabsf(add[b])) : (QT == 1 ? 128.0f : 8.0f) * d[b];
                 if (!bad[b]) top = fmaxf(top, most);
             }
-            const int e = max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 8, -90);
-            const float down = ldexpf(1.0f, -e);
+            int e = static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+            e = top == 0.0f || (e >= -10 && e < 7) ? 0 : max(e, -90);
+            const float down = ldexpf(kLift, -e);
             uint32_t any = 0;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 // keys: NaN through to the score; values: zero here, NaN for the rows that see it (`bad`)
                 const float nothing = lane >= 32 ? 0.0f : NAN;
-                s->scale[lane >> 5][0][b][key] = bad[b] ? nothing : QT == 0 ? down : d[b] * down;
-                if (QT != 0) s->scale[lane >> 5][QT == 0 ? 0 : 1][b][key] = bad[b] ? nothing : add[b] * down;
+                using T = typename std::remove_reference<decltype(s->scale[0][0][0][0])>::type;
+                s->scale[lane >> 5][0][b][key] = static_cast<T>(bad[b] ? nothing : QT == 0 ? down : d[b] * down);
+                if (QT == 3) s->scale[lane >> 5][QT == 3 ? 1 : 0][b][key] = static_cast<T>(bad[b] ? nothing : add[b] * down);
                 const uint32_t mask = static_cast<uint32_t>(__ballot(bad[b]) >> 32);
                 any |= mask;
                 if (lane == 0) s->bad[b] = mask;
@@ -195,49 +198,64 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
                 s->value_log[key] = static_cast<float>(e);
                 s->value_up[key] = ldexpf(1.0f, e);
             }
-            if (lane == 0) s->any_bad = any;
+            const bool far = __any(e != 0);
+            if (lane == 0) s->flags = (any != 0 ? kBad : 0u) | (far ? kFar : 0u);
         };
-        // Code j of an operand's raw words; 4-bit: the low or high nibbles (values: `t` says which).
-        auto key_code = [&](const uint32_t* raw, int j) -> float {
-            if (QT == 0) return bits<float>(raw[j]);
-            if (QT == 1) return static_cast<float>((raw[j >> 2] >> (8 * (j & 3))) & 0xffu);
-            return static_cast<float>((raw[0] >> (8 * (j & 3) + 4 * (j >> 2))) & 0xfu);
-        };
-        auto value_code = [&](const uint32_t* raw, int j, int t) -> float {
-            if (QT == 0) return bits<float>(raw[j]);
-            if (QT == 1) return static_cast<float>((raw[j >> 2] >> (8 * (j & 3))) & 0xffu);
-            return static_cast<float>((((raw[j >> 2] >> (4 * t)) & 0x0f0f0f0fu) >> (8 * (j & 3))) & 0xffu);
+        // Eight codes as fp16 (minus the stored offset): keys, values (`t`: which nibbles).
+        auto codes_of = [&](const uint32_t* raw, bool values, int t) -> h8_t {
+            if (QT == 1) return codes8(raw[0], raw[RAW_K - 1], static_cast<_Float16>(128.0f));
+            const _Float16 off = static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f);
+            if (values) return codes8((raw[0] >> (4 * t)) & 0x0f0f0f0fu, (raw[1] >> (4 * t)) & 0x0f0f0f0fu, off);
+            return codes8(raw[0] & 0x0f0f0f0fu, (raw[0] >> 4) & 0x0f0f0f0fu, off);
         };
         auto convert = [&](int buffer, const Scales* s) {
 #pragma unroll
             for (int k = 0; k < TASKS; ++k) {
                 const int f = wave + kKvWaves * k;
-                if (f >= FRAGS) continue;
+                if (FRAGS % kKvWaves != 0 && f >= FRAGS) continue;
                 const int h = f / NB, b = f % NB, bv = f >> 1, t = f & 1;
-                // The sum of a product and the scale's multiple is exact in f32 (19 bits; Q4_1: one rounding).
-                float x[8];
                 h8_t hi, lo;
-                const float d = s->scale[0][0][b][16 * h + i16];
-                const float add = QT == 0 ? 0.0f : s->scale[0][QT == 0 ? 0 : 1][b][16 * h + i16];
+                if constexpr (Scales::kPacked) {
+                    // code times scale: at most 19 bits, so hi and what is left of it are exact
+                    const _Float16 d = s->scale[0][0][b][16 * h + i16];
+                    const h8_t d8{d, d, d, d, d, d, d, d};
+                    h8_t c = codes_of(raw_k[k], false, 0);
+                    hi = c * d8;
+                    lo = __builtin_elementwise_fma(c, d8, -hi);
+                    operand(buffer, 0, f)[lane] = hi;
+                    operand(buffer, 1, f)[lane] = lo;
+                    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+                    const h4_t x = *reinterpret_cast<const h4_t*>(s->scale[1][0][bv] + 4 * g);
+                    const h4_t y = *reinterpret_cast<const h4_t*>(s->scale[1][0][bv] + 16 + 4 * g);
+                    const h8_t dv = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                    c = codes_of(raw_v[k], true, t);
+                    hi = c * dv;
+                    lo = __builtin_elementwise_fma(c, dv, -hi);
+                } else {
+                    float x[8];
+                    const float d = s->scale[0][0][b][16 * h + i16];
+                    const float add = QT == 3 ? s->scale[0][QT == 3 ? 1 : 0][b][16 * h + i16] : 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float c = key_code(raw_k[k], j);
-                    x[j] = QT == 0 ? c * d : fmaf(c, d, add);
-                }
-                split8(x, &hi, &lo);
-                operand(buffer, 0, f)[lane] = hi;
-                operand(buffer, 1, f)[lane] = lo;
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const f4_t d4 = *reinterpret_cast<const f4_t*>(s->scale[1][0][bv] + 16 * y + 4 * g);
-                    const f4_t a4 = *reinterpret_cast<const f4_t*>(s->scale[1][QT == 0 ? 0 : 1][bv] + 16 * y + 4 * g);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float c = value_code(raw_v[k], 4 * y + i, t);
-                        x[4 * y + i] = QT == 0 ? mul_or_zero(c, d4[i]) : fmaf(c, d4[i], a4[i]);
+                    for (int j = 0; j < 8; ++j) {
+                        x[j] = QT == 0 ? bits<float>(raw_k[k][j & (RAW_K - 1)]) * d
+                                       : fmaf(static_cast<float>((raw_k[k][0] >> (8 * (j & 3) + 4 * (j >> 2))) & 0xfu), d, add);
                     }
+                    split8(x, &hi, &lo);
+                    operand(buffer, 0, f)[lane] = hi;
+                    operand(buffer, 1, f)[lane] = lo;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const f4_t d4 = *reinterpret_cast<const f4_t*>(s->scale[1][0][bv] + 16 * y + 4 * g);
+                        const f4_t a4 = *reinterpret_cast<const f4_t*>(s->scale[1][QT == 3 ? 1 : 0][bv] + 16 * y + 4 * g);
+                        const uint32_t nibbles = (raw_v[k][y] >> (4 * t)) & 0x0f0f0f0fu;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[4 * y + i] = QT == 0 ? mul_or_zero(bits<float>(raw_v[k][(4 * y + i) & (RAW_V - 1)]), d4[i])
+                                                   : fmaf(static_cast<float>((nibbles >> (8 * i)) & 0xffu), d4[i], a4[i]);
+                        }
+                    }
+                    split8(x, &hi, &lo);
                 }
-                split8(x, &hi, &lo);
                 operand(buffer, 2, f)[lane] = hi;
                 operand(buffer, 3, f)[lane] = lo;
             }
@@ -263,6 +281,21 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
             const int buffer = (i - it.first) & 1;
             const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
             const Scales* const s = scales + slot;
+
+            f4_t sc[NQ][2];
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) sc[u][0] = sc[u][1] = zero;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const h8_t k0 = operand(buffer, 0, b)[lane], k1 = operand(buffer, 0, NB + b)[lane];
+                const h8_t l0 = operand(buffer, 1, b)[lane], l1 = operand(buffer, 1, NB + b)[lane];
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k0, qh[u][b], sc[u][0]), sc[u][1] = mfma(k1, qh[u][b], sc[u][1]);
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k0, ql[u][b], sc[u][0]), sc[u][1] = mfma(k1, ql[u][b], sc[u][1]);
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(l0, qh[u][b], sc[u][0]), sc[u][1] = mfma(l1, qh[u][b], sc[u][1]);
+            }
             // Ahead: convert i + 1, scales of i + 2, loads of i + 2 (raw) and i + 3 (scales).
             convert(buffer ^ 1, scales + slot1);
             make_scales(scales + slot2);
@@ -270,100 +303,86 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
             load_scales(base_of(i + 3));
 
             const int first = tile_of(i) * kKvTile;
-            const bool sees = first <= pos_hi && (a.window == 0 || first + kKvTile - 1 > pos_lo - a.window || first < a.sinks);
-            if (!idle && sees) {
-                f4_t sc[NQ][2];
+            const bool full = first + kKvTile - 1 <= pos_lo &&
+                              (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
+            const uint32_t flags = __builtin_amdgcn_readfirstlane(s->flags);
+            h8_t ph[NQ], pl[NQ];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) sc[u][0] = sc[u][1] = zero;
+            for (int u = 0; u < NQ; ++u) {
+                float t[8], top;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const h8_t k0 = operand(buffer, 0, b)[lane], k1 = operand(buffer, 0, NB + b)[lane];
-                    const h8_t l0 = operand(buffer, 1, b)[lane], l1 = operand(buffer, 1, NB + b)[lane];
+                for (int j = 0; j < 8; ++j) t[j] = sc[u][j >> 2][j & 3] * to_t[u];
+                if (flags & kFar) {
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k0, qh[u][b], sc[u][0]), sc[u][1] = mfma(k1, qh[u][b], sc[u][1]);
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k0, ql[u][b], sc[u][0]), sc[u][1] = mfma(k1, ql[u][b], sc[u][1]);
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(l0, qh[u][b], sc[u][0]), sc[u][1] = mfma(l1, qh[u][b], sc[u][1]);
+                    for (int j = 0; j < 8; ++j) t[j] *= s->key_up[(j >> 2) * 16 + 4 * g + (j & 3)];
                 }
-                float up[8], log[8], vup[8];
+                if (!full) {
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const f4_t x = *reinterpret_cast<const f4_t*>(s->key_up + 16 * y + 4 * g);
-                    const f4_t z = *reinterpret_cast<const f4_t*>(s->value_log + 16 * y + 4 * g);
-                    const f4_t v = *reinterpret_cast<const f4_t*>(s->value_up + 16 * y + 4 * g);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) up[4 * y + j] = x[j], log[4 * y + j] = z[j], vup[4 * y + j] = v[j];
+                    for (int j = 0; j < 8; ++j) {
+                        const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                        const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
+                        t[j] = seen ? t[j] : -INFINITY;
+                    }
                 }
-                const bool full = first + kKvTile - 1 <= pos_lo &&
-                                  (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
-                const bool bad = __builtin_amdgcn_readfirstlane(s->any_bad) != 0;
-                h8_t ph[NQ], pl[NQ];
+                if (flags & kFar) {
+                    top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j] + s->value_log[(j >> 2) * 16 + 4 * g + (j & 3)]);
+                } else {
+                    top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+                }
+                top = max_quarters(top);
+                if (__any(top > m[u] + kSlack)) {
+                    const float to = top > m[u] + kSlack ? top : m[u];
+                    const float c = __builtin_amdgcn_exp2f(m[u] - to);
+                    m[u] = to;
+                    l[u] *= c;
+#pragma unroll
+                    for (int x = 0; x < 2 * NB; ++x) o[u][x] *= c;
+                }
+                // P_j = p_j 2^ev_j up to 2^(6 + 8)
+                const float frame = m[u] - 8.0f;
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[j] = __builtin_amdgcn_exp2f(t[j] - frame);
+                    l[u] += p[j];
+                }
+                if (flags & kBad) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t mask = s->bad[b];
+                        bool hit = false;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            hit = hit || (((mask >> ((j >> 2) * 16 + 4 * g + (j & 3))) & 1u) != 0 && !(p[j] == 0.0f));
+                        }
+                        const float add = sum_quarters(hit ? NAN : 0.0f);
+                        o[u][2 * b] += add;
+                        o[u][2 * b + 1] += add;
+                    }
+                }
+                if (flags & kFar) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) p[j] *= s->value_up[(j >> 2) * 16 + 4 * g + (j & 3)];
+                }
+                split8(p, &ph[u], &pl[u]);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const h8_t v0 = operand(buffer, 2, 2 * b)[lane], v1 = operand(buffer, 2, 2 * b + 1)[lane];
+                const h8_t l0 = operand(buffer, 3, 2 * b)[lane], l1 = operand(buffer, 3, 2 * b + 1)[lane];
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
-                    float t[8], top = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        t[j] = sc[u][j >> 2][j & 3] * (up[j] * to_t[u]);
-                        if (!full) {
-                            const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
-                            const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
-                            t[j] = seen ? t[j] : -INFINITY;
-                        }
-                        top = fmaxf(top, t[j] + log[j]);
-                    }
-                    top = max_quarters(top);
-                    if (__any(top > m[u] + kSlack)) {
-                        const float to = top > m[u] + kSlack ? top : m[u];
-                        const float c = __builtin_amdgcn_exp2f(m[u] - to);
-                        m[u] = to;
-                        l[u] *= c;
-#pragma unroll
-                        for (int x = 0; x < 2 * NB; ++x) o[u][x] *= c;
-                    }
-                    // P_j = p_j 2^ev_j up to 2^(6 + kUp) < 2^15
-                    constexpr float kUp = 8.0f;
-                    const float frame = m[u] - kUp;
-                    float p[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        p[j] = __builtin_amdgcn_exp2f(t[j] - frame);
-                        l[u] += p[j];
-                    }
-                    if (bad) {
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const uint32_t mask = s->bad[b];
-                            bool hit = false;
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                hit = hit || (((mask >> ((j >> 2) * 16 + 4 * g + (j & 3))) & 1u) != 0 && !(p[j] == 0.0f));
-                            }
-                            const float add = sum_quarters(hit ? NAN : 0.0f);
-                            o[u][2 * b] += add;
-                            o[u][2 * b + 1] += add;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) p[j] *= vup[j];
-                    split8(p, &ph[u], &pl[u]);
+                    o[u][2 * b] = mfma(v0, ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v1, ph[u], o[u][2 * b + 1]);
                 }
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const h8_t v0 = operand(buffer, 2, 2 * b)[lane], v1 = operand(buffer, 2, 2 * b + 1)[lane];
-                    const h8_t l0 = operand(buffer, 3, 2 * b)[lane], l1 = operand(buffer, 3, 2 * b + 1)[lane];
+                for (int u = 0; u < NQ; ++u) {
+                    o[u][2 * b] = mfma(v0, pl[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v1, pl[u], o[u][2 * b + 1]);
+                }
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u) {
-                        o[u][2 * b] = mfma(v0, ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v1, ph[u], o[u][2 * b + 1]);
-                    }
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u) {
-                        o[u][2 * b] = mfma(v0, pl[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v1, pl[u], o[u][2 * b + 1]);
-                    }
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u) {
-                        o[u][2 * b] = mfma(l0, ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(l1, ph[u], o[u][2 * b + 1]);
-                    }
+                for (int u = 0; u < NQ; ++u) {
+                    o[u][2 * b] = mfma(l0, ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(l1, ph[u], o[u][2 * b + 1]);
                 }
             }
             __syncthreads();
@@ -398,7 +417,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
                 if (row0 + 16 * u + i16 >= row1) continue;
-                store_row<NB>(out + out_row[u], hd, g, o[u], 1.0f / l[u]);
+                store_row<NB>(out + out_row[u], hd, g, o[u], 1.0f / (l[u] * kLift));
             }
         }
     }

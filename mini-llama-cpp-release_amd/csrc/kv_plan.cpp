@@ -138,10 +138,23 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
                 whole.push_back(it);
             }
         }
-        // Parts of at most `most` tiles, as even as they come.
+        // Parts of at most `most` tiles, as even as they come: the fewest tiles that do not make more
+        // items than `target`, since those beyond one round of workgroups would take a second one.
         std::vector<KvAttnItem>& list = b.items[kind];
-        const int target = ceil_div(kTargetGroups[kind], s.n_kv_heads);
-        const int most = static_cast<int>(std::max<int64_t>(kLeastTiles, (tiles + target - 1) / target));
+        const int target = std::max(1, kTargetGroups[kind] / s.n_kv_heads);
+        auto items_of = [&](int64_t most) {
+            int64_t n = 0;
+            for (const KvAttnItem& w : whole) n += (w.count + most - 1) / most;
+            return n;
+        };
+        int64_t lo = std::max<int64_t>(kLeastTiles, tiles / target), hi = lo;
+        for (const KvAttnItem& w : whole) hi = std::max<int64_t>(hi, w.count);
+        while (lo < hi && static_cast<int>(whole.size()) < target) {
+            const int64_t mid = (lo + hi) / 2;
+            if (items_of(mid) <= target) hi = mid;
+            else lo = mid + 1;
+        }
+        const int most = static_cast<int>(std::max<int64_t>(1, lo));
         int slot = 0;
         for (const KvAttnItem& w : whole) {
             const int parts = ceil_div(w.count, most);
