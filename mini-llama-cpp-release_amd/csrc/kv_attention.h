@@ -140,12 +140,20 @@ __device__ __forceinline__ h8_t codes8(uint32_t w0, uint32_t w1, _Float16 off) {
 }
 // v = hi + lo, both fp16, for |v| < 65504: 2^-22 of v (or 2^-25) is lost.
 __device__ __forceinline__ void split8(const float* v, h8_t* hi, h8_t* lo) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    h2_t h[4], r[4];
+    // v - hi as a product with 1, one instruction that takes the fp16 operand as it is
+    // (v_fma_mix_f32); a 1 that the compiler knows would make it a conversion and a subtraction.
+    float one = 1.0f;
+    asm("" : "+s"(one));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const _Float16 h = static_cast<_Float16>(v[j]);
-        (*hi)[j] = h;
-        (*lo)[j] = static_cast<_Float16>(v[j] - static_cast<float>(h));
+    for (int j = 0; j < 4; ++j) {
+        h[j] = __builtin_convertvector((f2_t{v[2 * j], v[2 * j + 1]}), h2_t);
+        const f2_t rest{fmaf(-static_cast<float>(h[j].x), one, v[2 * j]), fmaf(-static_cast<float>(h[j].y), one, v[2 * j + 1])};
+        r[j] = __builtin_convertvector(rest, h2_t);
     }
+    *hi = join(h[0], h[1], h[2], h[3]);
+    *lo = join(r[0], r[1], r[2], r[3]);
 }
 // 1 / s for a power of two s from 2^-90 on; 0 for Inf.
 __device__ __forceinline__ float inverse_power(uint32_t s) {
@@ -175,8 +183,9 @@ __device__ __forceinline__ void load_query(const float* q, int hd, int g, float 
     top = max_quarters(top);
     // exponent, kept where 2^(13 - e) and its inverse are normal
     const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 127);
-    const float up = ldexpf(1.0f, 13 - e);
-    *to_t = ldexpf(scale, e - 13);
+    // a negative scale turns the queries; a score's factor is positive, so that -inf stays -inf
+    const float up = ldexpf(scale < 0.0f ? -1.0f : 1.0f, 13 - e);
+    *to_t = fmaxf(ldexpf(fabsf(scale), e - 13), 0x1p-126f);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         sum[b] = 0.0f;

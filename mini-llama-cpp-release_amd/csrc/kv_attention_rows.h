@@ -1,22 +1,26 @@
-// The paged attention for more than eight query rows a KV head: chunks of a prompt,
-// whole prompts (kv_attention.h has the formula and the kernel for few rows).
+// The paged attention for many query rows a KV head: chunks of a prompt, whole prompts
+// (kv_attention.h has the formula and the kernel for few rows).
 //
-// A workgroup takes 4 x 16 NQ rows of one KV head, a wave 16 NQ of them, and walks tiles of 32
-// positions that its waves convert for each other: a tile's keys and values are
-// decoded to f32 once, brought into fp16's range by a power of two per position and
-// split into two fp16 parts (hi + lo, 2^-22 is lost; the decoded product of a code and a
-// binary16 scale has at most 19 bits and is exact), and lie in LDS as the MFMA
-// operands they are.  Then, all in v_mfma_f32_16x16x32_f16, three products a pair:
+// A workgroup of four waves takes 4 x 16 NQ rows of one KV head, a wave 16 NQ of them, and walks
+// tiles of 32 positions that its waves convert for each other: a tile's keys and values are
+// decoded once, and lie in LDS as the MFMA operands they are, split into two fp16 parts
+// (hi + lo; 2^-22 is lost, nothing of a quantized element, which is a code times a binary16
+// scale: at most 19 bits).  Then, all in v_mfma_f32_16x16x32_f16, three products a pair:
 //
 //   S^T = K Q^T      A from LDS, B (queries, relative to the row's largest) in registers;
 //   O^T += V^T P^T   A from LDS, B the weights: a lane's eight scores are its eight weights.
 //
-// The powers of two come back per position: 2^ek into the score, 2^ev into the weight
-// (P_j = p_j 2^ev_j); the running maximum is that of t_j + ev_j, as in the kernel for few
-// rows, so what a row does not see cannot cost it a digit.
+// A position's elements are taken over a power of two where they are far from 1, which comes back
+// in the score (2^ek) and in the weight (P_j = p_j 2^ev_j); the running maximum is that of
+// t_j + ev_j, as in the kernel for few rows, so what a row does not see cannot cost it a digit.
 //
-// The loop is a pipeline over tiles i: compute on i, convert i + 1 into the other LDS buffer,
-// scales of i + 2, loads ahead of both; one barrier a tile.
+// One step a tile and one barrier: products of the last tile's values and this one's keys (96 at
+// head_dim 128), then the conversion of the next tile, the loads ahead and the softmax.  Two
+// workgroups fit a CU.  Bound: LDS and issue.  A wave's step reads 32 KB of operands and issues
+// 1540 cycles of products and about 290 vector instructions; eight waves a CU take 7000 cycles for
+// one step each, and 1900 for the products where only four run them.  Measured and no faster: eight
+// waves that share a conversion; halves of them in turn on the products and the rest; the
+// products' fences left out.
 #pragma once
 
 #include "kv_attention.h"
@@ -33,11 +37,11 @@ template <int QT, int NB>
 struct TileScales {
     static constexpr bool kPacked = QT == 1 || QT == 2;  // decoded in packed fp16
     typename std::conditional<kPacked, _Float16, float>::type scale[2][QT == 3 ? 2 : 1][NB][kKvTile];  // keys, values
-    float key_up[kKvTile];     // 2^ek
-    float value_log[kKvTile];  // ev
-    float value_up[kKvTile];   // 2^ev
-    uint32_t bad[NB];          // positions whose value block is not finite
-    uint32_t flags;            // kBad: any of `bad`; kFar: some power of two is not 1
+    float key_up[kKvTile];      // 2^ek
+    float value_log[kKvTile];   // ev
+    float value_down[kKvTile];  // 2^-ev
+    uint8_t bad[NB][kKvTile];  // whether a position's value block is not finite
+    uint32_t flags[kKvWaves];  // of the wave's part: kBad, some of `bad`; kFar, some power of two is not 1
 };
 constexpr uint32_t kBad = 1, kFar = 2;
 constexpr float kLift = 256.0f;  // operands lie in LDS times this
@@ -48,7 +52,7 @@ constexpr int rows_lds_bytes() {
 }
 
 template <int QT, int NB, int NQ>
-__global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kernel(KvAttention a, int count, const float* __restrict__ q,
+__global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention a, int count, const float* __restrict__ q,
                                                                       float* __restrict__ out) {
     using F = KvForm<QT>;
     using Scales = TileScales<QT, NB>;
@@ -58,6 +62,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
     constexpr int RAW_K = QT == 0 ? 8 : QT == 1 ? 2 : 1, RAW_V = QT == 0 ? 8 : 2;  // words a lane loads for an operand
     constexpr int QUADS = NQ * 2 * NB, STATE = (QUADS * 4 + 2 * NQ) * 64;
     constexpr int ROWS = 16 * NQ;
+    constexpr int PER = NB <= 4 ? 4 : 8, PASSES = 2 * kKvTile * PER / (kThreads);  // threads a position's scales, rounds of them
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     // [buffer][key hi, key lo, value hi, value lo][operand][lane] of 16 bytes, then the scales
     h8_t* const operands = reinterpret_cast<h8_t*>(lds);
@@ -71,6 +76,23 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
     const int page_tiles = a.kv.page_tiles, tile_shift = __builtin_ctz(page_tiles);
     const int total = (count > 0 ? count : uniform(a.lists.counts + kKvCountWide)) * n_kv;
 
+    // What this thread loads of a tile: a task is one operand of keys and one of values, both parts.
+    auto mine = [&](int x) { return FRAGS % kKvWaves == 0 || wave + kKvWaves * (x >> 1) < FRAGS; };
+    uint32_t key_off[TASKS], value_off[TASKS], scale_off[PASSES];
+#pragma unroll
+    for (int k = 0; k < TASKS; ++k) {
+        const int f = wave + kKvWaves * k, h = f / NB, b = f % NB, bv = f >> 1, t = f & 1;
+        key_off[k] = h * 64 * KL + F::at(KL, lane, b * F::kElemBits);
+        value_off[k] = F::half(NB) + F::at(VL, lane, QT < 2 ? (2 * bv + t) * F::kElemBits : 2 * bv * F::kElemBits);
+    }
+#pragma unroll
+    for (int z = 0; z < PASSES; ++z) {
+        const int block = min(static_cast<int>(threadIdx.x % PER), NB - 1), item = (threadIdx.x + z * (kThreads)) / PER;
+        const int key = item % kKvTile;
+        scale_off[z] = (item >= kKvTile ? F::half(NB) : 0) + F::codes(NB) +
+                       (item >= kKvTile ? F::value_scale(NB, key, block) : F::key_scale(NB, key, block)) * F::kScaleBytes;
+    }
+
     for (int w = blockIdx.x; w < total; w += gridDim.x) {
         const int head = w % n_kv;
         const KvAttnItem it = uniform(a.lists.items[1] + w / n_kv);
@@ -82,15 +104,17 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
         h8_t qh[NQ][NB], ql[NQ][NB];
         float to_t[NQ];
         int pos[NQ];
-        size_t out_row[NQ];
+        // This lane's row u of the batch, and where its elements start.
+        auto token_of = [&](int u) { return min(row0 + 16 * u + i16, rows - 1) / a.group; };
+        auto element_of = [&](int u) {
+            const int r = min(row0 + 16 * u + i16, rows - 1);
+            return (static_cast<size_t>(it.token0 + r / a.group) * heads + head * a.group + r % a.group) * hd;
+        };
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
-            const int r = min(row0 + 16 * u + i16, rows - 1);
-            const int token = r / a.group;
-            pos[u] = start + token;
-            out_row[u] = (static_cast<size_t>(it.token0 + token) * heads + head * a.group + r % a.group) * hd;
+            pos[u] = start + token_of(u);
             float v[NB][8], sum[NB];
-            load_query<NB>(q + out_row[u], hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
+            load_query<NB>(q + element_of(u), hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) split8(v[b], &qh[u][b], &ql[u][b]);
         }
@@ -106,100 +130,112 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
             for (int t = 0; t < 2 * NB; ++t) o[u][t] = zero;
         }
 
-        const int end = it.first + it.count;
-        auto tile_of = [&](int i) { return i < it.sinks ? i : i + it.shift; };
-        // Tiles past the end repeat the last one: loads stay in bounds, nothing uses them.
-        auto base_of = [&](int i) -> const uint8_t* {
-            const int t = tile_of(min(i, end - 1));
-            const int page = uniform(&a.lists.pages[it.page0 + (t >> tile_shift)].page);
-            return a.kv.base + ((static_cast<size_t>(page) * n_kv + head) * page_tiles + (t & (page_tiles - 1))) * F::tile(NB);
+        // Tiles counted from the item's first; those past the end repeat the last one: loads stay in
+        // bounds, nothing uses them.
+        auto tile_of = [&](int i) {
+            const int k = it.first + min(i, it.count - 1);
+            return k < it.sinks ? k : k + it.shift;
+        };
+        // (A vector load: one through the scalar cache would make every wait for LDS a wait for all of it.)
+        auto page_of = [&](int i) { return a.lists.pages[it.page0 + (tile_of(i) >> tile_shift)].page; };
+        // (And the address by vector arithmetic: there is no other wave to hide a chain of scalar steps.)
+        const uint8_t* const head_base = a.kv.base + static_cast<size_t>(head) * page_tiles * F::tile(NB);
+        const uint32_t page_bytes = static_cast<uint32_t>(page_tiles) * F::tile(NB);
+        auto address_of = [&](int i, int page) -> const uint8_t* {
+            const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(page) * static_cast<uint64_t>(n_kv)) * page_bytes;
+            return head_base + at + static_cast<uint32_t>((tile_of(i) & (page_tiles - 1)) * F::tile(NB));
         };
 
-        // Loads of a tile: this wave's operands, and (wave 0) lane's scales: keys' by
-        // lanes 0 .. 31, values' by lanes 32 .. 63.
+        // Loads of a tile: this wave's operands, and the scale of one (keys or values, position, block)
+        // a thread.
         uint32_t raw_k[TASKS][RAW_K], raw_v[TASKS][RAW_V];
-        uint32_t raw_s[F::kPlanes][NB];
-        auto load_raw = [&](const uint8_t* tile) {
+        uint32_t raw_s[PASSES][F::kPlanes];
+        auto load_keys = [&](const uint8_t* tile) {
 #pragma unroll
             for (int k = 0; k < TASKS; ++k) {
-                const int f = wave + kKvWaves * k;
-                if (f >= FRAGS) continue;
-                const int h = f / NB, b = f % NB;  // keys: half tile, block
-                const uint8_t* p = tile + h * 64 * KL;
-                const uint8_t* pv = tile + F::half(NB);
-                const int bv = f >> 1, t = f & 1;  // values: block, half of its dimensions
+                if (!mine(2 * k)) continue;
+                const uint8_t* p = tile + key_off[k];
+                if (QT == 0) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {  // the lane's two units
+                        const u4_t k4 = *reinterpret_cast<const u4_t*>(p + x * 1024);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) raw_k[k][(4 * x + i) & (RAW_K - 1)] = k4[i];
+                    }
+                } else if (QT == 1) {
+                    const uint2 k2 = *reinterpret_cast<const uint2*>(p);
+                    raw_k[k][0] = k2.x, raw_k[k][RAW_K - 1] = k2.y;
+                } else {
+                    raw_k[k][0] = *reinterpret_cast<const uint32_t*>(p);
+                }
+            }
+        };
+        auto load_values = [&](const uint8_t* tile) {
+#pragma unroll
+            for (int k = 0; k < TASKS; ++k) {
+                if (!mine(2 * k)) continue;
+                const uint8_t* p = tile + value_off[k];
                 if (QT == 0) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const u4_t k4 = *reinterpret_cast<const u4_t*>(p + F::at(KL, lane, b * 32 + 16 * x));
-                        const u4_t v4 = *reinterpret_cast<const u4_t*>(pv + F::at(VL, lane, bv * 64 + t * 32 + 16 * x));
+                        const u4_t v4 = *reinterpret_cast<const u4_t*>(p + x * 1024);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) raw_k[k][4 * x + i] = k4[i], raw_v[k][4 * x + i] = v4[i];
+                        for (int i = 0; i < 4; ++i) raw_v[k][(4 * x + i) & (RAW_V - 1)] = v4[i];
                     }
                 } else {
-                    if (QT == 1) {
-                        const uint2 k2 = *reinterpret_cast<const uint2*>(p + F::at(KL, lane, b * 8));
-                        raw_k[k][0] = k2.x, raw_k[k][RAW_K - 1] = k2.y;
-                    } else {
-                        raw_k[k][0] = *reinterpret_cast<const uint32_t*>(p + F::at(KL, lane, b * 4));
-                    }
-                    const uint2 v2 = *reinterpret_cast<const uint2*>(pv + F::at(VL, lane, QT == 1 ? bv * 16 + t * 8 : bv * 8));
+                    const uint2 v2 = *reinterpret_cast<const uint2*>(p);
                     raw_v[k][0] = v2.x, raw_v[k][1] = v2.y;
                 }
             }
         };
-        const int key = lane & 31;
         auto load_scales = [&](const uint8_t* tile) {
-            if (wave != 0) return;
-            const uint8_t* p = tile + (lane >= 32 ? F::half(NB) : 0) + F::codes(NB);
 #pragma unroll
-            for (int x = 0; x < F::kPlanes; ++x)
+            for (int z = 0; z < PASSES; ++z)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const int at = lane >= 32 ? F::value_scale(NB, key, b) : F::key_scale(NB, key, b);
-                    raw_s[x][b] = QT == 0 ? reinterpret_cast<const uint32_t*>(p)[at]
-                                          : reinterpret_cast<const uint16_t*>(p + x * F::plane(NB))[at];
+                for (int x = 0; x < F::kPlanes; ++x) {
+                    const uint8_t* p = tile + scale_off[z] + x * F::plane(NB);
+                    raw_s[z][x] = QT == 0 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
                 }
         };
         // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position: 1 where the
         // position's largest element is from 2^-10 to 2^7 (the parts then lose what they do at 1,
         // 2^-22, and none reaches 2^15), else what brings it to [1, 2).
         auto make_scales = [&](Scales* s) {
-            if (wave != 0) return;
-            float d[NB], add[NB];
-            float top = 0.0f;
-            bool bad[NB];
+            using T = typename std::remove_reference<decltype(s->scale[0][0][0][0])>::type;
+            uint32_t flags = 0;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                d[b] = QT == 0 ? bits<float>(raw_s[0][b]) : half_value(static_cast<uint16_t>(raw_s[0][b]));
-                add[b] = QT == 3 ? half_value(static_cast<uint16_t>(raw_s[F::kPlanes - 1][b])) : 0.0f;
-                bad[b] = !(fabsf(d[b]) < INFINITY) || !(fabsf(add[b]) < INFINITY);
-                const float most = QT == 0 ? d[b] : QT == 3 ? fmaf(16.0f, d[b], fabsf(add[b])) : (QT == 1 ? 128.0f : 8.0f) * d[b];
-                if (!bad[b]) top = fmaxf(top, most);
+            for (int z = 0; z < PASSES; ++z) {
+                const int block = threadIdx.x % PER, item = (threadIdx.x + z * (kThreads)) / PER;
+                const bool values = (wave * 64 + z * (kThreads)) / PER >= kKvTile;  // a wave has one or the other
+                const int key = item % kKvTile;
+                const float d = QT == 0 ? bits<float>(raw_s[z][0]) : half_value(static_cast<uint16_t>(raw_s[z][0]));
+                const float add = QT == 3 ? half_value(static_cast<uint16_t>(raw_s[z][F::kPlanes - 1])) : 0.0f;
+                const bool bad = !(fabsf(d) < INFINITY) || !(fabsf(add) < INFINITY);
+                float top = QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
+                top = bad ? 0.0f : top;
+                top = quad_max(top);  // over the position's blocks (lanes past the last repeat it)
+                if (PER == 8) top = fmaxf(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0x141, 0xf, 0xf, true)));
+                const bool near = top == 0.0f || (top >= 0x1p-10f && top < 0x1p7f);
+                float lift = kLift;
+                int e = 0;
+                if (!__all(near && !bad)) {
+                    e = near ? 0 : max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -90);
+                    lift = ldexpf(kLift, -e);
+                    flags |= kFar | (values && __any(bad) ? kBad : 0u);
+                }
+                if (block == 0) {
+                    (values ? s->value_down : s->key_up)[key] = ldexpf(1.0f, values ? -e : e);
+                    if (values) s->value_log[key] = static_cast<float>(e);
+                }
+                if (block < NB) {
+                    // keys: NaN through to the score; values: zero here, NaN for the rows that see it (`bad`)
+                    const float nothing = values ? 0.0f : NAN;
+                    if (values) s->bad[block][key] = bad;
+                    s->scale[values][0][block][key] = static_cast<T>(bad ? nothing : QT == 0 ? lift : d * lift);
+                    if (QT == 3) s->scale[values][QT == 3 ? 1 : 0][block][key] = static_cast<T>(bad ? nothing : add * lift);
+                }
             }
-            int e = static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-            e = top == 0.0f || (e >= -10 && e < 7) ? 0 : max(e, -90);
-            const float down = ldexpf(kLift, -e);
-            uint32_t any = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                // keys: NaN through to the score; values: zero here, NaN for the rows that see it (`bad`)
-                const float nothing = lane >= 32 ? 0.0f : NAN;
-                using T = typename std::remove_reference<decltype(s->scale[0][0][0][0])>::type;
-                s->scale[lane >> 5][0][b][key] = static_cast<T>(bad[b] ? nothing : QT == 0 ? down : d[b] * down);
-                if (QT == 3) s->scale[lane >> 5][QT == 3 ? 1 : 0][b][key] = static_cast<T>(bad[b] ? nothing : add[b] * down);
-                const uint32_t mask = static_cast<uint32_t>(__ballot(bad[b]) >> 32);
-                any |= mask;
-                if (lane == 0) s->bad[b] = mask;
-            }
-            if (lane < 32) {
-                s->key_up[key] = ldexpf(1.0f, e);
-            } else {
-                s->value_log[key] = static_cast<float>(e);
-                s->value_up[key] = ldexpf(1.0f, e);
-            }
-            const bool far = __any(e != 0);
-            if (lane == 0) s->flags = (any != 0 ? kBad : 0u) | (far ? kFar : 0u);
+            if (lane == 0) s->flags[wave] = flags;
         };
         // Eight codes as fp16 (minus the stored offset): keys, values (`t`: which nibbles).
         auto codes_of = [&](const uint32_t* raw, bool values, int t) -> h8_t {
@@ -208,189 +244,278 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
             if (values) return codes8((raw[0] >> (4 * t)) & 0x0f0f0f0fu, (raw[1] >> (4 * t)) & 0x0f0f0f0fu, off);
             return codes8(raw[0] & 0x0f0f0f0fu, (raw[0] >> 4) & 0x0f0f0f0fu, off);
         };
-        auto convert = [&](int buffer, const Scales* s) {
-#pragma unroll
-            for (int k = 0; k < TASKS; ++k) {
-                const int f = wave + kKvWaves * k;
-                if (FRAGS % kKvWaves != 0 && f >= FRAGS) continue;
-                const int h = f / NB, b = f % NB, bv = f >> 1, t = f & 1;
-                h8_t hi, lo;
+        // A tile's conversion in SLICES steps, two an operand pair (task): keys, values.  `begin` reads
+        // a step's scales, `finish` decodes, splits and stores.
+        constexpr int SLICES = 2 * TASKS;
+        typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+        struct SliceScales {
+            _Float16 d16;
+            h4_t v16[2];
+            float d, add;
+            f4_t v[2], vadd[2];
+        };
+        auto begin = [&](int x, const Scales* s, SliceScales& c) {
+            if (!mine(x)) return;
+            const int f = wave + kKvWaves * (x >> 1);
+            const int h = f / NB, b = f % NB, bv = f >> 1;
+            if (x % 2 == 0) {
                 if constexpr (Scales::kPacked) {
-                    // code times scale: at most 19 bits, so hi and what is left of it are exact
-                    const _Float16 d = s->scale[0][0][b][16 * h + i16];
-                    const h8_t d8{d, d, d, d, d, d, d, d};
-                    h8_t c = codes_of(raw_k[k], false, 0);
-                    hi = c * d8;
-                    lo = __builtin_elementwise_fma(c, d8, -hi);
-                    operand(buffer, 0, f)[lane] = hi;
-                    operand(buffer, 1, f)[lane] = lo;
-                    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-                    const h4_t x = *reinterpret_cast<const h4_t*>(s->scale[1][0][bv] + 4 * g);
-                    const h4_t y = *reinterpret_cast<const h4_t*>(s->scale[1][0][bv] + 16 + 4 * g);
-                    const h8_t dv = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-                    c = codes_of(raw_v[k], true, t);
-                    hi = c * dv;
-                    lo = __builtin_elementwise_fma(c, dv, -hi);
+                    c.d16 = s->scale[0][0][b][16 * h + i16];
                 } else {
-                    float x[8];
-                    const float d = s->scale[0][0][b][16 * h + i16];
-                    const float add = QT == 3 ? s->scale[0][QT == 3 ? 1 : 0][b][16 * h + i16] : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        x[j] = QT == 0 ? bits<float>(raw_k[k][j & (RAW_K - 1)]) * d
-                                       : fmaf(static_cast<float>((raw_k[k][0] >> (8 * (j & 3) + 4 * (j >> 2))) & 0xfu), d, add);
-                    }
-                    split8(x, &hi, &lo);
-                    operand(buffer, 0, f)[lane] = hi;
-                    operand(buffer, 1, f)[lane] = lo;
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const f4_t d4 = *reinterpret_cast<const f4_t*>(s->scale[1][0][bv] + 16 * y + 4 * g);
-                        const f4_t a4 = *reinterpret_cast<const f4_t*>(s->scale[1][QT == 3 ? 1 : 0][bv] + 16 * y + 4 * g);
-                        const uint32_t nibbles = (raw_v[k][y] >> (4 * t)) & 0x0f0f0f0fu;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[4 * y + i] = QT == 0 ? mul_or_zero(bits<float>(raw_v[k][(4 * y + i) & (RAW_V - 1)]), d4[i])
-                                                   : fmaf(static_cast<float>((nibbles >> (8 * i)) & 0xffu), d4[i], a4[i]);
-                        }
-                    }
-                    split8(x, &hi, &lo);
+                    c.d = s->scale[0][0][b][16 * h + i16];
+                    if (QT == 3) c.add = s->scale[0][QT == 3 ? 1 : 0][b][16 * h + i16];
                 }
-                operand(buffer, 2, f)[lane] = hi;
-                operand(buffer, 3, f)[lane] = lo;
+            } else {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    if constexpr (Scales::kPacked) {
+                        c.v16[y] = *reinterpret_cast<const h4_t*>(s->scale[1][0][bv] + 16 * y + 4 * g);
+                    } else {
+                        c.v[y] = *reinterpret_cast<const f4_t*>(s->scale[1][0][bv] + 16 * y + 4 * g);
+                        if (QT == 3) c.vadd[y] = *reinterpret_cast<const f4_t*>(s->scale[1][QT == 3 ? 1 : 0][bv] + 16 * y + 4 * g);
+                    }
+                }
             }
         };
-
-        // Fill the pipeline: tile `first` converted, `first + 1` loaded, scales of both.
-        const uint8_t* tile0 = base_of(it.first);
-        const uint8_t* tile1 = base_of(it.first + 1);
-        __syncthreads();  // the last item's readers are done
-        load_scales(tile0);
-        load_raw(tile0);
-        make_scales(scales + 0);
-        load_scales(tile1);
-        make_scales(scales + 1);
-        __syncthreads();
-        convert(0, scales + 0);
-        load_raw(tile1);
-        load_scales(base_of(it.first + 2));
-        __syncthreads();
-
-        int slot = 0;  // of tile i's scales
-        for (int i = it.first; i < end; ++i) {
-            const int buffer = (i - it.first) & 1;
-            const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
-            const Scales* const s = scales + slot;
-
-            f4_t sc[NQ][2];
+        auto finish = [&](int x, int buffer, const SliceScales& c) {
+            if (!mine(x)) return;
+            const int k = x >> 1, f = wave + kKvWaves * k, t = f & 1;
+            const bool values = x % 2 != 0;
+            h8_t hi, lo;
+            if constexpr (Scales::kPacked) {
+                // code times scale: at most 19 bits, so hi and what is left of it are exact
+                const h8_t d = values ? __builtin_shufflevector(c.v16[0], c.v16[1], 0, 1, 2, 3, 4, 5, 6, 7)
+                                      : h8_t{c.d16, c.d16, c.d16, c.d16, c.d16, c.d16, c.d16, c.d16};
+                const h8_t code = values ? codes_of(raw_v[k], true, t) : codes_of(raw_k[k], false, 0);
+                hi = code * d;
+                lo = __builtin_elementwise_fma(code, d, -hi);
+            } else {
+                float y[8];
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) sc[u][0] = sc[u][1] = zero;
+                for (int j = 0; j < 8; ++j) {
+                    if (QT == 0) {
+                        y[j] = values ? mul_or_zero(bits<float>(raw_v[k][j & (RAW_V - 1)]), c.v[j >> 2][j & 3])
+                                      : bits<float>(raw_k[k][j & (RAW_K - 1)]) * c.d;
+                    } else {
+                        const uint32_t nibbles = values ? raw_v[k][(j >> 2) & (RAW_V - 1)] >> (4 * t) : raw_k[k][0] >> (4 * (j >> 2));
+                        const float code = static_cast<float>(((nibbles & 0x0f0f0f0fu) >> (8 * (j & 3))) & 0xffu);
+                        y[j] = values ? fmaf(code, c.v[j >> 2][j & 3], c.vadd[j >> 2][j & 3]) : fmaf(code, c.d, c.add);
+                    }
+                }
+                split8(y, &hi, &lo);
+            }
+            operand(buffer, values ? 2 : 0, f)[lane] = hi;
+            operand(buffer, values ? 3 : 1, f)[lane] = lo;
+        };
+
+        auto barrier = [] {
+            __builtin_amdgcn_sched_barrier(0);  // a step's vector work stays out of the other's
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
+        // Converts the keys of tile i + 1 and the values of tile i, and loads those of the next.
+        auto convert_begin = [&](int i, SliceScales* c) {
+#pragma unroll
+            for (int x = 0; x < SLICES; ++x) begin(x, scales + slot_of(x % 2 == 0 ? i + 1 : i), c[x]);
+        };
+        auto convert_finish = [&](int i, const SliceScales* c, int page1, int page2) {
+#pragma unroll
+            for (int x = 0; x < SLICES; ++x) finish(x, x % 2 == 0 ? (i + 1) & 1 : i & 1, c[x]);
+            load_keys(address_of(i + 2, page2));
+            load_values(address_of(i + 1, page1));
+        };
+
+        // Fill the pipeline: scales of tiles 0 and 1 (counted from the item's first), keys of 0.
+        __syncthreads();  // the last item's readers are done
+        load_scales(address_of(0, page_of(0)));
+        load_keys(address_of(0, page_of(0)));
+        // what the first step takes for the values of a tile before the first
+        for (int f = wave; f < 2 * FRAGS; f += kKvWaves) operand(1, 2 + f / FRAGS, f % FRAGS)[lane] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        make_scales(scales + 0);
+        load_scales(address_of(1, page_of(1)));
+        make_scales(scales + 1);
+        load_scales(address_of(2, page_of(2)));
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < SLICES; x += 2) {
+            SliceScales c;
+            begin(x, scales + 0, c);
+            finish(x, 0, c);
+        }
+        load_keys(address_of(1, page_of(1)));
+        load_values(address_of(0, page_of(0)));
+        __syncthreads();
+
+        f4_t sc[NQ][2];
+        h8_t ph[NQ], pl[NQ];
+        uint32_t spoilt = 0;  // this lane's part: bit u NB + b
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) ph[u] = pl[u] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        // The products of a step: NB blocks of values of tile i - 1 (in the first step zeros times zeros) and, if
+        // `keys`, NB of keys of tile i; a block's operands are read a block ahead (the fences keep it so).
+        auto products = [&](bool keys, int i) {
+            h8_t frag[2][4];
+            auto read = [&](int x) {  // x: 0 .. NB - 1 values, NB .. 2 NB - 1 keys
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    frag[x & 1][y] = x < NB ? operand((i + 1) & 1, 2 + (y >> 1), 2 * x + (y & 1))[lane]
+                                            : operand(i & 1, y >> 1, (y & 1) * NB + x - NB)[lane];
+                }
+            };
+            __builtin_amdgcn_s_setprio(1);
+            read(0);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const h8_t k0 = operand(buffer, 0, b)[lane], k1 = operand(buffer, 0, NB + b)[lane];
-                const h8_t l0 = operand(buffer, 1, b)[lane], l1 = operand(buffer, 1, NB + b)[lane];
+                if (b + 1 < NB || keys) read(b + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                const h8_t* v = frag[b & 1];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k0, qh[u][b], sc[u][0]), sc[u][1] = mfma(k1, qh[u][b], sc[u][1]);
+                for (int u = 0; u < NQ; ++u) {
+                    o[u][2 * b] = mfma(v[0], ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v[1], ph[u], o[u][2 * b + 1]);
+                }
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k0, ql[u][b], sc[u][0]), sc[u][1] = mfma(k1, ql[u][b], sc[u][1]);
+                for (int u = 0; u < NQ; ++u) {
+                    o[u][2 * b] = mfma(v[0], pl[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v[1], pl[u], o[u][2 * b + 1]);
+                }
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(l0, qh[u][b], sc[u][0]), sc[u][1] = mfma(l1, qh[u][b], sc[u][1]);
+                for (int u = 0; u < NQ; ++u) {
+                    o[u][2 * b] = mfma(v[2], ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v[3], ph[u], o[u][2 * b + 1]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // Ahead: convert i + 1, scales of i + 2, loads of i + 2 (raw) and i + 3 (scales).
-            convert(buffer ^ 1, scales + slot1);
-            make_scales(scales + slot2);
-            load_raw(base_of(i + 2));
-            load_scales(base_of(i + 3));
-
+            if (keys) {
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) sc[u][0] = sc[u][1] = zero;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (b + 1 < NB) read(NB + b + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const h8_t* k = frag[(NB + b) & 1];
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k[0], qh[u][b], sc[u][0]), sc[u][1] = mfma(k[1], qh[u][b], sc[u][1]);
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k[0], ql[u][b], sc[u][0]), sc[u][1] = mfma(k[1], ql[u][b], sc[u][1]);
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) sc[u][0] = mfma(k[2], qh[u][b], sc[u][0]), sc[u][1] = mfma(k[3], qh[u][b], sc[u][1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            __builtin_amdgcn_s_setprio(0);
+        };
+        // The weights of tile i's scores.
+        auto softmax = [&](int i) {
+            const Scales* const s = scales + slot_of(i);
+            float x_[NQ][8];
+#pragma unroll
+            for (int u = 0; u < NQ; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x_[u][j] = sc[u][j >> 2][j & 3];
             const int first = tile_of(i) * kKvTile;
             const bool full = first + kKvTile - 1 <= pos_lo &&
                               (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
-            const uint32_t flags = __builtin_amdgcn_readfirstlane(s->flags);
-            h8_t ph[NQ], pl[NQ];
+            const u4_t all = *reinterpret_cast<const u4_t*>(s->flags);
+            const uint32_t flags = __builtin_amdgcn_readfirstlane(all.x | all.y | all.z | all.w);
+            if (!full || (flags & kFar) != 0) {
+                // (a value's power of two goes into the score here: P_j = p_j 2^ev_j; its sum is set right below)
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                float t[8], top;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = sc[u][j >> 2][j & 3] * to_t[u];
-                if (flags & kFar) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) t[j] *= s->key_up[(j >> 2) * 16 + 4 * g + (j & 3)];
-                }
-                if (!full) {
+                for (int u = 0; u < NQ; ++u) {
+                    const float inv = 1.0f / to_t[u];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                        const int at = (j >> 2) * 16 + 4 * g + (j & 3), k = first + at;
                         const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
-                        t[j] = seen ? t[j] : -INFINITY;
+                        float& x = x_[u][j];
+                        x = seen ? fmaf(s->value_log[at], inv, x * s->key_up[at]) : -INFINITY;
                     }
                 }
-                if (flags & kFar) {
-                    top = -INFINITY;
+            }
+            // The maximum moves when it is passed by kSlack.
+            float top[NQ];
+            bool passed = false;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) top = fmaxf(top, t[j] + s->value_log[(j >> 2) * 16 + 4 * g + (j & 3)]);
-                } else {
-                    top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
-                }
-                top = max_quarters(top);
-                if (__any(top > m[u] + kSlack)) {
-                    const float to = top > m[u] + kSlack ? top : m[u];
+            for (int u = 0; u < NQ; ++u) {
+                const float* x = x_[u];
+                top[u] = max_quarters(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])))) * to_t[u];
+                passed = passed || top[u] > m[u] + kSlack;
+            }
+            if (__any(passed)) {
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) {
+                    const float to = top[u] > m[u] + kSlack ? top[u] : m[u];
                     const float c = __builtin_amdgcn_exp2f(m[u] - to);
                     m[u] = to;
                     l[u] *= c;
 #pragma unroll
                     for (int x = 0; x < 2 * NB; ++x) o[u][x] *= c;
                 }
-                // P_j = p_j 2^ev_j up to 2^(6 + 8)
+            }
+            if ((flags & kBad) != 0) {
+                // rows that see a value block that is not finite: NaN in its dimensions, in the end
+#pragma unroll 1
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t bit = s->bad[b][(j >> 2) * 16 + 4 * g + (j & 3)];  // 0 or 1
+#pragma unroll
+                        for (int u = 0; u < NQ; ++u) spoilt |= (x_[u][j] != -INFINITY ? bit : 0u) << (u * NB + b);
+                    }
+            }
+
+            // P_j, up to 2^(6 + 8)
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
                 const float frame = m[u] - 8.0f;
-                float p[8];
+                float p[8], sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    p[j] = __builtin_amdgcn_exp2f(t[j] - frame);
-                    l[u] += p[j];
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(x_[u][j], to_t[u], -frame));
+                    sum += p[j];
                 }
-                if (flags & kBad) {
+                if ((flags & kFar) != 0) {
+                    sum = 0.0f;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint32_t mask = s->bad[b];
-                        bool hit = false;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            hit = hit || (((mask >> ((j >> 2) * 16 + 4 * g + (j & 3))) & 1u) != 0 && !(p[j] == 0.0f));
-                        }
-                        const float add = sum_quarters(hit ? NAN : 0.0f);
-                        o[u][2 * b] += add;
-                        o[u][2 * b + 1] += add;
-                    }
+                    for (int j = 0; j < 8; ++j) sum = fmaf(p[j], s->value_down[(j >> 2) * 16 + 4 * g + (j & 3)], sum);
                 }
-                if (flags & kFar) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) p[j] *= s->value_up[(j >> 2) * 16 + 4 * g + (j & 3)];
-                }
+                l[u] += sum;
                 split8(p, &ph[u], &pl[u]);
             }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const h8_t v0 = operand(buffer, 2, 2 * b)[lane], v1 = operand(buffer, 2, 2 * b + 1)[lane];
-                const h8_t l0 = operand(buffer, 3, 2 * b)[lane], l1 = operand(buffer, 3, 2 * b + 1)[lane];
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    o[u][2 * b] = mfma(v0, ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v1, ph[u], o[u][2 * b + 1]);
-                }
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    o[u][2 * b] = mfma(v0, pl[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(v1, pl[u], o[u][2 * b + 1]);
-                }
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    o[u][2 * b] = mfma(l0, ph[u], o[u][2 * b]), o[u][2 * b + 1] = mfma(l1, ph[u], o[u][2 * b + 1]);
-                }
-            }
-            __syncthreads();
-            slot = slot1;
+        };
+
+        const int n = it.count;
+        int page1 = page_of(1), page2 = page_of(2), page3 = page_of(3);
+        for (int i = 0; i < n; ++i) {
+            products(true, i);
+            __builtin_amdgcn_sched_barrier(0);
+            // All that a tile loads is used a tile later: its own waits are for loads long done.
+            // (The pages are opaque until then, or their products would be computed as they arrive.)
+            asm volatile("" : "+v"(page1), "+v"(page2), "+v"(page3));
+            SliceScales c[SLICES];
+            convert_begin(i, c);
+            make_scales(scales + slot_of(i + 2));
+            convert_finish(i, c, page1, page2);
+            load_scales(address_of(i + 3, page3));
+            page1 = page2;
+            page2 = page3;
+            page3 = page_of(i + 4);
+            __builtin_amdgcn_sched_barrier(0);
+            softmax(i);
+            barrier();
         }
+        products(false, n);
 
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) l[u] = sum_quarters(l[u]);
+        for (int u = 0; u < NQ; ++u) {
+            l[u] = sum_quarters(l[u]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
+                o[u][2 * b] += add;
+                o[u][2 * b + 1] += add;
+            }
+        }
 
         if (it.nsplit > 1) {
             // Every wave's state to memory; the workgroup that arrives last merges the parts, each wave its rows.
@@ -417,7 +542,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void attention_rows_kern
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
                 if (row0 + 16 * u + i16 >= row1) continue;
-                store_row<NB>(out + out_row[u], hd, g, o[u], 1.0f / (l[u] * kLift));
+                store_row<NB>(out + element_of(u), hd, g, o[u], 1.0f / (l[u] * kLift));
             }
         }
     }

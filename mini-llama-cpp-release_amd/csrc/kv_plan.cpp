@@ -32,7 +32,8 @@ Seen seen_tiles(const KvPlanShape& s, int lo, int hi) {
 
 KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     const int64_t rows = static_cast<int64_t>(s.max_tokens) * s.group;
-    const int whole[2] = {s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
+    const int64_t narrow = std::min(rows / kKvNarrowRows, static_cast<int64_t>(s.max_seqs) * (kKvNarrowMost / kKvNarrowRows - 1));
+    const int whole[2] = {static_cast<int>(narrow) + s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
     KvPlanLimits l;
     for (int kind = 0; kind < 2; ++kind) {
         // Only an item of n parts adds to the list, n - 1 items, and all parts take slots: at
@@ -105,7 +106,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
         }
         if (n > 0) {
             const int rows = n * s.group;
-            const int kind = rows <= kKvNarrowRows ? 0 : 1;
+            const int kind = rows <= kKvNarrowMost ? 0 : 1;
             base[kind].push_back(KvAttnItem{token0, n, len, page0, 0, 0, 0, 0, 0, 0, 1, 0});
         }
         token0 += n;
@@ -147,7 +148,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
             for (const KvAttnItem& w : whole) n += (w.count + most - 1) / most;
             return n;
         };
-        int64_t lo = std::max<int64_t>(kLeastTiles, tiles / target), hi = lo;
+        int64_t lo = std::max<int64_t>(kLeastTiles, (tiles + target - 1) / target), hi = lo;
         for (const KvAttnItem& w : whole) hi = std::max<int64_t>(hi, w.count);
         while (lo < hi && static_cast<int>(whole.size()) < target) {
             const int64_t mid = (lo + hi) / 2;

@@ -10,7 +10,8 @@
 namespace mlq {
 
 constexpr int kKvTile = 32;       // positions per tile: the depth of one MFMA over keys
-constexpr int kKvNarrowRows = 8;  // query rows of the kernel for few rows (fp16 hi and lo parts side by side)
+constexpr int kKvNarrowRows = 8;  // query rows of a workgroup of the kernel for few rows (fp16 hi and lo parts side by side)
+constexpr int kKvNarrowMost = 64;  // rows of a sequence up to which it runs them
 constexpr int kKvWaves = 4;       // waves of an attention workgroup
 
 // New tokens in one tile: positions pos .. pos + n - 1 at slots slot .. of tile

@@ -39,7 +39,7 @@ void one(std::mt19937& rng, int trial) {
     s.page_size = pick(rng, {32, 64, 256, 4096});
     s.n_kv_heads = pick(rng, {1, 2, 8, 32});
     s.group = pick(rng, {1, 2, 7, 8, 16});
-    s.wide_rows = pick(rng, {64, 128});
+    s.wide_rows = pick(rng, {128, 256});
     s.window = pick(rng, {0, 0, 1, 20, 32, 33, 100, 1000});
     s.sinks = s.window ? pick(rng, {0, 1, 4, 32, 40, 3000}) : 0;
     const int n_seqs = rng() % 6;
@@ -141,7 +141,7 @@ void refused(const KvPlanShape& s, std::vector<int> fresh, std::vector<int> len,
 int main() {
     std::mt19937 rng(7);
     for (int t = 0; t < 200; ++t) one(rng, t);
-    const KvPlanShape s{64, 10, 2, 4, 128, 0, 0, 3, 100, 6};
+    const KvPlanShape s{64, 10, 2, 4, 256, 0, 0, 3, 100, 6};
     refused(s, {1, 1, 1, 1}, {1, 1, 1, 1}, {0, 1, 2, 3}, "4 sequences, the plan holds 3");
     refused(s, {-1}, {4}, {0}, "negative token count");
     refused(s, {5}, {4}, {0}, "5 new tokens in a length of 4");
