@@ -366,7 +366,7 @@ int mlq_hip_kv_write(mlq_kv_plan_t p, int layer, const float* k, const float* v,
         p->rope.on = theta > 0.0f;
         p->rope.neox = neox != 0;
         const hipError_t e = mlq::launch_kv_write(p->view(layer), p->device_lists(), recorded ? 0 : p->counts[mlq::kKvCountFresh],
-                                                  k, v, q, q_out, p->n_heads, p->rope, s);
+                                                  static_cast<int>(rows), k, v, q, q_out, p->n_heads, p->rope, s);
         return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
     });
 }

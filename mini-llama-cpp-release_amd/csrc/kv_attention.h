@@ -218,7 +218,6 @@ __device__ __forceinline__ void leave_state(__amdgpu_buffer_rsrc_t rs, int lane,
         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[u]), rs,
                                               (QUADS * 256 + (2 * u + 1) * 64 + lane) * 4, 0, kCoherent);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
 }
 // Takes another state of the same rows into one's own.
 __device__ __forceinline__ void fold(float& m, float& l, float m1, float l1, float* w0, float* w1) {
@@ -266,8 +265,8 @@ __device__ __forceinline__ void store_row(float* out, int hd, int g, const f4_t*
 }
 
 template <int QT, int NB>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(KvAttention a, int count, const float* __restrict__ q,
-                                                                 float* __restrict__ out) {
+__global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) void attention_kernel(
+    KvAttention a, int count, const float* __restrict__ q, float* __restrict__ out) {
     using F = KvForm<QT>;
     constexpr int SB = F::kScaleBytes;
     constexpr int KL = F::key_lane(NB), VL = F::value_lane(NB);
@@ -536,8 +535,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(KvAttention a, i
             auto rsrc_of = [&](int split) {
                 return state_rsrc(a.partial, static_cast<size_t>(it.slot + split) * n_kv + head, STATE);
             };
+            const bool live = !low && it.row0 + i16 < row1;  // the lane's column is a row's
             if (wave == 0) {
-                leave_state<1, NB>(rsrc_of(it.split), lane, o, &m, &l);
+                if (live) leave_state<1, NB>(rsrc_of(it.split), lane, o, &m, &l);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
                 if (lane == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);
             }
             __syncthreads();
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(KvAttention a, i
             l = 0.0f;
 #pragma unroll
             for (int x = 0; x < 2 * NB; ++x) o[0][x] = zero;
-            for (int part = wave; part < it.nsplit; part += kKvWaves) take_state<1, NB>(rsrc_of(part), lane, o, &m, &l);
+            for (int part = wave; live && part < it.nsplit; part += kKvWaves) take_state<1, NB>(rsrc_of(part), lane, o, &m, &l);
             merge_waves();
         }
 

@@ -523,6 +523,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 return state_rsrc(a.partial, (static_cast<size_t>(it.slot + split) * n_kv + head) * kKvWaves + wave, STATE);
             };
             leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
             __syncthreads();
             if (threadIdx.x == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);
             __syncthreads();

@@ -7,7 +7,6 @@
 // once, angles reduced to a fraction of a turn first, so a far position's angle
 // costs no digits and a code next to a border falls as the definition says.
 
-#include "kv_device.h"
 #include "kv_layout.h"
 #include "quant_device.h"
 
@@ -16,7 +15,8 @@
 namespace mlq {
 namespace {
 
-constexpr int kKvThreads = 256;
+constexpr int kWriteThreads = 512;  // at the most
+constexpr int kReadThreads = 256;
 constexpr int kRecordedGroups = 1024;  // workgroups of a recorded launch: four a CU
 
 __global__ __launch_bounds__(256) void kv_upload_kernel(KvParts p) {
@@ -189,8 +189,7 @@ __device__ __forceinline__ void load8_rotated(const float* x, int e, int half, i
     }
 }
 
-// Heads first .. last - 1 of the item's tokens: KV heads (keys and values into
-// `tile(head)`), then query heads.
+// One KV head of an item's tokens: keys (rotated) and values, quantized, to `out`.
 template <int QT, typename Tile>
 __device__ __forceinline__ void write_kv_head(const KvTileItem& it, int head, const Tile& out, const KvView& kv,
                                               const float* __restrict__ k, const float* __restrict__ v, int rope, int neox,
@@ -199,7 +198,7 @@ __device__ __forceinline__ void write_kv_head(const KvTileItem& it, int head, co
     const int per = 4 * nb;  // tasks of a row: (block, eight elements), a quad of lanes a block
     const int tasks = it.n * per;
     // every quad is whole: `per` and the workgroup are multiples of four
-    for (int t = threadIdx.x; t < tasks; t += kKvThreads) {
+    for (int t = threadIdx.x; t < tasks; t += blockDim.x) {
         const int s = t / per, b = t % per >> 2, g = t & 3;
         const int e = 32 * b + 8 * g;
         const bool here = e < hd;
@@ -235,7 +234,7 @@ __device__ __forceinline__ void write_kv_head(const KvTileItem& it, int head, co
 // stored where they belong, values byte by byte, so that slots of other
 // sequences or earlier tokens in the same words are never rewritten.
 template <int QT>
-__global__ __launch_bounds__(kKvThreads) void kv_write_kernel(KvView kv, const KvTileItem* __restrict__ items,
+__global__ __launch_bounds__(kWriteThreads) void kv_write_kernel(KvView kv, const KvTileItem* __restrict__ items,
                                                               const int* __restrict__ counts, int count,
                                                               const float* __restrict__ k, const float* __restrict__ v,
                                                               const float* q, float* q_out, int n_heads, int per_group,
@@ -253,7 +252,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_write_kernel(KvView kv, const K
         const int h0 = w % chunks * per_group, h1 = min(heads, h0 + per_group);
         if (rope.on) {
             __syncthreads();  // the last item's readers are done
-            for (int i = threadIdx.x; i < it.n * half; i += kKvThreads) {
+            for (int i = threadIdx.x; i < it.n * half; i += blockDim.x) {
                 const double a = static_cast<double>(it.pos + i / half) * rope.turns[i % half];
                 double2 t;
                 sincospi(2.0 * (a - rint(a)), &t.y, &t.x);
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_write_kernel(KvView kv, const K
             if (it.n == kKvTile) {
                 write_kv_head<QT>(it, h, TileOut<QT>{image, kv.nb}, kv, k, v, rope.on, rope.neox, turn);
                 __syncthreads();
-                for (int i = threadIdx.x * 16; i < tile_bytes; i += kKvThreads * 16) {
+                for (int i = threadIdx.x * 16; i < tile_bytes; i += blockDim.x * 16) {
                     *reinterpret_cast<uint4*>(tile + i) = *reinterpret_cast<const uint4*>(image + i);
                 }
                 __syncthreads();
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_write_kernel(KvView kv, const K
         // Query heads: a thread rotates four pairs, both members, so q_out may be q.
         const int q0 = max(h0, kv.n_kv) - kv.n_kv, nq = h1 - kv.n_kv - q0;
         const int per = hd / 8;
-        for (int t = threadIdx.x; t < nq * it.n * per; t += kKvThreads) {
+        for (int t = threadIdx.x; t < nq * it.n * per; t += blockDim.x) {
             const int r = t % per * 4, s = t / per % it.n, h = q0 + t / per / it.n;
             const size_t row = (static_cast<size_t>(it.row + s) * n_heads + h) * hd;
             const int e0 = rope.neox ? r : 2 * r, e1 = rope.neox ? r + half : 2 * r + 4;
@@ -303,10 +302,18 @@ __global__ __launch_bounds__(kKvThreads) void kv_write_kernel(KvView kv, const K
     }
 }
 
-// Bound: memory (cache bytes in, 4-byte elements out).  A workgroup brings one tile
-// to LDS with 16-byte loads and writes its positions' rows, a float4 a thread.
+// Byte i of a word of codes (4-bit: its low nibble) times its scale, exactly.
 template <int QT>
-__global__ __launch_bounds__(kKvThreads) void kv_read_kernel(KvView kv, KvLists lists, bool fresh, int count,
+__device__ __forceinline__ float value_of(uint32_t w, int i, float d, float m) {
+    const int c = static_cast<int>((w >> (8 * i)) & (QT == 1 ? 0xffu : 0xfu));
+    const float y = static_cast<float>(c - (QT == 1 ? 128 : QT == 2 ? 8 : 0)) * d;
+    return QT == 3 ? y + m : y;
+}
+
+// Bound: memory (cache bytes in, 4-byte elements out).  A workgroup brings one tile
+// to LDS with 16-byte loads and writes its positions' rows.
+template <int QT>
+__global__ __launch_bounds__(kReadThreads) void kv_read_kernel(KvView kv, KvLists lists, bool fresh, int count,
                                                              float* __restrict__ k, float* __restrict__ v) {
     using F = KvForm<QT>;
     extern __shared__ __attribute__((aligned(16))) uint8_t image[];
@@ -330,19 +337,64 @@ __global__ __launch_bounds__(kKvThreads) void kv_read_kernel(KvView kv, KvLists 
         if (n <= 0) continue;
         const uint8_t* src = kv.base + ((static_cast<size_t>(page) * kv.n_kv + head) * kv.page_tiles + tile) * tile_bytes;
         __syncthreads();  // the last tile's readers are done
-        for (int i = threadIdx.x * 16; i < tile_bytes; i += kKvThreads * 16) {
+        for (int i = threadIdx.x * 16; i < tile_bytes; i += kReadThreads * 16) {
             *reinterpret_cast<uint4*>(image + i) = *reinterpret_cast<const uint4*>(src + i);
         }
         __syncthreads();
-        const int per = hd / 4;
-        for (int t = threadIdx.x; t < 2 * n * per; t += kKvThreads) {
-            const int e = t % per * 4, s = t / per % n;
-            const bool values = t >= n * per;
+        // Keys: four elements of a position a thread, which share a word of codes and a scale.
+        const size_t first = (static_cast<size_t>(row) * kv.n_kv + head) * hd, step = static_cast<size_t>(kv.n_kv) * hd;
+        const int per = hd / 4, at_once = kReadThreads / per;
+        const uint16_t* scale = reinterpret_cast<const uint16_t*>(image + F::codes(nb));
+        const uint16_t* minimum = reinterpret_cast<const uint16_t*>(image + F::codes(nb) + F::plane(nb));
+        {
+            const int e = threadIdx.x % per * 4, b = e >> 5, r = e & 31;
+            const int lb = F::key_lane(nb);
+            for (int s = threadIdx.x / per; s < n; s += at_once) {
+                if (static_cast<int>(threadIdx.x) >= at_once * per) break;
+                const int key = slot + s, lane = 16 * (r >> 3) + (key & 15);
+                const uint8_t* p = image + (key >> 4) * 64 * lb;
+                float4 y;
+                if (QT == 0) {
+                    y = *reinterpret_cast<const float4*>(p + F::at(lb, lane, (b * 8 + (r & 7)) * 4));
+                } else {
+                    const int si = F::key_scale(nb, key, b);
+                    const float d = half_value(scale[si]), m = QT == 3 ? half_value(minimum[si]) : 0.0f;
+                    uint32_t w;
+                    if (QT == 1) w = *reinterpret_cast<const uint32_t*>(p + F::at(lb, lane, b * 8 + (r & 7)));
+                    else w = *reinterpret_cast<const uint32_t*>(p + F::at(lb, lane, b * 4)) >> (r & 4);
+                    y = make_float4(value_of<QT>(w, 0, d, m), value_of<QT>(w, 1, d, m), value_of<QT>(w, 2, d, m), value_of<QT>(w, 3, d, m));
+                }
+                *reinterpret_cast<float4*>(k + first + s * step + e) = y;
+            }
+        }
+        // Values: a thread takes the four positions of one dimension that share a word.
+        scale = reinterpret_cast<const uint16_t*>(image + F::half(nb) + F::codes(nb));
+        minimum = reinterpret_cast<const uint16_t*>(image + F::half(nb) + F::codes(nb) + F::plane(nb));
+        const int lb = F::value_lane(nb);
+        for (int t = threadIdx.x; t < 8 * hd; t += kReadThreads) {
+            const int d = t % hd, quad = t / hd;  // positions 4 quad ..
+            if (4 * quad + 3 < slot || 4 * quad >= slot + n) continue;
+            const int b = d >> 5, r = d & 31, lane = 16 * (quad & 3) + (r & 15), x = (r >> 4) * 8 + (quad >> 2) * 4;
+            const uint8_t* p = image + F::half(nb);
             float y[4];
+            if (QT == 0) {
+                const float4 f = *reinterpret_cast<const float4*>(p + F::at(lb, lane, (b * 16 + x) * 4));
+                y[0] = f.x, y[1] = f.y, y[2] = f.z, y[3] = f.w;
+            } else {
+                uint32_t w;
+                if (QT == 1) w = *reinterpret_cast<const uint32_t*>(p + F::at(lb, lane, b * 16 + x));
+                else w = *reinterpret_cast<const uint32_t*>(p + F::at(lb, lane, b * 8 + (x & 7))) >> (r >> 4 << 2);
+                const int si = F::value_scale(nb, 4 * quad, b);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = kv_element<QT>(image, nb, values, slot + s, e + i);
-            float* o = (values ? v : k) + (static_cast<size_t>(row + s) * kv.n_kv + head) * hd + e;
-            *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = value_of<QT>(w, i, half_value(scale[si + i]), QT == 3 ? half_value(minimum[si + i]) : 0.0f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = 4 * quad + i - slot;
+                if (s >= 0 && s < n) v[first + s * step + d] = y[i];
+            }
         }
     }
 }
@@ -354,7 +406,7 @@ hipError_t allow_lds(K kernel, int bytes) {
 }
 
 template <int QT>
-hipError_t write(const KvView& kv, const KvLists& lists, int count, const float* k, const float* v, const float* q,
+hipError_t write(const KvView& kv, const KvLists& lists, int count, int tokens, const float* k, const float* v, const float* q,
                  float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
     const int heads = kv.n_kv + (q != nullptr ? n_heads : 0);
     // Heads a workgroup takes: the angles are computed once for them, as long as
@@ -363,10 +415,13 @@ hipError_t write(const KvView& kv, const KvLists& lists, int count, const float*
     const long long groups = static_cast<long long>(count) * ((heads + per_group - 1) / per_group);
     const int lds = KvForm<QT>::tile(kv.nb) +
                     (rope.on ? kKvTile * (kv.head_dim / 2) * static_cast<int>(sizeof(double2)) : 0);
+    // Whole tiles keep 512 threads busy (2048 tokens, 32 + 32 heads of 128: 62 us with the read back, 92
+    // with 256); a token or two do not (64 sequences: 14 us, 17 with 512).
+    const unsigned threads = tokens > 4ll * count ? kWriteThreads : kWriteThreads / 2;
     const hipError_t e = allow_lds(kv_write_kernel<QT>, lds);
     if (e != hipSuccess) return e;
     const unsigned grid = count > 0 ? static_cast<unsigned>(std::min<long long>(groups, 1 << 20)) : kRecordedGroups;
-    kv_write_kernel<QT><<<grid, kKvThreads, lds, s>>>(kv, lists.fresh, lists.counts, count, k, v, q, q_out, n_heads,
+    kv_write_kernel<QT><<<grid, threads, lds, s>>>(kv, lists.fresh, lists.counts, count, k, v, q, q_out, n_heads,
                                                       count > 0 ? per_group : 4, rope);
     return hipGetLastError();
 }
@@ -378,7 +433,7 @@ hipError_t read(const KvView& kv, const KvLists& lists, bool fresh, int count, f
     const hipError_t e = allow_lds(kv_read_kernel<QT>, lds);
     if (e != hipSuccess) return e;
     const unsigned grid = count > 0 ? static_cast<unsigned>(std::min<long long>(groups, 1 << 20)) : kRecordedGroups;
-    kv_read_kernel<QT><<<grid, kKvThreads, lds, s>>>(kv, lists, fresh, count, k, v);
+    kv_read_kernel<QT><<<grid, kReadThreads, lds, s>>>(kv, lists, fresh, count, k, v);
     return hipGetLastError();
 }
 
@@ -391,13 +446,13 @@ hipError_t launch_kv_upload(const KvParts& parts, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, int count, const float* k, const float* v, const float* q,
+hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, int count, int tokens, const float* k, const float* v, const float* q,
                            float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
     switch (kv.qtype) {
-        case 0: return write<0>(kv, lists, count, k, v, q, q_out, n_heads, rope, s);
-        case 1: return write<1>(kv, lists, count, k, v, q, q_out, n_heads, rope, s);
-        case 2: return write<2>(kv, lists, count, k, v, q, q_out, n_heads, rope, s);
-        case 3: return write<3>(kv, lists, count, k, v, q, q_out, n_heads, rope, s);
+        case 0: return write<0>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 1: return write<1>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 2: return write<2>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 3: return write<3>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
         default: return hipErrorInvalidValue;
     }
 }

@@ -103,10 +103,10 @@ struct KvParts {
 };
 hipError_t launch_kv_upload(const KvParts& parts, hipStream_t s);
 
-// `groups` workgroups walk the list of which `count` items are in use (0: as the
-// device says, for launches that are recorded and replayed with other lists).
-hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, int count, const float* k, const float* v, const float* q,
-                           float* q_out, int n_heads, const KvRope& rope, hipStream_t s);
+// `count`: the items of the list in use (0: as many as the device says, for launches
+// that are recorded and replayed with other lists); `tokens`: new tokens of the batch.
+hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, int count, int tokens, const float* k, const float* v,
+                           const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s);
 hipError_t launch_kv_read(const KvView& kv, const KvLists& lists, bool fresh, int count, float* k, float* v, hipStream_t s);
 
 struct KvAttention {

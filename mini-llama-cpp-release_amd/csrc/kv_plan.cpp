@@ -7,10 +7,13 @@
 namespace mlq {
 namespace {
 
-// A split makes workgroups until there are this many (few rows, many rows: four and
-// two a CU), and no more.
-constexpr int kTargetGroups[2] = {1024, 512};
-// Fewer tiles than this are not split further: the parts' merge would cost more.
+// A split makes workgroups until there are this many, two a CU as either kernel's registers
+// allow, and no more.  One token over 100000 positions (Q4_0, 8 KV heads), 256 / 512 / 1024 of
+// them: 48 / 46 / 57 us; 8 sequences of 4000 (Q8_0) 21 / 21 / 26.
+constexpr int kTargetGroups = 512;
+// Fewer tiles than this are not split further, as the parts' merge would cost more.  One token over
+// 4000 positions, at least 4 / 8 / 16 tiles: 14.9 / 12.8 / 13.8 us; over 700 9.6 / 10.3 / 11.6; 128 rows
+// over 4000 53 / 46 / 54.
 constexpr int kLeastTiles = 8;
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -38,7 +41,7 @@ KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     for (int kind = 0; kind < 2; ++kind) {
         // Only an item of n parts adds to the list, n - 1 items, and all parts take slots: at
         // most twice what is added.
-        const int extra = ceil_div(kTargetGroups[kind], s.n_kv_heads);
+        const int extra = ceil_div(kTargetGroups, s.n_kv_heads);
         l.items[kind] = whole[kind] + extra;
         l.slots[kind] = 2 * extra;
     }
@@ -142,15 +145,19 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
         // Parts of at most `most` tiles, as even as they come: the fewest tiles that do not make more
         // items than `target`, since those beyond one round of workgroups would take a second one.
         std::vector<KvAttnItem>& list = b.items[kind];
-        const int target = std::max(1, kTargetGroups[kind] / s.n_kv_heads);
+        const int target = std::max(1, kTargetGroups / s.n_kv_heads);
         auto items_of = [&](int64_t most) {
             int64_t n = 0;
             for (const KvAttnItem& w : whole) n += (w.count + most - 1) / most;
             return n;
         };
-        int64_t lo = std::max<int64_t>(kLeastTiles, (tiles + target - 1) / target), hi = lo;
+        // Where there is a round without splits, only items of twice the average are split (64 ragged
+        // sequences of up to 4000: 79 us, 85 with those over the average split).
+        // (Not a prompt's row groups, whose lengths are spread: 2048 tokens, 32 heads: 167 us, 193 unsplit.)
+        const bool enough = static_cast<int>(whole.size()) >= target;
+        int64_t lo = std::max<int64_t>(kLeastTiles, (enough && kind == 0 ? 2 : 1) * ((tiles + target - 1) / target)), hi = lo;
         for (const KvAttnItem& w : whole) hi = std::max<int64_t>(hi, w.count);
-        while (lo < hi && static_cast<int>(whole.size()) < target) {
+        while (lo < hi && !enough) {
             const int64_t mid = (lo + hi) / 2;
             if (items_of(mid) <= target) hi = mid;
             else lo = mid + 1;
