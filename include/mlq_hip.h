@@ -414,11 +414,12 @@ int mlq_hip_kv_cache_destroy(mlq_kv_cache_t cache);
  * and, from each set, the batch with its work lists in device memory.
  * A token at position i sees positions j <= i; with window > 0 only those with
  * j > i - window or j < sinks (the sequence's first tokens, which stay visible).
- * scale: of the scores, 0 for 1/sqrt(head_dim).  n_heads: a multiple of the
- * cache's KV heads (query head h reads KV head h / (n_heads / n_kv_heads)).
+ * scale: of the scores, 0 for 1/sqrt(head_dim), else of magnitude 2^-100 to
+ * 2^100.  n_heads: a multiple of the cache's KV heads (query head h reads KV head
+ * h / (n_heads / n_kv_heads)).
  * max_seqs, max_tokens and max_pages bound a set's sequences, new tokens and
  * page entries (max_pages * page_size up to 2^30, max_tokens * n_heads up to
- * 2^30).  A plan holds device memory of its own (about 55 MB at head_dim 128,
+ * 2^30).  A plan holds device memory of its own (about 80 MB at head_dim 128,
  * for results of work that is split over long contexts): its calls must not
  * overlap in time (one stream, or events), graph replays included, and one host
  * thread uses it at a time. */
@@ -459,8 +460,9 @@ int mlq_hip_kv_read(mlq_kv_plan_t plan, int layer, int new_only, float* k, float
  * products run as pairs of fp16 parts.  A position a token does not see has no
  * part in its result, whatever it holds.  A 32-element block of a key or value
  * that holds an element that is not finite (in f32 caches also one of magnitude
- * 2^110 or more, in quantized ones a scale that is not finite) counts as NaN
- * for the tokens that see it.  The same call gives the same bits. */
+ * 2^80 or more, in quantized ones a scale that is not finite) counts as NaN for
+ * the tokens that see it; f32 elements below 2^-80 are taken to 2^-100.  The same
+ * call gives the same bits. */
 int mlq_hip_kv_attention(mlq_kv_plan_t plan, int layer, const float* q, float* out, void* stream);
 
 /* Kernel selection introspection: name of the kernel the next call with this

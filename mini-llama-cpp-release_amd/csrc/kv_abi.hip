@@ -222,7 +222,9 @@ int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int si
         }
         if (window < 0 || sinks < 0) return abi_fail(MLQ_ERR_INVALID, who + ": negative window or sinks");
         if (sinks > 0 && window == 0) return abi_fail(MLQ_ERR_INVALID, who + ": sinks need a window");
-        if (!std::isfinite(scale)) return abi_fail(MLQ_ERR_INVALID, who + ": scale is not finite");
+        if (!(scale == 0.0f || (std::fabs(scale) >= 0x1p-100f && std::fabs(scale) <= 0x1p100f))) {
+            return abi_fail(MLQ_ERR_INVALID, who + ": scale is neither 0 nor of magnitude 2^-100 to 2^100");
+        }
         if (max_seqs <= 0 || max_tokens <= 0 || max_pages <= 0) {
             return abi_fail(MLQ_ERR_SHAPE, who + ": empty plans are not supported");
         }

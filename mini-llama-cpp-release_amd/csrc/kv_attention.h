@@ -155,7 +155,7 @@ __device__ __forceinline__ void split8(const float* v, h8_t* hi, h8_t* lo) {
     *hi = join(h[0], h[1], h[2], h[3]);
     *lo = join(r[0], r[1], r[2], r[3]);
 }
-// 1 / s for a power of two s from 2^-90 on; 0 for Inf.
+// 1 / s for a power of two s from 2^-80 on; 0 for Inf.
 __device__ __forceinline__ float inverse_power(uint32_t s) {
     return bits<float>(static_cast<uint32_t>(max(static_cast<int>(0x7f000000u) - static_cast<int>(s), 0)));
 }
@@ -181,11 +181,13 @@ __device__ __forceinline__ void load_query(const float* q, int hd, int g, float 
         for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[b][j]));
     }
     top = max_quarters(top);
-    // exponent, kept where 2^(13 - e) and its inverse are normal
-    const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 127);
+    // exponent, kept where 2^(13 - e) is finite and to_t is 2^-112 or more (a row of zeros or nearly: its
+    // scores are then as near to 0 as to_t says, and what is taken over to_t stays finite)
+    const int log_scale = static_cast<int>(__builtin_bit_cast(uint32_t, fabsf(scale)) >> 23) - 127;
+    const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, max(-110, -99 - log_scale)), 127);
     // a negative scale turns the queries; a score's factor is positive, so that -inf stays -inf
     const float up = ldexpf(scale < 0.0f ? -1.0f : 1.0f, 13 - e);
-    *to_t = fmaxf(ldexpf(fabsf(scale), e - 13), 0x1p-126f);
+    *to_t = ldexpf(fabsf(scale), e - 13);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         sum[b] = 0.0f;
@@ -219,13 +221,18 @@ __device__ __forceinline__ void leave_state(__amdgpu_buffer_rsrc_t rs, int lane,
                                               (QUADS * 256 + (2 * u + 1) * 64 + lane) * 4, 0, kCoherent);
     }
 }
+// l 2^d, in halves: d is a difference of scores *and* of f32 values' exponents, and a sum of weights whose
+// values are small may be far above 1, so it counts where 2^d itself is below what f32 holds.
+__device__ __forceinline__ float down(float l, float d, float* w) {
+    const float half = __builtin_amdgcn_exp2f(0.5f * d);
+    *w = half * half;
+    return l * half * half;
+}
 // Takes another state of the same rows into one's own.
 __device__ __forceinline__ void fold(float& m, float& l, float m1, float l1, float* w0, float* w1) {
     const float to = fmaxf(m, m1);
-    *w0 = __builtin_amdgcn_exp2f(m - to);
-    *w1 = __builtin_amdgcn_exp2f(m1 - to);
+    l = down(l, m - to, w0) + down(l1, m1 - to, w1);
     m = to;
-    l = l * *w0 + l1 * *w1;
 }
 template <int NQ, int NB>
 __device__ __forceinline__ void take_state(__amdgpu_buffer_rsrc_t rs, int lane, f4_t (*o)[2 * NB], float* m, float* l) {
@@ -438,9 +445,9 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             top = max_quarters(top);
             if (__any(top > m + kSlack)) {
                 const float to = top > m + kSlack ? top : m;
-                const float c = __builtin_amdgcn_exp2f(m - to);
+                float c;
+                l = down(l, m - to, &c);
                 m = to;
-                l *= c;
 #pragma unroll
                 for (int x = 0; x < 2 * NB; ++x) o[0][x] *= c;
 #pragma unroll

@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 float lift = kLift;
                 int e = 0;
                 if (!__all(near && !bad)) {
-                    e = near ? 0 : max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -90);
+                    e = near ? 0 : max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -80);
                     lift = ldexpf(kLift, -e);
                     flags |= kFar | (values && __any(bad) ? kBad : 0u);
                 }
@@ -445,9 +445,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
                     const float to = top[u] > m[u] + kSlack ? top[u] : m[u];
-                    const float c = __builtin_amdgcn_exp2f(m[u] - to);
+                    float c;
+                    l[u] = down(l[u], m[u] - to, &c);
                     m[u] = to;
-                    l[u] *= c;
 #pragma unroll
                     for (int x = 0; x < 2 * NB; ++x) o[u][x] *= c;
                 }
@@ -475,9 +475,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     sum += p[j];
                 }
                 if ((flags & kFar) != 0) {
+                    // p_j = P_j 2^-ev_j, which may count where P_j is below what f32 holds
                     sum = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum = fmaf(p[j], s->value_down[(j >> 2) * 16 + 4 * g + (j & 3)], sum);
+                    for (int j = 0; j < 8; ++j) {
+                        const float y = fmaf(x_[u][j], to_t[u], -frame);
+                        const float down = s->value_down[(j >> 2) * 16 + 4 * g + (j & 3)];
+                        const bool deep = y < -60.0f;
+                        sum = fmaf(__builtin_amdgcn_exp2f(deep ? y + 100.0f : y), deep ? down * 0x1p-100f : down, sum);
+                    }
                 }
                 l[u] += sum;
                 split8(p, &ph[u], &pl[u]);

@@ -100,14 +100,15 @@ __device__ __forceinline__ void quantize_block(const float* y, bool here, int g,
 #pragma clang fp contract(off)
     *m = 0;
     if (QT == 0) {
-        // 2^e with the block's largest element in [2^e, 2^(e+1)), e at least -90
+        // 2^e with the block's largest element in [2^e, 2^(e+1)), e at least -80; Inf from 2^80 on (sums of
+        // products of such elements and their powers of two stay in f32's range)
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, f32_bits(y[i]) & 0x7fffffffu);
         top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xf, 0xf, true)));
         top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x4E, 0xf, 0xf, true)));
         const uint32_t e = top >> 23;
-        *d = e >= 127 + 110 ? 0x7f800000u : max(e, 127u - 90u) << 23;
+        *d = e >= 127 + 80 ? 0x7f800000u : max(e, 127u - 80u) << 23;
         return;
     }
     if (QT == 3) {

@@ -18,7 +18,7 @@
 // dimensions i and 16 + i).  Scales are binary16 (Q4_1: scales, then minima), in
 // the order of the lanes that use them.  F32 elements are stored as they are; per
 // block there is a power of two (f32) that brings them into fp16's range, Inf
-// where a block holds something that is not finite or reaches 2^110.
+// where a block holds something that is not finite or reaches 2^80.
 #pragma once
 
 #include "kv_plan.h"

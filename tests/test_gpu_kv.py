@@ -302,6 +302,43 @@ def test_attention_value_range(hip, orc, size):
     Case(hip, orc, "f32", [(7, 150)], 4, 2, 64, keys=k, scale=float(0.1 / size)).check()
 
 
+@pytest.mark.parametrize("size", [1e-20, 1e-6, 1e5, 1e20])
+@pytest.mark.parametrize("new", [3, 70])
+def test_attention_range_of_all_three(hip, orc, new, size):
+    """Queries of zeros and tiny ones beside ordinary ones, keys and values far from 1."""
+    rng = np.random.default_rng(14)
+    v = (rng.standard_normal((150, 2, 64)) * size).astype(np.float32)
+    k = rng.standard_normal((150, 2, 64)).astype(np.float32)
+    for keys, scale in ((k, 0.0), ((k * size).astype(np.float32), float(0.1 / size))):
+        c = Case(hip, orc, "f32", [(new, 150)], 4, 2, 64, keys=keys, values=v, scale=scale)
+        c.q[0] = 0.0
+        c.q[1, 1] *= np.float32(1e-30)
+        c.q[2, 3] *= np.float32(1e-36)
+        c.q[1, 2, 1:] = 0.0
+        c.check()
+    # keys near the largest that count as finite, small queries
+    c = Case(hip, orc, "f32", [(new, 150)], 4, 2, 64, keys=(k * 2e23).astype(np.float32), values=v)
+    c.q *= np.float32(2e-23)
+    c.check()
+
+
+@pytest.mark.parametrize("new", [3, 70])
+def test_attention_values_of_many_sizes(hip, orc, new):
+    """f32 values whose sizes differ by 2^150 between positions: the sum of the weights holds those of the
+    positions whose values are small, also where a tile of large ones comes behind them."""
+    rng = np.random.default_rng(15)
+    k, v = (rng.standard_normal((300, 2, 64)).astype(np.float32) for _ in range(2))
+    any_size = (v * 10.0 ** rng.uniform(-22, 22, (300, 1, 1))).astype(np.float32)
+    Case(hip, orc, "f32", [(new, 300)], 4, 2, 64, keys=k, values=any_size).check()
+    for first, then in ((1e-23, 1e23), (1e23, 1e-23)):
+        sizes = np.where(np.arange(300) < 150, first, then)[:, None, None]
+        # scores of 0 where values are tiny, of about -14 where they are large
+        keys = np.where(sizes < 1, 0.0, np.float32(-14.0 / 64)).astype(np.float32) * np.ones_like(k)
+        c = Case(hip, orc, "f32", [(new, 300)], 4, 2, 64, keys=keys, values=(v * sizes).astype(np.float32), scale=1.0)
+        c.q[:] = 1.0
+        c.check()
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, np.float32(-3.4e38)])
 def test_attention_unseen_places(hip, orc, kind, bad):
@@ -554,7 +591,9 @@ def test_refusals(hip):
     for a, code, what in (((3, 0, 0, 0.0, 1, 1, 1), 2, "3 heads over 2 KV heads"), ((0, 0, 0, 0.0, 1, 1, 1), 2, "0 heads"),
                           ((4, -1, 0, 0.0, 1, 1, 1), 1, "negative window"), ((4, 0, 2, 0.0, 1, 1, 1), 1, "sinks need a window"),
                           ((4, 5, -2, 0.0, 1, 1, 1), 1, "negative window or sinks"),
-                          ((4, 0, 0, float("nan"), 1, 1, 1), 1, "scale"), ((4, 0, 0, 0.0, 0, 1, 1), 2, "empty plans"),
+                          ((4, 0, 0, float("nan"), 1, 1, 1), 1, "scale"), ((4, 0, 0, 1e31, 1, 1, 1), 1, "2^100"),
+                          ((4, 0, 0, float("-inf"), 1, 1, 1), 1, "scale"), ((4, 0, 0, -1e-31, 1, 1, 1), 1, "scale"),
+                          ((4, 0, 0, 0.0, 0, 1, 1), 2, "empty plans"),
                           ((4, 0, 0, 0.0, 1, 0, 1), 2, "empty plans"), ((4, 0, 0, 0.0, 1, 1, -1), 2, "empty plans"),
                           ((4, 0, 0, 0.0, 1, 1 << 29, 1), 6, "2^30"), ((4, 0, 0, 0.0, 1, 1, 1 << 25), 6, "2^30")):
         assert plan(*a) == code, (a, hip.last_error())
