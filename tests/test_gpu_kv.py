@@ -279,6 +279,48 @@ def test_attention_long(hip, orc, kind):
     assert np.array_equal(got, wide.run())
 
 
+HEAD_DIMS = [8, 24, 40, 72, 104, 136, 160, 192, 200, 224, 248, 256]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd", HEAD_DIMS)
+def test_attention_head_dims(hip, orc, kind, hd):
+    """Every number of blocks a head, whole and not, with one row, some and many."""
+    say("head_dim", kind, hd)
+    Case(hip, orc, kind, [(1, 70), (70, 101), (13, 45)], 4, 2, hd, 32, seed=hd).check()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows", [7, 8, 9, 16, 17, 63, 64, 65, 127, 128, 129, 191, 257])
+def test_attention_row_counts(hip, orc, kind, rows):
+    """Rows at and around what one workgroup takes, over short contexts and ones that are split."""
+    say("rows", kind, rows)
+    for t in (rows, rows + 31, rows + 2500):
+        Case(hip, orc, kind, [(rows, t)], 1, 1, 64, 64, seed=rows).check()
+    Case(hip, orc, kind, [(rows, rows + 1700), (1, 33)], 6, 2, 32, 64, window=1500, sinks=5, seed=rows).check()
+
+
+def test_attention_of_many_sequences(hip, orc):
+    """A batch of 300 short sequences of every kind, and one sequence listed twice (a page may be
+    in several sequences as long as no two new tokens share a slot)."""
+    rng = np.random.default_rng(31)
+    lens = [(int(min(n, t)), int(t)) for n, t in zip(rng.choice([0, 1, 1, 1, 2, 9, 40], 300), rng.integers(0, 150, 300))]
+    Case(hip, orc, "q4_0", lens, 8, 2, 64, 32, seed=32).check()
+    c = Case(hip, orc, "q8_0", [(1, 90)], 4, 2, 64, 32, seed=33)
+    twice = hip.KvPlan(c.cache, 4, max_seqs=2, max_tokens=2, max_pages=6)
+    pages = c.batch.pages
+    with pytest.raises(hip.MlqError, match="slot"):
+        twice.set([1, 1], [90, 90], pages + pages)
+    twice.set([1, 1], [90, 89], pages + pages)
+    q = np.concatenate([c.q, c.q])
+    out = hip.DeviceBuffer(q.nbytes)
+    twice.attention(0, dev(hip, q), out)
+    got = back(hip, out, q.shape)
+    for i, t in enumerate((90, 89)):
+        want, bound = attention(c.q, c.held[0][:t], c.held[1][:t])
+        assert (np.abs(got[i] - want[0]) <= bound[0]).all()
+
+
 def test_attention_scale_and_peaks(hip, orc):
     """A scale of one's own, scores of hundreds (one position takes all), equal scores."""
     Case(hip, orc, "q8_0", [(5, 200), (1, 90)], 4, 2, 64, scale=0.02, seed=1).check()
@@ -550,6 +592,45 @@ def test_graph_serves_later_batches(hip, orc):
     short = hip.DeviceBuffer(4 * 95 * heads * hd)
     with pytest.raises(hip.MlqError, match="too small"):
         hip.Graph.record(lambda: plan.attention(0, short, out, stream=s), stream=s)
+    g.destroy()
+    hip.stream_destroy(s)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_recorded_write_of_whole_tiles(hip, orc, kind):
+    """A recorded rotation and write, replayed with whole tiles, single tokens and parts of tiles, eager calls
+    between the replays."""
+    rng = np.random.default_rng(19)
+    heads, kv, hd, page, most = 4, 2, 64, 64, 200
+    cache, want = (hip.KvCache(QT[kind], 1, 12, page, kv, hd) for _ in range(2))
+    plan, eager = (hip.KvPlan(c, heads, max_seqs=3, max_tokens=most, max_pages=12) for c in (cache, want))
+    s = hip.stream_create()
+    dk, dv = (hip.DeviceBuffer(4 * most * kv * hd) for _ in range(2))
+    dq, oq, eq = (hip.DeviceBuffer(4 * most * heads * hd) for _ in range(3))
+    reads = [hip.DeviceBuffer(4 * 12 * page * kv * hd) for _ in range(4)]
+    plan.set([1], [1], [0], stream=s)
+    hip.synchronize(s)
+    g = hip.Graph.record(lambda: plan.write(0, dk, dv, q=dq, q_out=oq, theta=THETA, neox=True, stream=s), stream=s)
+    for new, length in (([128], [128]), ([1, 64, 3], [129, 64, 3]), ([0, 0, 1], [129, 64, 4]), ([31, 1, 100], [160, 65, 104])):
+        pages = sum(([4 * i + j for j in range(-(-t // page))] for i, t in enumerate(length)), [])
+        for d, n in ((dk, kv), (dv, kv), (dq, heads)):
+            d.upload(rng.standard_normal(most * n * hd).astype(np.float32))
+        for p in (plan, eager):
+            p.set(new, length, pages, stream=s)
+        oq.upload(np.full(most * heads * hd, 3.5, np.float32))
+        eq.upload(np.full(most * heads * hd, 3.5, np.float32))
+        for _ in range(2):
+            g.launch(s)
+            eager.write(0, dk, dv, q=dq, q_out=eq, theta=THETA, neox=True, stream=s)
+            hip.synchronize(s)
+        n = most * heads * hd
+        assert np.array_equal(oq.download(np.float32, n), eq.download(np.float32, n))
+        for p, (rk, rv) in ((plan, reads[:2]), (eager, reads[2:])):
+            p.read(0, rk, rv, stream=s)
+        hip.synchronize(s)
+        n = sum(length) * kv * hd
+        a, b, x, y = (r.download(np.float32, n) for r in reads)
+        assert np.array_equal(a, x) and np.array_equal(b, y) and np.abs(a).max() > 0
     g.destroy()
     hip.stream_destroy(s)
 
