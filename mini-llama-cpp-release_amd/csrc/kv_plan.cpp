@@ -16,7 +16,7 @@ constexpr int kTargetGroups = 512;
 // over 4000 53 / 46 / 54.
 constexpr int kLeastTiles = 8;
 
-int ceil_div(int a, int b) { return (a + b - 1) / b; }
+int ceil_div(int a, int b) { return a / b + (a % b != 0); }  // (sinks go up to the largest int)
 
 // Tiles that query rows at positions lo .. hi can see, in the numbering of KvAttnItem.
 struct Seen {

@@ -40,8 +40,8 @@ void one(std::mt19937& rng, int trial) {
     s.n_kv_heads = pick(rng, {1, 2, 8, 32});
     s.group = pick(rng, {1, 2, 7, 8, 16});
     s.wide_rows = pick(rng, {128, 256});
-    s.window = pick(rng, {0, 0, 1, 20, 32, 33, 100, 1000});
-    s.sinks = s.window ? pick(rng, {0, 1, 4, 32, 40, 3000}) : 0;
+    s.window = pick(rng, {0, 0, 1, 20, 32, 33, 100, 1000, 2147483647});
+    s.sinks = s.window ? pick(rng, {0, 1, 4, 32, 40, 3000, 2147483647}) : 0;
     const int n_seqs = rng() % 6;
     std::vector<int> fresh(n_seqs), len(n_seqs), pages;
     int tokens = 0, entries = 0;
