@@ -422,7 +422,7 @@ int mlq_hip_kv_cache_destroy(mlq_kv_cache_t cache);
  * 2^30).  A plan holds device memory of its own (about 80 MB at head_dim 128,
  * for results of work that is split over long contexts): its calls must not
  * overlap in time (one stream, or events), graph replays included, and one host
- * thread uses it at a time. */
+ * thread uses it at a time.  It outlives the graphs that recorded its calls. */
 typedef struct mlq_kv_plan_s* mlq_kv_plan_t;
 int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
                            int max_tokens, int max_pages, mlq_kv_plan_t* out);

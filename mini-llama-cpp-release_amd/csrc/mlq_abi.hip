@@ -474,7 +474,10 @@ int grow_stage(DeviceState& st, size_t bytes) {
 namespace mlq {
 
 int abi_fail(int code, const std::string& msg) { return fail(code, msg); }
-int abi_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+int abi_hip_fail(hipError_t e, const char* what) {
+    (void)hipGetLastError();  // reported here: not to be taken for the next launch's
+    return hip_fail(e, what);
+}
 int abi_device(int device) { return ensure_device(device); }
 hipStream_t abi_stream(int device, void* stream) { return resolve_stream(device, stream); }
 bool abi_capturing(hipStream_t s) { return capturing(s); }

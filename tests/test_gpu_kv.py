@@ -596,12 +596,12 @@ def test_graph_serves_later_batches(hip, orc):
     hip.stream_destroy(s)
 
 
-@pytest.mark.parametrize("kind", TYPES)
-def test_recorded_write_of_whole_tiles(hip, orc, kind):
+@pytest.mark.parametrize("kind,hd", [(kind, 64) for kind in TYPES] + [("f32", 256), ("q4_1", 200)])
+def test_recorded_write_of_whole_tiles(hip, orc, kind, hd):
     """A recorded rotation and write, replayed with whole tiles, single tokens and parts of tiles, eager calls
     between the replays."""
     rng = np.random.default_rng(19)
-    heads, kv, hd, page, most = 4, 2, 64, 64, 200
+    heads, kv, page, most = 4, 2, 64, 200
     cache, want = (hip.KvCache(QT[kind], 1, 12, page, kv, hd) for _ in range(2))
     plan, eager = (hip.KvPlan(c, heads, max_seqs=3, max_tokens=most, max_pages=12) for c in (cache, want))
     s = hip.stream_create()
@@ -709,6 +709,16 @@ def test_refusals(hip):
         with pytest.raises(hip.MlqError, match=what):
             call()
     hip.synchronize(hip.stream(0))
+
+
+def test_a_failed_allocation_is_reported_once(hip, orc):
+    """A cache that no card holds is refused with the allocation's error, and the calls after it work."""
+    c = Case(hip, orc, "q8_0", [(1, 40)], 4, 2, 64)
+    with pytest.raises(hip.MlqError, match="HIP error"):
+        hip.KvCache(QT["f32"], 1000, 4000, 65536, 8, 128)  # 2 PB
+    with pytest.raises(hip.MlqError, match="too large"):
+        hip.KvCache(QT["f32"], 2 ** 31 - 1, 2 ** 31 - 1, 65536, 65536, 256)
+    c.check()
 
 
 def test_plan_outlives_its_cache_handle(hip, orc):
