@@ -7,8 +7,8 @@
 // A wave walks tiles of 32 positions of one KV head for up to eight query rows (row =
 // token * group + query head of the group, so grouped heads share what is read), the
 // four waves of a workgroup every fourth tile each, and workgroups parts of a long context; the
-// states are merged in a fixed order, the last workgroup to arrive merging the parts.  Per tile, in v_mfma_f32_16x16x32_f16 with operands that come
-// from memory as they lie there:
+// states are merged in a fixed order, the last workgroup to arrive merging the parts.  Per tile,
+// in v_mfma_f32_16x16x32_f16 with operands that come from memory as they lie there:
 //
 //   S^T = K Q^T   per block b of 32 elements: the codes are whole numbers (exact in
 //                 fp16), the queries pairs of fp16 parts hi + lo relative to the row's
@@ -30,6 +30,14 @@
 //
 // What a row does not see gets weight 0, and 0 times a scale that is Inf or NaN is 0
 // (v_mul_legacy_f32); codes are finite always.
+//
+// Bound: memory where the rows of a KV head are few and the contexts fill the chip (64
+// sequences of up to 4000 positions, Q8_0, 8 KV heads of 128, four query heads each: 75 us,
+// 4.7 TB/s of cache); with 4-bit codes half the bytes cost about as many instructions, some
+// 550 a tile, and issue bounds it (100 000 positions, Q4_0: 49 us, 2.3 TB/s, vector
+// instructions issue in half of the cycles). Short ones: launch, a chain of four trips to
+// memory (list, page, tile, parts) and the merge (700 positions 10.4 us).  Two workgroups a CU;
+// a third (fewer registers, Q4_0) was no faster, and parts beyond one round of them slower.
 #pragma once
 
 #include "kv_layout.h"
