@@ -240,7 +240,7 @@ int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int si
                                     window, sinks, max_seqs, max_tokens, max_pages};
         const mlq::KvPlanLimits lim = mlq::kv_plan_limits(p->shape);
         const size_t sizes[mlq::kKvParts] = {
-            mlq::kKvCounts * sizeof(int), static_cast<size_t>(max_tokens) * sizeof(mlq::KvTileItem),
+            mlq::kKvCounts * sizeof(int), static_cast<size_t>(lim.fresh) * sizeof(mlq::KvTileItem),
             static_cast<size_t>(max_pages) * sizeof(mlq::KvPage), static_cast<size_t>(lim.items[0]) * sizeof(mlq::KvAttnItem),
             static_cast<size_t>(lim.items[1]) * sizeof(mlq::KvAttnItem)};
         for (int i = 0; i < mlq::kKvParts; ++i) {

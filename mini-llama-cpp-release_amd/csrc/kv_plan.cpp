@@ -38,6 +38,8 @@ KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     const int64_t narrow = std::min(rows / kKvNarrowRows, static_cast<int64_t>(s.max_seqs) * (kKvNarrowMost / kKvNarrowRows - 1));
     const int whole[2] = {static_cast<int>(narrow) + s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
     KvPlanLimits l;
+    // a sequence's new tokens begin and end inside a tile at the most
+    l.fresh = static_cast<int>(std::min<int64_t>(s.max_tokens, s.max_tokens / kKvTile + 2ll * s.max_seqs));
     for (int kind = 0; kind < 2; ++kind) {
         // Only an item of n parts adds to the list, n - 1 items, and all parts take slots: at
         // most twice what is added.

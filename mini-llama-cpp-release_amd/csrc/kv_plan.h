@@ -50,6 +50,7 @@ struct KvPlanShape {
 
 // What a set of a plan of this shape can need at the most.
 struct KvPlanLimits {
+    int fresh;     // tiles with new tokens
     int items[2];  // narrow, wide
     int slots[2];  // partial results
 };

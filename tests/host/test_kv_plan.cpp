@@ -66,7 +66,7 @@ void one(std::mt19937& rng, int trial) {
     const std::string wrong = mlq::kv_plan_build(s, n_seqs, fresh.data(), len.data(), pages.data(), &b);
     CHECK(wrong.empty(), "trial %d: %s", trial, wrong.c_str());
     const mlq::KvPlanLimits lim = mlq::kv_plan_limits(s);
-    CHECK(static_cast<int>(b.fresh.size()) <= s.max_tokens, "trial %d", trial);
+    CHECK(static_cast<int>(b.fresh.size()) <= lim.fresh && lim.fresh <= s.max_tokens, "trial %d", trial);
     CHECK(static_cast<int>(b.pages.size()) == entries, "trial %d", trial);
     CHECK(b.n_tokens == tokens, "trial %d", trial);
 
