@@ -399,7 +399,8 @@ int mlq_hip_matmul_f32(int device, const float* a, const float* b, int m, int k,
  * caller's business: a sequence's pages are a list of page ids, entry i holding
  * positions i * page_size .., the same for every layer.  Sequences may share
  * pages (a common prefix).  page_size: a power of two, 32 to 65536; head_dim: a
- * multiple of 8, up to 256.  The cache starts out as zeros. */
+ * multiple of 8, up to 256.  The cache starts out as zeros.  Caches and plans are
+ * created outside graph capture. */
 typedef struct mlq_kv_cache_s* mlq_kv_cache_t;
 int mlq_hip_kv_cache_create(int device, int type, int n_layers, int n_pages, int page_size, int n_kv_heads,
                             int head_dim, mlq_kv_cache_t* out);

@@ -176,11 +176,12 @@ int mlq_hip_kv_cache_create(int device, int type, int n_layers, int n_pages, int
         kv->layer_bytes = mlq::kv_tile_bytes(type, kv->nb) * (page_size / mlq::kKvTile) * n_kv_heads * n_pages;
         const int rc = mlq::abi_device(device);
         if (rc != MLQ_OK) return rc;
+        const hipStream_t s = mlq::abi_stream(device, nullptr);
+        if (mlq::abi_capturing(s)) return abi_fail(MLQ_ERR_INVALID, who + ": not under graph capture");
         void* mem = nullptr;
         MLQ_KV_HIP(hipMalloc(&mem, kv->bytes()));
         kv->mem = static_cast<uint8_t*>(mem);
         // Zeros: a slot that nothing has been written to holds finite values.
-        const hipStream_t s = mlq::abi_stream(device, nullptr);
         MLQ_KV_HIP(hipMemsetAsync(mem, 0, kv->bytes(), s));
         MLQ_KV_HIP(hipStreamSynchronize(s));
         *out = new mlq_kv_cache_s{std::move(kv)};
@@ -249,6 +250,8 @@ int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int si
         }
         const int rc = mlq::abi_device(kv.device);
         if (rc != MLQ_OK) return rc;
+        const hipStream_t s = mlq::abi_stream(kv.device, nullptr);
+        if (mlq::abi_capturing(s)) return abi_fail(MLQ_ERR_INVALID, who + ": not under graph capture");
         void* mem = nullptr;
         MLQ_KV_HIP(hipMalloc(&mem, p->list_bytes));
         p->lists = static_cast<uint8_t*>(mem);
@@ -268,7 +271,6 @@ int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int si
         p->arrived[1] = p->arrived[0] + words[0];
         p->partial[0] = reinterpret_cast<float*>(p->arrived[1] + words[1]);
         p->partial[1] = p->partial[0] + floats[0];
-        const hipStream_t s = mlq::abi_stream(kv.device, nullptr);
         MLQ_KV_HIP(hipMemsetAsync(p->work, 0, (words[0] + words[1]) * 4, s));
         MLQ_KV_HIP(hipStreamSynchronize(s));
         *out = p.release();

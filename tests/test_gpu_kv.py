@@ -588,6 +588,10 @@ def test_graph_serves_later_batches(hip, orc):
         assert np.array_equal(out.download(np.float32, most * heads * hd).reshape(got.shape), got), lens
     with pytest.raises(hip.MlqError, match="graph capture"):
         hip.Graph.record(lambda: plan.set([1], [1], [0], stream=s), stream=s)
+    for create in (lambda: hip.KvCache(QT["q8_0"], 1, 4, 64, 2, 64),
+                   lambda: hip.KvPlan(cache, heads, max_seqs=1, max_tokens=1, max_pages=1)):
+        with pytest.raises(hip.MlqError, match="graph capture"):
+            hip.Graph.record(create, stream=hip.stream(0))
     # recorded calls need room for the largest batch
     short = hip.DeviceBuffer(4 * 95 * heads * hd)
     with pytest.raises(hip.MlqError, match="too small"):
