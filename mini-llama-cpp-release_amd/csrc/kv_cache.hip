@@ -230,7 +230,8 @@ __device__ __forceinline__ void write_kv_head(const KvTileItem& it, int head, co
 
 // Bound: memory (4-byte elements in, cache bytes and rotated queries out: 2048 tokens of
 // 32 + 32 heads of 128 in Q8_0 50 us, 3.0 TB/s), for single tokens launch and a chain of
-// loads, angles and stores (5 us for one, 10.8 for 64 sequences of 32 + 8 heads).  A
+// loads, angles and stores (5 us for one, 10.8 for 64 sequences of 32 + 8 heads).  115
+// registers, 16 waves a CU; 80 (some spilled) took as long, 64 up to a third longer.  A
 // workgroup takes `per_group` heads of one tile's new tokens; the pairs' cosines and
 // sines, in 64 bits, are computed once for them.  A tile that is written whole
 // gathers in LDS and leaves as 16-byte stores; of others the new slots are
