@@ -624,6 +624,14 @@ def _ptr(b):
     return b if b is None or isinstance(b, int) else b.ptr
 
 
+def _ints(x, what: str) -> np.ndarray:
+    """x as an int32 vector; what does not fit is refused rather than wrapped or cut off."""
+    a = np.asarray(x).ravel()
+    if a.size and (a.dtype.kind not in "iu" or int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
+        raise ValueError(f"{what}: not a list of 32-bit integers")
+    return np.ascontiguousarray(a, np.int32)
+
+
 class KvCache:
     """Pages of keys and values that several sequences share (mlq_hip_kv_cache_*)."""
 
@@ -666,9 +674,7 @@ class KvPlan:
 
     def set(self, new_tokens, kv_len, pages, stream=None) -> None:
         """new_tokens and kv_len per sequence; pages: their page ids, one sequence's after the other's."""
-        n = np.ascontiguousarray(new_tokens, np.int32).ravel()
-        t = np.ascontiguousarray(kv_len, np.int32).ravel()
-        p = np.ascontiguousarray(pages, np.int32).ravel()
+        n, t, p = _ints(new_tokens, "new_tokens"), _ints(kv_len, "kv_len"), _ints(pages, "pages")
         if n.size != t.size:
             raise ValueError("one length per sequence")
         need = int(sum(-(-int(x) // self._page_size) for x in t if x > 0))

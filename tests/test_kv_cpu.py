@@ -56,6 +56,27 @@ def test_null_handles():
     assert lib.mlq_hip_kv_cache_destroy(None) == 0 and lib.mlq_hip_kv_plan_destroy(None) == 0
 
 
+def test_batches_hold_32_bit_integers():
+    """Lists that would be wrapped or cut off on their way into int arrays are refused."""
+    import numpy as np
+    import pytest
+
+    mlq_hip.load()
+    plan = mlq_hip.KvPlan.__new__(mlq_hip.KvPlan)
+    plan.h, plan._page_size = None, 64
+    for bad in ([1.0], [2 ** 31], np.array([2 ** 32 + 1]), [-2 ** 40], [True], ["1"]):
+        for args in ((bad, [1], [0]), ([1], bad, [0]), ([1], [1], bad)):
+            with pytest.raises(ValueError):
+                plan.set(*args)
+    with pytest.raises(ValueError, match="one length per sequence"):
+        plan.set([1, 1], [1], [0])
+    with pytest.raises(ValueError, match="2 page ids, the lengths need 1"):
+        plan.set([1], [64], [0, 1])
+    for good in ((np.array([1], np.uint8), np.array([65], np.int64), (0, 1)), ([], [], [])):
+        with pytest.raises(mlq_hip.MlqError, match="null plan"):  # past the lists' checks
+            plan.set(*good)
+
+
 def test_reference_quantizes_as_its_formulas(orc):
     """The values the device tests compare with, against the formats' formulas in 64 bits: a
     value is at most half a step (plus the scale's own rounding) from what is held for it."""
