@@ -33,9 +33,10 @@
 //
 // Bound: memory where the rows of a KV head are few and the contexts fill the chip (64
 // sequences of up to 4000 positions, Q8_0, 8 KV heads of 128, four query heads each: 75 us,
-// 4.7 TB/s of cache); with 4-bit codes half the bytes cost about as many instructions, some
-// 550 a tile, and issue bounds it (100 000 positions, Q4_0: 49 us, 2.3 TB/s, vector
-// instructions issue in half of the cycles). Short ones: launch, a chain of four trips to
+// 4.7 TB/s of cache); with 4-bit codes half the bytes take about as many instructions, some
+// 550 a tile, in one chain from loads over scores to weights, at two waves a SIMD (100 000
+// positions, Q4_0: 49 us, 2.3 TB/s, vector instructions issue in half of the cycles; 64 more
+// of them a tile cost 1 us).  Short contexts: launch, a chain of four trips to
 // memory (list, page, tile, parts) and the merge (700 positions 10.4 us).  Two workgroups a CU;
 // a third (fewer registers, Q4_0) was no faster, and parts beyond one round of them slower.
 #pragma once
@@ -162,6 +163,18 @@ __device__ __forceinline__ void split8(const float* v, h8_t* hi, h8_t* lo) {
     }
     *hi = join(h[0], h[1], h[2], h[3]);
     *lo = join(r[0], r[1], r[2], r[3]);
+}
+// The one part a lane has: hi where `low` is 0, lo where it is 1.
+__device__ __forceinline__ h8_t split8_one(const float* v, float low) {
+    typedef float f2_t __attribute__((ext_vector_type(2)));
+    h2_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const h2_t h = __builtin_convertvector((f2_t{v[2 * j], v[2 * j + 1]}), h2_t);
+        const f2_t rest{fmaf(-static_cast<float>(h.x), low, v[2 * j]), fmaf(-static_cast<float>(h.y), low, v[2 * j + 1])};
+        r[j] = __builtin_convertvector(rest, h2_t);
+    }
+    return join(r[0], r[1], r[2], r[3]);
 }
 // 1 / s for a power of two s from 2^-80 on; 0 for Inf.
 __device__ __forceinline__ float inverse_power(uint32_t s) {
@@ -476,8 +489,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                 h8_t hi, lo;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[j], scale_at(vs, 8 * b + j));
-                split8(v, &hi, &lo);
-                const h8_t ps = low ? lo : hi;
+                const h8_t ps = split8_one(v, low ? 1.0f : 0.0f);
                 if (QT == 3) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) om[b] += mul_or_zero(p[j], scale_at(vm, 8 * b + j));
