@@ -17,13 +17,14 @@
 //                 its minimum times the queries' sum.  f32 keys are split the same way,
 //                 relative to the block's power of two: three products.
 //   O^T += V^T P^T   the value scale d_jb belongs to key and block, so it goes into the
-//                 weights: P_b = p_j d_jb, split into hi + lo, times the codes.
+//                 weights: P_b = p_j d_jb f_b, split into hi + lo, times the codes.
 //
-// The running maximum m of a row is that of t_j + e_j, t the score in base 2 and 2^e_j
-// (nearly) the largest value scale of position j: then no P_b passes 2^15 and what is
-// large in the sum is what keeps all its digits, whatever the values' size; a value of
-// zero takes no digits from the others.  It moves only when t + e passes it by 6, so the
-// accumulators are seldom rescaled.  The sum of the weights is f32 in the same frame.
+// p_j = 2^(t_j - m), t the score in base 2 and m a running maximum of it, a whole number that moves
+// only when t passes it by 6; the sum of the weights is f32.  f_b, a power of two of every row and
+// block, takes the block's largest p_j d_jb so far to 2^9 .. 2^15: what is large in a block's sum keeps
+// all its digits in fp16 (2^-34 of it is lost of a small weight), whatever the values' size and
+// whatever other blocks of the head or positions with values of zero hold.  When m moves, f_b takes the
+// step up and the accumulators stay; they are rescaled when a weight passes 2^15.
 //
 // The hi parts are columns 0 .. 7 of the query operand and the lo parts columns 8 .. 15, of
 // the weights as well: one product where there would be two, the halves added at the end.
@@ -59,6 +60,8 @@ typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 64 * kKvWaves;
 constexpr int kCoherent = 16;   // sc1: through to / from the point of coherence
 constexpr float kSlack = 6.0f;  // a row's maximum moves when it is passed by this
+constexpr int kMostFrame = 126;  // f_b is at most 2^this: what is lost by it is below f32's range
+constexpr float kElementLift = 8192.0f;  // f32 elements are split times this over their block's power of two
 
 template <typename T>
 __device__ __forceinline__ T bits(uint32_t v) { return __builtin_bit_cast(T, v); }
@@ -180,6 +183,8 @@ __device__ __forceinline__ h8_t split8_one(const float* v, float low) {
 __device__ __forceinline__ float inverse_power(uint32_t s) {
     return bits<float>(static_cast<uint32_t>(max(static_cast<int>(0x7f000000u) - static_cast<int>(s), 0)));
 }
+// e of a positive v in [2^e, 2^(e+1)); 128 for Inf.
+__device__ __forceinline__ int exponent(float v) { return static_cast<int>(__builtin_bit_cast(uint32_t, v) >> 23) - 127; }
 
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
@@ -326,7 +331,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
         float qsum[NB], to_t;
         {
             float v[NB][8];
-            load_query<NB>(q + out_row, hd, g, a.scale, v, qsum, &to_t);
+            load_query<NB>(q + out_row, hd, g, a.scale * (QT == 0 ? 1.0f / kElementLift : 1.0f), v, qsum, &to_t);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 h8_t hi, lo;
@@ -339,11 +344,12 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
         const f4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
         f4_t o[1][2 * NB];
         float om[NB];  // Q4_1: this lane's part of the sum of weights times minima
+        int frame[NB];  // log2 f_b
         float m = -3.402823466e38f, l = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2 * NB; ++t) o[0][t] = zero;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) om[b] = 0.0f;
+        for (int b = 0; b < NB; ++b) om[b] = 0.0f, frame[b] = kMostFrame;
 
         // This wave's tiles: every fourth of the item's.
         const int end = it.first + it.count;
@@ -407,11 +413,11 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                     if (QT == 0) {
                         h8_t hi, lo;
                         float v[8];
-                        const float inv = inverse_power(kp[h][b]);
+                        const float inv = inverse_power(kp[h][b]) * kElementLift;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(bits<float>(kw[h][8 * b + j]), inv);
                         split8(v, &hi, &lo);
-                        acc = mfma(lo, qs[b], mfma(hi, qs[b], zero));
+                        acc = mfma(lo, qs[b], mfma(hi, qs[b], zero));  // (times kElementLift, taken back with to_t)
                     } else if (QT == 1) {
                         acc = mfma(codes8(kw[h][2 * b], kw[h][2 * b + 1], static_cast<_Float16>(128.0f)), qs[b], zero);
                     } else {
@@ -431,23 +437,6 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             if (more) load_keys(next);
 
             // Weights.
-            float e[8];  // log2 of a position's largest value scale, nearly, plus a constant
-#pragma unroll
-            for (int j = 0; j < 8; j += QT == 0 ? 1 : 2) {
-                if (QT == 0) {
-                    uint32_t top = vs[j];
-#pragma unroll
-                    for (int b = 1; b < NB; ++b) top = max(top, vs[8 * b + j]);
-                    e[j] = static_cast<float>(top) * 0x1p-23f;
-                } else {
-                    us2_t top = bits<us2_t>(vs[j / 2]);
-#pragma unroll
-                    for (int b = 1; b < NB; ++b) top = __builtin_elementwise_max(top, bits<us2_t>(vs[4 * b + j / 2]));
-                    e[j] = static_cast<float>(top.x) * 0x1p-10f;
-                    e[j + 1] = static_cast<float>(top.y) * 0x1p-10f;
-                }
-            }
-            constexpr float kBias = (QT == 0 ? 127.0f : 15.0f) + 8.0f;
             const bool full = first + kKvTile - 1 <= pos_lo &&
                               (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
             float top = -INFINITY;
@@ -461,24 +450,30 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                     const bool seen = key <= pos && (a.window == 0 || key > pos - a.window || key < a.sinks);
                     t[j] = seen ? t[j] : -INFINITY;
                 }
-                top = fmaxf(top, t[j] + e[j]);
+                top = fmaxf(top, t[j]);
             }
             top = max_quarters(top);
             if (__any(top > m + kSlack)) {
-                const float to = top > m + kSlack ? top : m;
-                float c;
-                l = down(l, m - to, &c);
-                m = to;
+                const bool moves = top > m + kSlack;
+                const float to = ceilf(top);
+                const int up = moves ? static_cast<int>(fminf(to - m, 1000.0f)) : 0;
+                m = moves ? to : m;
+                l = ldexpf(l, -up);
 #pragma unroll
-                for (int x = 0; x < 2 * NB; ++x) o[0][x] *= c;
+                for (int b = 0; b < NB; ++b) {
+                    const int over = max(frame[b] + up - kMostFrame, 0);
+                    frame[b] += up - over;
+                    om[b] = ldexpf(om[b], -up);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) om[b] *= c;
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[0][2 * b + x][i] = ldexpf(o[0][2 * b + x][i], -over);
+                }
             }
-            const float frame = m - kBias;
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[j] = __builtin_amdgcn_exp2f(t[j] - frame);
+                p[j] = __builtin_amdgcn_exp2f(t[j] - m);
                 l += p[j];
             }
 
@@ -489,6 +484,18 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                 h8_t hi, lo;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[j], scale_at(vs, 8 * b + j));
+                float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+                if (__any(ldexpf(most, frame[b]) > 0x1p15f)) {
+                    most = max_quarters(most);
+                    const int to = ldexpf(most, frame[b]) > 0x1p15f ? 9 - exponent(most) : frame[b];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[0][2 * b + x][i] = ldexpf(o[0][2 * b + x][i], to - frame[b]);
+                    frame[b] = to;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = ldexpf(v[j], frame[b]);
                 const h8_t ps = split8_one(v, low ? 1.0f : 0.0f);
                 if (QT == 3) {
 #pragma unroll
@@ -500,7 +507,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                     if (QT == 0) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            v[j] = mul_or_zero(bits<float>(vw[16 * b + 8 * x + j]), inverse_power(vs[8 * b + j]));
+                            v[j] = mul_or_zero(bits<float>(vw[16 * b + 8 * x + j]), inverse_power(vs[8 * b + j]) * kElementLift);
                         }
                         split8(v, &hi, &lo);
                         acc = mfma(lo, ps, mfma(hi, ps, acc));
@@ -516,7 +523,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             if (more) load_values(next);
         }
 
-        // The lanes' sums, the halves and the minima's part together.
+        // The lanes' sums, the halves and the minima's part together, out of the blocks' frames.
         l = sum_quarters(l);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -526,7 +533,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float y = o[0][2 * b + x][i];
-                    o[0][2 * b + x][i] = y + other_half(y) + add;
+                    o[0][2 * b + x][i] = ldexpf(y + other_half(y), -frame[b] - (QT == 0 ? 13 : 0)) + add;
                 }
         }
         // The four waves' states into wave 0, in a fixed order.

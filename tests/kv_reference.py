@@ -92,3 +92,38 @@ class Batch:
             out.append(np.arange(at + t - n, at + t))
             at += t
         return np.concatenate(out + [np.zeros(0, int)]).astype(int)
+
+
+def attention_by_block(q, k, v, window=0, sinks=0, scale=0.0):
+    """As `attention`, with a bound of its own for each of a head's blocks of 32 dimensions: (out, bound),
+    both [n, heads, hd].
+
+    A block's results are weighted sums of that block's values, so f32 arithmetic is off by what it
+    loses of W = sum_j p_j max|v_j| over the block, whatever other blocks hold and however small the weights
+    of the positions that hold its values.  A probability is off by the 2 `each` of `attention`, and by three
+    roundings (in base 2) of the values' exponents where these go into the scores; an element and a weight by
+    3 2^-22 for their parts; a sum over `length` positions by as many roundings of it (weights too small for
+    fp16 beside a block's largest one are lost in there: 2^-34 of that each, 2^-24 where the positions'
+    values differ by 2^10), and 96 more for parts and merges."""
+    n, heads, hd = q.shape
+    length, kv = k.shape[:2]
+    factor = scale or 1.0 / np.sqrt(hd)
+    see = visible(n, length, window, sinks)
+    out, bound = np.empty(q.shape, np.float64), np.empty(q.shape, np.float64)
+    q, k, v = (np.asarray(t, np.float64) for t in (q, k, v))
+    starts = np.arange(0, hd, 32)
+    for h in range(heads):
+        kh, vh = k[:, h // (heads // kv)], v[:, h // (heads // kv)]
+        s = np.where(see, factor * (q[:, h] @ kh.T), -np.inf)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        out[:, h] = p @ vh
+        size = np.where(see, abs(factor) * (np.abs(q[:, h]) @ np.abs(kh).T), 0).max(-1)
+        reach = np.where(see, np.abs(s), 0).max(-1)
+        top = np.maximum.reduceat(np.abs(vh), starts, axis=1)  # [length, blocks]
+        largest = top.max(-1)
+        log = np.abs(np.log2(largest[largest > 0])).max(initial=0.0)
+        each = size * (3 * 2.0 ** -22 + (hd + 16) * 2.0 ** -24) + 6 * reach * 2.0 ** -24 + 3 * log * 2.0 ** -24 + 2.0 ** -22
+        rel = 2 * each + 3 * 2.0 ** -22 + (length + 96) * 2.0 ** -24
+        bound[:, h] = np.repeat((p @ top) * rel[:, None], 32, axis=1)[:, :hd]
+    return out, bound

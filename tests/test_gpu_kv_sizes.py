@@ -1,0 +1,69 @@
+"""Attention over the paged cache where sizes differ inside a head: every block of 32 dimensions is
+held to a bound of its own (kv_reference.attention_by_block), whatever the blocks beside it hold."""
+
+import numpy as np
+import pytest
+
+from kv_reference import QT, attention_by_block
+from test_gpu_kv import Case, say
+
+pytestmark = pytest.mark.gpu
+
+
+def check(c, dims=slice(None), heads=slice(None)):
+    """The output against the 64-bit result, in `dims` of `heads`."""
+    got = c.run()
+    at = qat = 0
+    for n, t in c.batch.lens:
+        k, v = (x[at:at + t] for x in c.held)
+        want, bound = attention_by_block(c.q[qat:qat + n], k, v, c.window, c.sinks, c.scale)
+        err = np.abs(got[qat:qat + n] - want)
+        ok = (err <= bound)[:, heads, dims]
+        assert ok.all(), (n, t, float((err / np.maximum(bound, 1e-300))[:, heads, dims].max()))
+        at, qat = at + t, qat + n
+    return got
+
+
+def spread(rng, positions, kv, hd, sizes):
+    """Normal values whose blocks of 32 are of `sizes` in turn."""
+    by = np.repeat(np.resize(np.asarray(sizes, np.float64), -(-hd // 32)), 32)[:hd]
+    return (rng.standard_normal((positions, kv, hd)) * by).astype(np.float32)
+
+
+FEW = [[(3, 60)], [(1, 90), (2, 40)], [(1, 5000)]]
+VALUE_SIZES = [("f32", (1.0, 1e4)), ("f32", (1.0, 1e8)), ("f32", (1e20, 1e-3)), ("f32", (1e-20, 1e20)),
+               ("q8_0", (1.0, 2e-4)), ("q8_0", (1e-3, 1e3)), ("q4_0", (2e-3, 1e4)), ("q4_1", (1e-3, 1e3))]
+
+
+@pytest.mark.parametrize("kind,sizes", VALUE_SIZES)
+@pytest.mark.parametrize("lens", FEW)
+def test_few_rows_value_blocks_of_different_size(hip, orc, lens, kind, sizes):
+    say("few rows, value blocks", kind, sizes, lens)
+    for hd in (64, 80, 160):
+        rng = np.random.default_rng(hd)
+        c = Case(hip, orc, kind, lens, 4, 2, hd, values=spread(rng, sum(t for _, t in lens), 2, hd, sizes))
+        check(c)
+
+
+@pytest.mark.parametrize("kind,size", [("f32", 1e8), ("f32", 1e19), ("q8_0", 1e4), ("q4_0", 1e4), ("q4_1", 1e4)])
+def test_few_rows_one_position_with_a_large_block(hip, orc, kind, size):
+    """One position among sixty holds a block that is large; the other block of the head is as it was."""
+    rng = np.random.default_rng(1)
+    v = rng.standard_normal((60, 2, 64)).astype(np.float32)
+    v[23, :, 32:] *= np.float32(size)
+    check(Case(hip, orc, kind, [(3, 60)], 4, 2, 64, values=v))
+
+
+@pytest.mark.parametrize("kind,bad", [("f32", np.inf), ("f32", np.nan), ("f32", 3e30), ("q8_0", 1e30), ("q4_0", -np.inf)])
+def test_few_rows_healthy_block_beside_a_bad_one(hip, orc, kind, bad):
+    """A value block that is not finite is NaN for what sees it, the head's other block what it is without it."""
+    rng = np.random.default_rng(2)
+    v = rng.standard_normal((60, 2, 64)).astype(np.float32)
+    c = Case(hip, orc, kind, [(3, 60)], 4, 2, 64, values=v.copy())
+    v[20, 0, 40] = bad
+    with np.errstate(all="ignore"):
+        worse = Case(hip, orc, kind, [(3, 60)], 4, 2, 64, values=v, keys=c.k)
+    worse.held = c.held
+    got = check(worse, dims=slice(0, 32))
+    check(worse, heads=slice(2, 4))
+    assert np.isnan(got[:, :2, 32:]).all()
