@@ -30,7 +30,8 @@
 // the weights as well: one product where there would be two, the halves added at the end.
 //
 // What a row does not see gets weight 0, and 0 times a scale that is Inf or NaN is 0
-// (v_mul_legacy_f32); codes are finite always.
+// (v_mul_legacy_f32); codes are finite always.  A weight that is not 0 times such a scale (or minimum)
+// ends as NaN; one that a row sees but that is below f32's range is looked for (`spoilt`).
 //
 // Bound: memory where the rows of a KV head are few and the contexts fill the chip (64
 // sequences of up to 4000 positions, Q8_0, 8 KV heads of 128, four query heads each: 75 us,
@@ -61,6 +62,7 @@ constexpr int kThreads = 64 * kKvWaves;
 constexpr int kCoherent = 16;   // sc1: through to / from the point of coherence
 constexpr float kSlack = 6.0f;  // a row's maximum moves when it is passed by this
 constexpr int kMostFrame = 126;  // f_b is at most 2^this: what is lost by it is below f32's range
+constexpr int kFirstUp = 1000;   // steps of a maximum beyond this are as good as infinite, the first one is
 constexpr float kElementLift = 8192.0f;  // f32 elements are split times this over their block's power of two
 
 template <typename T>
@@ -345,11 +347,12 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
         f4_t o[1][2 * NB];
         float om[NB];  // Q4_1: this lane's part of the sum of weights times minima
         int frame[NB];  // log2 f_b
+        uint32_t spoilt = 0;  // bit b: this lane's part of the row sees a block that is not finite with a weight of 0
         float m = -3.402823466e38f, l = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2 * NB; ++t) o[0][t] = zero;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) om[b] = 0.0f, frame[b] = kMostFrame;
+        for (int b = 0; b < NB; ++b) om[b] = 0.0f, frame[b] = kMostFrame - kFirstUp;
 
         // This wave's tiles: every fourth of the item's.
         const int end = it.first + it.count;
@@ -439,35 +442,43 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             // Weights.
             const bool full = first + kKvTile - 1 <= pos_lo &&
                               (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
+            auto seen = [&](int j) {
+                const int key = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                return key <= pos && (a.window == 0 || key > pos - a.window || key < a.sinks);
+            };
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 t[j] = (t[j] + other_half(t[j])) * to_t;
                 // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
                 if (QT >= 2) t[j] = fmaf(t[j], 0.0f, t[j]);
-                if (!full) {
-                    const int key = first + (j >> 2) * 16 + 4 * g + (j & 3);
-                    const bool seen = key <= pos && (a.window == 0 || key > pos - a.window || key < a.sinks);
-                    t[j] = seen ? t[j] : -INFINITY;
-                }
+                if (!full) t[j] = seen(j) ? t[j] : -INFINITY;
                 top = fmaxf(top, t[j]);
             }
             top = max_quarters(top);
             if (__any(top > m + kSlack)) {
                 const bool moves = top > m + kSlack;
                 const float to = ceilf(top);
-                const int up = moves ? static_cast<int>(fminf(to - m, 1000.0f)) : 0;
+                const int up = moves ? static_cast<int>(fminf(to - m, static_cast<float>(kFirstUp))) : 0;
                 m = moves ? to : m;
                 l = ldexpf(l, -up);
+                int over = 0;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const int over = max(frame[b] + up - kMostFrame, 0);
-                    frame[b] += up - over;
-                    om[b] = ldexpf(om[b], -up);
+                    frame[b] += up;
+                    over = max(over, frame[b] - kMostFrame);
+                    if (QT == 3) om[b] = ldexpf(om[b], -up);
+                }
+                if (__builtin_expect(__any(over > 0), 0)) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
+                    for (int b = 0; b < NB; ++b) {
+                        const int less = max(frame[b] - kMostFrame, 0);
+                        frame[b] -= less;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[0][2 * b + x][i] = ldexpf(o[0][2 * b + x][i], -over);
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[0][2 * b + x][i] = ldexpf(o[0][2 * b + x][i], -less);
+                    }
                 }
             }
             float p[8];
@@ -475,6 +486,38 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             for (int j = 0; j < 8; ++j) {
                 p[j] = __builtin_amdgcn_exp2f(t[j] - m);
                 l += p[j];
+            }
+            if (__builtin_expect(__any(fminf(fminf(fminf(p[0], p[1]), fminf(p[2], p[3])), fminf(fminf(p[4], p[5]), fminf(p[6], p[7]))) == 0.0f), 0)) {
+                // (the largest of all scales and minima tells whether there is anything to look for)
+                uint32_t any_bad;
+                if (QT == 0) {
+                    uint32_t x = vs[0];
+#pragma unroll
+                    for (int i = 1; i < VS; ++i) x = max(x, vs[i]);
+                    any_bad = x >= 0x7f800000u;
+                } else {
+                    us2_t x{0, 0};
+#pragma unroll
+                    for (int i = 0; i < VS; ++i) {
+                        x = __builtin_elementwise_max(x, bits<us2_t>(vs[i]));
+                        if (QT == 3) x = __builtin_elementwise_max(x, bits<us2_t>(vm[QT == 3 ? i : 0] & 0x7fff7fffu));
+                    }
+                    any_bad = max(x.x, x.y) >= 0x7c00;
+                }
+                if (__builtin_expect(__any(any_bad != 0), 0)) {
+                    auto bad_at = [&](const uint32_t* s, int i) {
+                        return QT == 0 ? s[i] >= 0x7f800000u : ((s[i / 2] >> (i % 2 * 16)) & 0x7fffu) >= 0x7c00u;
+                    };
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bool lost = p[j] == 0.0f && seen(j);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const bool bad = bad_at(vs, 8 * b + j) || (QT == 3 && bad_at(vm, QT == 3 ? 8 * b + j : 0));
+                            spoilt |= (lost && bad ? 1u : 0u) << b;
+                        }
+                    }
+                }
             }
 
             // Values.
@@ -527,7 +570,9 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
         l = sum_quarters(l);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const float add = QT == 3 ? sum_quarters(om[b]) : 0.0f;
+            float add = QT == 3 ? sum_quarters(om[b]) : 0.0f;
+            add = fmaf(add, 0.0f, add);  // an infinite minimum: NaN
+            add += sum_quarters((spoilt >> b) & 1u ? NAN : 0.0f);
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll

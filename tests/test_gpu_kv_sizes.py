@@ -67,3 +67,38 @@ def test_few_rows_healthy_block_beside_a_bad_one(hip, orc, kind, bad):
     got = check(worse, dims=slice(0, 32))
     check(worse, heads=slice(2, 4))
     assert np.isnan(got[:, :2, 32:]).all()
+
+
+@pytest.mark.parametrize("new", [3, 70])
+@pytest.mark.parametrize("size", [1e6, -1e6])
+def test_infinite_minimum_counts_as_nan(hip, orc, new, size):
+    """A Q4_1 block of one large constant has a finite scale (0) and an infinite minimum: NaN for what sees it,
+    whichever kernel the number of rows chooses."""
+    rng = np.random.default_rng(3)
+    v = rng.standard_normal((100, 2, 64)).astype(np.float32)
+    c = Case(hip, orc, "q4_1", [(new, 100)], 4, 2, 64, values=v.copy())
+    v[10, 1, 32:] = size
+    worse = Case(hip, orc, "q4_1", [(new, 100)], 4, 2, 64, values=v, keys=c.k)
+    worse.held = c.held
+    got = check(worse, dims=slice(0, 32))
+    check(worse, heads=slice(0, 2))
+    assert np.isnan(got[:, 2:, 32:]).all()
+
+
+@pytest.mark.parametrize("new", [3, 70])
+@pytest.mark.parametrize("kind", list(QT))
+def test_bad_block_counts_however_small_its_weight(hip, orc, kind, new):
+    """A seen value block that is not finite is NaN for a token whose weight for it is below f32's range, and
+    nothing to the tokens before it."""
+    rng = np.random.default_rng(4)
+    k, v = (rng.standard_normal((100, 2, 64)).astype(np.float32) for _ in range(2))
+    k[98] = -40.0
+    c = Case(hip, orc, kind, [(new, 100)], 4, 2, 64, keys=k, values=v.copy(), scale=1.0)
+    c.q[:] = rng.uniform(1, 2, c.q.shape).astype(np.float32)
+    v[98, 0, :32] = -1e30
+    with np.errstate(all="ignore"):
+        worse = Case(hip, orc, kind, [(new, 100)], 4, 2, 64, keys=k, values=v, scale=1.0)
+    worse.q, worse.held = c.q, c.held
+    got = check(worse, dims=slice(32, 64))
+    check(worse, heads=slice(2, 4))
+    assert np.isnan(got[-2:, :2, :32]).all() and np.isfinite(got[:-2]).all()
