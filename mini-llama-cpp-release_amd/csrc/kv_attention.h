@@ -11,7 +11,7 @@
 // in v_mfma_f32_16x16x32_f16 with operands that come from memory as they lie there:
 //
 //   S^T = K Q^T   per block b of 32 elements: the codes are whole numbers (exact in
-//                 fp16), the queries pairs of fp16 parts hi + lo relative to the row's
+//                 fp16), the queries pairs of fp16 parts hi + lo relative to the block's
 //                 largest (2^-22 of it is lost), so a product is exact and the sum
 //                 f32; times the block's scale it goes into the score.  A Q4_1 block adds
 //                 its minimum times the queries' sum.  f32 keys are split the same way,
@@ -190,11 +190,12 @@ __device__ __forceinline__ int exponent(float v) { return static_cast<int>(__bui
 
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// A lane's part of a query row (elements 8 g .. of every block), relative to the row's
-// largest, which becomes 2^13 .. 2^14; the blocks' sums; what takes a score to base 2.
-template <int NB>
+// A lane's part of a query row (elements 8 g .. of every block), relative to the row's largest (EACH: to
+// the block's), which becomes 2^13 .. 2^14; the blocks' sums; what takes a score (EACH: a block's part of
+// it) to base 2.
+template <int NB, bool EACH>
 __device__ __forceinline__ void load_query(const float* q, int hd, int g, float scale, float (*v)[8], float* sum, float* to_t) {
-    float top = 0.0f;
+    float tops[NB], top = 0.0f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int e = 32 * b + 8 * g;
@@ -205,19 +206,21 @@ __device__ __forceinline__ void load_query(const float* q, int hd, int g, float 
         }
         v[b][0] = x.x, v[b][1] = x.y, v[b][2] = x.z, v[b][3] = x.w;
         v[b][4] = y.x, v[b][5] = y.y, v[b][6] = y.z, v[b][7] = y.w;
+        tops[b] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[b][j]));
+        for (int j = 0; j < 8; ++j) tops[b] = fmaxf(tops[b], fabsf(v[b][j]));
+        top = fmaxf(top, tops[b]);
     }
-    top = max_quarters(top);
-    // exponent, kept where 2^(13 - e) is finite and to_t is 2^-112 or more (a row of zeros or nearly: its
-    // scores are then as near to 0 as to_t says, and what is taken over to_t stays finite)
-    const int log_scale = static_cast<int>(__builtin_bit_cast(uint32_t, fabsf(scale)) >> 23) - 127;
-    const int e = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, max(-110, -99 - log_scale)), 127);
-    // a negative scale turns the queries; a score's factor is positive, so that -inf stays -inf
-    const float up = ldexpf(scale < 0.0f ? -1.0f : 1.0f, 13 - e);
-    *to_t = ldexpf(fabsf(scale), e - 13);
+    if (!EACH) top = max_quarters(top);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+        // exponent, kept where 2^(13 - e) is finite and to_t is 2^-112 or more (a row of zeros or nearly: its
+        // scores are then as near to 0 as to_t says, and what is taken over to_t stays finite)
+        const int log_scale = exponent(fabsf(scale));
+        const int e = min(max(exponent(EACH ? max_quarters(tops[b]) : top), max(-110, -99 - log_scale)), 127);
+        // a negative scale turns the queries; a score's factor is positive, so that -inf stays -inf
+        const float up = ldexpf(scale < 0.0f ? -1.0f : 1.0f, 13 - e);
+        if (b == 0 || EACH) to_t[b] = ldexpf(fabsf(scale), e - 13);
         sum[b] = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -330,16 +333,16 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             (static_cast<size_t>(it.token0 + row / a.group) * heads + head * a.group + row % a.group) * hd;
 
         h8_t qs[NB];
-        float qsum[NB], to_t;
+        float qsum[NB], to_t[NB];
         {
             float v[NB][8];
-            load_query<NB>(q + out_row, hd, g, a.scale * (QT == 0 ? 1.0f / kElementLift : 1.0f), v, qsum, &to_t);
+            load_query<NB, true>(q + out_row, hd, g, a.scale * (QT == 0 ? 1.0f / kElementLift : 1.0f), v, qsum, to_t);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 h8_t hi, lo;
                 split8(v[b], &hi, &lo);
                 qs[b] = low ? lo : hi;
-                if (QT == 3) qsum[b] = low ? 0.0f : sum_quarters(qsum[b]);
+                if (QT == 3) qsum[b] = low ? 0.0f : sum_quarters(qsum[b]) * to_t[b];
             }
         }
 
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(bits<float>(kw[h][8 * b + j]), inv);
                         split8(v, &hi, &lo);
-                        acc = mfma(lo, qs[b], mfma(hi, qs[b], zero));  // (times kElementLift, taken back with to_t)
+                        acc = mfma(lo, qs[b], mfma(hi, qs[b], zero));  // (times kElementLift, which to_t takes back)
                     } else if (QT == 1) {
                         acc = mfma(codes8(kw[h][2 * b], kw[h][2 * b + 1], static_cast<_Float16>(128.0f)), qs[b], zero);
                     } else {
@@ -428,6 +431,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                         acc = mfma(codes8(x & 0x0f0f0f0fu, (x >> 4) & 0x0f0f0f0fu, static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f)),
                                    qs[b], zero);
                     }
+                    acc *= to_t[b];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         s[i] = fmaf(scale_at(ks[h], 4 * b + i), acc[i], s[i]);
@@ -449,7 +453,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                t[j] = (t[j] + other_half(t[j])) * to_t;
+                t[j] += other_half(t[j]);
                 // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
                 if (QT >= 2) t[j] = fmaf(t[j], 0.0f, t[j]);
                 if (!full) t[j] = seen(j) ? t[j] : -INFINITY;

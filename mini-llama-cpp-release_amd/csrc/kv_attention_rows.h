@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         for (int u = 0; u < NQ; ++u) {
             pos[u] = start + token_of(u);
             float v[NB][8], sum[NB];
-            load_query<NB>(q + element_of(u), hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
+            load_query<NB, false>(q + element_of(u), hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) split8(v[b], &qh[u][b], &ql[u][b]);
         }

@@ -102,3 +102,19 @@ def test_bad_block_counts_however_small_its_weight(hip, orc, kind, new):
     got = check(worse, dims=slice(32, 64))
     check(worse, heads=slice(2, 4))
     assert np.isnan(got[-2:, :2, :32]).all() and np.isfinite(got[:-2]).all()
+
+
+@pytest.mark.parametrize("kind,sizes", [("f32", (1.0, 1e-5)), ("f32", (1e8, 1.0)), ("f32", (1e18, 1e-18)), ("f32", (1.0, 0.0)),
+                                        ("q8_0", (1e3, 1e-3)), ("q4_0", (1e4, 1e-3)), ("q4_1", (1e-3, 1e3))])
+@pytest.mark.parametrize("lens", FEW)
+def test_few_rows_query_blocks_of_different_size(hip, orc, lens, kind, sizes):
+    """Small query blocks beside large ones, over keys whose blocks make up for it: both count in the score."""
+    say("few rows, query blocks", kind, sizes, lens)
+    rng = np.random.default_rng(5)
+    for hd in (64, 80, 160):
+        inverse = [1 / s if s else 1.0 for s in sizes]
+        keys = spread(rng, sum(t for _, t in lens), 2, hd, inverse)
+        c = Case(hip, orc, kind, lens, 4, 2, hd, keys=keys)
+        c.q[::2] = spread(rng, len(c.q[::2]), 4, hd, sizes)
+        c.q[1::2] = spread(rng, len(c.q[1::2]), 4, hd, [min(1.0, s) for s in sizes])
+        check(c)
