@@ -193,8 +193,9 @@ __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) { return __builtin_
 // A lane's part of a query row (elements 8 g .. of every block), relative to the row's largest (EACH: to
 // the block's), which becomes 2^13 .. 2^14; the blocks' sums; what takes a score (EACH: a block's part of
 // it) to base 2.
+// Whether a block of the row is far below the largest (2^-13 of it, and not zeros).
 template <int NB, bool EACH>
-__device__ __forceinline__ void load_query(const float* q, int hd, int g, float scale, float (*v)[8], float* sum, float* to_t) {
+__device__ __forceinline__ bool load_query(const float* q, int hd, int g, float scale, float (*v)[8], float* sum, float* to_t) {
     float tops[NB], top = 0.0f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -212,8 +213,13 @@ __device__ __forceinline__ void load_query(const float* q, int hd, int g, float 
         top = fmaxf(top, tops[b]);
     }
     if (!EACH) top = max_quarters(top);
+    bool apart = false;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+        if (!EACH) {
+            tops[b] = max_quarters(tops[b]);
+            apart = apart || (tops[b] > 0.0f && exponent(tops[b]) < exponent(top) - 13);
+        }
         // exponent, kept where 2^(13 - e) is finite and to_t is 2^-112 or more (a row of zeros or nearly: its
         // scores are then as near to 0 as to_t says, and what is taken over to_t stays finite)
         const int log_scale = exponent(fabsf(scale));
@@ -228,6 +234,7 @@ __device__ __forceinline__ void load_query(const float* q, int hd, int g, float 
             sum[b] += v[b][j];
         }
     }
+    return apart;
 }
 
 // The state of a wave's rows (accumulators, running maximum, sum) in memory, for parts

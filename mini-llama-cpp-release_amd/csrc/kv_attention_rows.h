@@ -47,10 +47,203 @@ struct TileScales {
 };
 constexpr uint32_t kBad = 1, kFar = 2;
 constexpr float kLift = 256.0f;  // operands lie in LDS times this
+constexpr float kFloor = 0x1p-80f;  // f32: the power of two of a block of zeros, or of elements this small
 
 template <int QT, int NB>
 constexpr int rows_lds_bytes() {
     return 2 * 8 * NB * 1024 + 3 * static_cast<int>(sizeof(TileScales<QT, NB>));
+}
+
+// Element `i` of a word of codes, times its scale.
+template <int QT>
+__device__ __forceinline__ float element(uint32_t w, int i, float d, float add) {
+    const float c = static_cast<float>(static_cast<int>((w >> (8 * i)) & (QT == 1 ? 0xffu : 0xfu)) - (QT == 1 ? 128 : QT == 2 ? 8 : 0));
+    return QT == 3 ? fmaf(c, d, add) : c * d;
+}
+
+// The rows of one wave of an item (ROWS from row_base on), in plain f32: what a wave of attention_rows_kernel does
+// where blocks of a position or of a query differ too much in size for its operands.  Four rows at a time; a lane takes one
+// position's half of every block for the scores, every 64th dimension for the values.  Five times as slow, in few
+// registers: the kernel's own are not touched by it.  lds: the wave's, 4 (32 NB + 32) floats.
+template <int QT, int NB, int NQ>
+__device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnItem& it, int head, int row_base, int wave, int lane,
+                                           const float* __restrict__ q, float* __restrict__ out, float* lds) {
+    using F = KvForm<QT>;
+    constexpr int KL = F::key_lane(NB), VL = F::value_lane(NB), HD = 32 * NB, DIMS = (HD + 63) / 64;
+    constexpr int QUADS = NQ * 2 * NB, STATE = (QUADS * 4 + 2 * NQ) * 64;
+    const int hd = a.kv.head_dim, n_kv = a.kv.n_kv, heads = n_kv * a.group;
+    const int rows = it.new_tokens * a.group, start = it.len - it.new_tokens;
+    const int page_tiles = a.kv.page_tiles, tile_shift = __builtin_ctz(page_tiles);
+    // (opaque here, or what depends on it would be computed ahead of the kernel's loop, in registers that it needs)
+    asm volatile("" : "+v"(lane));
+    float* const weights = lds + 4 * HD;  // [position][row]
+    auto over_lanes = [](float x, auto two) {  // of 32: both halves of the wave have the same
+#pragma unroll
+        for (int s = 1; s < 32; s *= 2) x = two(x, __shfl_xor(x, s));
+        return x;
+    };
+    auto larger = [](float x, float y) { return fmaxf(x, y); };
+    auto plus = [](float x, float y) { return x + y; };
+    auto in_order = [] {  // what the wave has written to LDS is there for all its lanes
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto scale_of = [](const uint8_t* plane, int i) {
+        return QT == 0 ? reinterpret_cast<const float*>(plane)[i] : half_value(reinterpret_cast<const uint16_t*>(plane)[i]);
+    };
+#pragma unroll 1
+    for (int r = 0; r < 16 * NQ && row_base + r < rows; r += 4) {
+        // Queries over the power of two of the row's largest; a score's factor to base 2.
+        float to_t[4], m[4], l[4], acc[DIMS][4];
+        int pos[4];
+        size_t at[4];
+        in_order();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int row = min(row_base + r + k, rows - 1);
+            pos[k] = start + row / a.group;
+            at[k] = (static_cast<size_t>(it.token0 + row / a.group) * heads + head * a.group + row % a.group) * hd;
+            float x[DIMS], top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DIMS; ++c) {
+                const int e = lane + 64 * c;
+                x[c] = e < hd ? q[at[k] + e] : 0.0f;
+                top = fmaxf(top, fabsf(x[c]));
+            }
+            top = over_lanes(top, larger);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const int e = min(max(exponent(top), -120), 127);
+            to_t[k] = ldexpf(a.scale, e);
+#pragma unroll
+            for (int c = 0; c < DIMS; ++c) {
+                if (lane + 64 * c < HD) lds[k * HD + lane + 64 * c] = ldexpf(x[c], -e);
+                acc[c][k] = 0.0f;
+            }
+            m[k] = -3.402823466e38f;
+            l[k] = 0.0f;
+        }
+        in_order();
+#pragma unroll 1
+        for (int i = it.first; i < it.first + it.count; ++i) {
+            const int t = i < it.sinks ? i : i + it.shift;
+            const int page = uniform(&a.lists.pages[it.page0 + (t >> tile_shift)].page);
+            const uint8_t* const tile =
+                a.kv.base + ((static_cast<size_t>(page) * n_kv + head) * page_tiles + (t & (page_tiles - 1))) * F::tile(NB);
+            // Scores: this lane's position, half of every block's elements.
+            const int slot = lane & 31, key = t * kKvTile + slot;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            bool bad_value = false;
+#pragma unroll 1
+            for (int x = 0; x < 2 * NB; ++x) {
+                const int b = x >> 1, g = (lane >> 5) * 2 + (x & 1);
+                const uint8_t* const from = tile + (slot >> 4) * 64 * KL;
+                const int of_lane = 16 * g + (slot & 15);
+                float d = scale_of(tile + F::codes(NB), F::key_scale(NB, slot, b)), y[8];
+                if (QT == 0) {
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const f4_t four = *reinterpret_cast<const f4_t*>(from + F::at(KL, of_lane, b * 32 + 16 * z));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[4 * z + e] = d < INFINITY ? four[e] : NAN;
+                    }
+                } else {
+                    const float add = QT == 3 ? scale_of(tile + F::codes(NB) + F::plane(NB), F::key_scale(NB, slot, b)) : 0.0f;
+                    const uint8_t* const p = from + F::at(KL, of_lane, b * F::kElemBits);
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const uint32_t w = QT == 1 ? reinterpret_cast<const uint32_t*>(p)[z] : *reinterpret_cast<const uint32_t*>(p) >> (4 * z);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[4 * z + e] = element<QT>(w, e, d, add);
+                    }
+                }
+                d = scale_of(tile + F::half(NB) + F::codes(NB), F::value_scale(NB, slot, b));
+                bad_value = bad_value || !(d < INFINITY);
+                if (QT == 3) {
+                    d = scale_of(tile + F::half(NB) + F::codes(NB) + F::plane(NB), F::value_scale(NB, slot, b));
+                    bad_value = bad_value || !(fabsf(d) < INFINITY);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f4_t* const of_row = reinterpret_cast<const f4_t*>(lds + k * HD + 32 * b + 8 * g);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[k] = fmaf(of_row[e >> 2][e & 3], y[e], s[k]);
+                }
+            }
+            // Weights.
+            f4_t p;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float x = (s[k] + __shfl_xor(s[k], 32)) * to_t[k];
+                x = fmaf(x, 0.0f, x);  // an infinite scale: NaN
+                const bool seen = key <= pos[k] && (a.window == 0 || key > pos[k] - a.window || key < a.sinks);
+                x = seen ? x : -INFINITY;
+                const float to = fmaxf(m[k], over_lanes(x, larger)), c = __builtin_amdgcn_exp2f(m[k] - to);
+                m[k] = to;
+                p[k] = __builtin_amdgcn_exp2f(x - to);
+                l[k] = l[k] * c + over_lanes(p[k], plus);
+                // (a block that is not finite counts however small its weight)
+                if (bad_value && seen) p[k] = fmaxf(p[k], 0x1p-126f);
+#pragma unroll
+                for (int z = 0; z < DIMS; ++z) acc[z][k] *= c;
+            }
+            in_order();
+            if (lane < 32) *reinterpret_cast<f4_t*>(weights + 4 * slot) = p;
+            in_order();
+            // Values: four positions of a dimension share a word.
+#pragma unroll
+            for (int c = 0; c < DIMS; ++c) {
+                const int dim = min(lane + 64 * c, HD - 1), b = dim >> 5, side = (dim >> 4) & 1;
+#pragma unroll 1
+                for (int quad = 0; quad < 8; ++quad) {
+                    const uint8_t* const from = tile + F::half(NB);
+                    const int of_lane = 16 * (quad & 3) + (dim & 15), x = side * 8 + (quad >> 2) * 4;
+                    const int first_scale = F::value_scale(NB, 4 * quad, b);
+                    f4_t y;
+                    uint32_t w = 0;
+                    if (QT == 0) y = *reinterpret_cast<const f4_t*>(from + F::at(VL, of_lane, (b * 16 + x) * 4));
+                    else if (QT == 1) w = *reinterpret_cast<const uint32_t*>(from + F::at(VL, of_lane, b * 16 + x));
+                    else w = *reinterpret_cast<const uint32_t*>(from + F::at(VL, of_lane, b * 8 + (x & 7))) >> (4 * side);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float d = scale_of(from + F::codes(NB), first_scale + e);
+                        const float add = QT == 3 ? scale_of(from + F::codes(NB) + F::plane(NB), first_scale + e) : 0.0f;
+                        float v = QT == 0 ? y[e] : element<QT>(w, e, d, add);
+                        if (!(d < INFINITY) || !(fabsf(add) < INFINITY)) v = NAN;
+                        const f4_t of_rows = *reinterpret_cast<const f4_t*>(weights + 4 * (4 * quad + e));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[c][k] += mul_or_zero(of_rows[k], v);
+                    }
+                }
+            }
+        }
+        // The output, or the state as leave_state lays it out, in the units of the others (weights times 2^8, values
+        // times kLift).
+        const __amdgpu_buffer_rsrc_t rs =
+            state_rsrc(a.partial, (static_cast<size_t>(it.slot + it.split) * n_kv + head) * kKvWaves + wave, STATE);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (row_base + r + k >= rows) continue;
+            const int u = (r + k) >> 4, column = (r + k) & 15;
+#pragma unroll
+            for (int c = 0; c < DIMS; ++c) {
+                const int dim = lane + 64 * c;
+                if (it.nsplit == 1) {
+                    if (dim < hd) out[at[k] + dim] = acc[c][k] / l[k];
+                } else if (dim < HD) {
+                    const int of_lane = column + 16 * ((dim & 15) >> 2);
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, acc[c][k] * kLift), rs,
+                                                          ((u * 2 * NB + (dim >> 4)) * 64 + of_lane) * 16 + (dim & 3) * 4, 0, kCoherent);
+                }
+            }
+            if (it.nsplit > 1 && lane < 4) {
+                const int of_lane = column + 16 * lane;
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[k] + 8.0f), rs,
+                                                      (QUADS * 256 + 2 * u * 64 + of_lane) * 4, 0, kCoherent);
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[k]), rs,
+                                                      (QUADS * 256 + (2 * u + 1) * 64 + of_lane) * 4, 0, kCoherent);
+            }
+        }
+    }
 }
 
 template <int QT, int NB, int NQ>
@@ -70,7 +263,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
     h8_t* const operands = reinterpret_cast<h8_t*>(lds);
     Scales* const scales = reinterpret_cast<Scales*>(lds + 2 * 8 * NB * 1024);
     auto operand = [&](int buffer, int part, int f) { return operands + ((buffer * 4 + part) * FRAGS + f) * 64; };
-    __shared__ unsigned last;
+    __shared__ unsigned last, meets[kKvWaves];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
@@ -80,13 +273,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 
     // What this thread loads of a tile: a task is one operand of keys and one of values, both parts.
     auto mine = [&](int x) { return FRAGS % kKvWaves == 0 || wave + kKvWaves * (x >> 1) < FRAGS; };
-    uint32_t key_off[TASKS], value_off[TASKS], scale_off[PASSES];
+    // (Task k's offsets are those of task 0 and a constant, for keys where the waves share out whole halves: a register each.)
+    constexpr bool WHOLE = NB % kKvWaves == 0;
+    uint32_t key_off[WHOLE ? 1 : TASKS], scale_off[PASSES];
 #pragma unroll
-    for (int k = 0; k < TASKS; ++k) {
-        const int f = wave + kKvWaves * k, h = f / NB, b = f % NB, bv = f >> 1, t = f & 1;
-        key_off[k] = h * 64 * KL + F::at(KL, lane, b * F::kElemBits);
-        value_off[k] = F::half(NB) + F::at(VL, lane, QT < 2 ? (2 * bv + t) * F::kElemBits : 2 * bv * F::kElemBits);
+    for (int k = 0; k < (WHOLE ? 1 : TASKS); ++k) {
+        const int f = wave + kKvWaves * k, h = f / NB, b = f % NB;
+        key_off[k] = WHOLE ? F::at(KL, lane, wave * F::kElemBits) : h * 64 * KL + F::at(KL, lane, b * F::kElemBits);
     }
+    auto key_at = [&](const uint8_t* tile, int k) {
+        const int b = kKvWaves * k;  // of task k, less the wave
+        return WHOLE ? tile + key_off[0] + (b / NB * 64 * KL + F::at(KL, 0, b % NB * F::kElemBits)) : tile + key_off[WHOLE ? 0 : k];
+    };
+    const uint32_t value_off = F::half(NB) + F::at(VL, lane, (QT < 2 ? wave : wave & ~1) * F::kElemBits);
+    auto value_at = [&](const uint8_t* tile, int k) { return tile + value_off + F::at(VL, 0, kKvWaves * k * F::kElemBits); };
 #pragma unroll
     for (int z = 0; z < PASSES; ++z) {
         const int block = min(static_cast<int>(threadIdx.x % PER), NB - 1), item = (threadIdx.x + z * (kThreads)) / PER;
@@ -106,6 +306,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         h8_t qh[NQ][NB], ql[NQ][NB];
         float to_t[NQ];
         int pos[NQ];
+        bool uneven = false;  // blocks of a row or a position that this wave has met are too far apart in size
         // This lane's row u of the batch, and where its elements start.
         auto token_of = [&](int u) { return min(row0 + 16 * u + i16, rows - 1) / a.group; };
         auto element_of = [&](int u) {
@@ -116,7 +317,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         for (int u = 0; u < NQ; ++u) {
             pos[u] = start + token_of(u);
             float v[NB][8], sum[NB];
-            load_query<NB, false>(q + element_of(u), hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
+            const bool apart = load_query<NB, false>(q + element_of(u), hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
+            uneven = uneven || __any(apart);
 #pragma unroll
             for (int b = 0; b < NB; ++b) split8(v[b], &qh[u][b], &ql[u][b]);
         }
@@ -156,7 +358,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 #pragma unroll
             for (int k = 0; k < TASKS; ++k) {
                 if (!mine(2 * k)) continue;
-                const uint8_t* p = tile + key_off[k];
+                const uint8_t* p = key_at(tile, k);
                 if (QT == 0) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {  // the lane's two units
@@ -176,7 +378,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 #pragma unroll
             for (int k = 0; k < TASKS; ++k) {
                 if (!mine(2 * k)) continue;
-                const uint8_t* p = tile + value_off[k];
+                const uint8_t* p = value_at(tile, k);
                 if (QT == 0) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -199,10 +401,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     raw_s[z][x] = QT == 0 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
                 }
         };
-        // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position: 1 where the
-        // position's largest element is from 2^-10 to 2^7 (the parts then lose what they do at 1,
-        // 2^-22, and none reaches 2^15), else what brings it to [1, 2).
-        auto make_scales = [&](Scales* s) {
+        auto over_blocks = [&](float x, auto two) {  // over a position's blocks, PER lanes in a row
+            x = two(x, quad_peer<0xB1>(x));
+            x = two(x, quad_peer<0x4E>(x));
+            if (PER == 8) x = two(x, quad_peer<0x141>(x));  // (the mirror of eight lanes)
+            return x;
+        };
+        auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
+        const int item_lo = start + it.row0 / a.group, item_hi = start + (min(rows, it.row0 + kKvWaves * ROWS) - 1) / a.group;
+        // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position: 1 where all of the
+        // position's blocks are of sizes from 2^-10 to 2^7 (the parts then lose what they do at 1,
+        // 2^-22, and none reaches 2^15), else what brings the largest to [1, 2).  That serves its blocks as long as none
+        // is below 2^-9 of the largest for keys, 2^-6 for values, whose weights share it; a key's block of zeros adds
+        // nothing and loses nothing.  Otherwise the rows are left to plain_rows.  Positions that no row of the item
+        // sees are zeros.
+        auto make_scales = [&](int i) {
+            Scales* const s = scales + slot_of(i);
             using T = typename std::remove_reference<decltype(s->scale[0][0][0][0])>::type;
             uint32_t flags = 0;
 #pragma unroll
@@ -212,16 +426,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 const int key = item % kKvTile;
                 const float d = QT == 0 ? bits<float>(raw_s[z][0]) : half_value(static_cast<uint16_t>(raw_s[z][0]));
                 const float add = QT == 3 ? half_value(static_cast<uint16_t>(raw_s[z][F::kPlanes - 1])) : 0.0f;
-                const bool bad = !(fabsf(d) < INFINITY) || !(fabsf(add) < INFINITY);
-                float top = QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
-                top = bad ? 0.0f : top;
-                top = quad_max(top);  // over the position's blocks (lanes past the last repeat it)
-                if (PER == 8) top = fmaxf(top, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, top), 0x141, 0xf, 0xf, true)));
-                const bool near = top == 0.0f || (top >= 0x1p-10f && top < 0x1p7f);
+                // a bound of the block's elements, within a factor of 3 (lanes past the last block repeat it)
+                const float size = QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
                 float lift = kLift;
                 int e = 0;
-                if (!__all(near && !bad)) {
-                    e = near ? 0 : max(static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -80);
+                bool bad = false, nothing = false;
+                if (!__all((size >= 0x1p-10f && size < 0x1p7f) || 32 * block >= hd)) {
+                    const int at = tile_of(i) * kKvTile + key;
+                    nothing = !(at <= item_hi && (a.window == 0 || at > item_lo - a.window || at < a.sinks));
+                    bad = !nothing && !(size < INFINITY);
+                    const bool counts = !nothing && !bad && 32 * block < hd;
+                    const float top = over_blocks(counts ? size : 0.0f, [](float x, float y) { return fmaxf(x, y); });
+                    const float least = over_blocks(counts && (values || size > (QT == 0 ? kFloor : 0.0f)) ? size : INFINITY,
+                                                    [](float x, float y) { return fminf(x, y); });
+                    const bool near = top == 0.0f || (least >= 0x1p-10f && top < 0x1p7f);
+                    uneven = uneven || !__all(near || least >= top * (values ? 0x1p-6f : 0x1p-9f));
+                    e = near ? 0 : exponent(top);
                     lift = ldexpf(kLift, -e);
                     flags |= kFar | (values && __any(bad) ? kBad : 0u);
                 }
@@ -231,10 +451,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 }
                 if (block < NB) {
                     // keys: NaN through to the score; values: zero here, NaN for the rows that see it (`bad`)
-                    const float nothing = values ? 0.0f : NAN;
+                    const bool other = bad || nothing;
+                    const float instead = values || nothing ? 0.0f : NAN;
                     if (values) s->bad[block][key] = bad;
-                    s->scale[values][0][block][key] = static_cast<T>(bad ? nothing : QT == 0 ? lift : d * lift);
-                    if (QT == 3) s->scale[values][QT == 3 ? 1 : 0][block][key] = static_cast<T>(bad ? nothing : add * lift);
+                    s->scale[values][0][block][key] = static_cast<T>(other ? instead : QT == 0 ? lift : d * lift);
+                    if (QT == 3) s->scale[values][QT == 3 ? 1 : 0][block][key] = static_cast<T>(other ? instead : add * lift);
                 }
             }
             if (lane == 0) s->flags[wave] = flags;
@@ -317,7 +538,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
         // Converts the keys of tile i + 1 and the values of tile i, and loads those of the next.
         auto convert_begin = [&](int i, SliceScales* c) {
 #pragma unroll
@@ -336,9 +556,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         load_keys(address_of(0, page_of(0)));
         // what the first step takes for the values of a tile before the first
         for (int f = wave; f < 2 * FRAGS; f += kKvWaves) operand(1, 2 + f / FRAGS, f % FRAGS)[lane] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
-        make_scales(scales + 0);
+        make_scales(0);
         load_scales(address_of(1, page_of(1)));
-        make_scales(scales + 1);
+        make_scales(1);
         load_scales(address_of(2, page_of(2)));
         __syncthreads();
 #pragma unroll
@@ -503,7 +723,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             asm volatile("" : "+v"(page1), "+v"(page2), "+v"(page3));
             SliceScales c[SLICES];
             convert_begin(i, c);
-            make_scales(scales + slot_of(i + 2));
+            make_scales(i + 2);
             convert_finish(i, c, page1, page2);
             load_scales(address_of(i + 3, page3));
             page1 = page2;
@@ -513,16 +733,24 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             softmax(i);
             barrier();
         }
-        products(false, n);
+        if (lane == 0) meets[wave] = uneven;
+        __syncthreads();
+        const bool plain = (meets[0] | meets[1] | meets[2] | meets[3]) != 0;
+        if (__builtin_expect(plain, 0)) {
+            plain_rows<QT, NB, NQ>(a, it, head, row0, wave, lane, q, out, reinterpret_cast<float*>(lds) + wave * 4 * (32 * NB + 32));
+            if (it.nsplit == 1) continue;
+        } else {
+            products(false, n);
 
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            l[u] = sum_quarters(l[u]);
+            for (int u = 0; u < NQ; ++u) {
+                l[u] = sum_quarters(l[u]);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
-                o[u][2 * b] += add;
-                o[u][2 * b + 1] += add;
+                for (int b = 0; b < NB; ++b) {
+                    const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
+                    o[u][2 * b] += add;
+                    o[u][2 * b + 1] += add;
+                }
             }
         }
 
@@ -531,7 +759,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             auto rsrc_of = [&](int split) {
                 return state_rsrc(a.partial, (static_cast<size_t>(it.slot + split) * n_kv + head) * kKvWaves + wave, STATE);
             };
-            leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
+            if (!plain) leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
             __syncthreads();
             if (threadIdx.x == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);

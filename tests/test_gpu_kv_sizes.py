@@ -118,3 +118,62 @@ def test_few_rows_query_blocks_of_different_size(hip, orc, lens, kind, sizes):
         c.q[::2] = spread(rng, len(c.q[::2]), 4, hd, sizes)
         c.q[1::2] = spread(rng, len(c.q[1::2]), 4, hd, [min(1.0, s) for s in sizes])
         check(c)
+
+
+MANY = [[(70, 100)], [(200, 230), (1, 40)], [(33, 2500)]]
+
+
+@pytest.mark.parametrize("kind,sizes", VALUE_SIZES)
+@pytest.mark.parametrize("lens", MANY)
+def test_many_rows_value_blocks_of_different_size(hip, orc, lens, kind, sizes):
+    say("many rows, value blocks", kind, sizes, lens)
+    for hd in (64, 80, 160):
+        rng = np.random.default_rng(hd)
+        check(Case(hip, orc, kind, lens, 4, 2, hd, values=spread(rng, sum(t for _, t in lens), 2, hd, sizes)))
+
+
+@pytest.mark.parametrize("kind,sizes", [("f32", (1.0, 1e-5)), ("f32", (1e8, 1.0)), ("f32", (1e18, 1e-18)), ("f32", (1.0, 0.0)),
+                                        ("q8_0", (1e3, 1e-3)), ("q4_0", (1e4, 1e-3)), ("q4_1", (1e-3, 1e3))])
+@pytest.mark.parametrize("lens", MANY)
+def test_many_rows_query_and_key_blocks_of_different_size(hip, orc, lens, kind, sizes):
+    """Keys' blocks far apart in size, under queries that make up for it and under ones that read the small ones
+    only; queries' blocks far apart."""
+    say("many rows, key blocks", kind, sizes, lens)
+    rng = np.random.default_rng(6)
+    for hd in (64, 80, 160):
+        inverse = [1 / s if s else 1.0 for s in sizes]
+        c = Case(hip, orc, kind, lens, 4, 2, hd, keys=spread(rng, sum(t for _, t in lens), 2, hd, inverse))
+        c.q[::2] = spread(rng, len(c.q[::2]), 4, hd, sizes)
+        c.q[1::2] = spread(rng, len(c.q[1::2]), 4, hd, [min(1.0, s) if i < 1 else 0.0 for i, s in enumerate(sizes)])
+        check(c)
+        c = Case(hip, orc, kind, lens, 4, 2, hd)
+        c.q[:] = spread(rng, len(c.q), 4, hd, [min(1.0, s) for s in sizes])
+        check(c)
+
+
+@pytest.mark.parametrize("kind", list(QT))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+def test_many_rows_a_few_uneven_positions(hip, orc, kind, window, sinks):
+    """Uneven positions that some rows see, in the middle of a long context whose parts are merged."""
+    rng = np.random.default_rng(7)
+    v, k = (rng.standard_normal((3000, 2, 96)).astype(np.float32) for _ in range(2))
+    v[1500, :, 32:64] *= np.float32(3e4)
+    v[2950, 1, :32] *= np.float32(1e-4)
+    k[700, 0, 64:] *= np.float32(2e4)
+    check(Case(hip, orc, kind, [(140, 3000)], 4, 2, 96, window=window, sinks=sinks, values=v, keys=k))
+
+
+@pytest.mark.parametrize("kind,bad", [("f32", np.inf), ("f32", np.nan), ("f32", 3e30), ("q8_0", 1e30), ("q4_0", -np.inf)])
+def test_many_rows_healthy_block_beside_a_bad_one(hip, orc, kind, bad):
+    """As for few rows; the head's other blocks differ in size or not."""
+    for size in (1.0, 1e-5):
+        rng = np.random.default_rng(8)
+        v = spread(rng, 100, 2, 96, (1.0, 1.0, size))
+        c = Case(hip, orc, kind, [(70, 100)], 4, 2, 96, values=v.copy())
+        v[20, 0, 40] = bad
+        with np.errstate(all="ignore"):
+            worse = Case(hip, orc, kind, [(70, 100)], 4, 2, 96, values=v, keys=c.k)
+        worse.held = c.held
+        got = check(worse, dims=np.r_[0:32, 64:96])
+        check(worse, heads=slice(2, 4))
+        assert np.isnan(got[:, :2, 32:64]).all()
