@@ -439,7 +439,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     const float top = over_blocks(counts ? size : 0.0f, [](float x, float y) { return fmaxf(x, y); });
                     const float least = over_blocks(counts && (values || size > (QT == 0 ? kFloor : 0.0f)) ? size : INFINITY,
                                                     [](float x, float y) { return fminf(x, y); });
-                    const bool near = top == 0.0f || (least >= 0x1p-10f && top < 0x1p7f);
+                    const bool near = top == 0.0f || (least >= 0x1p-10f && top < 0x1p7f && (QT != 0 || top > kFloor));
                     uneven = uneven || !__all(near || least >= top * (values ? 0x1p-6f : 0x1p-9f));
                     e = near ? 0 : exponent(top);
                     lift = ldexpf(kLift, -e);

@@ -177,3 +177,11 @@ def test_many_rows_healthy_block_beside_a_bad_one(hip, orc, kind, bad):
         got = check(worse, dims=np.r_[0:32, 64:96])
         check(worse, heads=slice(2, 4))
         assert np.isnan(got[:, :2, 32:64]).all()
+
+
+@pytest.mark.parametrize("new", [3, 70])
+def test_keys_below_the_floor_of_a_block(hip, orc, new):
+    """f32 keys below 2^-80, which share one power of two, under a scale that makes their scores count."""
+    rng = np.random.default_rng(9)
+    k = (rng.standard_normal((150, 2, 64)) * 1e-25).astype(np.float32)
+    check(Case(hip, orc, "f32", [(new, 150)], 4, 2, 64, keys=k, scale=1e24))
