@@ -47,6 +47,8 @@ struct TileScales {
 };
 constexpr uint32_t kBad = 1, kFar = 2;
 constexpr float kLift = 256.0f;  // operands lie in LDS times this
+constexpr float kWeightLift = 9.0f;  // log2 of what weights are split times, at the running maximum
+constexpr int kZeroLog = -90;  // taken for a position whose values are zeros: others count until weights differ by 2^90
 constexpr float kFloor = 0x1p-80f;  // f32: the power of two of a block of zeros, or of elements this small
 
 template <int QT, int NB>
@@ -61,13 +63,13 @@ __device__ __forceinline__ float element(uint32_t w, int i, float d, float add) 
     return QT == 3 ? fmaf(c, d, add) : c * d;
 }
 
-// The rows of one wave of an item (ROWS from row_base on), in plain f32: what a wave of attention_rows_kernel does
-// where blocks of a position or of a query differ too much in size for its operands.  Four rows at a time; a lane takes one
-// position's half of every block for the scores, every 64th dimension for the values.  Five times as slow, in few
-// registers: the kernel's own are not touched by it.  lds: the wave's, 4 (32 NB + 32) floats.
+// Rows of one wave of an item (those of the mask `which`, from row_base on), in plain f32: what a wave of
+// attention_rows_kernel does where blocks of a position that the row sees or of its query differ too much in size for
+// its operands.  Four rows at a time; a lane takes one position's half of every block for the scores, every 64th dimension for
+// the values.  In few registers: the kernel's own are not touched by it.  lds: the wave's, 4 (32 NB + 32) floats.
 template <int QT, int NB, int NQ>
-__device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnItem& it, int head, int row_base, int wave, int lane,
-                                           const float* __restrict__ q, float* __restrict__ out, float* lds) {
+__device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnItem& it, int head, int row_base, uint32_t which, int wave,
+                                           int lane, const float* __restrict__ q, float* __restrict__ out, float* lds) {
     using F = KvForm<QT>;
     constexpr int KL = F::key_lane(NB), VL = F::value_lane(NB), HD = 32 * NB, DIMS = (HD + 63) / 64;
     constexpr int QUADS = NQ * 2 * NB, STATE = (QUADS * 4 + 2 * NQ) * 64;
@@ -92,7 +94,8 @@ __device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnIte
         return QT == 0 ? reinterpret_cast<const float*>(plane)[i] : half_value(reinterpret_cast<const uint16_t*>(plane)[i]);
     };
 #pragma unroll 1
-    for (int r = 0; r < 16 * NQ && row_base + r < rows; r += 4) {
+    for (int r = 0; r < 16 * NQ; r += 4) {
+        if ((which >> r & 15u) == 0) continue;
         // Queries over the power of two of the row's largest; a score's factor to base 2.
         float to_t[4], m[4], l[4], acc[DIMS][4];
         int pos[4];
@@ -216,13 +219,13 @@ __device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnIte
                 }
             }
         }
-        // The output, or the state as leave_state lays it out, in the units of the others (weights times 2^8, values
-        // times kLift).
+        // The output, or the state as leave_state lays it out, in the units of the others (weights times 2^kWeightLift,
+        // values times kLift).
         const __amdgpu_buffer_rsrc_t rs =
             state_rsrc(a.partial, (static_cast<size_t>(it.slot + it.split) * n_kv + head) * kKvWaves + wave, STATE);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (row_base + r + k >= rows) continue;
+            if ((which >> (r + k) & 1u) == 0) continue;
             const int u = (r + k) >> 4, column = (r + k) & 15;
 #pragma unroll
             for (int c = 0; c < DIMS; ++c) {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnIte
             }
             if (it.nsplit > 1 && lane < 4) {
                 const int of_lane = column + 16 * lane;
-                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[k] + 8.0f), rs,
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, m[k] + kWeightLift), rs,
                                                       (QUADS * 256 + 2 * u * 64 + of_lane) * 4, 0, kCoherent);
                 __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, l[k]), rs,
                                                       (QUADS * 256 + (2 * u + 1) * 64 + of_lane) * 4, 0, kCoherent);
@@ -263,7 +266,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
     h8_t* const operands = reinterpret_cast<h8_t*>(lds);
     Scales* const scales = reinterpret_cast<Scales*>(lds + 2 * 8 * NB * 1024);
     auto operand = [&](int buffer, int part, int f) { return operands + ((buffer * 4 + part) * FRAGS + f) * 64; };
-    __shared__ unsigned last, meets[kKvWaves];
+    __shared__ unsigned last;
+    __shared__ int item_range[2];  // positions of the item's rows (in LDS, as few tiles ask for them)
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
@@ -306,7 +310,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         h8_t qh[NQ][NB], ql[NQ][NB];
         float to_t[NQ];
         int pos[NQ];
-        bool uneven = false;  // blocks of a row or a position that this wave has met are too far apart in size
         // This lane's row u of the batch, and where its elements start.
         auto token_of = [&](int u) { return min(row0 + 16 * u + i16, rows - 1) / a.group; };
         auto element_of = [&](int u) {
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             pos[u] = start + token_of(u);
             float v[NB][8], sum[NB];
             const bool apart = load_query<NB, false>(q + element_of(u), hd, g, a.scale * (1.0f / kLift), v, sum, &to_t[u]);
-            uneven = uneven || __any(apart);
+            if (apart) to_t[u] = NAN;  // (the row is done in plain f32: below)
 #pragma unroll
             for (int b = 0; b < NB; ++b) split8(v[b], &qh[u][b], &ql[u][b]);
         }
@@ -408,13 +411,25 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             return x;
         };
         auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
-        const int item_lo = start + it.row0 / a.group, item_hi = start + (min(rows, it.row0 + kKvWaves * ROWS) - 1) / a.group;
-        // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position: 1 where all of the
-        // position's blocks are of sizes from 2^-10 to 2^7 (the parts then lose what they do at 1,
-        // 2^-22, and none reaches 2^15), else what brings the largest to [1, 2).  That serves its blocks as long as none
-        // is below 2^-9 of the largest for keys, 2^-6 for values, whose weights share it; a key's block of zeros adds
-        // nothing and loses nothing.  Otherwise the rows are left to plain_rows.  Positions that no row of the item
-        // sees are zeros.
+        // A position, a block and a bound of the block's elements, within a factor of 3; whether a row of the item sees it.
+        auto size_of = [&](float d, float add) {
+            return QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
+        };
+        auto scale_in = [&](const uint32_t* raw, int plane) {
+            return QT == 0 ? bits<float>(raw[0]) : half_value(static_cast<uint16_t>(raw[F::kPlanes == 2 ? plane : 0]));
+        };
+        auto seen_by_some = [&](int i, int key) {
+            const int at = tile_of(i) * kKvTile + key;
+            return at <= item_range[1] && (a.window == 0 || at > item_range[0] - a.window || at < a.sinks);
+        };
+        // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position, so that what they lose,
+        // 2^-25, is 2^-22 of every block's largest, and none reaches 2^15.  Keys: 1 where all blocks are of sizes from
+        // 2^-10 to 2^7, else what brings the largest to [2^5, 2^6), which serves blocks from 2^-14 of it on; a block of
+        // zeros adds nothing and loses nothing.  Values: 1 where all blocks are from 2^-6 to 2^4, else
+        // what brings the largest to [2^3, 2^4), which serves blocks from 2^-9 of it on.  (The range is narrow as a weight
+        // keeps 2^-34 of the row's largest: a position that has that one then has values of at least 2^-10 of any
+        // other's.)  What else there is, a value's block of zeros beside others too, leaves the rows that see it to plain_rows.
+        // Positions that no row of the item sees are zeros.
         auto make_scales = [&](int i) {
             Scales* const s = scales + slot_of(i);
             using T = typename std::remove_reference<decltype(s->scale[0][0][0][0])>::type;
@@ -424,35 +439,38 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 const int block = threadIdx.x % PER, item = (threadIdx.x + z * (kThreads)) / PER;
                 const bool values = (wave * 64 + z * (kThreads)) / PER >= kKvTile;  // a wave has one or the other
                 const int key = item % kKvTile;
-                const float d = QT == 0 ? bits<float>(raw_s[z][0]) : half_value(static_cast<uint16_t>(raw_s[z][0]));
-                const float add = QT == 3 ? half_value(static_cast<uint16_t>(raw_s[z][F::kPlanes - 1])) : 0.0f;
-                // a bound of the block's elements, within a factor of 3 (lanes past the last block repeat it)
-                const float size = QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
+                const float d = scale_in(raw_s[z], 0), add = QT == 3 ? scale_in(raw_s[z], 1) : 0.0f;
+                const float size = size_of(d, add);  // (lanes past the last block repeat it)
                 float lift = kLift;
                 int e = 0;
-                bool bad = false, nothing = false;
-                if (!__all((size >= 0x1p-10f && size < 0x1p7f) || 32 * block >= hd)) {
-                    const int at = tile_of(i) * kKvTile + key;
-                    nothing = !(at <= item_hi && (a.window == 0 || at > item_lo - a.window || at < a.sinks));
+                bool bad = false, nothing = false, uneven = false;
+                const float high = values ? 0x1p4f : 0x1p7f, low = values ? 0x1p-6f : 0x1p-10f;
+                if (!__all((size >= low && size < high) || 32 * block >= hd)) {
+                    nothing = !seen_by_some(i, key);
                     bad = !nothing && !(size < INFINITY);
                     const bool counts = !nothing && !bad && 32 * block < hd;
                     const float top = over_blocks(counts ? size : 0.0f, [](float x, float y) { return fmaxf(x, y); });
-                    const float least = over_blocks(counts && (values || size > (QT == 0 ? kFloor : 0.0f)) ? size : INFINITY,
+                    constexpr float kZeros = QT == 0 ? kFloor : 0.0f;  // what a block of zeros, or nearly, has
+                    const float least = over_blocks(counts && (values || size > kZeros) ? size : INFINITY,
                                                     [](float x, float y) { return fminf(x, y); });
-                    const bool near = top == 0.0f || (least >= 0x1p-10f && top < 0x1p7f && (QT != 0 || top > kFloor));
-                    uneven = uneven || !__all(near || least >= top * (values ? 0x1p-6f : 0x1p-9f));
-                    e = near ? 0 : exponent(top);
+                    // (no block that counts leaves the infinity)
+                    const bool near = values ? least >= low && top < high
+                                             : top == 0.0f || (least >= low && top < high && (QT != 0 || top > kFloor));
+                    const bool even = values ? least >= top * 0x1p-9f && (least > kZeros || top <= kZeros) : least >= top * 0x1p-14f;
+                    uneven = !(near || even);
+                    e = near || uneven ? 0 : top == 0.0f ? kZeroLog : exponent(top) - (values ? 3 : 5);
                     lift = ldexpf(kLift, -e);
-                    flags |= kFar | (values && __any(bad) ? kBad : 0u);
+                    flags |= (__any(e != 0 || bad || uneven) ? kFar : 0u) | (values && __any(bad) ? kBad : 0u);
                 }
                 if (block == 0) {
-                    (values ? s->value_down : s->key_up)[key] = ldexpf(1.0f, values ? -e : e);
-                    if (values) s->value_log[key] = static_cast<float>(e);
+                    // (the scores of an uneven position are NaN)
+                    (values ? s->value_down : s->key_up)[key] = uneven && !values ? NAN : ldexpf(1.0f, values ? -e : e);
+                    if (values) s->value_log[key] = uneven ? NAN : static_cast<float>(e);
                 }
                 if (block < NB) {
                     // keys: NaN through to the score; values: zero here, NaN for the rows that see it (`bad`)
-                    const bool other = bad || nothing;
-                    const float instead = values || nothing ? 0.0f : NAN;
+                    const bool other = bad || nothing || uneven;
+                    const float instead = values || !bad ? 0.0f : NAN;
                     if (values) s->bad[block][key] = bad;
                     s->scale[values][0][block][key] = static_cast<T>(other ? instead : QT == 0 ? lift : d * lift);
                     if (QT == 3) s->scale[values][QT == 3 ? 1 : 0][block][key] = static_cast<T>(other ? instead : add * lift);
@@ -551,6 +569,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         };
 
         // Fill the pipeline: scales of tiles 0 and 1 (counted from the item's first), keys of 0.
+        if (threadIdx.x == 0) {
+            item_range[0] = start + it.row0 / a.group;
+            item_range[1] = start + (min(rows, it.row0 + kKvWaves * ROWS) - 1) / a.group;
+        }
         __syncthreads();  // the last item's readers are done
         load_scales(address_of(0, page_of(0)));
         load_keys(address_of(0, page_of(0)));
@@ -640,19 +662,30 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                               (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
             const u4_t all = *reinterpret_cast<const u4_t*>(s->flags);
             const uint32_t flags = __builtin_amdgcn_readfirstlane(all.x | all.y | all.z | all.w);
-            if (!full || (flags & kFar) != 0) {
+            // (a lane's positions are 4 g .. and 16 + 4 g ..)
+            auto of_tile = [&](const float* x) {
+                const f4_t lo = *reinterpret_cast<const f4_t*>(x + 4 * g), hi = *reinterpret_cast<const f4_t*>(x + 16 + 4 * g);
+                return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            if ((flags & kFar) != 0) {
                 // (a value's power of two goes into the score here: P_j = p_j 2^ev_j; its sum is set right below)
+                const auto up = of_tile(s->key_up), log = of_tile(s->value_log);
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
                     const float inv = 1.0f / to_t[u];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int at = (j >> 2) * 16 + 4 * g + (j & 3), k = first + at;
-                        const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
-                        float& x = x_[u][j];
-                        x = seen ? fmaf(s->value_log[at], inv, x * s->key_up[at]) : -INFINITY;
-                    }
+                    for (int j = 0; j < 8; ++j) x_[u][j] = fmaf(log[j], inv, x_[u][j] * up[j]);
                 }
+            }
+            if (!full) {
+#pragma unroll
+                for (int u = 0; u < NQ; ++u)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                        const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
+                        x_[u][j] = seen ? x_[u][j] : -INFINITY;
+                    }
             }
             // The maximum moves when it is passed by kSlack.
             float top[NQ];
@@ -687,10 +720,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     }
             }
 
-            // P_j, up to 2^(6 + 8)
+            // P_j, up to 2^15
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
-                const float frame = m[u] - 8.0f;
+                const float frame = m[u] - kWeightLift;
                 float p[8], sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -699,13 +732,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 }
                 if ((flags & kFar) != 0) {
                     // p_j = P_j 2^-ev_j, which may count where P_j is below what f32 holds
+                    const auto down = of_tile(s->value_down);
                     sum = 0.0f;
+                    bool deep = false;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float y = fmaf(x_[u][j], to_t[u], -frame);
-                        const float down = s->value_down[(j >> 2) * 16 + 4 * g + (j & 3)];
-                        const bool deep = y < -60.0f;
-                        sum = fmaf(__builtin_amdgcn_exp2f(deep ? y + 100.0f : y), deep ? down * 0x1p-100f : down, sum);
+                        sum = fmaf(p[j], down[j], sum);
+                        deep = deep || (p[j] < 0x1p-60f && down[j] > 1.0f && x_[u][j] != -INFINITY);
+                    }
+                    if (__any(deep)) {
+                        sum = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float y = fmaf(x_[u][j], to_t[u], -frame);
+                            const bool far = y < -60.0f;
+                            sum = fmaf(__builtin_amdgcn_exp2f(far ? y + 100.0f : y), far ? down[j] * 0x1p-100f : down[j], sum);
+                        }
                     }
                 }
                 l[u] += sum;
@@ -733,33 +775,41 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             softmax(i);
             barrier();
         }
-        if (lane == 0) meets[wave] = uneven;
-        __syncthreads();
-        const bool plain = (meets[0] | meets[1] | meets[2] | meets[3]) != 0;
-        if (__builtin_expect(plain, 0)) {
-            plain_rows<QT, NB, NQ>(a, it, head, row0, wave, lane, q, out, reinterpret_cast<float*>(lds) + wave * 4 * (32 * NB + 32));
-            if (it.nsplit == 1) continue;
-        } else {
-            products(false, n);
+        products(false, n);
 
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                l[u] = sum_quarters(l[u]);
+        for (int u = 0; u < NQ; ++u) {
+            l[u] = sum_quarters(l[u]);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
-                    o[u][2 * b] += add;
-                    o[u][2 * b + 1] += add;
-                }
+            for (int b = 0; b < NB; ++b) {
+                const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
+                o[u][2 * b] += add;
+                o[u][2 * b + 1] += add;
             }
         }
+
+        // Rows that are NaN: for what they are made of, or for blocks that differ too much in size, and then done again.
+        uint32_t again = 0;
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            const uint64_t lanes = __ballot(l[u] != l[u] && row0 + 16 * u + i16 < row1);
+            again |= static_cast<uint32_t>((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffffu) << (16 * u);
+        }
+        auto plain = [&] {
+            // (in the LDS of the first keys' operands, which no wave reads any more)
+            plain_rows<QT, NB, NQ>(a, it, head, row0, again, wave, lane, q, out, reinterpret_cast<float*>(lds) + wave * 4 * (32 * NB + 32));
+        };
 
         if (it.nsplit > 1) {
             // Every wave's state to memory; the workgroup that arrives last merges the parts, each wave its rows.
             auto rsrc_of = [&](int split) {
                 return state_rsrc(a.partial, (static_cast<size_t>(it.slot + split) * n_kv + head) * kKvWaves + wave, STATE);
             };
-            if (!plain) leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
+            leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
+            if (__builtin_expect(again != 0, 0)) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                plain();
+            }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
             __syncthreads();
             if (threadIdx.x == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);
@@ -781,6 +831,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             for (int u = 0; u < NQ; ++u) {
                 if (row0 + 16 * u + i16 >= row1) continue;
                 store_row<NB>(out + element_of(u), hd, g, o[u], 1.0f / (l[u] * kLift));
+            }
+            if (__builtin_expect(it.nsplit == 1 && again != 0, 0)) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                plain();
             }
         }
     }

@@ -185,3 +185,35 @@ def test_keys_below_the_floor_of_a_block(hip, orc, new):
     rng = np.random.default_rng(9)
     k = (rng.standard_normal((150, 2, 64)) * 1e-25).astype(np.float32)
     check(Case(hip, orc, "f32", [(new, 150)], 4, 2, 64, keys=k, scale=1e24))
+
+
+@pytest.mark.parametrize("kind", list(QT))
+@pytest.mark.parametrize("new", [3, 70])
+@pytest.mark.parametrize("size", [0.0, 1e-3, 1e-2])
+def test_a_sink_with_small_values(hip, orc, kind, new, size):
+    """A first position that takes nearly all the weight and whose values are zeros or small: the others' part of
+    the result is what the smaller weights make it."""
+    rng = np.random.default_rng(10)
+    for gap in (12.0, 15.0, 20.0, 40.0):
+        k, v = (rng.standard_normal((200, 2, 64)).astype(np.float32) for _ in range(2))
+        k *= np.float32(0.05)
+        k[0] = gap / 64
+        v[0] *= np.float32(size)
+        c = Case(hip, orc, kind, [(new, 200)], 4, 2, 64, keys=k, values=v, scale=1.0)
+        c.q[:] = rng.uniform(0.9, 1.1, c.q.shape).astype(np.float32)
+        check(c)
+
+
+@pytest.mark.parametrize("kind", ["f32", "q8_0"])
+@pytest.mark.parametrize("new", [3, 70])
+def test_values_of_all_sizes_beside_each_other(hip, orc, kind, new):
+    """Values of zero, tiny and large ones in turn, and a position that is all zeros in the middle of a tile."""
+    rng = np.random.default_rng(11)
+    v = rng.standard_normal((300, 2, 96)).astype(np.float32)
+    v[1::5] = 0.0
+    v[2::7] *= np.float32(3e-3)
+    v[3::11] *= np.float32(100.0)
+    check(Case(hip, orc, kind, [(new, 300)], 4, 2, 96, values=v))
+    v = rng.standard_normal((300, 2, 96)).astype(np.float32)
+    v[100] = 0.0
+    check(Case(hip, orc, kind, [(new, 300)], 4, 2, 96, values=v))
