@@ -28,6 +28,7 @@
 #include "kv_attention.h"
 #include "quant_device.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mlq {
@@ -842,10 +843,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 
 // Workgroups of a recorded launch, which walks whatever list is set by then.
 constexpr unsigned kRecorded = 1024;
+constexpr long long kMostGroups = 1 << 20;
 
 template <int QT, int NB>
 hipError_t launch_blocks(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
-    const unsigned grid = count > 0 ? static_cast<unsigned>(count) * a.kv.n_kv : kRecorded;
+    // (a launch holds less than 2^32 threads; the kernels walk their lists whatever the grid)
+    const unsigned grid =
+        count > 0 ? static_cast<unsigned>(std::min<long long>(static_cast<long long>(count) * a.kv.n_kv, kMostGroups)) : kRecorded;
     if (kind == 0) {
         attention_kernel<QT, NB><<<grid, kThreads, 0, s>>>(a, count, q, out);
     } else {

@@ -4,8 +4,8 @@ held to a bound of its own (kv_reference.attention_by_block), whatever the block
 import numpy as np
 import pytest
 
-from kv_reference import QT, attention_by_block
-from test_gpu_kv import Case, say
+from kv_reference import QT, attention, attention_by_block, held
+from test_gpu_kv import Case, back, dev, say
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,27 @@ def test_values_of_all_sizes_beside_each_other(hip, orc, kind, new):
     v = rng.standard_normal((300, 2, 96)).astype(np.float32)
     v[100] = 0.0
     check(Case(hip, orc, kind, [(new, 300)], 4, 2, 96, values=v))
+
+
+def test_more_workgroups_than_a_launch_holds(hip, orc):
+    """16400 decoding sequences of 1024 heads: 2^24 items and a few, whose workgroups would be more threads than a
+    launch may have."""
+    n, heads, hd, page = 16400, 1024, 8, 32
+    rng = np.random.default_rng(12)
+    some = rng.standard_normal((97, heads, hd)).astype(np.float32)
+    k, v, q = (np.take(some, (np.arange(n) * step + 5) % 97, axis=0) for step in (1, 3, 7))
+    cache = hip.KvCache(QT["q8_0"], 1, -(-n // page), page, heads, hd)
+    plan = hip.KvPlan(cache, heads, max_seqs=n, max_tokens=n, max_pages=n)
+    # sequence i: the first i % 32 + 1 slots of a page it shares with up to 31 others
+    length, pages = np.arange(n) % page + 1, np.arange(n) // page
+    plan.set(np.ones(n, int), length, pages)
+    plan.write(0, dev(hip, k), dev(hip, v))
+    out = dev(hip, np.full_like(q, 7.25))
+    plan.attention(0, dev(hip, q), out)
+    got = back(hip, out, q.shape)
+    assert np.isfinite(got).all() and not (got == 7.25).all(-1).any()
+    for i in (0, 1, 31, 32, 8191, 16383, 16384, 16399):
+        first = i - i % page
+        kk, vv = (held(orc, "q8_0", x[first:i + 1]) for x in (k, v))
+        want, bound = attention(q[i:i + 1], kk, vv)
+        assert (np.abs(got[i] - want[0]) <= bound[0]).all(), i
