@@ -268,6 +268,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
     Scales* const scales = reinterpret_cast<Scales*>(lds + 2 * 8 * NB * 1024);
     auto operand = [&](int buffer, int part, int f) { return operands + ((buffer * 4 + part) * FRAGS + f) * 64; };
     __shared__ unsigned last;
+    __shared__ float block_tops[kKvWaves][PER];  // the largest of the first tile's values, by wave that looked
     __shared__ int item_range[2];  // positions of the item's rows (in LDS, as few tiles ask for them)
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -412,6 +413,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             return x;
         };
         auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
+        // log2 of a block's power of two for values; one over it, of the block whose scales this thread makes.
+        auto block_exponent = [&](int b) {
+            const float top = fmaxf(fmaxf(block_tops[0][b], block_tops[1][b]), fmaxf(block_tops[2][b], block_tops[3][b]));
+            return top > 0.0f ? min(max(exponent(top), -20), 20) : 0;  // (what is beyond that, in f32's range, stays so over it)
+        };
+        float value_unit;
         // A position, a block and a bound of the block's elements, within a factor of 3; whether a row of the item sees it.
         auto size_of = [&](float d, float add) {
             return QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
@@ -426,8 +433,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position, so that what they lose,
         // 2^-25, is 2^-22 of every block's largest, and none reaches 2^15.  Keys: 1 where all blocks are of sizes from
         // 2^-10 to 2^7, else what brings the largest to [2^5, 2^6), which serves blocks from 2^-14 of it on; a block of
-        // zeros adds nothing and loses nothing.  Values: 1 where all blocks are from 2^-6 to 2^4, else
-        // what brings the largest to [2^3, 2^4), which serves blocks from 2^-9 of it on.  (The range is narrow as a weight
+        // zeros adds nothing and loses nothing.  Values are first taken over the block's own power of two, that of its
+        // largest in the item's first tile; then 1 where all blocks are from 2^-7 to 2^3, else
+        // what brings the largest to [2^2, 2^3), which serves blocks from 2^-9 of it on.  (The range is narrow as a weight
         // keeps 2^-34 of the row's largest: a position that has that one then has values of at least 2^-10 of any
         // other's.)  What else there is, a value's block of zeros beside others too, leaves the rows that see it to plain_rows.
         // Positions that no row of the item sees are zeros.
@@ -441,26 +449,29 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 const bool values = (wave * 64 + z * (kThreads)) / PER >= kKvTile;  // a wave has one or the other
                 const int key = item % kKvTile;
                 const float d = scale_in(raw_s[z], 0), add = QT == 3 ? scale_in(raw_s[z], 1) : 0.0f;
-                const float size = size_of(d, add);  // (lanes past the last block repeat it)
-                float lift = kLift;
+                const float unit = values ? value_unit : 1.0f;
+                const float size = size_of(d, add) * unit;  // (lanes past the last block repeat it)
+                float lift = kLift * unit;
                 int e = 0;
                 bool bad = false, nothing = false, uneven = false;
-                const float high = values ? 0x1p4f : 0x1p7f, low = values ? 0x1p-6f : 0x1p-10f;
+                const float high = values ? 0x1p3f : 0x1p7f, low = values ? 0x1p-7f : 0x1p-10f;
                 if (!__all((size >= low && size < high) || 32 * block >= hd)) {
                     nothing = !seen_by_some(i, key);
                     bad = !nothing && !(size < INFINITY);
                     const bool counts = !nothing && !bad && 32 * block < hd;
                     const float top = over_blocks(counts ? size : 0.0f, [](float x, float y) { return fmaxf(x, y); });
-                    constexpr float kZeros = QT == 0 ? kFloor : 0.0f;  // what a block of zeros, or nearly, has
-                    const float least = over_blocks(counts && (values || size > kZeros) ? size : INFINITY,
-                                                    [](float x, float y) { return fminf(x, y); });
-                    // (no block that counts leaves the infinity)
-                    const bool near = values ? least >= low && top < high
-                                             : top == 0.0f || (least >= low && top < high && (QT != 0 || top > kFloor));
-                    const bool even = values ? least >= top * 0x1p-9f && (least > kZeros || top <= kZeros) : least >= top * 0x1p-14f;
+                    // a block of zeros, or nearly
+                    const bool zeros = size_of(d, add) <= (QT == 0 ? kFloor : 0.0f);
+                    const float least = over_blocks(counts && !zeros ? size : INFINITY, [](float x, float y) { return fminf(x, y); });
+                    const float any_zeros = over_blocks(counts && zeros ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); });
+                    // (no block that counts leaves the infinity; where all are zeros a power of two far below the others')
+                    const bool all_zeros = least == INFINITY && any_zeros != 0.0f;
+                    const bool near = values ? least >= low && top < high && any_zeros == 0.0f
+                                             : top == 0.0f || (least >= low && top < high && !(QT == 0 && all_zeros));
+                    const bool even = least >= top * (values ? 0x1p-9f : 0x1p-14f) && (!values || any_zeros == 0.0f || all_zeros);
                     uneven = !(near || even);
-                    e = near || uneven ? 0 : top == 0.0f ? kZeroLog : exponent(top) - (values ? 3 : 5);
-                    lift = ldexpf(kLift, -e);
+                    e = near || uneven ? 0 : values ? (all_zeros ? kZeroLog : exponent(top) - 2) : exponent(top) - 5;
+                    lift = ldexpf(kLift * unit, -e);
                     flags |= (__any(e != 0 || bad || uneven) ? kFar : 0u) | (values && __any(bad) ? kBad : 0u);
                 }
                 if (block == 0) {
@@ -577,6 +588,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         __syncthreads();  // the last item's readers are done
         load_scales(address_of(0, page_of(0)));
         load_keys(address_of(0, page_of(0)));
+        // The blocks' powers of two for values.
+        {
+            float top = 0.0f;
+#pragma unroll
+            for (int z = 0; z < PASSES; ++z) {
+                const int block = threadIdx.x % PER, item = (threadIdx.x + z * (kThreads)) / PER;
+                const float size = size_of(scale_in(raw_s[z], 0), QT == 3 ? scale_in(raw_s[z], 1) : 0.0f);
+                if (item >= kKvTile && 32 * block < hd && size < INFINITY && seen_by_some(0, item % kKvTile)) top = fmaxf(top, size);
+            }
+            // over the wave's positions (row_ror)
+            if (PER == 4) top = fmaxf(top, quad_peer<0x124>(top));
+            top = max_quarters(fmaxf(top, quad_peer<0x128>(top)));
+            if (lane < PER) block_tops[wave][lane] = top;
+        }
+        __syncthreads();
+        value_unit = ldexpf(1.0f, -block_exponent(threadIdx.x % PER));
         // what the first step takes for the values of a tile before the first
         for (int f = wave; f < 2 * FRAGS; f += kKvWaves) operand(1, 2 + f / FRAGS, f % FRAGS)[lane] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
         make_scales(0);
@@ -784,8 +811,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
-                o[u][2 * b] += add;
-                o[u][2 * b + 1] += add;
+                const int e = block_exponent(b);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], e) + add;
             }
         }
 

@@ -241,3 +241,15 @@ def test_more_workgroups_than_a_launch_holds(hip, orc):
         kk, vv = (held(orc, "q8_0", x[first:i + 1]) for x in (k, v))
         want, bound = attention(q[i:i + 1], kk, vv)
         assert (np.abs(got[i] - want[0]) <= bound[0]).all(), i
+
+
+@pytest.mark.parametrize("kind", list(QT))
+@pytest.mark.parametrize("first,then", [(1.0, 1e-3), (1e-3, 1.0), (1.0, 300.0), (0.0, 1.0)])
+def test_values_change_size_behind_the_first_tile(hip, orc, kind, first, then):
+    """The first 32 positions' values are of another size than the rest, in all blocks or in one."""
+    rng = np.random.default_rng(13)
+    for dims in (slice(None), slice(32, 64)):
+        v = rng.standard_normal((200, 2, 96)).astype(np.float32)
+        v[:32, :, dims] *= np.float32(first)
+        v[32:, :, dims] *= np.float32(then)
+        check(Case(hip, orc, kind, [(70, 200)], 4, 2, 96, values=v))
