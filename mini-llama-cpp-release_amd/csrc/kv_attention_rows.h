@@ -455,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 int e = 0;
                 bool bad = false, nothing = false, uneven = false;
                 const float high = values ? 0x1p3f : 0x1p7f, low = values ? 0x1p-7f : 0x1p-10f;
-                if (!__all((size >= low && size < high) || 32 * block >= hd)) {
+                if (__builtin_expect(!__all((size >= low && size < high) || 32 * block >= hd), 0)) {
                     nothing = !seen_by_some(i, key);
                     bad = !nothing && !(size < INFINITY);
                     const bool counts = !nothing && !bad && 32 * block < hd;
@@ -695,7 +695,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 const f4_t lo = *reinterpret_cast<const f4_t*>(x + 4 * g), hi = *reinterpret_cast<const f4_t*>(x + 16 + 4 * g);
                 return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             };
-            if ((flags & kFar) != 0) {
+            if (__builtin_expect((flags & kFar) != 0, 0)) {
                 // (a value's power of two goes into the score here: P_j = p_j 2^ev_j; its sum is set right below)
                 const auto up = of_tile(s->key_up), log = of_tile(s->value_log);
 #pragma unroll
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     for (int x = 0; x < 2 * NB; ++x) o[u][x] *= c;
                 }
             }
-            if ((flags & kBad) != 0) {
+            if (__builtin_expect((flags & kBad) != 0, 0)) {
                 // rows that see a value block that is not finite: NaN in its dimensions, in the end
 #pragma unroll 1
                 for (int b = 0; b < NB; ++b)
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     p[j] = __builtin_amdgcn_exp2f(fmaf(x_[u][j], to_t[u], -frame));
                     sum += p[j];
                 }
-                if ((flags & kFar) != 0) {
+                if (__builtin_expect((flags & kFar) != 0, 0)) {
                     // p_j = P_j 2^-ev_j, which may count where P_j is below what f32 holds
                     const auto down = of_tile(s->value_down);
                     sum = 0.0f;
@@ -768,7 +768,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                         sum = fmaf(p[j], down[j], sum);
                         deep = deep || (p[j] < 0x1p-60f && down[j] > 1.0f && x_[u][j] != -INFINITY);
                     }
-                    if (__any(deep)) {
+                    if (__builtin_expect(__any(deep), 0)) {
                         sum = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
