@@ -401,9 +401,11 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             return static_cast<float>(i % 2 == 0 ? p.x : p.y);
         };
 
+        // The next tile's loads are under way during this one's work, unless its registers are not enough for both.
+        constexpr bool AHEAD = QT != 0 || NB <= 4;
         int at = it.first + wave;
         int next_page = 0;
-        if (at < end) {
+        if (AHEAD && at < end) {
             const uint8_t* tile = base_of(at, page_of(at));
             load_keys(tile);
             load_values(tile);
@@ -411,9 +413,11 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
         }
         for (; at < end; at += kKvWaves) {
             const int first = tile_of(at) * kKvTile;
-            const bool more = at + kKvWaves < end;
+            const bool more = AHEAD && at + kKvWaves < end;
+            if (!AHEAD) next_page = page_of(at);
             const uint8_t* next = base_of(more ? at + kKvWaves : at, next_page);
-            if (at + 2 * kKvWaves < end) next_page = page_of(at + 2 * kKvWaves);
+            if (AHEAD && at + 2 * kKvWaves < end) next_page = page_of(at + 2 * kKvWaves);
+            if (!AHEAD) load_keys(next);
 
             // Scores, halves apart.
             float t[8];
@@ -449,23 +453,26 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
                 for (int i = 0; i < 4; ++i) t[4 * h + i] = s[i];
             }
             if (more) load_keys(next);
+            if (!AHEAD) load_values(next);
 
             // Weights.
             const bool full = first + kKvTile - 1 <= pos_lo &&
                               (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
             auto seen = [&](int j) {
                 const int key = first + (j >> 2) * 16 + 4 * g + (j & 3);
-                return key <= pos && (a.window == 0 || key > pos - a.window || key < a.sinks);
+                return (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.sinks));
             };
-            float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 t[j] += other_half(t[j]);
                 // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
                 if (QT >= 2) t[j] = fmaf(t[j], 0.0f, t[j]);
-                if (!full) t[j] = seen(j) ? t[j] : -INFINITY;
-                top = fmaxf(top, t[j]);
             }
+            if (!full) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = seen(j) ? t[j] : -INFINITY;
+            }
+            float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
             top = max_quarters(top);
             if (__any(top > m + kSlack)) {
                 const bool moves = top > m + kSlack;
@@ -539,7 +546,7 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[j], scale_at(vs, 8 * b + j));
                 float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
-                if (__any(ldexpf(most, frame[b]) > 0x1p15f)) {
+                if (__builtin_expect(__any(ldexpf(most, frame[b]) > 0x1p15f), 0)) {
                     most = max_quarters(most);
                     const int to = ldexpf(most, frame[b]) > 0x1p15f ? 9 - exponent(most) : frame[b];
 #pragma unroll
@@ -579,11 +586,12 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
 
         // The lanes' sums, the halves and the minima's part together, out of the blocks' frames.
         l = sum_quarters(l);
+        const bool any_spoilt = __any(spoilt != 0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float add = QT == 3 ? sum_quarters(om[b]) : 0.0f;
             add = fmaf(add, 0.0f, add);  // an infinite minimum: NaN
-            add += sum_quarters((spoilt >> b) & 1u ? NAN : 0.0f);
+            if (__builtin_expect(any_spoilt, 0)) add += sum_quarters((spoilt >> b) & 1u ? NAN : 0.0f);
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
