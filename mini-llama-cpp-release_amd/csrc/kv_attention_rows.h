@@ -49,7 +49,7 @@ struct TileScales {
 constexpr uint32_t kBad = 1, kFar = 2;
 constexpr float kLift = 256.0f;  // operands lie in LDS times this
 constexpr float kWeightLift = 9.0f;  // log2 of what weights are split times, at the running maximum
-constexpr int kZeroLog = -90;  // taken for a position whose values are zeros: others count until weights differ by 2^90
+constexpr int kLeastLog = -90;  // of a position's values over their blocks' powers of two, zeros too (sums of 2^-ev stay finite)
 constexpr float kFloor = 0x1p-80f;  // f32: the power of two of a block of zeros, or of elements this small
 
 template <int QT, int NB>
@@ -464,13 +464,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     const bool zeros = size_of(d, add) <= (QT == 0 ? kFloor : 0.0f);
                     const float least = over_blocks(counts && !zeros ? size : INFINITY, [](float x, float y) { return fminf(x, y); });
                     const float any_zeros = over_blocks(counts && zeros ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); });
-                    // (no block that counts leaves the infinity; where all are zeros a power of two far below the others')
+                    // (no block that counts leaves the infinity; where all are zeros the power of two is far below the others')
                     const bool all_zeros = least == INFINITY && any_zeros != 0.0f;
                     const bool near = values ? least >= low && top < high && any_zeros == 0.0f
                                              : top == 0.0f || (least >= low && top < high && !(QT == 0 && all_zeros));
                     const bool even = least >= top * (values ? 0x1p-9f : 0x1p-14f) && (!values || any_zeros == 0.0f || all_zeros);
                     uneven = !(near || even);
-                    e = near || uneven ? 0 : values ? (all_zeros ? kZeroLog : exponent(top) - 2) : exponent(top) - 5;
+                    e = near || uneven ? 0 : values ? max(exponent(top) - 2, kLeastLog) : exponent(top) - 5;
                     lift = ldexpf(kLift * unit, -e);
                     flags |= (__any(e != 0 || bad || uneven) ? kFar : 0u) | (values && __any(bad) ? kBad : 0u);
                 }

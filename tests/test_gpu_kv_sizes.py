@@ -253,3 +253,16 @@ def test_values_change_size_behind_the_first_tile(hip, orc, kind, first, then):
         v[:32, :, dims] *= np.float32(first)
         v[32:, :, dims] *= np.float32(then)
         check(Case(hip, orc, kind, [(70, 200)], 4, 2, 96, values=v))
+
+
+@pytest.mark.parametrize("new", [3, 70])
+@pytest.mark.parametrize("before", [1.0, 1e-7, 1e7])
+def test_values_below_the_floor_of_a_block(hip, orc, new, before):
+    """f32 values below 2^-80, which share one power of two, behind ones of other sizes that nobody sees any more."""
+    rng = np.random.default_rng(14)
+    v = rng.standard_normal((300, 2, 64)).astype(np.float32)
+    v[:64] *= np.float32(before)
+    v[64:] *= np.float32(4e-25)
+    check(Case(hip, orc, "f32", [(new, 300)], 4, 2, 64, values=v, window=100, seed=1))
+    v[:64] = 0.0
+    check(Case(hip, orc, "f32", [(new, 300)], 4, 2, 64, values=v, seed=1))
