@@ -457,13 +457,21 @@ int mlq_hip_kv_write(mlq_kv_plan_t plan, int layer, const float* k, const float*
  * != 0, the new tokens' alone. */
 int mlq_hip_kv_read(mlq_kv_plan_t plan, int layer, int new_only, float* k, float* v, void* stream);
 /* out [tokens][n_heads][head_dim]: attention of the new tokens' q over the pages
- * of `layer`, which hold the new tokens too (write first).  f32 throughout: the
- * products run as pairs of fp16 parts.  A position a token does not see has no
- * part in its result, whatever it holds.  A 32-element block of a key or value
- * that holds an element that is not finite (in f32 caches also one of magnitude
- * 2^80 or more, in quantized ones a scale that is not finite) counts as NaN for
- * the tokens that see it; f32 elements below 2^-80 are taken to 2^-100.  The same
- * call gives the same bits. */
+ * of `layer`, which hold the new tokens too (write first).  A position a token does
+ * not see has no part in its result, whatever it holds.  A 32-element block of a key
+ * or value that holds an element that is not finite (in f32 caches also one of
+ * magnitude 2^80 or more, in quantized ones a scale or minimum that is not finite)
+ * counts as NaN for the tokens that see it; f32 elements below 2^-80 are taken to
+ * 2^-100.  The same call gives the same bits.
+ * Scores, weights and sums are f32, the products pairs of fp16 parts: an element of q
+ * and of an f32 cache keeps 2^-22 of the largest of its 32-element block, and a
+ * result is as near as f32 sums of its block's values are, whatever the head's other
+ * blocks hold.  (Weights below 2^-90 of a row's largest may be lost where that one's
+ * values are zeros.)  With more than 64 query rows a KV head in a sequence (new
+ * tokens times grouped heads), rows whose query has blocks more than 2^13 apart, or
+ * that see a position whose key blocks lie more than 2^14 apart, or whose value blocks
+ * lie more than 2^9 apart beside what the sequence's other positions hold in them, are
+ * done in plain f32, 12 to 30 times as slow. */
 int mlq_hip_kv_attention(mlq_kv_plan_t plan, int layer, const float* q, float* out, void* stream);
 
 /* Kernel selection introspection: name of the kernel the next call with this

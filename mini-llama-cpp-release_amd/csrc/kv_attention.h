@@ -36,11 +36,17 @@
 // Bound: memory where the rows of a KV head are few and the contexts fill the chip (64
 // sequences of up to 4000 positions, Q8_0, 8 KV heads of 128, four query heads each: 75 us,
 // 4.7 TB/s of cache); with 4-bit codes half the bytes take about as many instructions, some
-// 550 a tile, in one chain from loads over scores to weights, at two waves a SIMD (100 000
-// positions, Q4_0: 49 us, 2.3 TB/s, vector instructions issue in half of the cycles; 64 more
-// of them a tile cost 1 us).  Short contexts: launch, a chain of four trips to
-// memory (list, page, tile, parts) and the merge (700 positions 10.4 us).  Two workgroups a CU;
-// a third (fewer registers, Q4_0) was no faster, and parts beyond one round of them slower.
+// 625 a tile (75 of them for the blocks' frames and factors).  100 000 positions, Q4_0: 51 us, 2.2 TB/s;
+// a wave lives for 31 of them, and vector instructions issue in four fifths of its cycles at two waves a SIMD;
+// the rest is the launch and the merge of 64 parts, which takes each wave of the last workgroup 16 trips
+// to memory one after the other.  Short contexts: launch, a chain of four trips to
+// memory (list, page, tile, parts) and the merge (700 positions 11.4 us).  Two workgroups a CU up to a
+// head_dim of 128 (f32: 64), one above; a third (fewer registers, Q4_0, 128) was no faster, and parts beyond one
+// round of them slower.
+//
+// Measured and no faster: a branch that skips the blocks' factors where a query needs none (Q8_0, 64 sequences
+// 78 us), the largest scale of a walk kept in a register (84), the first tile's frames found for all blocks at
+// once.
 #pragma once
 
 #include "kv_layout.h"
@@ -401,7 +407,8 @@ __global__ __launch_bounds__(kThreads, (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1) vo
             return static_cast<float>(i % 2 == 0 ? p.x : p.y);
         };
 
-        // The next tile's loads are under way during this one's work, unless its registers are not enough for both.
+        // The next tile's loads are under way during this one's work, unless its registers are not enough for both:
+        // f32 heads of 256 would keep 2.6 KB a lane in scratch (32 sequences of 4000, 8 KV heads: 1015 us, 399 so).
         constexpr bool AHEAD = QT != 0 || NB <= 4;
         int at = it.first + wave;
         int next_page = 0;

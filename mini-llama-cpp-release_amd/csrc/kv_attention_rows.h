@@ -4,25 +4,33 @@
 // A workgroup of four waves takes 4 x 16 NQ rows of one KV head, a wave 16 NQ of them, and walks
 // tiles of 32 positions that its waves convert for each other: a tile's keys and values are
 // decoded once, and lie in LDS as the MFMA operands they are, split into two fp16 parts
-// (hi + lo; 2^-22 is lost, nothing of a quantized element, which is a code times a binary16
-// scale: at most 19 bits).  Then, all in v_mfma_f32_16x16x32_f16, three products a pair:
+// (hi + lo; 2^-22 of a block's largest is lost, nothing of a Q8_0 or Q4_0 element, which is a code times a
+// binary16 scale: at most 19 bits).  Then, all in v_mfma_f32_16x16x32_f16, three products a pair (low parts
+// times low parts, 2^-22 of an element, are left out):
 //
 //   S^T = K Q^T      A from LDS, B (queries, relative to the row's largest) in registers;
 //   O^T += V^T P^T   A from LDS, B the weights: a lane's eight scores are its eight weights.
 //
-// A position's elements are taken over a power of two where they are far from 1, which comes back
-// in the score (2^ek) and in the weight (P_j = p_j 2^ev_j); the running maximum is that of
-// t_j + ev_j, as in the kernel for few rows, so what a row does not see cannot cost it a digit.
+// A value block is taken over a power of two of its own for the whole item, and a position's elements over
+// one where they are still far from 1, which comes back in the score (2^ek) and in the weight (P_j = p_j 2^ev_j);
+// the running maximum is that of t_j + ev_j.  The weights are one operand for all blocks of a head, so this
+// holds what the few-row kernel's frames do as long as a position's blocks do not differ too much
+// (make_scales); rows that see one where they do become NaN and are done again in plain f32 (plain_rows).
 //
 // One step a tile and one barrier: products of the last tile's values and this one's keys (96 at
 // head_dim 128), then the conversion of the next tile, the loads ahead and the softmax.  Two
 // workgroups fit a CU.  Bound: issue and LDS.  A wave's step issues 1540 cycles of products, about
 // 290 vector instructions and reads 32 KB of operands from LDS; the matrix cores are busy 37 % of the
 // time.  512 tokens of 32 heads after 3500 positions (Q8_0, 8 KV heads of 128): 105 us, 300 TFLOP/s of
-// the formula's operations (900 with the parts); a prompt of 2048 in f32, 32 heads: 170 us, 205.
-// Measured and no faster: eight waves that share a conversion; halves of them in turn on the
-// products and the rest; the products' fences left out; several parts of a split in flight in the
-// merge (spills).
+// the formula's operations (900 with the parts); a prompt of 2048 in f32, 32 heads: 170 us, 204.
+// At head_dim 128 all 256 registers are in use and 35 to 49 more lie in scratch, all but one or two outside of
+// the main loop (two there, before one wait for all loads, cost 9 %).
+// Keys far from 1 take a sixth longer (125 -> 150 us a call).  Rows in plain f32 take 12 to 30 times as long
+// (2.7 ms): one of the last positions' value blocks 1000 times below its others is enough.
+// Measured and no faster: those rows by the kernel for few rows' steps, inline (three times the time of all
+// rows, for want of registers), in a function (127 us) or in a launch behind (4 us a call); eight waves that
+// share a conversion; halves of them in turn on the products and the rest; the products' fences left out;
+// several parts of a split in flight in the merge (spills).
 #pragma once
 
 #include "kv_attention.h"

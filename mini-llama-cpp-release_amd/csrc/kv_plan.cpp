@@ -7,9 +7,10 @@
 namespace mlq {
 namespace {
 
-// A split makes workgroups until there are this many, two a CU as either kernel's registers
-// allow, and no more.  One token over 100000 positions (Q4_0, 8 KV heads), 256 / 512 / 1024 of
-// them: 48 / 46 / 57 us; 8 sequences of 4000 (Q8_0) 21 / 21 / 26.
+// A split makes workgroups until there are this many, two a CU, and no more.  Measured at a head_dim of
+// 128, where either kernel's registers allow two: one token over 100000 positions (Q4_0, 8 KV heads), 256 /
+// 512 / 1024 of them: 48 / 46 / 57 us; 8 sequences of 4000 (Q8_0) 21 / 21 / 26.  (Above 128 one fits a CU and
+// these are two rounds, at 64 three or four fit: not tuned.)
 constexpr int kTargetGroups = 512;
 // Fewer tiles than this are not split further, as the parts' merge would cost more.  One token over
 // 4000 positions, at least 4 / 8 / 16 tiles: 14.9 / 12.8 / 13.8 us; over 700 9.6 / 10.3 / 11.6; 128 rows

@@ -11,8 +11,9 @@ namespace mlq {
 
 constexpr int kKvTile = 32;       // positions per tile: the depth of one MFMA over keys
 constexpr int kKvNarrowRows = 8;  // query rows of a workgroup of the kernel for few rows (fp16 hi and lo parts side by side)
-// Rows of a sequence up to which it runs them.  64 rows over 4000 positions (Q8_0) 26 us, 43 in the
-// kernel for many rows; 128 rows 32 and 45; 16 such sequences of 2000 74 and 69, 142 and 76.
+// Rows of a sequence up to which it runs them.  64 rows over 4000 positions (Q8_0) 21 us, 45 in the
+// kernel for many rows; 128 rows 30 and 46; 16 such sequences of 2000 85 and 77, 150 and 78.  (The number of
+// sequences has no say, so one of 128 rows takes the slower kernel.)
 constexpr int kKvNarrowMost = 64;
 constexpr int kKvWaves = 4;       // waves of an attention workgroup
 
