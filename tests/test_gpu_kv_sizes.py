@@ -266,3 +266,27 @@ def test_values_below_the_floor_of_a_block(hip, orc, new, before):
     check(Case(hip, orc, "f32", [(new, 300)], 4, 2, 64, values=v, window=100, seed=1))
     v[:64] = 0.0
     check(Case(hip, orc, "f32", [(new, 300)], 4, 2, 64, values=v, seed=1))
+
+
+@pytest.mark.parametrize("kind", ["f32", "q4_1"])
+def test_recorded_uneven_rows(hip, orc, kind):
+    """A recorded attention whose workgroups take several items each, some of them with rows that are done in plain
+    f32: replayed, with eager calls in between, it gives the eager call's bits and the 64-bit result."""
+    rng = np.random.default_rng(15)
+    lens = [(70, 90)] * 38 + [(33, 700), (70, 1300)]
+    positions = sum(t for _, t in lens)
+    v = rng.standard_normal((positions, 32, 64)).astype(np.float32)
+    v[rng.random(positions) < 0.004, :, 32:] *= np.float32(1e-4)
+    c = Case(hip, orc, kind, lens, 32, 32, 64, 64, values=v, seed=2)
+    want = check(c)
+    s = hip.stream_create()
+    dq, out = dev(hip, c.q), dev(hip, np.zeros_like(c.q))
+    g = hip.Graph.record(lambda: c.plan.attention(0, dq, out, stream=s), stream=s)
+    for _ in range(3):
+        out.upload(np.zeros(c.q.size, np.float32))
+        g.launch(s)
+        hip.synchronize(s)
+        assert np.array_equal(out.download(np.float32, c.q.size).reshape(c.q.shape), want)
+        assert np.array_equal(c.run(), want)
+    g.destroy()
+    hip.stream_destroy(s)
