@@ -421,12 +421,17 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             return x;
         };
         auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
-        // log2 of a block's power of two for values; one over it, of the block whose scales this thread makes.
-        auto block_exponent = [&](int b) {
-            const float top = fmaxf(fmaxf(block_tops[0][b], block_tops[1][b]), fmaxf(block_tops[2][b], block_tops[3][b]));
-            return top > 0.0f ? min(max(exponent(top), -20), 20) : 0;  // (what is beyond that, in f32's range, stays so over it)
+        // log2 of a block's power of two for values: of its largest in the first tile, -20 .. 20 (what is beyond that,
+        // in f32's range, stays so over it).  A block of zeros there beside others (`asleep`: padded heads) is taken to stay so.
+        constexpr float kZeros = QT == 0 ? kFloor : 0.0f;  // a block of zeros, or nearly
+        auto first_top = [&](int b) {
+            return fmaxf(fmaxf(block_tops[0][b], block_tops[1][b]), fmaxf(block_tops[2][b], block_tops[3][b]));
         };
-        float value_unit;
+        auto block_exponent = [&](float top, bool block_asleep) {
+            return block_asleep ? (QT == 0 ? -80 : 0) : top > 0.0f ? min(max(exponent(top), -20), 20) : 0;
+        };
+        float value_unit;  // one over it, of the block whose scales this thread makes
+        bool asleep;
         // A position, a block and a bound of the block's elements, within a factor of 3; whether a row of the item sees it.
         auto size_of = [&](float d, float add) {
             return QT == 0 ? d : QT == 3 ? fmaf(16.0f, d, fabsf(add)) : (QT == 1 ? 128.0f : 8.0f) * d;
@@ -445,7 +450,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         // largest in the item's first tile; then 1 where all blocks are from 2^-7 to 2^3, else
         // what brings the largest to [2^2, 2^3), which serves blocks from 2^-9 of it on.  (The range is narrow as a weight
         // keeps 2^-34 of the row's largest: a position that has that one then has values of at least 2^-10 of any
-        // other's.)  What else there is, a value's block of zeros beside others too, leaves the rows that see it to plain_rows.
+        // other's.)  What else there is, a value's block of zeros beside others too unless it is asleep, leaves the rows
+        // that see it to plain_rows.
         // Positions that no row of the item sees are zeros.
         auto make_scales = [&](int i) {
             Scales* const s = scales + slot_of(i);
@@ -463,13 +469,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 int e = 0;
                 bool bad = false, nothing = false, uneven = false;
                 const float high = values ? 0x1p3f : 0x1p7f, low = values ? 0x1p-7f : 0x1p-10f;
-                if (__builtin_expect(!__all((size >= low && size < high) || 32 * block >= hd), 0)) {
+                const bool quiet = 32 * block >= hd || (QT != 0 && size == 0.0f && (!values || asleep));
+                if (__builtin_expect(!__all((size >= low && size < high) || quiet), 0)) {
                     nothing = !seen_by_some(i, key);
-                    bad = !nothing && !(size < INFINITY);
-                    const bool counts = !nothing && !bad && 32 * block < hd;
+                    bad = !nothing && !(size_of(d, add) < INFINITY);
+                    const bool zeros = size_of(d, add) <= kZeros, rests = values && asleep;
+                    const bool real = !nothing && !bad && 32 * block < hd, counts = real && !rests;
                     const float top = over_blocks(counts ? size : 0.0f, [](float x, float y) { return fmaxf(x, y); });
-                    // a block of zeros, or nearly
-                    const bool zeros = size_of(d, add) <= (QT == 0 ? kFloor : 0.0f);
+                    // (a block that wakes makes the position uneven)
+                    const float wakes = over_blocks(real && rests && !zeros ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); });
                     const float least = over_blocks(counts && !zeros ? size : INFINITY, [](float x, float y) { return fminf(x, y); });
                     const float any_zeros = over_blocks(counts && zeros ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); });
                     // (no block that counts leaves the infinity; where all are zeros the power of two is far below the others')
@@ -477,7 +485,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     const bool near = values ? least >= low && top < high && any_zeros == 0.0f
                                              : top == 0.0f || (least >= low && top < high && !(QT == 0 && all_zeros));
                     const bool even = least >= top * (values ? 0x1p-9f : 0x1p-14f) && (!values || any_zeros == 0.0f || all_zeros);
-                    uneven = !(near || even);
+                    uneven = !(near || even) || wakes != 0.0f;
                     e = near || uneven ? 0 : values ? max(exponent(top) - 2, kLeastLog) : exponent(top) - 5;
                     lift = ldexpf(kLift * unit, -e);
                     flags |= (__any(e != 0 || bad || uneven) ? kFar : 0u) | (values && __any(bad) ? kBad : 0u);
@@ -489,7 +497,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 }
                 if (block < NB) {
                     // keys: NaN through to the score; values: zero here, NaN for the rows that see it (`bad`)
-                    const bool other = bad || nothing || uneven;
+                    const bool other = bad || nothing || uneven || !(lift < INFINITY);
                     const float instead = values || !bad ? 0.0f : NAN;
                     if (values) s->bad[block][key] = bad;
                     s->scale[values][0][block][key] = static_cast<T>(other ? instead : QT == 0 ? lift : d * lift);
@@ -611,7 +619,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
             if (lane < PER) block_tops[wave][lane] = top;
         }
         __syncthreads();
-        value_unit = ldexpf(1.0f, -block_exponent(threadIdx.x % PER));
+        {
+            const float top = first_top(threadIdx.x % PER);
+            const float any = over_blocks(top, [](float x, float y) { return fmaxf(x, y); });
+            asleep = top <= kZeros && any > kZeros;
+            value_unit = ldexpf(1.0f, -block_exponent(top, asleep));
+        }
         // what the first step takes for the values of a tile before the first
         for (int f = wave; f < 2 * FRAGS; f += kKvWaves) operand(1, 2 + f / FRAGS, f % FRAGS)[lane] = h8_t{0, 0, 0, 0, 0, 0, 0, 0};
         make_scales(0);
@@ -813,13 +826,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         }
         products(false, n);
 
+        float any_first = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) any_first = fmaxf(any_first, first_top(b));
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
             l[u] = sum_quarters(l[u]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float add = sum_quarters((spoilt >> (u * NB + b)) & 1u ? NAN : 0.0f);
-                const int e = block_exponent(b);
+                const int e = block_exponent(first_top(b), first_top(b) <= kZeros && any_first > kZeros);
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll

@@ -290,3 +290,26 @@ def test_recorded_uneven_rows(hip, orc, kind):
         assert np.array_equal(c.run(), want)
     g.destroy()
     hip.stream_destroy(s)
+
+
+@pytest.mark.parametrize("kind", list(QT))
+@pytest.mark.parametrize("new", [3, 70])
+def test_padded_heads(hip, orc, kind, new):
+    """A head's last blocks are zeros in keys, values and queries, up to some position or throughout; rows that
+    see where they are not, zeros in all blocks behind, tiny ones."""
+    rng = np.random.default_rng(16)
+    for hd, until, behind in ((128, 300, 1.0), (96, 300, 1.0), (128, 250, 1.0), (128, 290, 1e-3), (128, 299, 300.0), (192, 40, 1.0)):
+        k, v = (rng.standard_normal((300, 2, hd)).astype(np.float32) for _ in range(2))
+        k[:, :, hd - 32:] = 0
+        v[until:] *= np.float32(behind)
+        v[:until, :, hd - 32:] = 0
+        v[270:275] = 0
+        c = Case(hip, orc, kind, [(new, 300)], 4, 2, hd, keys=k, values=v)
+        c.q[:, :, hd - 32:] = 0
+        check(c)
+    v = rng.standard_normal((300, 2, 64)).astype(np.float32)
+    v[:32] = 0  # nothing to go by in the first tile
+    check(Case(hip, orc, kind, [(new, 300)], 4, 2, 64, values=v))
+    v[:, :, 32:] *= np.float32(1e-25)
+    v[100:110, :, :32] = 0
+    check(Case(hip, orc, kind, [(new, 300)], 4, 2, 64, values=v), dims=slice(0, 32))
