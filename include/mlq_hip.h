@@ -471,8 +471,9 @@ int mlq_hip_kv_read(mlq_kv_plan_t plan, int layer, int new_only, float* k, float
  * tokens times grouped heads), rows whose query has blocks more than 2^13 apart, or
  * that see a position whose key blocks lie more than 2^14 apart, or whose value blocks
  * lie more than 2^9 apart beside what the sequence's other positions hold in them
- * (blocks of zeros throughout, as in padded heads, do not count), are done in plain
- * f32, 12 to 30 times as slow. */
+ * (blocks of zeros throughout, as in padded heads, do not count, in f32 only where the
+ * position's others lie within 2^-9 and 2^8 of what the sequence holds in them), are
+ * done in plain f32, 12 to 30 times as slow. */
 int mlq_hip_kv_attention(mlq_kv_plan_t plan, int layer, const float* q, float* out, void* stream);
 
 /* Kernel selection introspection: name of the kernel the next call with this

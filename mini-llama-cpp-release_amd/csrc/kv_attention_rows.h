@@ -423,12 +423,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         auto slot_of = [](int i) { return i % 3; };  // of tile i's scales
         // log2 of a block's power of two for values: of its largest in the first tile, -20 .. 20 (what is beyond that,
         // in f32's range, stays so over it).  A block of zeros there beside others (`asleep`: padded heads) is taken to stay so.
+        // (In f32 it may hold elements up to kFloor: over 2^-74 they are operands up to 2^3 (times 2^-ev), and 2^-100 is far
+        // above what operands lose, 2^-25.)
         constexpr float kZeros = QT == 0 ? kFloor : 0.0f;  // a block of zeros, or nearly
         auto first_top = [&](int b) {
             return fmaxf(fmaxf(block_tops[0][b], block_tops[1][b]), fmaxf(block_tops[2][b], block_tops[3][b]));
         };
         auto block_exponent = [&](float top, bool block_asleep) {
-            return block_asleep ? (QT == 0 ? -80 : 0) : top > 0.0f ? min(max(exponent(top), -20), 20) : 0;
+            return block_asleep ? (QT == 0 ? -74 : 0) : top > 0.0f ? min(max(exponent(top), -20), 20) : 0;
         };
         float value_unit;  // one over it, of the block whose scales this thread makes
         bool asleep;
@@ -476,8 +478,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     const bool zeros = size_of(d, add) <= kZeros, rests = values && asleep;
                     const bool real = !nothing && !bad && 32 * block < hd, counts = real && !rests;
                     const float top = over_blocks(counts ? size : 0.0f, [](float x, float y) { return fmaxf(x, y); });
-                    // (a block that wakes makes the position uneven)
-                    const float wakes = over_blocks(real && rests && !zeros ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); });
+                    // 1: a block is asleep, 2: and wakes, which makes the position uneven
+                    const float sleeps = over_blocks(real && rests ? (zeros ? 1.0f : 2.0f) : 0.0f, [](float x, float y) { return fmaxf(x, y); });
                     const float least = over_blocks(counts && !zeros ? size : INFINITY, [](float x, float y) { return fminf(x, y); });
                     const float any_zeros = over_blocks(counts && zeros ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); });
                     // (no block that counts leaves the infinity; where all are zeros the power of two is far below the others')
@@ -485,8 +487,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                     const bool near = values ? least >= low && top < high && any_zeros == 0.0f
                                              : top == 0.0f || (least >= low && top < high && !(QT == 0 && all_zeros));
                     const bool even = least >= top * (values ? 0x1p-9f : 0x1p-14f) && (!values || any_zeros == 0.0f || all_zeros);
-                    uneven = !(near || even) || wakes != 0.0f;
-                    e = near || uneven ? 0 : values ? max(exponent(top) - 2, kLeastLog) : exponent(top) - 5;
+                    e = near ? 0 : values ? max(exponent(top) - 2, kLeastLog) : exponent(top) - 5;
+                    // (elements up to kFloor of a block asleep: below 2^15 from 2^-12 on, held to 2^-100 up to 2^6)
+                    uneven = !(near || even) || sleeps == 2.0f || (QT == 0 && sleeps != 0.0f && (e < -12 || e > 6));
+                    if (uneven) e = 0;
                     lift = ldexpf(kLift * unit, -e);
                     flags |= (__any(e != 0 || bad || uneven) ? kFar : 0u) | (values && __any(bad) ? kBad : 0u);
                 }

@@ -313,3 +313,24 @@ def test_padded_heads(hip, orc, kind, new):
     v[:, :, 32:] *= np.float32(1e-25)
     v[100:110, :, :32] = 0
     check(Case(hip, orc, kind, [(new, 300)], 4, 2, 64, values=v), dims=slice(0, 32))
+
+
+@pytest.mark.parametrize("new", [3, 70])
+@pytest.mark.parametrize("size", [1.0, 300.0, 1e-3, 1e12, 1e-12, 1e-20, 1e-24])
+def test_value_blocks_below_the_floor_beside_larger_ones(hip, orc, new, size):
+    """f32 values below 2^-80 throughout a block, but not zeros, beside a block of another size: they are taken to
+    2^-100, and no size beside them makes them overflow.  (The tolerance is the bound and that 2^-100, once: the
+    weights sum to one.)"""
+    rng = np.random.default_rng(17)
+    for tiny, total in ((1e-25, 300), (1e-26, 1500)):
+        v = rng.standard_normal((total, 2, 64)).astype(np.float32)
+        v[:, :, :32] *= np.float32(size)
+        v[:, :, 32:] = np.clip(v[:, :, 32:], -4, 4) * np.float32(tiny)
+        v[total - 60:total - 50, :, :32] *= np.float32(1e-4)  # positions with a power of two of their own
+        v[total - 40:total - 30, :, :32] *= np.float32(1e4)
+        v[total - 20:total - 10, :, :32] = 0
+        c = Case(hip, orc, "f32", [(new, total)], 4, 2, 64, values=v, seed=3)
+        got = c.run()
+        want, bound = attention_by_block(c.q, c.held[0], c.held[1])
+        err = np.abs(got - want) / (bound + 2.0 ** -100)
+        assert (err <= 1).all(), (tiny, float(np.max(err)), int(np.isnan(err).sum()))
