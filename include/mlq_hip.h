@@ -467,13 +467,14 @@ int mlq_hip_kv_read(mlq_kv_plan_t plan, int layer, int new_only, float* k, float
  * and of an f32 cache keeps 2^-22 of the largest of its 32-element block, and a
  * result is as near as f32 sums of its block's values are, whatever the head's other
  * blocks hold.  (Weights below 2^-90 of a row's largest may be lost where that one's
- * values are zeros, weights below 2^-126 of it anyhow.)  With more than 64 query rows a KV head in a sequence (new
- * tokens times grouped heads), rows whose query has blocks more than 2^13 apart, or
- * that see a position whose key blocks lie more than 2^14 apart, or whose value blocks
- * lie more than 2^9 apart beside what the sequence's other positions hold in them
- * (blocks of zeros throughout, as in padded heads, do not count, in f32 only where the
- * position's others lie within 2^-9 and 2^8 of what the sequence holds in them), are
- * done in plain f32, 12 to 30 times as slow. */
+ * values are zeros, weights below 2^-126 of it anyhow.)  With more than 64 query
+ * rows a KV head in a sequence (new tokens times grouped heads), rows whose query
+ * has blocks more than 2^13 apart, or that see a position whose key blocks lie more
+ * than 2^14 apart, or whose value blocks lie more than 2^9 apart beside what the
+ * sequence's other positions hold in them (blocks of zeros throughout, as in padded
+ * heads, do not count, in f32 only where the position's others lie within 2^-9 and
+ * 2^8 of what the sequence holds in them), are done in plain f32, 12 to 30 times as
+ * slow. */
 int mlq_hip_kv_attention(mlq_kv_plan_t plan, int layer, const float* q, float* out, void* stream);
 
 /* Kernel selection introspection: name of the kernel the next call with this
