@@ -477,6 +477,81 @@ int mlq_hip_kv_read(mlq_kv_plan_t plan, int layer, int new_only, float* k, float
  * slow. */
 int mlq_hip_kv_attention(mlq_kv_plan_t plan, int layer, const float* q, float* out, void* stream);
 
+/* ---- Decoding with several candidates over the paged cache ----
+ * No counterpart in the reference, which decodes one token of one sequence at a
+ * time (src/forward.cpp:865-903).
+ *
+ * A plan of trees: a step's new tokens of a sequence may be a tree of drafted
+ * tokens, which one pass through the model checks together.  The arguments are
+ * mlq_hip_kv_plan_create's; max_nodes, up to 1024: of a sequence's tree. */
+int mlq_hip_kv_tree_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
+                                int max_tokens, int max_pages, int max_nodes, mlq_kv_plan_t* out);
+/* The batch of a plan of trees, as mlq_hip_kv_plan_set: sequence s has
+ * kv_len[s] - new_tokens[s] positions before its tree of new_tokens[s] nodes (0:
+ * none).  parents [tokens of the batch]: each node's parent among its sequence's
+ * nodes, an earlier one, or -1 where it follows what came before the tree (more
+ * than one may); NULL: every node follows the one before it, and so does
+ * mlq_hip_kv_plan_set.  Node i lies in slot kv_len - new_tokens + i of its
+ * sequence and has position kv_len - new_tokens + its depth: mlq_hip_kv_write
+ * rotates by that, and in mlq_hip_kv_attention it sees what came before the tree,
+ * its ancestors and itself, as far as the window (of positions) and the first
+ * tokens go. */
+int mlq_hip_kv_plan_set_tree(mlq_kv_plan_t plan, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
+                             const int* parents, void* stream);
+/* Checks drafted trees greedily.  logits [tokens][vocab]: what the model says
+ * after each node; tokens: the nodes' tokens.  picks [tokens] is the first index
+ * of each row's largest logit, -1 where one is infinite or NaN (as
+ * mlq_hip_quant_linear_argmax).  A sequence's first node is its last token, which
+ * is certain; from there its path goes on to the lowest child whose token is the
+ * last node's pick.  n_kept [sequences]: the path's nodes (0 of an empty tree);
+ * kept [tokens]: at the sequence's rows, the path's node indexes, then -1; next
+ * [sequences]: the pick of the path's last node (-1 of an empty tree).  Device buffers
+ * that start 4-byte aligned, outputs apart from each other and the inputs.
+ * Asynchronous on `stream`; under graph capture as the calls above (max_tokens
+ * rows, max_seqs sequences). */
+int mlq_hip_kv_tree_pick(mlq_kv_plan_t plan, const float* logits, int vocab, const int32_t* tokens, int32_t* picks,
+                         int32_t* n_kept, int32_t* kept, int32_t* next, void* stream);
+/* Keeps a path of each sequence's tree: n_kept[s] nodes (0: none), the first one
+ * without a parent, each other one a child of the one before; kept: their
+ * indexes, one sequence's after the other's (host arrays).  Their keys and values
+ * move, in every layer, to the first slots of the tree, so that the sequence goes
+ * on with kv_len - new_tokens + n_kept[s] positions; what the tree's other slots
+ * hold is then undefined.  The batch stays set.  Asynchronous on `stream`; not
+ * under graph capture. */
+int mlq_hip_kv_keep(mlq_kv_plan_t plan, const int* n_kept, const int* kept, void* stream);
+/* Copies the first positions[i] positions (NULL: all) of page from[i] to page
+ * to[i], in every layer: a sequence that forks keeps its full pages in common and
+ * takes a copy of its last one.  No page may be written twice, or read and
+ * written.  Positions up to the next multiple of 32 are copied with them.  Host
+ * arrays, copied before the call returns.  Asynchronous on `stream`; a recorded
+ * call copies the same pages at every replay. */
+int mlq_hip_kv_copy_pages(mlq_kv_cache_t cache, int n, const int* from, const int* to, const int* positions, void* stream);
+
+/* Beam search's selection.  Each of `groups` sequences has `beams` beams: their
+ * scores (log probabilities so far) [groups][beams] and logits
+ * [groups][beams][vocab].  A continuation of beam b with token t has the value
+ * score + log_softmax(logits)[t], taken in 64 bits; the `keep` largest of a group
+ * come out, largest first, as the beam (parents), the token and the value rounded
+ * to f32 [groups][keep].  Of equal values the lower beam comes first, in a beam
+ * the larger logit, then the lower token.
+ * A logit of -Inf is no continuation, and a beam whose score is -Inf has none (a
+ * search starts with one beam).  ended (NULL: none) [groups][beams]: a beam with
+ * another value than 0 has one continuation, end_token at its own score, and its
+ * logits are not looked at.  Where there are fewer than `keep`, the rest is beam
+ * -1, token -1, value -Inf.  A group with a score that is NaN or +Inf, or such a
+ * logit of a beam that goes on, comes out as -1, -1, NaN throughout.
+ * A handle holds the workspace: its calls must not overlap in time (one stream,
+ * or events), graph replays included, and it outlives the graphs that recorded
+ * them.  max_beams and max_keep: up to 64.  Created outside graph capture.  Device
+ * buffers that start 4-byte aligned, outputs apart from each other and the
+ * inputs.  Asynchronous on `stream`; the same call gives the same bits. */
+typedef struct mlq_beam_s* mlq_beam_t;
+int mlq_hip_beam_create(int device, int max_groups, int max_beams, int max_vocab, int max_keep, mlq_beam_t* out);
+int mlq_hip_beam_destroy(mlq_beam_t beam);
+int mlq_hip_beam_select(mlq_beam_t beam, const float* logits, const float* scores, const int32_t* ended, int end_token,
+                        int groups, int beams, int vocab, int keep, int32_t* parents, int32_t* tokens,
+                        float* out_scores, void* stream);
+
 /* Kernel selection introspection: name of the kernel the next call with this
  * shape would launch (for profiles and tests). */
 int mlq_hip_kernel_name(int qtype, int rows, int out_features, int in_features, char* buf,

@@ -1,0 +1,37 @@
+// Beam selection (beam.hip): what its launch takes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace mlq {
+
+constexpr int kBeamMostBeams = 64;  // of a group
+constexpr int kBeamMostKeep = 64;
+constexpr int kBeamPart = 8192;     // logits of a part of a row
+
+inline int beam_parts(int vocab) { return (vocab + kBeamPart - 1) / kBeamPart; }
+
+// A part of a row: its largest logit and the sum of exp(logit - largest).
+struct BeamPart {
+    double sum;
+    float largest;  // NaN: a logit is NaN or +Inf
+    int pad;
+};
+
+struct BeamCall {
+    const float* logits;  // [groups][beams][vocab]
+    const float* scores;  // [groups][beams]
+    const int* ended;     // [groups][beams], or null
+    int end_token, groups, beams, vocab, keep;
+    int *parents, *tokens;  // [groups][keep]
+    float* out_scores;      // [groups][keep]
+    // Workspace: of every part its BeamPart and the keys of its best `keep` logits, best first.
+    BeamPart* parts;
+    unsigned long long* best;
+};
+hipError_t launch_beam_select(const BeamCall& c, hipStream_t s);
+
+}  // namespace mlq

@@ -28,6 +28,9 @@ struct KvMemory {
     uint8_t* mem = nullptr;
 
     size_t bytes() const { return layer_bytes * n_layers; }
+    mlq::KvView view(int layer) const {
+        return mlq::KvView{mem + layer_bytes * layer, qtype, nb, head_dim, n_kv, page_size / mlq::kKvTile};
+    }
     ~KvMemory() {
         if (mem == nullptr) return;
         (void)hipSetDevice(device);
@@ -57,9 +60,12 @@ struct mlq_kv_plan_s {
     float* partial[2] = {nullptr, nullptr};
     unsigned* arrived[2] = {nullptr, nullptr};
     void* work = nullptr;
-    // The batch.
+    // Of trees: keys of the picks' parts.
+    unsigned long long* keys = nullptr;
+    // The batch; of trees also its sequences, parents and pages (for what is kept of it).
     bool set = false;
     int n_tokens = 0, n_positions = 0;
+    mlq::KvBatch batch;
     int counts[mlq::kKvCounts] = {};
     // Turns per position of the last theta.
     float theta = 0.0f;
@@ -74,10 +80,20 @@ struct mlq_kv_plan_s {
         l.items[1] = reinterpret_cast<const mlq::KvAttnItem*>(lists + at[4]);
         return l;
     }
-    mlq::KvView view(int layer) const {
-        return mlq::KvView{kv->mem + kv->layer_bytes * layer, kv->qtype, kv->nb, kv->head_dim, kv->n_kv,
-                           kv->page_size / mlq::kKvTile};
+    mlq::KvTreeLists tree_lists() const {
+        mlq::KvTreeLists l;
+        l.counts = reinterpret_cast<const int*>(lists + at[0]);
+        l.pages = reinterpret_cast<const mlq::KvPage*>(lists + at[2]);
+        l.items[0] = reinterpret_cast<const mlq::KvTreeItem*>(lists + at[3]);
+        l.items[1] = reinterpret_cast<const mlq::KvTreeItem*>(lists + at[4]);
+        l.seqs = reinterpret_cast<const mlq::KvTreeSeq*>(lists + at[5]);
+        l.pos = reinterpret_cast<const int*>(lists + at[6]);
+        l.parents = reinterpret_cast<const int*>(lists + at[7]);
+        l.masks = reinterpret_cast<const uint32_t*>(lists + at[8]);
+        return l;
     }
+    bool trees() const { return shape.max_nodes > 0; }
+    mlq::KvView view(int layer) const { return kv->view(layer); }
     ~mlq_kv_plan_s() {
         if (kv) (void)hipSetDevice(kv->device);
         for (int i = 0; i < 2; ++i) {
@@ -134,9 +150,166 @@ int check_rows(const void* ptr, mlq_kv_plan_t p, const char* caller, const char*
                                static_cast<size_t>(rows) * heads * p->kv->head_dim * sizeof(float));
 }
 
+// A call that only batches of trees have.
+int check_trees(mlq_kv_plan_t p, const char* caller) {
+    if (p == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null plan");
+    if (!p->trees()) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": the plan holds no trees");
+    if (!p->set) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": the plan holds no batch");
+    return mlq::abi_device(p->kv->device);
+}
+
+int check_words(const void* ptr, int device, const char* caller, const char* what, size_t words) {
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0) {
+        return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": " + what + " is not 4-byte aligned");
+    }
+    return mlq::abi_device_ptr(ptr, device, caller, what, words * 4);
+}
+
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x < y + nb && y < x + na;
+}
+
+// max_nodes 0: a plan of plain sequences.
+int create_plan(const char* caller, mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
+                int max_tokens, int max_pages, int max_nodes, mlq_kv_plan_t* out) {
+    if (out == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null output handle");
+    *out = nullptr;
+    return entry(caller, [&]() -> int {
+        const std::string who(caller);
+        if (cache == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null cache");
+        const KvMemory& kv = *cache->kv;
+        if (n_heads <= 0 || n_heads % kv.n_kv != 0) {
+            return abi_fail(MLQ_ERR_SHAPE, who + ": " + std::to_string(n_heads) + " heads over " + std::to_string(kv.n_kv) +
+                                               " KV heads");
+        }
+        if (window < 0 || sinks < 0) return abi_fail(MLQ_ERR_INVALID, who + ": negative window or sinks");
+        if (sinks > 0 && window == 0) return abi_fail(MLQ_ERR_INVALID, who + ": sinks need a window");
+        if (!(scale == 0.0f || (std::fabs(scale) >= 0x1p-100f && std::fabs(scale) <= 0x1p100f))) {
+            return abi_fail(MLQ_ERR_INVALID, who + ": scale is neither 0 nor of magnitude 2^-100 to 2^100");
+        }
+        if (max_seqs <= 0 || max_tokens <= 0 || max_pages <= 0) {
+            return abi_fail(MLQ_ERR_SHAPE, who + ": empty plans are not supported");
+        }
+        if (static_cast<int64_t>(max_tokens) * n_heads > kMost || static_cast<int64_t>(max_pages) * kv.page_size > kMost ||
+            max_seqs > 1 << 20) {
+            return abi_fail(MLQ_ERR_LIMIT, who + ": more than 2^30 token heads or positions, or 2^20 sequences");
+        }
+        auto p = std::make_unique<mlq_kv_plan_s>();
+        p->kv = cache->kv;
+        p->n_heads = n_heads;
+        p->scale = scale != 0.0f ? scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(kv.head_dim)));
+        p->shape = mlq::KvPlanShape{kv.page_size, kv.n_pages, kv.n_kv, n_heads / kv.n_kv, mlq::kv_wide_rows(kv.nb),
+                                    window, sinks, max_seqs, max_tokens, max_pages, max_nodes,
+                                    mlq::kv_tree_rows(kv.nb)};
+        const mlq::KvPlanLimits lim = mlq::kv_plan_limits(p->shape);
+        if (lim.masks > kMost) return abi_fail(MLQ_ERR_LIMIT, who + ": more than 2^30 words of who sees whom");
+        const bool trees = max_nodes > 0;
+        const size_t item = trees ? sizeof(mlq::KvTreeItem) : sizeof(mlq::KvAttnItem), of_trees = trees ? 1 : 0;
+        const size_t sizes[mlq::kKvParts] = {
+            mlq::kKvCounts * sizeof(int), static_cast<size_t>(lim.fresh) * sizeof(mlq::KvTileItem),
+            static_cast<size_t>(max_pages) * sizeof(mlq::KvPage), static_cast<size_t>(lim.items[0]) * item,
+            static_cast<size_t>(lim.items[1]) * item, of_trees * max_seqs * sizeof(mlq::KvTreeSeq),
+            of_trees * max_tokens * sizeof(int), of_trees * max_tokens * sizeof(int),
+            static_cast<size_t>(lim.masks) * sizeof(uint32_t)};
+        for (int i = 0; i < mlq::kKvParts; ++i) {
+            p->at[i] = p->list_bytes;
+            p->list_bytes += (sizes[i] + 255) / 256 * 256;
+        }
+        const int rc = mlq::abi_device(kv.device);
+        if (rc != MLQ_OK) return rc;
+        const hipStream_t s = mlq::abi_stream(kv.device, nullptr);
+        if (mlq::abi_capturing(s)) return abi_fail(MLQ_ERR_INVALID, who + ": not under graph capture");
+        void* mem = nullptr;
+        MLQ_KV_HIP(hipMalloc(&mem, p->list_bytes));
+        p->lists = static_cast<uint8_t*>(mem);
+        for (int i = 0; i < 2; ++i) {
+            void* host = nullptr;
+            MLQ_KV_HIP(hipHostMalloc(&host, p->list_bytes, hipHostMallocDefault));
+            p->pinned[i] = static_cast<uint8_t*>(host);
+            MLQ_KV_HIP(hipEventCreateWithFlags(&p->uploaded[i], hipEventDisableTiming));
+        }
+        size_t floats[2], words[2];
+        for (int i = 0; i < 2; ++i) {
+            words[i] = (static_cast<size_t>(lim.slots[i]) * kv.n_kv + 63) / 64 * 64;
+            floats[i] = static_cast<size_t>(lim.slots[i]) * kv.n_kv *
+                        (trees ? mlq::kv_tree_partial_floats(kv.nb, i) : mlq::kv_partial_floats(kv.nb, i));
+        }
+        const size_t keys = trees ? std::max(max_tokens, mlq::kKvPickParts) : 0;
+        MLQ_KV_HIP(hipMalloc(&p->work, (words[0] + words[1] + floats[0] + floats[1]) * 4 + keys * 8));
+        p->arrived[0] = static_cast<unsigned*>(p->work);
+        p->arrived[1] = p->arrived[0] + words[0];
+        p->partial[0] = reinterpret_cast<float*>(p->arrived[1] + words[1]);
+        p->partial[1] = p->partial[0] + floats[0];
+        p->keys = reinterpret_cast<unsigned long long*>(p->partial[1] + floats[1]);
+        MLQ_KV_HIP(hipMemsetAsync(p->work, 0, (words[0] + words[1]) * 4, s));
+        MLQ_KV_HIP(hipStreamSynchronize(s));
+        *out = p.release();
+        return MLQ_OK;
+    });
+}
+
+int set_plan(const char* caller, mlq_kv_plan_t p, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
+             const int* parents, void* stream) {
+    return entry(caller, [&]() -> int {
+        if (p == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null plan");
+        mlq::KvBatch b;
+        const std::string wrong = mlq::kv_plan_build(p->shape, n_seqs, new_tokens, kv_len, pages, parents, &b);
+        if (!wrong.empty()) return abi_fail(MLQ_ERR_SHAPE, std::string(caller) + ": " + wrong);
+        const int rc = mlq::abi_device(p->kv->device);
+        if (rc != MLQ_OK) return rc;
+        const hipStream_t s = mlq::abi_stream(p->kv->device, stream);
+        if (mlq::abi_capturing(s)) {
+            return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": a batch cannot be set under graph capture");
+        }
+        const bool trees = p->trees();
+        int counts[mlq::kKvCounts];
+        counts[mlq::kKvCountFresh] = static_cast<int>(b.fresh.size());
+        counts[mlq::kKvCountPages] = static_cast<int>(b.pages.size());
+        counts[mlq::kKvCountNarrow] = static_cast<int>(trees ? b.trees[0].size() : b.items[0].size());
+        counts[mlq::kKvCountWide] = static_cast<int>(trees ? b.trees[1].size() : b.items[1].size());
+        counts[mlq::kKvCountSeqs] = static_cast<int>(b.seqs.size());
+        counts[mlq::kKvCountTokens] = b.n_tokens;
+        const void* items[2];
+        size_t item_bytes[2];
+        for (int i = 0; i < 2; ++i) {
+            items[i] = trees ? static_cast<const void*>(b.trees[i].data()) : b.items[i].data();
+            item_bytes[i] = trees ? b.trees[i].size() * sizeof b.trees[i][0] : b.items[i].size() * sizeof b.items[i][0];
+        }
+        const void* from[mlq::kKvParts] = {counts,   b.fresh.data(), b.pages.data(),   items[0],      items[1], b.seqs.data(),
+                                           b.pos.data(), b.parents.data(), b.masks.data()};
+        const size_t bytes[mlq::kKvParts] = {sizeof counts,
+                                             b.fresh.size() * sizeof b.fresh[0],
+                                             b.pages.size() * sizeof b.pages[0],
+                                             item_bytes[0],
+                                             item_bytes[1],
+                                             b.seqs.size() * sizeof b.seqs[0],
+                                             b.pos.size() * sizeof b.pos[0],
+                                             b.parents.size() * sizeof b.parents[0],
+                                             b.masks.size() * sizeof b.masks[0]};
+        const int t = p->turn;
+        MLQ_KV_HIP(hipEventSynchronize(p->uploaded[t]));  // the block's last upload (none yet: done)
+        mlq::KvParts parts;
+        for (int i = 0; i < mlq::kKvParts; ++i) {
+            if (p->at[i] + bytes[i] > (i + 1 < mlq::kKvParts ? p->at[i + 1] : p->list_bytes)) {
+                return abi_fail(MLQ_ERR_LIMIT, std::string(caller) + ": a work list is longer than the plan holds");
+            }
+            if (bytes[i] > 0) std::memcpy(p->pinned[t] + p->at[i], from[i], bytes[i]);
+            parts.src[i] = reinterpret_cast<const uint32_t*>(p->pinned[t] + p->at[i]);
+            parts.dst[i] = reinterpret_cast<uint32_t*>(p->lists + p->at[i]);
+            parts.words[i] = static_cast<int>(bytes[i] / 4);
+        }
+        const hipError_t e = mlq::launch_kv_upload(parts, s);
+        if (e != hipSuccess) return abi_hip_fail(e, caller);
+        MLQ_KV_HIP(hipEventRecord(p->uploaded[t], s));
+        p->turn ^= 1;
+        std::copy(counts, counts + mlq::kKvCounts, p->counts);
+        p->n_tokens = b.n_tokens;
+        p->n_positions = b.n_positions;
+        if (trees) p->batch = std::move(b);
+        p->set = true;
+        return MLQ_OK;
+    });
 }
 
 }  // namespace
@@ -210,119 +383,31 @@ int mlq_hip_kv_cache_destroy(mlq_kv_cache_t cache) {
 
 int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
                            int max_tokens, int max_pages, mlq_kv_plan_t* out) {
-    const char* caller = "hip_kv_plan_create";
-    if (out == nullptr) return abi_fail(MLQ_ERR_INVALID, "hip_kv_plan_create: null output handle");
-    *out = nullptr;
-    return entry(caller, [&]() -> int {
-        const std::string who(caller);
-        if (cache == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null cache");
-        const KvMemory& kv = *cache->kv;
-        if (n_heads <= 0 || n_heads % kv.n_kv != 0) {
-            return abi_fail(MLQ_ERR_SHAPE, who + ": " + std::to_string(n_heads) + " heads over " + std::to_string(kv.n_kv) +
-                                               " KV heads");
-        }
-        if (window < 0 || sinks < 0) return abi_fail(MLQ_ERR_INVALID, who + ": negative window or sinks");
-        if (sinks > 0 && window == 0) return abi_fail(MLQ_ERR_INVALID, who + ": sinks need a window");
-        if (!(scale == 0.0f || (std::fabs(scale) >= 0x1p-100f && std::fabs(scale) <= 0x1p100f))) {
-            return abi_fail(MLQ_ERR_INVALID, who + ": scale is neither 0 nor of magnitude 2^-100 to 2^100");
-        }
-        if (max_seqs <= 0 || max_tokens <= 0 || max_pages <= 0) {
-            return abi_fail(MLQ_ERR_SHAPE, who + ": empty plans are not supported");
-        }
-        if (static_cast<int64_t>(max_tokens) * n_heads > kMost || static_cast<int64_t>(max_pages) * kv.page_size > kMost ||
-            max_seqs > 1 << 20) {
-            return abi_fail(MLQ_ERR_LIMIT, who + ": more than 2^30 token heads or positions, or 2^20 sequences");
-        }
-        auto p = std::make_unique<mlq_kv_plan_s>();
-        p->kv = cache->kv;
-        p->n_heads = n_heads;
-        p->scale = scale != 0.0f ? scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(kv.head_dim)));
-        p->shape = mlq::KvPlanShape{kv.page_size, kv.n_pages, kv.n_kv, n_heads / kv.n_kv, mlq::kv_wide_rows(kv.nb),
-                                    window, sinks, max_seqs, max_tokens, max_pages};
-        const mlq::KvPlanLimits lim = mlq::kv_plan_limits(p->shape);
-        const size_t sizes[mlq::kKvParts] = {
-            mlq::kKvCounts * sizeof(int), static_cast<size_t>(lim.fresh) * sizeof(mlq::KvTileItem),
-            static_cast<size_t>(max_pages) * sizeof(mlq::KvPage), static_cast<size_t>(lim.items[0]) * sizeof(mlq::KvAttnItem),
-            static_cast<size_t>(lim.items[1]) * sizeof(mlq::KvAttnItem)};
-        for (int i = 0; i < mlq::kKvParts; ++i) {
-            p->at[i] = p->list_bytes;
-            p->list_bytes += (sizes[i] + 255) / 256 * 256;
-        }
-        const int rc = mlq::abi_device(kv.device);
-        if (rc != MLQ_OK) return rc;
-        const hipStream_t s = mlq::abi_stream(kv.device, nullptr);
-        if (mlq::abi_capturing(s)) return abi_fail(MLQ_ERR_INVALID, who + ": not under graph capture");
-        void* mem = nullptr;
-        MLQ_KV_HIP(hipMalloc(&mem, p->list_bytes));
-        p->lists = static_cast<uint8_t*>(mem);
-        for (int i = 0; i < 2; ++i) {
-            void* host = nullptr;
-            MLQ_KV_HIP(hipHostMalloc(&host, p->list_bytes, hipHostMallocDefault));
-            p->pinned[i] = static_cast<uint8_t*>(host);
-            MLQ_KV_HIP(hipEventCreateWithFlags(&p->uploaded[i], hipEventDisableTiming));
-        }
-        size_t floats[2], words[2];
-        for (int i = 0; i < 2; ++i) {
-            words[i] = (static_cast<size_t>(lim.slots[i]) * kv.n_kv + 63) / 64 * 64;
-            floats[i] = static_cast<size_t>(lim.slots[i]) * kv.n_kv * mlq::kv_partial_floats(kv.nb, i);
-        }
-        MLQ_KV_HIP(hipMalloc(&p->work, (words[0] + words[1] + floats[0] + floats[1]) * 4));
-        p->arrived[0] = static_cast<unsigned*>(p->work);
-        p->arrived[1] = p->arrived[0] + words[0];
-        p->partial[0] = reinterpret_cast<float*>(p->arrived[1] + words[1]);
-        p->partial[1] = p->partial[0] + floats[0];
-        MLQ_KV_HIP(hipMemsetAsync(p->work, 0, (words[0] + words[1]) * 4, s));
-        MLQ_KV_HIP(hipStreamSynchronize(s));
-        *out = p.release();
-        return MLQ_OK;
-    });
+    return create_plan("hip_kv_plan_create", cache, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages, 0, out);
+}
+
+int mlq_hip_kv_tree_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
+                                int max_tokens, int max_pages, int max_nodes, mlq_kv_plan_t* out) {
+    const char* caller = "hip_kv_tree_plan_create";
+    if (max_nodes < 1 || max_nodes > mlq::kKvMostNodes) {
+        if (out != nullptr) *out = nullptr;
+        return abi_fail(MLQ_ERR_LIMIT, std::string(caller) + ": trees of " + std::to_string(max_nodes) + " nodes, not 1 to " +
+                                           std::to_string(mlq::kKvMostNodes));
+    }
+    return create_plan(caller, cache, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages, max_nodes, out);
 }
 
 int mlq_hip_kv_plan_set(mlq_kv_plan_t p, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
                         void* stream) {
-    const char* caller = "hip_kv_plan_set";
-    return entry(caller, [&]() -> int {
-        if (p == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null plan");
-        mlq::KvBatch b;
-        const std::string wrong = mlq::kv_plan_build(p->shape, n_seqs, new_tokens, kv_len, pages, &b);
-        if (!wrong.empty()) return abi_fail(MLQ_ERR_SHAPE, std::string(caller) + ": " + wrong);
-        const int rc = mlq::abi_device(p->kv->device);
-        if (rc != MLQ_OK) return rc;
-        const hipStream_t s = mlq::abi_stream(p->kv->device, stream);
-        if (mlq::abi_capturing(s)) {
-            return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": a batch cannot be set under graph capture");
-        }
-        int counts[mlq::kKvCounts];
-        counts[mlq::kKvCountFresh] = static_cast<int>(b.fresh.size());
-        counts[mlq::kKvCountPages] = static_cast<int>(b.pages.size());
-        counts[mlq::kKvCountNarrow] = static_cast<int>(b.items[0].size());
-        counts[mlq::kKvCountWide] = static_cast<int>(b.items[1].size());
-        const void* from[mlq::kKvParts] = {counts, b.fresh.data(), b.pages.data(), b.items[0].data(), b.items[1].data()};
-        const size_t bytes[mlq::kKvParts] = {sizeof counts, b.fresh.size() * sizeof b.fresh[0],
-                                             b.pages.size() * sizeof b.pages[0], b.items[0].size() * sizeof b.items[0][0],
-                                             b.items[1].size() * sizeof b.items[1][0]};
-        const int t = p->turn;
-        MLQ_KV_HIP(hipEventSynchronize(p->uploaded[t]));  // the block's last upload (none yet: done)
-        mlq::KvParts parts;
-        for (int i = 0; i < mlq::kKvParts; ++i) {
-            if (p->at[i] + bytes[i] > (i + 1 < mlq::kKvParts ? p->at[i + 1] : p->list_bytes)) {
-                return abi_fail(MLQ_ERR_LIMIT, std::string(caller) + ": a work list is longer than the plan holds");
-            }
-            if (bytes[i] > 0) std::memcpy(p->pinned[t] + p->at[i], from[i], bytes[i]);
-            parts.src[i] = reinterpret_cast<const uint32_t*>(p->pinned[t] + p->at[i]);
-            parts.dst[i] = reinterpret_cast<uint32_t*>(p->lists + p->at[i]);
-            parts.words[i] = static_cast<int>(bytes[i] / 4);
-        }
-        const hipError_t e = mlq::launch_kv_upload(parts, s);
-        if (e != hipSuccess) return abi_hip_fail(e, caller);
-        MLQ_KV_HIP(hipEventRecord(p->uploaded[t], s));
-        p->turn ^= 1;
-        std::copy(counts, counts + mlq::kKvCounts, p->counts);
-        p->n_tokens = b.n_tokens;
-        p->n_positions = b.n_positions;
-        p->set = true;
-        return MLQ_OK;
-    });
+    return set_plan("hip_kv_plan_set", p, n_seqs, new_tokens, kv_len, pages, nullptr, stream);
+}
+
+int mlq_hip_kv_plan_set_tree(mlq_kv_plan_t p, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
+                             const int* parents, void* stream) {
+    const char* caller = "hip_kv_plan_set_tree";
+    if (p == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null plan");
+    if (!p->trees()) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": the plan holds no trees");
+    return set_plan(caller, p, n_seqs, new_tokens, kv_len, pages, parents, stream);
 }
 
 int mlq_hip_kv_plan_destroy(mlq_kv_plan_t p) {
@@ -369,8 +454,9 @@ int mlq_hip_kv_write(mlq_kv_plan_t p, int layer, const float* k, const float* v,
         }
         p->rope.on = theta > 0.0f;
         p->rope.neox = neox != 0;
-        const hipError_t e = mlq::launch_kv_write(p->view(layer), p->device_lists(), recorded ? 0 : p->counts[mlq::kKvCountFresh],
-                                                  static_cast<int>(rows), k, v, q, q_out, p->n_heads, p->rope, s);
+        const hipError_t e = mlq::launch_kv_write(p->view(layer), p->device_lists(), p->trees() ? p->tree_lists().pos : nullptr,
+                                                  recorded ? 0 : p->counts[mlq::kKvCountFresh], static_cast<int>(rows), k, v, q,
+                                                  q_out, p->n_heads, p->rope, s);
         return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
     });
 }
@@ -412,12 +498,125 @@ int mlq_hip_kv_attention(mlq_kv_plan_t p, int layer, const float* q, float* out,
         for (int kind = 0; kind < 2; ++kind) {
             const int count = p->counts[mlq::kKvCountNarrow + kind];
             if (count == 0 && !recorded) continue;
+            if (kind == 1 && p->trees() && p->shape.tree_rows == mlq::kKvTreeRows) continue;  // (all are in the first list)
+            const float to_base_2 = static_cast<float>(p->scale * 1.4426950408889634);
+            if (p->trees()) {
+                const mlq::KvTreeAttention a{p->view(layer), p->tree_lists(), p->shape.group, p->shape.window, p->shape.sinks,
+                                             to_base_2, p->partial[kind], p->arrived[kind]};
+                const hipError_t e = mlq::launch_kv_tree_attention(a, kind, recorded ? 0 : count, q, out, s);
+                if (e != hipSuccess) return abi_hip_fail(e, caller);
+                continue;
+            }
             const mlq::KvAttention a{p->view(layer), p->device_lists(), p->shape.group, p->shape.window, p->shape.sinks,
-                                     static_cast<float>(p->scale * 1.4426950408889634), p->partial[kind], p->arrived[kind]};
+                                     to_base_2, p->partial[kind], p->arrived[kind]};
             const hipError_t e = mlq::launch_kv_attention(a, kind, recorded ? 0 : count, q, out, s);
             if (e != hipSuccess) return abi_hip_fail(e, caller);
         }
         return MLQ_OK;
+    });
+}
+
+int mlq_hip_kv_tree_pick(mlq_kv_plan_t p, const float* logits, int vocab, const int32_t* tokens, int32_t* picks,
+                         int32_t* n_kept, int32_t* kept, int32_t* next, void* stream) {
+    const char* caller = "hip_kv_tree_pick";
+    return entry(caller, [&]() -> int {
+        int rc = check_trees(p, caller);
+        if (rc != MLQ_OK) return rc;
+        if (vocab <= 0) return abi_fail(MLQ_ERR_SHAPE, std::string(caller) + ": vocabulary of " + std::to_string(vocab));
+        const hipStream_t s = mlq::abi_stream(p->kv->device, stream);
+        const bool recorded = mlq::abi_capturing(s);
+        const size_t rows = recorded ? p->shape.max_tokens : p->n_tokens;
+        const size_t seqs = recorded ? p->shape.max_seqs : p->batch.seqs.size();
+        if (seqs == 0) return MLQ_OK;
+        struct Buffer {
+            const void* ptr;
+            const char* what;
+            size_t words;
+        };
+        const Buffer in[2] = {{logits, "logits", rows * vocab}, {tokens, "tokens", rows}};
+        const Buffer out[4] = {{picks, "picks", rows}, {n_kept, "n_kept", seqs}, {kept, "kept", rows}, {next, "next", seqs}};
+        const int device = p->kv->device;
+        for (const Buffer& b : in) {
+            if (b.words > 0 && (rc = check_words(b.ptr, device, caller, b.what, b.words)) != MLQ_OK) return rc;
+        }
+        for (int i = 0; i < 4; ++i) {
+            const Buffer& b = out[i];
+            if (b.words == 0) continue;
+            if ((rc = check_words(b.ptr, device, caller, b.what, b.words)) != MLQ_OK) return rc;
+            for (int j = 0; j < 2 + i; ++j) {
+                const Buffer& o = j < 2 ? in[j] : out[j - 2];
+                if (overlap(b.ptr, b.words * 4, o.ptr, o.words * 4)) {
+                    return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": " + b.what + " overlaps " + o.what);
+                }
+            }
+        }
+        const mlq::KvPick k{p->tree_lists(), logits, vocab, tokens, picks, n_kept, kept, next, p->keys};
+        const hipError_t e = mlq::launch_kv_pick(k, recorded ? -1 : static_cast<int>(rows), recorded ? -1 : static_cast<int>(seqs), s);
+        return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
+    });
+}
+
+int mlq_hip_kv_keep(mlq_kv_plan_t p, const int* n_kept, const int* kept, void* stream) {
+    const char* caller = "hip_kv_keep";
+    return entry(caller, [&]() -> int {
+        const int rc = check_trees(p, caller);
+        if (rc != MLQ_OK) return rc;
+        std::vector<mlq::KvMove> moves;
+        std::vector<int> ends;
+        const std::string wrong = mlq::kv_keep_build(p->shape, p->batch, n_kept, kept, &moves, &ends);
+        if (!wrong.empty()) return abi_fail(MLQ_ERR_SHAPE, std::string(caller) + ": " + wrong);
+        const hipStream_t s = mlq::abi_stream(p->kv->device, stream);
+        if (mlq::abi_capturing(s)) {
+            return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": what is kept of a batch cannot be recorded");
+        }
+        if (moves.empty()) return MLQ_OK;
+        const hipError_t e = mlq::launch_kv_moves(p->view(0), p->kv->n_layers, p->kv->layer_bytes, moves.data(), ends.data(),
+                                                  static_cast<int>(ends.size()), s);
+        return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
+    });
+}
+
+int mlq_hip_kv_copy_pages(mlq_kv_cache_t cache, int n, const int* from, const int* to, const int* positions, void* stream) {
+    const char* caller = "hip_kv_copy_pages";
+    return entry(caller, [&]() -> int {
+        const std::string who(caller);
+        if (cache == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null cache");
+        const KvMemory& kv = *cache->kv;
+        if (n < 0) return abi_fail(MLQ_ERR_SHAPE, who + ": negative page count");
+        if (n == 0) return MLQ_OK;
+        if (from == nullptr || to == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null page list");
+        std::vector<mlq::KvCopy> copies;
+        std::vector<int> sources(from, from + n), targets(to, to + n);
+        for (int i = 0; i < n; ++i) {
+            const int used = positions != nullptr ? positions[i] : kv.page_size;
+            if (from[i] < 0 || from[i] >= kv.n_pages || to[i] < 0 || to[i] >= kv.n_pages) {
+                return abi_fail(MLQ_ERR_SHAPE, who + ": copy " + std::to_string(i) + " is from page " + std::to_string(from[i]) + " to " +
+                                                   std::to_string(to[i]) + ", the cache has " + std::to_string(kv.n_pages));
+            }
+            if (used < 0 || used > kv.page_size) {
+                return abi_fail(MLQ_ERR_SHAPE, who + ": copy " + std::to_string(i) + ": " + std::to_string(used) +
+                                                   " positions of a page of " + std::to_string(kv.page_size));
+            }
+            if (used > 0) copies.push_back(mlq::KvCopy{from[i], to[i], (used + mlq::kKvTile - 1) / mlq::kKvTile});
+        }
+        // Copies run side by side: no page is written twice, or both read and written.
+        std::sort(sources.begin(), sources.end());
+        std::sort(targets.begin(), targets.end());
+        for (int i = 0; i < n; ++i) {
+            if (i > 0 && targets[i] == targets[i - 1]) {
+                return abi_fail(MLQ_ERR_SHAPE, who + ": page " + std::to_string(targets[i]) + " is written twice");
+            }
+            if (std::binary_search(sources.begin(), sources.end(), targets[i])) {
+                return abi_fail(MLQ_ERR_SHAPE, who + ": page " + std::to_string(targets[i]) + " is read and written");
+            }
+        }
+        const int rc = mlq::abi_device(kv.device);
+        if (rc != MLQ_OK) return rc;
+        const hipStream_t s = mlq::abi_stream(kv.device, stream);
+        if (copies.empty()) return MLQ_OK;
+        const hipError_t e = mlq::launch_kv_copy(kv.view(0), kv.n_layers, kv.layer_bytes, copies.data(),
+                                                 static_cast<int>(copies.size()), s);
+        return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
     });
 }
 

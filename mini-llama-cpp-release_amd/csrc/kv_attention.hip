@@ -10,6 +10,11 @@ hipError_t launch_kv_attention_q8_0(const KvAttention& a, int kind, int count, c
 hipError_t launch_kv_attention_q4_0(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
 hipError_t launch_kv_attention_q4_1(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
 
+hipError_t launch_kv_tree_attention_f32(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+hipError_t launch_kv_tree_attention_q8_0(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+hipError_t launch_kv_tree_attention_q4_0(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+hipError_t launch_kv_tree_attention_q4_1(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+
 int kv_wide_rows(int nb) { return nb <= 4 ? 128 : 64; }
 
 size_t kv_partial_floats(int nb, int kind) {
@@ -22,6 +27,23 @@ hipError_t launch_kv_attention(const KvAttention& a, int kind, int count, const 
         case 1: return launch_kv_attention_q8_0(a, kind, count, q, out, s);
         case 2: return launch_kv_attention_q4_0(a, kind, count, q, out, s);
         case 3: return launch_kv_attention_q4_1(a, kind, count, q, out, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+// (Above 128 elements the registers hold sixteen rows.)
+int kv_tree_rows(int nb) { return nb <= 4 ? 2 * kKvTreeRows : kKvTreeRows; }
+
+size_t kv_tree_partial_floats(int nb, int kind) {
+    return static_cast<size_t>(kind == 0 ? 1 : kv_tree_rows(nb) / kKvTreeRows) * 64 * (8 * nb + 2);
+}
+
+hipError_t launch_kv_tree_attention(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
+    switch (a.kv.qtype) {
+        case 0: return launch_kv_tree_attention_f32(a, kind, count, q, out, s);
+        case 1: return launch_kv_tree_attention_q8_0(a, kind, count, q, out, s);
+        case 2: return launch_kv_tree_attention_q4_0(a, kind, count, q, out, s);
+        case 3: return launch_kv_tree_attention_q4_1(a, kind, count, q, out, s);
         default: return hipErrorInvalidValue;
     }
 }

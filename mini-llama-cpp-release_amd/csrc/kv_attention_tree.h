@@ -1,0 +1,460 @@
+// Attention of drafted trees over the paged cache (kv_layout.h) on MFMA.
+//
+// A sequence's new tokens are the nodes of a tree, in an order that has parents first; node i lies in slot
+// start + i and has position start + depth.  It sees what came before the tree (within the window, and the first
+// positions), its ancestors and itself:
+//
+//   out = softmax_j(scale q . k_j) v   over these j.
+//
+// Who sees whom among the nodes is a bit a slot, laid out by tiles when the batch is set (kv_plan.cpp), so a tile of
+// nodes costs a lane one word; tiles before the tree are as in kv_attention.h, whose arithmetic this is: codes as they
+// lie, queries split in two fp16 parts over their block's largest, value scales in the weights, which are split over a
+// power of two of every row and block that keeps its largest at 2^9 .. 2^15.  There eight rows stand beside their own
+// low parts in an operand's sixteen columns; a tree has more rows than that, so here the sixteen columns are sixteen
+// rows, a block takes two products (f32: three, as low parts times low parts, 2^-22 of an element, are left out), and a
+// wave has NQ such groups for one decoding of a tile.
+#pragma once
+
+#include "kv_attention.h"
+
+#include <algorithm>
+
+namespace mlq {
+namespace kv {
+
+__device__ __forceinline__ KvTreeItem uniform(const KvTreeItem* p) {
+    constexpr int N = sizeof(KvTreeItem) / sizeof(int);
+    struct Words {
+        int v[N];
+    } w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w.v[i] = uniform(reinterpret_cast<const int*>(p) + i);
+    return __builtin_bit_cast(KvTreeItem, w);
+}
+
+// (Two waves a SIMD where the registers allow it.)
+template <int QT, int NB, int NQ>
+constexpr int tree_waves() {
+    return (QT == 0 ? NB * NQ <= 2 : NB * NQ <= 4) ? 2 : 1;
+}
+
+template <int QT, int NB, int NQ>
+__global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attention_tree_kernel(
+    KvTreeAttention a, int count, const float* __restrict__ q, float* __restrict__ out) {
+    using F = KvForm<QT>;
+    constexpr int SB = F::kScaleBytes;
+    constexpr int KL = F::key_lane(NB), VL = F::value_lane(NB);
+    constexpr int KW = KL / 4, VW = VL / 4;
+    constexpr int KS = NB * SB, VS = 2 * NB * SB;  // words of a lane's scales: 4 keys a half tile, 8 keys
+    constexpr int STATE = (8 * NB + 2) * 64;       // floats of a wave's state of sixteen rows
+    __shared__ float merge[2 * STATE];
+    __shared__ unsigned last;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i16 = lane & 15, g = lane >> 4;
+    const int n_kv = a.kv.n_kv, hd = a.kv.head_dim, heads = n_kv * a.group;
+    const int page_tiles = a.kv.page_tiles, tile_shift = __builtin_ctz(page_tiles);
+    const int total = (count > 0 ? count : uniform(a.lists.counts + kKvCountNarrow + NQ - 1)) * n_kv;
+
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
+        const int head = w % n_kv;
+        const KvTreeItem it = uniform(a.lists.items[NQ - 1] + w / n_kv);
+        const int rows = it.new_tokens * a.group, start = it.len - it.new_tokens;
+        const int first_node_tile = start / kKvTile;
+
+        // Lane's row u: its token, its position (only a window asks for it), where its bits and elements start.
+        auto row_of = [&](int u) { return min(it.row0 + 16 * u + i16, rows - 1); };
+        auto element_of = [&](int u) {
+            const int row = row_of(u);
+            return (static_cast<size_t>(it.token0 + row / a.group) * heads + head * a.group + row % a.group) * hd;
+        };
+        int pos[NQ];
+        const uint32_t* mask[NQ];
+        h8_t qh[NQ][NB], ql[NQ][NB];
+        float qsum[NQ][NB], to_t[NQ][NB];
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            const int token = row_of(u) / a.group;
+            pos[u] = a.window > 0 ? a.lists.pos[it.token0 + token] : 0;
+            mask[u] = a.lists.masks + (it.mask0 + token * it.words - first_node_tile);
+            float v[NB][8];
+            load_query<NB, true>(q + element_of(u), hd, g, a.scale * (QT == 0 ? 1.0f / kElementLift : 1.0f), v, qsum[u], to_t[u]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                split8(v[b], &qh[u][b], &ql[u][b]);
+                if (QT == 3) qsum[u][b] = sum_quarters(qsum[u][b]) * to_t[u][b];
+            }
+        }
+
+        const f4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        f4_t o[NQ][2 * NB];
+        float om[NQ][NB];   // Q4_1: this lane's part of the sum of weights times minima
+        int frame[NQ][NB];  // log2 f_b
+        uint32_t spoilt[NQ];  // bit b: this lane's part of the row sees a block that is not finite with a weight of 0
+        float m[NQ], l[NQ];
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            m[u] = -3.402823466e38f, l[u] = 0.0f, spoilt[u] = 0;
+#pragma unroll
+            for (int t = 0; t < 2 * NB; ++t) o[u][t] = zero;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) om[u][b] = 0.0f, frame[u][b] = kMostFrame - kFirstUp;
+        }
+
+        // This wave's tiles: every fourth of the item's.
+        const int end = it.first + it.count;
+        auto tile_of = [&](int i) { return i < it.sinks ? i : i + it.shift; };
+        auto page_of = [&](int i) { return uniform(&a.lists.pages[it.page0 + (tile_of(i) >> tile_shift)].page); };
+        auto base_of = [&](int i, int page) {
+            return a.kv.base + ((static_cast<size_t>(page) * n_kv + head) * page_tiles + (tile_of(i) & (page_tiles - 1))) * F::tile(NB);
+        };
+
+        uint32_t kw[2][KW], ks[2][KS], km[2][QT == 3 ? KS : 1];
+        uint32_t kp[2][QT == 0 ? NB : 1];  // f32: the scales of the lane's own key (ks: of the keys of its scores)
+        uint32_t vw[VW], vs[VS], vm[QT == 3 ? VS : 1];
+        auto load_keys = [&](const uint8_t* tile) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                load_units<KL>(tile + h * 64 * KL, lane, kw[h]);
+                load_run<4 * KS>(tile + F::codes(NB) + (4 * h + g) * 4 * KS, ks[h]);
+                if (QT == 3) load_run<4 * KS>(tile + F::codes(NB) + F::plane(NB) + (4 * h + g) * 4 * KS, km[h]);
+                if (QT == 0) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        kp[h][b] = reinterpret_cast<const uint32_t*>(tile + F::codes(NB))[F::key_scale(NB, 16 * h + i16, b)];
+                    }
+                }
+            }
+        };
+        auto load_values = [&](const uint8_t* tile) {
+            load_units<VL>(tile + F::half(NB), lane, vw);
+            load_run<4 * VS>(tile + F::half(NB) + F::codes(NB) + g * 4 * VS, vs);
+            if (QT == 3) load_run<4 * VS>(tile + F::half(NB) + F::codes(NB) + F::plane(NB) + g * 4 * VS, vm);
+        };
+        // f16 scale i of an array of words (f32: word i)
+        auto scale_at = [&](const uint32_t* s, int i) -> float {
+            if (QT == 0) return bits<float>(s[i]);
+            const h2_t p = bits<h2_t>(s[i / 2]);
+            return static_cast<float>(i % 2 == 0 ? p.x : p.y);
+        };
+
+        // The next tile's loads are under way during this one's work, unless its registers are not enough for both.
+        constexpr bool AHEAD = QT == 0 ? NB * NQ <= 4 : QT != 3 || NB * NQ <= 6;
+        int at = it.first + wave;
+        int next_page = 0;
+        if (AHEAD && at < end) {
+            const uint8_t* tile = base_of(at, page_of(at));
+            load_keys(tile);
+            load_values(tile);
+            if (at + kKvWaves < end) next_page = page_of(at + kKvWaves);
+        }
+        for (; at < end; at += kKvWaves) {
+            const int tile_index = tile_of(at), first = tile_index * kKvTile;
+            const bool more = AHEAD && at + kKvWaves < end;
+            if (!AHEAD) next_page = page_of(at);
+            const uint8_t* next = base_of(more ? at + kKvWaves : at, next_page);
+            if (AHEAD && at + 2 * kKvWaves < end) next_page = page_of(at + 2 * kKvWaves);
+            if (!AHEAD) load_keys(next);
+            const bool nodes = tile_index >= first_node_tile;
+            const bool full = !nodes && (a.window == 0 || first > it.far - a.window || first + kKvTile <= a.sinks);
+            uint32_t word[NQ];  // the tile's bits of the rows: of the nodes' tiles alone
+            if (nodes) {
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) word[u] = mask[u][tile_index];
+            }
+
+            // Scores.
+            float t[NQ][8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f4_t s[NQ];
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) s[u] = zero;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    h8_t hi, lo;
+                    if (QT == 0) {
+                        float v[8];
+                        const float inv = inverse_power(kp[h][b]) * kElementLift;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(bits<float>(kw[h][8 * b + j]), inv);
+                        split8(v, &hi, &lo);
+                    } else if (QT == 1) {
+                        hi = codes8(kw[h][2 * b], kw[h][2 * b + 1], static_cast<_Float16>(128.0f));
+                    } else {
+                        const uint32_t x = kw[h][b];
+                        hi = codes8(x & 0x0f0f0f0fu, (x >> 4) & 0x0f0f0f0fu, static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f));
+                    }
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) {
+                        f4_t acc = mfma(hi, ql[u][b], mfma(hi, qh[u][b], zero));
+                        if (QT == 0) acc = mfma(lo, qh[u][b], acc);  // (times kElementLift, which to_t takes back)
+                        acc *= to_t[u][b];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            s[u][i] = fmaf(scale_at(ks[h], 4 * b + i), acc[i], s[u][i]);
+                            if (QT == 3) s[u][i] = fmaf(scale_at(km[h], 4 * b + i), qsum[u][b], s[u][i]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < NQ; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[u][4 * h + i] = s[u][i];
+            }
+            if (more) load_keys(next);
+            if (!AHEAD) load_values(next);
+
+            // Weights.
+            auto key_in_tile = [&](int j) { return (j >> 2) * 16 + 4 * g + (j & 3); };
+            float p[NQ][8];
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                auto seen = [&](int j) -> bool {
+                    const int k = key_in_tile(j), key = first + k;
+                    return nodes ? (word[u] >> k & 1u) != 0 : (a.window == 0) | (key > pos[u] - a.window) | (key < a.sinks);
+                };
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
+                    if (QT >= 2) t[u][j] = fmaf(t[u][j], 0.0f, t[u][j]);
+                }
+                if (!full) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[u][j] = seen(j) ? t[u][j] : -INFINITY;
+                }
+                float top = fmaxf(fmaxf(fmaxf(t[u][0], t[u][1]), fmaxf(t[u][2], t[u][3])),
+                                  fmaxf(fmaxf(t[u][4], t[u][5]), fmaxf(t[u][6], t[u][7])));
+                top = max_quarters(top);
+                if (__any(top > m[u] + kSlack)) {
+                    const bool moves = top > m[u] + kSlack;
+                    const float to = ceilf(top);
+                    const int up = moves ? static_cast<int>(fminf(to - m[u], static_cast<float>(kFirstUp))) : 0;
+                    m[u] = moves ? to : m[u];
+                    l[u] = ldexpf(l[u], -up);
+                    int over = 0;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        frame[u][b] += up;
+                        over = max(over, frame[u][b] - kMostFrame);
+                        if (QT == 3) om[u][b] = ldexpf(om[u][b], -up);
+                    }
+                    if (__builtin_expect(__any(over > 0), 0)) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const int less = max(frame[u][b] - kMostFrame, 0);
+                            frame[u][b] -= less;
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], -less);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[u][j] = __builtin_amdgcn_exp2f(t[u][j] - m[u]);
+                    l[u] += p[u][j];
+                }
+                const float least = fminf(fminf(fminf(p[u][0], p[u][1]), fminf(p[u][2], p[u][3])),
+                                          fminf(fminf(p[u][4], p[u][5]), fminf(p[u][6], p[u][7])));
+                if (__builtin_expect(__any(least == 0.0f), 0)) {
+                    // (the largest of all scales and minima tells whether there is anything to look for)
+                    uint32_t any_bad;
+                    if (QT == 0) {
+                        uint32_t x = vs[0];
+#pragma unroll
+                        for (int i = 1; i < VS; ++i) x = max(x, vs[i]);
+                        any_bad = x >= 0x7f800000u;
+                    } else {
+                        us2_t x{0, 0};
+#pragma unroll
+                        for (int i = 0; i < VS; ++i) {
+                            x = __builtin_elementwise_max(x, bits<us2_t>(vs[i]));
+                            if (QT == 3) x = __builtin_elementwise_max(x, bits<us2_t>(vm[QT == 3 ? i : 0] & 0x7fff7fffu));
+                        }
+                        any_bad = max(x.x, x.y) >= 0x7c00;
+                    }
+                    if (__builtin_expect(__any(any_bad != 0), 0)) {
+                        auto bad_at = [&](const uint32_t* s, int i) {
+                            return QT == 0 ? s[i] >= 0x7f800000u : ((s[i / 2] >> (i % 2 * 16)) & 0x7fffu) >= 0x7c00u;
+                        };
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const bool lost = p[u][j] == 0.0f && seen(j);
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) {
+                                const bool bad = bad_at(vs, 8 * b + j) || (QT == 3 && bad_at(vm, QT == 3 ? 8 * b + j : 0));
+                                spoilt[u] |= (lost && bad ? 1u : 0u) << b;
+                            }
+                        }
+                    }
+                }
+            }
+
+            // Values.
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                h8_t vh[2], vl[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (QT == 0) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            v[j] = mul_or_zero(bits<float>(vw[16 * b + 8 * x + j]), inverse_power(vs[8 * b + j]) * kElementLift);
+                        }
+                        split8(v, &vh[x], &vl[x]);
+                    } else if (QT == 1) {
+                        vh[x] = codes8(vw[4 * b + 2 * x], vw[4 * b + 2 * x + 1], static_cast<_Float16>(128.0f));
+                    } else {
+                        const uint32_t y = vw[2 * b], z = vw[2 * b + 1];
+                        vh[x] = codes8((x == 0 ? y : y >> 4) & 0x0f0f0f0fu, (x == 0 ? z : z >> 4) & 0x0f0f0f0fu,
+                                       static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[u][j], scale_at(vs, 8 * b + j));
+                    float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+                    if (__builtin_expect(__any(ldexpf(most, frame[u][b]) > 0x1p15f), 0)) {
+                        most = max_quarters(most);
+                        const int to = ldexpf(most, frame[u][b]) > 0x1p15f ? 9 - exponent(most) : frame[u][b];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], to - frame[u][b]);
+                        frame[u][b] = to;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = ldexpf(v[j], frame[u][b]);
+                    if (QT == 3) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) om[u][b] += mul_or_zero(p[u][j], scale_at(vm, 8 * b + j));
+                    }
+                    h8_t ph, pl;
+                    split8(v, &ph, &pl);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        f4_t& acc = o[u][2 * b + x];
+                        acc = mfma(vh[x], pl, mfma(vh[x], ph, acc));
+                        if (QT == 0) acc = mfma(vl[x], ph, acc);
+                    }
+                }
+            }
+            if (more) load_values(next);
+        }
+
+        // The lanes' sums and the minima's part, out of the blocks' frames.
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            l[u] = sum_quarters(l[u]);
+            const bool any_spoilt = __any(spoilt[u] != 0);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float add = QT == 3 ? sum_quarters(om[u][b]) : 0.0f;
+                add = fmaf(add, 0.0f, add);  // an infinite minimum: NaN
+                if (__builtin_expect(any_spoilt, 0)) add += sum_quarters((spoilt[u] >> b) & 1u ? NAN : 0.0f);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], -frame[u][b] - (QT == 0 ? 13 : 0)) + add;
+                    }
+            }
+        }
+        // The four waves' states into wave 0, in a fixed order, sixteen rows at a time.
+        auto leave = [&](int u, float* to) {
+#pragma unroll
+            for (int x = 0; x < 2 * NB; ++x) *reinterpret_cast<f4_t*>(to + (x * 64 + lane) * 4) = o[u][x];
+            to[2 * NB * 256 + lane] = m[u];
+            to[2 * NB * 256 + 64 + lane] = l[u];
+        };
+        auto take = [&](int u, const float* from) {
+            float w0, w1;
+            fold(m[u], l[u], from[2 * NB * 256 + lane], from[2 * NB * 256 + 64 + lane], &w0, &w1);
+#pragma unroll
+            for (int x = 0; x < 2 * NB; ++x) {
+                o[u][x] = o[u][x] * w0 + *reinterpret_cast<const f4_t*>(from + (x * 64 + lane) * 4) * w1;
+            }
+        };
+        auto merge_waves = [&] {
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                __syncthreads();
+                if (wave >= 2) leave(u, merge + (wave - 2) * STATE);
+                __syncthreads();
+                if (wave < 2) take(u, merge + wave * STATE);
+                __syncthreads();
+                if (wave == 1) leave(u, merge);
+                __syncthreads();
+                if (wave == 0) take(u, merge);
+            }
+        };
+        merge_waves();
+
+        if (it.nsplit > 1) {
+            // This part's state to memory; the workgroup that arrives last merges all parts, wave w
+            // taking w, w + 4, ...
+            auto rsrc_of = [&](int split) {
+                return state_rsrc(a.partial, static_cast<size_t>(it.slot + split) * n_kv + head, NQ * STATE);
+            };
+            if (wave == 0) {
+                leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
+                if (lane == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);
+            }
+            __syncthreads();
+            const bool mine = last != 0u;
+            __syncthreads();
+            if (!mine) continue;
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                m[u] = -3.402823466e38f;
+                l[u] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 2 * NB; ++x) o[u][x] = zero;
+            }
+            for (int part = wave; part < it.nsplit; part += kKvWaves) take_state<NQ, NB>(rsrc_of(part), lane, o, m, l);
+            merge_waves();
+        }
+
+        if (wave == 0) {
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                if (it.row0 + 16 * u + i16 < rows) store_row<NB>(out + element_of(u), hd, g, o[u], 1.0f / l[u]);
+            }
+        }
+    }
+}
+
+// Workgroups of a recorded launch, which walks whatever list is set by then.
+constexpr unsigned kTreeRecorded = 1024;
+
+template <int QT, int NB>
+hipError_t launch_tree_blocks(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
+    // (a launch holds less than 2^32 threads; the kernel walks its list whatever the grid)
+    const unsigned grid =
+        count > 0 ? static_cast<unsigned>(std::min<long long>(static_cast<long long>(count) * a.kv.n_kv, 1 << 20)) : kTreeRecorded;
+    if (kind == 0) attention_tree_kernel<QT, NB, 1><<<grid, kThreads, 0, s>>>(a, count, q, out);
+    else if constexpr (NB <= 4) attention_tree_kernel<QT, NB, 2><<<grid, kThreads, 0, s>>>(a, count, q, out);
+    return hipGetLastError();
+}
+
+template <int QT>
+hipError_t launch_tree(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
+    switch (a.kv.nb) {
+        case 1: return launch_tree_blocks<QT, 1>(a, kind, count, q, out, s);
+        case 2: return launch_tree_blocks<QT, 2>(a, kind, count, q, out, s);
+        case 3: return launch_tree_blocks<QT, 3>(a, kind, count, q, out, s);
+        case 4: return launch_tree_blocks<QT, 4>(a, kind, count, q, out, s);
+        case 6: return launch_tree_blocks<QT, 6>(a, kind, count, q, out, s);
+        case 8: return launch_tree_blocks<QT, 8>(a, kind, count, q, out, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace kv
+}  // namespace mlq

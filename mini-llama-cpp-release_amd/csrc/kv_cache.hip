@@ -237,9 +237,10 @@ __device__ __forceinline__ void write_kv_head(const KvTileItem& it, int head, co
 // gathers in LDS and leaves as 16-byte stores; of others the new slots are
 // stored where they belong, values byte by byte, so that slots of other
 // sequences or earlier tokens in the same words are never rewritten.
-template <int QT>
+// TREE: the tokens' positions are those of a list, as a tree's nodes do not follow each other.
+template <int QT, bool TREE>
 __global__ __launch_bounds__(kWriteThreads) void kv_write_kernel(KvView kv, const KvTileItem* __restrict__ items,
-                                                              const int* __restrict__ counts, int count,
+                                                              const int* __restrict__ counts, const int* __restrict__ pos, int count,
                                                               const float* __restrict__ k, const float* __restrict__ v,
                                                               const float* q, float* q_out, int n_heads, int per_group,
                                                               KvRope rope) {
@@ -257,7 +258,8 @@ __global__ __launch_bounds__(kWriteThreads) void kv_write_kernel(KvView kv, cons
         if (rope.on) {
             __syncthreads();  // the last item's readers are done
             for (int i = threadIdx.x; i < it.n * half; i += blockDim.x) {
-                const double a = static_cast<double>(it.pos + i / half) * rope.turns[i % half];
+                const int at = TREE ? pos[it.row + i / half] : it.pos + i / half;
+                const double a = static_cast<double>(at) * rope.turns[i % half];
                 double2 t;
                 sincospi(2.0 * (a - rint(a)), &t.y, &t.x);
                 turn[i] = t;
@@ -410,9 +412,9 @@ hipError_t allow_lds(K kernel, int bytes) {
     return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <int QT>
-hipError_t write(const KvView& kv, const KvLists& lists, int count, int tokens, const float* k, const float* v, const float* q,
-                 float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
+template <int QT, bool TREE>
+hipError_t write(const KvView& kv, const KvLists& lists, const int* pos, int count, int tokens, const float* k, const float* v,
+                 const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
     const int heads = kv.n_kv + (q != nullptr ? n_heads : 0);
     // Heads a workgroup takes: the angles are computed once for them, as long as there are workgroups
     // enough (2048 tokens, 64 heads, 1 / 2 / 4 / 8 a workgroup: 75 / 71 / 64 / 62 us with the read
@@ -424,12 +426,19 @@ hipError_t write(const KvView& kv, const KvLists& lists, int count, int tokens, 
     // Whole tiles keep 512 threads busy (2048 tokens, 32 + 32 heads of 128: 62 us with the read back, 92
     // with 256); a token or two do not (64 sequences: 14 us, 17 with 512).
     const unsigned threads = tokens > 4ll * count ? kWriteThreads : kWriteThreads / 2;
-    const hipError_t e = allow_lds(kv_write_kernel<QT>, lds);
+    const hipError_t e = allow_lds(kv_write_kernel<QT, TREE>, lds);
     if (e != hipSuccess) return e;
     const unsigned grid = count > 0 ? static_cast<unsigned>(std::min<long long>(groups, 1 << 20)) : kRecordedGroups;
-    kv_write_kernel<QT><<<grid, threads, lds, s>>>(kv, lists.fresh, lists.counts, count, k, v, q, q_out, n_heads,
-                                                      count > 0 ? per_group : 4, rope);
+    kv_write_kernel<QT, TREE><<<grid, threads, lds, s>>>(kv, lists.fresh, lists.counts, pos, count, k, v, q, q_out, n_heads,
+                                                            count > 0 ? per_group : 4, rope);
     return hipGetLastError();
+}
+
+template <int QT>
+hipError_t write(const KvView& kv, const KvLists& lists, const int* pos, int count, int tokens, const float* k, const float* v,
+                 const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
+    return pos != nullptr ? write<QT, true>(kv, lists, pos, count, tokens, k, v, q, q_out, n_heads, rope, s)
+                          : write<QT, false>(kv, lists, pos, count, tokens, k, v, q, q_out, n_heads, rope, s);
 }
 
 template <int QT>
@@ -452,13 +461,13 @@ hipError_t launch_kv_upload(const KvParts& parts, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, int count, int tokens, const float* k, const float* v,
-                           const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
+hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, const int* pos, int count, int tokens, const float* k,
+                           const float* v, const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s) {
     switch (kv.qtype) {
-        case 0: return write<0>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
-        case 1: return write<1>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
-        case 2: return write<2>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
-        case 3: return write<3>(kv, lists, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 0: return write<0>(kv, lists, pos, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 1: return write<1>(kv, lists, pos, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 2: return write<2>(kv, lists, pos, count, tokens, k, v, q, q_out, n_heads, rope, s);
+        case 3: return write<3>(kv, lists, pos, count, tokens, k, v, q, q_out, n_heads, rope, s);
         default: return hipErrorInvalidValue;
     }
 }

@@ -86,7 +86,19 @@ struct KvLists {
     const KvPage* pages;
     const KvAttnItem* items[2];
 };
-enum { kKvCountFresh, kKvCountPages, kKvCountNarrow, kKvCountWide, kKvCounts };
+enum { kKvCountFresh, kKvCountPages, kKvCountNarrow, kKvCountWide, kKvCountSeqs, kKvCountTokens, kKvCounts };
+
+// What a plan of trees has beside `counts`, `fresh` and `pages` (its items are counted in kKvCountNarrow and
+// kKvCountWide).
+struct KvTreeLists {
+    const int* counts;
+    const KvPage* pages;
+    const KvTreeItem* items[2];
+    const KvTreeSeq* seqs;
+    const int* pos;      // of each token
+    const int* parents;  // of each token, among its sequence's
+    const uint32_t* masks;
+};
 
 // RoPE of a write: turns per position of pair r, and how elements pair.
 struct KvRope {
@@ -95,7 +107,7 @@ struct KvRope {
 };
 
 // Copies `n` parts of pinned host memory to the lists (one launch, any stream).
-constexpr int kKvParts = 5;
+constexpr int kKvParts = 9;
 struct KvParts {
     const uint32_t* src[kKvParts];
     uint32_t* dst[kKvParts];
@@ -105,8 +117,9 @@ hipError_t launch_kv_upload(const KvParts& parts, hipStream_t s);
 
 // `count`: the items of the list in use (0: as many as the device says, for launches
 // that are recorded and replayed with other lists); `tokens`: new tokens of the batch.
-hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, int count, int tokens, const float* k, const float* v,
-                           const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s);
+// pos: the tokens' positions where they do not follow each other (trees), or null.
+hipError_t launch_kv_write(const KvView& kv, const KvLists& lists, const int* pos, int count, int tokens, const float* k,
+                           const float* v, const float* q, float* q_out, int n_heads, const KvRope& rope, hipStream_t s);
 hipError_t launch_kv_read(const KvView& kv, const KvLists& lists, bool fresh, int count, float* k, float* v, hipStream_t s);
 
 struct KvAttention {
@@ -123,5 +136,41 @@ int kv_wide_rows(int nb);
 size_t kv_partial_floats(int nb, int kind);
 // count: items of the narrow (kind 0) or wide list, 0 as above.
 hipError_t launch_kv_attention(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+
+// The same of trees (kv_attention_tree.h).
+struct KvTreeAttention {
+    KvView kv;
+    KvTreeLists lists;
+    int group;
+    int window, sinks;
+    float scale;
+    float* partial;
+    unsigned* arrived;
+};
+// Query rows of a workgroup of the second list.
+int kv_tree_rows(int nb);
+size_t kv_tree_partial_floats(int nb, int kind);
+hipError_t launch_kv_tree_attention(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
+
+// Positions and pages moved within a cache, in all layers (kv_moves.hip).
+struct KvCopy {
+    int from, to, tiles;
+};
+hipError_t launch_kv_copy(const KvView& kv, int n_layers, size_t layer_bytes, const KvCopy* copies, int n, hipStream_t s);
+hipError_t launch_kv_moves(const KvView& kv, int n_layers, size_t layer_bytes, const KvMove* moves, const int* ends, int n_ends,
+                           hipStream_t s);
+
+// Picks of a batch of trees and the paths they confirm (kv_pick.hip).  keys: a word a row and part, as many as rows,
+// kKvPickParts at the least.  tokens and seqs: of the batch, or -1: as many as the device says.
+constexpr int kKvPickParts = 1024;
+struct KvPick {
+    KvTreeLists lists;
+    const float* logits;
+    int vocab;
+    const int* tokens;
+    int *picks, *n_kept, *kept, *next;
+    unsigned long long* keys;
+};
+hipError_t launch_kv_pick(const KvPick& p, int tokens, int seqs, hipStream_t s);
 
 }  // namespace mlq

@@ -24,12 +24,93 @@ struct Seen {
     int sinks, shift, count;
 };
 
-Seen seen_tiles(const KvPlanShape& s, int lo, int hi) {
+// (`most`: of a position in the first tile of the window.)
+Seen seen_tiles(const KvPlanShape& s, int lo, int hi, int most) {
     const int last = hi / kKvTile;
-    const int first = s.window > 0 ? std::max(0, lo - s.window + 1) / kKvTile : 0;
+    const int first = s.window > 0 ? std::max(0, std::min(most, lo - s.window + 1)) / kKvTile : 0;
     // the sinks are first positions: below `first` they are whole tiles of their own
     const int sinks = s.window > 0 ? std::min(first, ceil_div(s.sinks, kKvTile)) : 0;
     return Seen{sinks, first - sinks, sinks + last - first + 1};
+}
+
+// Adds the items of `whole` to `list`, split along their tiles where there are too few: parts of at most
+// `most` tiles, as even as they come: the fewest tiles that do not make more items than `target`, since those
+// beyond one round of workgroups would take a second one.
+// Where there is a round without splits, only items of twice the average are split if `lone` (64 ragged
+// sequences of up to 4000: 79 us, 85 with those over the average split).
+// (Not a prompt's row groups, whose lengths are spread: 2048 tokens, 32 heads: 167 us, 193 unsplit.)
+template <typename Item>
+void split_items(const std::vector<Item>& whole, int n_kv_heads, bool lone, std::vector<Item>& list) {
+    int64_t tiles = 0;
+    for (const Item& w : whole) tiles += w.count;
+    const int target = std::max(1, kTargetGroups / n_kv_heads);
+    auto items_of = [&](int64_t most) {
+        int64_t n = 0;
+        for (const Item& w : whole) n += (w.count + most - 1) / most;
+        return n;
+    };
+    const bool enough = static_cast<int>(whole.size()) >= target;
+    int64_t lo = std::max<int64_t>(kLeastTiles, (enough && lone ? 2 : 1) * ((tiles + target - 1) / target)), hi = lo;
+    for (const Item& w : whole) hi = std::max<int64_t>(hi, w.count);
+    while (lo < hi && !enough) {
+        const int64_t mid = (lo + hi) / 2;
+        if (items_of(mid) <= target) hi = mid;
+        else lo = mid + 1;
+    }
+    const int most = static_cast<int>(std::max<int64_t>(1, lo));
+    int slot = 0;
+    for (const Item& w : whole) {
+        const int parts = ceil_div(w.count, most);
+        for (int p = 0; p < parts; ++p) {
+            Item it = w;
+            it.first = static_cast<int>(static_cast<int64_t>(w.count) * p / parts);
+            it.count = static_cast<int>(static_cast<int64_t>(w.count) * (p + 1) / parts) - it.first;
+            it.split = p;
+            it.nsplit = parts;
+            it.slot = slot;
+            list.push_back(it);
+        }
+        if (parts > 1) slot += parts;
+    }
+    // The longest first: what starts last is short.
+    std::stable_sort(list.begin(), list.end(), [](const Item& x, const Item& y) { return x.count > y.count; });
+}
+
+// The tree of one sequence, n nodes after `start` positions: checks `parents` (null: a chain) and adds positions,
+// parents and bits to the batch.  Bit k of node i's word w: whether it sees position 32 (start / 32 + w) + k,
+// counted in slots.
+std::string add_tree(const KvPlanShape& s, const std::string& who, int n, int start, const int* parents, KvBatch& b) {
+    const int t0 = start / kKvTile, words = (start + n - 1) / kKvTile - t0 + 1, base = start % kKvTile;
+    const size_t first = b.masks.size(), pos0 = b.pos.size();
+    b.masks.resize(first + static_cast<size_t>(n) * words, 0);
+    for (int i = 0; i < n; ++i) {
+        const int parent = parents != nullptr ? parents[i] : i - 1;
+        if (parent < -1 || parent >= i) {
+            return who + ": node " + std::to_string(i) + " has parent " + std::to_string(parent) + ", not -1 or an earlier node";
+        }
+        b.parents.push_back(parent);
+        const int pos = parent < 0 ? start : b.pos[pos0 + parent] + 1;
+        b.pos.push_back(pos);
+        uint32_t* const mask = &b.masks[first + static_cast<size_t>(i) * words];
+        const int lo = s.window > 0 ? pos - s.window : -1;  // positions up to here are seen as sinks only
+        auto set = [&](int bit) { mask[bit / kKvTile] |= 1u << (bit % kKvTile); };
+        if (lo < start && parent >= 0) {
+            // all nodes of the path are seen
+            const uint32_t* const of_parent = &b.masks[first + static_cast<size_t>(parent) * words];
+            std::copy(of_parent, of_parent + words, mask);
+            mask[0] &= ~((1u << base) - 1u);
+        } else {
+            for (int p = parent; p >= 0; p = b.parents[pos0 + p]) {
+                if (b.pos[pos0 + p] > lo || b.pos[pos0 + p] < s.sinks) set(base + p);
+            }
+        }
+        for (int k = 0; k < base; ++k) {
+            const int p = t0 * kKvTile + k;
+            if (p > lo || p < s.sinks) set(k);
+        }
+        set(base + i);
+    }
+    return "";
 }
 
 }  // namespace
@@ -37,8 +118,14 @@ Seen seen_tiles(const KvPlanShape& s, int lo, int hi) {
 KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     const int64_t rows = static_cast<int64_t>(s.max_tokens) * s.group;
     const int64_t narrow = std::min(rows / kKvNarrowRows, static_cast<int64_t>(s.max_seqs) * (kKvNarrowMost / kKvNarrowRows - 1));
-    const int whole[2] = {static_cast<int>(narrow) + s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
+    int whole[2] = {static_cast<int>(narrow) + s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
     KvPlanLimits l;
+    if (s.max_nodes > 0) {
+        // (a node's bits begin inside a tile at the most)
+        whole[0] = static_cast<int>(s.tree_rows > kKvTreeRows ? 0 : rows / kKvTreeRows) + s.max_seqs;
+        whole[1] = static_cast<int>(rows / s.tree_rows) + s.max_seqs;
+        l.masks = static_cast<int64_t>(s.max_tokens) * (s.max_nodes / kKvTile + 2);
+    }
     // a sequence's new tokens begin and end inside a tile at the most
     l.fresh = static_cast<int>(std::min<int64_t>(s.max_tokens, s.max_tokens / kKvTile + 2ll * s.max_seqs));
     for (int kind = 0; kind < 2; ++kind) {
@@ -52,7 +139,7 @@ KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
 }
 
 std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
-                          KvBatch* out) {
+                          const int* parents, KvBatch* out) {
     if (n_seqs < 0 || n_seqs > s.max_seqs) {
         return std::to_string(n_seqs) + " sequences, the plan holds " + std::to_string(s.max_seqs);
     }
@@ -63,6 +150,9 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
         if (new_tokens[i] < 0) return who + ": negative token count";
         if (kv_len[i] < new_tokens[i]) {
             return who + ": " + std::to_string(new_tokens[i]) + " new tokens in a length of " + std::to_string(kv_len[i]);
+        }
+        if (s.max_nodes > 0 && new_tokens[i] > s.max_nodes) {
+            return who + ": " + std::to_string(new_tokens[i]) + " nodes, the plan's trees hold " + std::to_string(s.max_nodes);
         }
         tokens += new_tokens[i];
         positions += kv_len[i];
@@ -93,7 +183,29 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     };
     std::vector<Written> written;
     std::vector<KvAttnItem> base[2];
+    std::vector<KvTreeItem> of_trees[2];
     int token0 = 0, row0 = 0, page0 = 0;
+    // The row groups of sequence i's tree.
+    auto add_item = [&](int i, int token, int page) -> std::string {
+        const int n = new_tokens[i], start = kv_len[i] - n, rows = n * s.group;
+        const int kind = rows <= kKvTreeRows || s.tree_rows <= kKvTreeRows ? 0 : 1, step = kind == 0 ? kKvTreeRows : s.tree_rows;
+        const int mask0 = static_cast<int>(b.masks.size()), words = (kv_len[i] - 1) / kKvTile - start / kKvTile + 1;
+        const std::string wrong =
+            add_tree(s, "sequence " + std::to_string(i), n, start, parents != nullptr ? parents + token : nullptr, b);
+        if (!wrong.empty()) return wrong;
+        for (int r = 0; r < rows; r += step) {
+            const int last = (std::min(rows, r + step) - 1) / s.group;
+            int near = b.pos[token + r / s.group], far = near;
+            for (int t = r / s.group; t <= last; ++t) {
+                near = std::min(near, b.pos[token + t]);
+                far = std::max(far, b.pos[token + t]);
+            }
+            // (from the tree's first tile at the latest: a node may be seen as a sink wherever it lies)
+            const Seen t = seen_tiles(s, near, start + last, start);
+            of_trees[kind].push_back(KvTreeItem{token, n, kv_len[i], page, r, 0, t.count, t.sinks, t.shift, 0, 1, 0, mask0, words, far, 0});
+        }
+        return "";
+    };
     for (int i = 0; i < n_seqs; ++i) {
         const int len = kv_len[i], n = new_tokens[i], start = len - n;
         for (int p = 0; p < len; p += s.page_size) {
@@ -110,7 +222,15 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
             written.push_back(Written{pages[page0 + p / s.page_size], p % s.page_size, (end - 1) % s.page_size});
             p = end;
         }
-        if (n > 0) {
+        if (s.max_nodes > 0) {
+            if (n > 0) {
+                const std::string wrong = add_item(i, token0, page0);
+                if (!wrong.empty()) return wrong;
+            }
+            b.seqs.push_back(KvTreeSeq{token0, n});
+            b.starts.push_back(start);
+            b.first_page.push_back(page0);
+        } else if (n > 0) {
             const int rows = n * s.group;
             const int kind = rows <= kKvNarrowMost ? 0 : 1;
             base[kind].push_back(KvAttnItem{token0, n, len, page0, 0, 0, 0, 0, 0, 0, 1, 0});
@@ -129,60 +249,60 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     }
 
     for (int kind = 0; kind < 2; ++kind) {
+        split_items(of_trees[kind], s.n_kv_heads, true, b.trees[kind]);
         const int step = kind == 0 ? kKvNarrowRows : s.wide_rows;
         std::vector<KvAttnItem> whole;
-        int64_t tiles = 0;
         for (const KvAttnItem& q : base[kind]) {
             const int rows = q.new_tokens * s.group, start = q.len - q.new_tokens;
             for (int r = 0; r < rows; r += step) {
-                const Seen t = seen_tiles(s, start + r / s.group, start + (std::min(rows, r + step) - 1) / s.group);
+                const Seen t = seen_tiles(s, start + r / s.group, start + (std::min(rows, r + step) - 1) / s.group, q.len);
                 KvAttnItem it = q;
                 it.row0 = r;
                 it.count = t.count;
                 it.sinks = t.sinks;
                 it.shift = t.shift;
-                tiles += t.count;
                 whole.push_back(it);
             }
         }
-        // Parts of at most `most` tiles, as even as they come: the fewest tiles that do not make more
-        // items than `target`, since those beyond one round of workgroups would take a second one.
-        std::vector<KvAttnItem>& list = b.items[kind];
-        const int target = std::max(1, kTargetGroups / s.n_kv_heads);
-        auto items_of = [&](int64_t most) {
-            int64_t n = 0;
-            for (const KvAttnItem& w : whole) n += (w.count + most - 1) / most;
-            return n;
-        };
-        // Where there is a round without splits, only items of twice the average are split (64 ragged
-        // sequences of up to 4000: 79 us, 85 with those over the average split).
-        // (Not a prompt's row groups, whose lengths are spread: 2048 tokens, 32 heads: 167 us, 193 unsplit.)
-        const bool enough = static_cast<int>(whole.size()) >= target;
-        int64_t lo = std::max<int64_t>(kLeastTiles, (enough && kind == 0 ? 2 : 1) * ((tiles + target - 1) / target)), hi = lo;
-        for (const KvAttnItem& w : whole) hi = std::max<int64_t>(hi, w.count);
-        while (lo < hi && !enough) {
-            const int64_t mid = (lo + hi) / 2;
-            if (items_of(mid) <= target) hi = mid;
-            else lo = mid + 1;
+        split_items(whole, s.n_kv_heads, kind == 0, b.items[kind]);
+    }
+    return "";
+}
+
+std::string kv_keep_build(const KvPlanShape& s, const KvBatch& b, const int* n_kept, const int* kept, std::vector<KvMove>* moves,
+                          std::vector<int>* ends) {
+    moves->clear();
+    ends->clear();
+    if (!b.seqs.empty() && n_kept == nullptr) return "null counts";
+    size_t at = 0;
+    int64_t total = 0;
+    for (size_t i = 0; i < b.seqs.size(); ++i) {
+        const std::string who = "sequence " + std::to_string(i);
+        if (n_kept[i] < 0 || n_kept[i] > b.seqs[i].nodes) {
+            return who + ": " + std::to_string(n_kept[i]) + " of " + std::to_string(b.seqs[i].nodes) + " nodes kept";
         }
-        const int most = static_cast<int>(std::max<int64_t>(1, lo));
-        int slot = 0;
-        for (const KvAttnItem& w : whole) {
-            const int parts = ceil_div(w.count, most);
-            for (int p = 0; p < parts; ++p) {
-                KvAttnItem it = w;
-                it.first = static_cast<int>(static_cast<int64_t>(w.count) * p / parts);
-                it.count = static_cast<int>(static_cast<int64_t>(w.count) * (p + 1) / parts) - it.first;
-                it.split = p;
-                it.nsplit = parts;
-                it.slot = slot;
-                list.push_back(it);
+        total += n_kept[i];
+    }
+    if (total > 0 && kept == nullptr) return "null list";
+    for (size_t i = 0; i < b.seqs.size(); ++i) {
+        const KvTreeSeq& q = b.seqs[i];
+        for (int j = 0; j < n_kept[i]; ++j) {
+            const int node = kept[at + j], before = j > 0 ? kept[at + j - 1] : -1;
+            if (node < 0 || node >= q.nodes || b.parents[q.token0 + node] != before) {
+                return "sequence " + std::to_string(i) + ": kept node " + std::to_string(node) + " is not a child of " +
+                       (j > 0 ? "node " + std::to_string(before) : "what came before the tree");
             }
-            if (parts > 1) slot += parts;
+            // A path's nodes ascend, so node j lies at slot j or later.
+            if (node != j) {
+                const int from = b.starts[i] + node, to = b.starts[i] + j;
+                moves->push_back(KvMove{b.pages[b.first_page[i] + from / s.page_size].page, b.pages[b.first_page[i] + to / s.page_size].page,
+                                        static_cast<uint16_t>(from % s.page_size), static_cast<uint16_t>(to % s.page_size)});
+            }
         }
-        // The longest first: what starts last is short.
-        std::stable_sort(list.begin(), list.end(),
-                         [](const KvAttnItem& x, const KvAttnItem& y) { return x.count > y.count; });
+        at += n_kept[i];
+        if (!moves->empty() && (ends->empty() || ends->back() != static_cast<int>(moves->size()))) {
+            ends->push_back(static_cast<int>(moves->size()));
+        }
     }
     return "";
 }

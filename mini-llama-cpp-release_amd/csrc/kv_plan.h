@@ -41,19 +41,44 @@ struct KvAttnItem {
     int split, nsplit, slot;  // part `split` of nsplit; the parts' first slot in the partial results
 };
 
+// The same of a batch of trees (kv_attention_tree.h).  The sequence's nodes see each other by bits: those of its
+// node i start at word mask0 + i * words of the masks, a word a tile from that of the first node on.
+struct KvTreeItem {
+    int token0, new_tokens, len, page0;
+    int row0, first, count;
+    int sinks, shift;
+    int split, nsplit, slot;
+    int mask0, words;
+    int far;  // the largest position of the item's rows
+    int pad;
+};
+
+// A sequence of a batch of trees: its first row in the token buffers, and its nodes.
+struct KvTreeSeq {
+    int token0, nodes;
+};
+
+// Query rows of a workgroup of the trees' first list: the columns of an MFMA operand.
+constexpr int kKvTreeRows = 16;
+constexpr int kKvMostNodes = 1024;
+
 struct KvPlanShape {
     int page_size, n_pages, n_kv_heads;
     int group;      // query heads per KV head
     int wide_rows;  // query rows of a workgroup of the kernel for many rows
     int window, sinks;
     int max_seqs, max_tokens, max_pages;
+    int max_nodes = 0;  // of a sequence's tree; 0: batches of plain sequences
+    int tree_rows = 2 * kKvTreeRows;  // query rows of a workgroup of the trees' second list
 };
+
 
 // What a set of a plan of this shape can need at the most.
 struct KvPlanLimits {
     int fresh;     // tiles with new tokens
-    int items[2];  // narrow, wide
+    int items[2];  // narrow, wide (of trees: few rows, many)
     int slots[2];  // partial results
+    int64_t masks = 0;  // words of the trees' bits
 };
 KvPlanLimits kv_plan_limits(const KvPlanShape& s);
 
@@ -62,11 +87,32 @@ struct KvBatch {
     std::vector<KvTileItem> fresh;     // tiles with new tokens
     std::vector<KvPage> pages;
     std::vector<KvAttnItem> items[2];  // narrow, wide
+    // Of trees, in place of `items`.
+    std::vector<KvTreeItem> trees[2];
+    std::vector<KvTreeSeq> seqs;
+    std::vector<int> starts, first_page;  // of each sequence: positions before its tree, first entry in `pages`
+    std::vector<int> pos, parents;  // of each token: its position, the parent among its sequence's nodes
+    std::vector<uint32_t> masks;
 };
 
 // Checks a batch and builds its lists.  Returns "" or what is wrong with it;
-// `out` is complete only on "".
+// `out` is complete only on "".  parents: of shapes with max_nodes, each new token's
+// parent among its sequence's new tokens, an earlier one, or -1 (null: chains).
 std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
-                          KvBatch* out);
+                          const int* parents, KvBatch* out);
+inline std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
+                                 KvBatch* out) {
+    return kv_plan_build(s, n_seqs, new_tokens, kv_len, pages, nullptr, out);
+}
+
+// Moves of a path's tokens behind what came before the tree: slots of the cache's pages.
+struct KvMove {
+    int from_page, to_page;
+    uint16_t from_slot, to_slot;  // (a page has 65536 at the most)
+};
+// Checks what is kept of a batch (of each sequence n_kept[s] of its new tokens, each the child of the one before)
+// and lists the moves, one sequence's after the other's, `ends` the list's length after each sequence that has some.
+std::string kv_keep_build(const KvPlanShape& s, const KvBatch& b, const int* n_kept, const int* kept, std::vector<KvMove>* moves,
+                          std::vector<int>* ends);
 
 }  // namespace mlq

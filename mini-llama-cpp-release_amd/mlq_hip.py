@@ -154,6 +154,16 @@ _SIGS = {
     "mlq_hip_kv_write": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_float, ctypes.c_int, _vp]),
     "mlq_hip_kv_read": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp]),
     "mlq_hip_kv_attention": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
+    "mlq_hip_kv_tree_plan_create": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
+                                                   ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                                   ctypes.POINTER(_vp)]),
+    "mlq_hip_kv_plan_set_tree": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp]),
+    "mlq_hip_kv_tree_pick": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mlq_hip_kv_keep": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
+    "mlq_hip_kv_copy_pages": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp]),
+    "mlq_hip_beam_create": (ctypes.c_int, [ctypes.c_int] * 5 + [ctypes.POINTER(_vp)]),
+    "mlq_hip_beam_destroy": (ctypes.c_int, [_vp]),
+    "mlq_hip_beam_select": (ctypes.c_int, [_vp, _vp, _vp, _vp] + [ctypes.c_int] * 5 + [_vp, _vp, _vp, _vp]),
     "mlq_hip_kernel_name": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                             ctypes.c_char_p, ctypes.c_size_t]),
 }
@@ -648,6 +658,15 @@ class KvCache:
         _check(_LIB.mlq_hip_kv_cache_info(self.h, *[ctypes.byref(x) for x in v], ctypes.byref(n)))
         return {**{k: x.value for k, x in zip(names, v)}, "bytes": n.value}
 
+    def copy_pages(self, src, dst, positions=None, stream=None) -> None:
+        """The first positions of each page (all by default) into another page, in every layer."""
+        a, b = _ints(src, "src"), _ints(dst, "dst")
+        n = _ints(positions, "positions") if positions is not None else None
+        if a.size != b.size or (n is not None and n.size != a.size):
+            raise ValueError("one destination, and one count of positions, per page")
+        _check(_LIB.mlq_hip_kv_copy_pages(self.h, a.size, a.ctypes.data, b.ctypes.data,
+                                          n.ctypes.data if n is not None else None, stream))
+
     def destroy(self) -> None:
         if getattr(self, "h", None):
             _LIB.mlq_hip_kv_cache_destroy(self.h)
@@ -662,25 +681,41 @@ class KvCache:
 
 class KvPlan:
     """A batch over a KvCache and its calls (mlq_hip_kv_plan_*, _write, _read, _attention).
-    Buffers are DeviceBuffers or device pointers; every call is asynchronous."""
+    Buffers are DeviceBuffers or device pointers; every call is asynchronous.
+    max_nodes > 0: the new tokens of a sequence may be a tree of drafted tokens of up to that
+    many nodes (mlq_hip_kv_tree_plan_create, _plan_set_tree, _tree_pick, _keep)."""
 
     def __init__(self, cache: KvCache, n_heads: int, max_seqs: int, max_tokens: int, max_pages: int, window: int = 0,
-                 sinks: int = 0, scale: float = 0.0):
+                 sinks: int = 0, scale: float = 0.0, max_nodes: int = 0):
         h = _vp()
-        _check(load().mlq_hip_kv_plan_create(cache.h, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages,
-                                             ctypes.byref(h)))
+        if max_nodes != 0:
+            _check(load().mlq_hip_kv_tree_plan_create(cache.h, n_heads, window, sinks, scale, max_seqs, max_tokens,
+                                                      max_pages, max_nodes, ctypes.byref(h)))
+        else:
+            _check(load().mlq_hip_kv_plan_create(cache.h, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages,
+                                                 ctypes.byref(h)))
         self.h = h.value
         self._page_size = cache.info()["page_size"]
+        self._n_seqs = 0
 
-    def set(self, new_tokens, kv_len, pages, stream=None) -> None:
-        """new_tokens and kv_len per sequence; pages: their page ids, one sequence's after the other's."""
+    def set(self, new_tokens, kv_len, pages, stream=None, parents=None) -> None:
+        """new_tokens and kv_len per sequence; pages: their page ids, one sequence's after the other's.  parents: of
+        trees, each new token's parent among its sequence's (-1: what came before the tree)."""
         n, t, p = _ints(new_tokens, "new_tokens"), _ints(kv_len, "kv_len"), _ints(pages, "pages")
         if n.size != t.size:
             raise ValueError("one length per sequence")
         need = int(sum(-(-int(x) // self._page_size) for x in t if x > 0))
         if p.size != need:
             raise ValueError(f"{p.size} page ids, the lengths need {need}")
-        _check(_LIB.mlq_hip_kv_plan_set(self.h, n.size, n.ctypes.data, t.ctypes.data, p.ctypes.data, stream))
+        if parents is not None:
+            up = _ints(parents, "parents")
+            if up.size != sum(int(x) for x in n if x > 0):
+                raise ValueError("one parent per new token")
+            _check(_LIB.mlq_hip_kv_plan_set_tree(self.h, n.size, n.ctypes.data, t.ctypes.data, p.ctypes.data,
+                                                 up.ctypes.data, stream))
+        else:
+            _check(_LIB.mlq_hip_kv_plan_set(self.h, n.size, n.ctypes.data, t.ctypes.data, p.ctypes.data, stream))
+        self._n_seqs = n.size
 
     def write(self, layer: int, k, v, q=None, q_out=None, theta: float = 0.0, neox: bool = False, stream=None) -> None:
         """k and v into the batch's pages; theta > 0 rotates k, and q into q_out."""
@@ -693,9 +728,50 @@ class KvPlan:
     def attention(self, layer: int, q, out, stream=None) -> None:
         _check(_LIB.mlq_hip_kv_attention(self.h, layer, _ptr(q), _ptr(out), stream))
 
+    def pick(self, logits, vocab: int, tokens, picks, n_kept, kept, next_token, stream=None) -> None:
+        """Greedy picks of the nodes' logits and the paths of drafted tokens that they confirm (device buffers)."""
+        _check(_LIB.mlq_hip_kv_tree_pick(self.h, _ptr(logits), vocab, _ptr(tokens), _ptr(picks), _ptr(n_kept), _ptr(kept),
+                                         _ptr(next_token), stream))
+
+    def keep(self, n_kept, kept, stream=None) -> None:
+        """Moves the kept nodes of each sequence's tree (host lists, one sequence's after the other's) to its first
+        slots, in every layer."""
+        n, k = _ints(n_kept, "n_kept"), _ints(kept, "kept")
+        if n.size != self._n_seqs:
+            raise ValueError("one count per sequence of the batch")
+        if k.size != sum(int(x) for x in n if x > 0):
+            raise ValueError(f"{k.size} kept nodes, the counts need {sum(int(x) for x in n if x > 0)}")
+        _check(_LIB.mlq_hip_kv_keep(self.h, n.ctypes.data, k.ctypes.data, stream))
+
     def destroy(self) -> None:
         if getattr(self, "h", None):
             _LIB.mlq_hip_kv_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+class BeamSelect:
+    """Beam search's selection and its workspace (mlq_hip_beam_*)."""
+
+    def __init__(self, max_groups: int, max_beams: int, max_vocab: int, max_keep: int, device: int = 0):
+        h = _vp()
+        _check(load().mlq_hip_beam_create(device, max_groups, max_beams, max_vocab, max_keep, ctypes.byref(h)))
+        self.h = h.value
+
+    def select(self, logits, scores, groups: int, beams: int, vocab: int, keep: int, parents, tokens, out_scores,
+               ended=None, end_token: int = 0, stream=None) -> None:
+        """The `keep` best continuations of each group's beams: parents, tokens and values [groups][keep]."""
+        _check(_LIB.mlq_hip_beam_select(self.h, _ptr(logits), _ptr(scores), _ptr(ended), end_token, groups, beams, vocab,
+                                        keep, _ptr(parents), _ptr(tokens), _ptr(out_scores), stream))
+
+    def destroy(self) -> None:
+        if getattr(self, "h", None):
+            _LIB.mlq_hip_beam_destroy(self.h)
             self.h = None
 
     def __del__(self):
