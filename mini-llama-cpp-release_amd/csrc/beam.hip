@@ -22,113 +22,160 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 
-// Orders by value, then by lower index.
-__device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) {
+// Unsigned numbers in the order of the values (-0 is 0), and back.
+__device__ __forceinline__ uint32_t order_of(float v) {
     uint32_t b = __builtin_bit_cast(uint32_t, v);
     b = b == 0x80000000u ? 0u : b;
-    const uint32_t order = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return static_cast<unsigned long long>(order) << 32 | static_cast<uint32_t>(~index);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float logit_of(unsigned long long key) {
-    const uint32_t order = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float value_of(uint32_t order) {
     return __builtin_bit_cast(float, (order & 0x80000000u) ? order & 0x7fffffffu : ~order);
 }
+// Orders by value, then by lower index.
+__device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) {
+    return static_cast<unsigned long long>(order_of(v)) << 32 | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ float logit_of(unsigned long long key) { return value_of(static_cast<uint32_t>(key >> 32)); }
 __device__ __forceinline__ uint32_t index_of(unsigned long long key) { return ~static_cast<uint32_t>(key); }
 constexpr unsigned long long kNoKey = 0;  // below every logit's key, -Inf's too
 
-// exp(d) for d <= 0 in 64 bits, 2^-36 of it off at the most: 2^n times the series to degree 9 of the rest, at most
-// 0.35 (0.35^10 / 10! = 7.6e-12).  0 below -700.
+// exp(d) for d <= 0 in 64 bits, 2^-39 of it off at the most: 2^n times a polynomial of the rest, at most 0.3466 (of
+// degree 8, through exp at the Chebyshev points; 1.1e-12 off, the series to degree 9 6.9e-12).  0 below -800.  n is
+// rounded by a sum whose last places are whole numbers: its low word is n.
 __device__ __forceinline__ double exp64(double d) {
-    const double n = rint(d * 1.4426950408889634);
-    const double r = fma(n, -0.6931471805599453, d);
-    double y = 1.0 / 362880;
-    y = fma(y, r, 1.0 / 40320);
-    y = fma(y, r, 1.0 / 5040);
-    y = fma(y, r, 1.0 / 720);
-    y = fma(y, r, 1.0 / 120);
-    y = fma(y, r, 1.0 / 24);
-    y = fma(y, r, 1.0 / 6);
-    y = fma(y, r, 0.5);
+    constexpr double kWhole = 6755399441055744.0;  // 1.5 x 2^52
+    d = fmax(d, -800.0);
+    const double t = fma(d, 1.4426950408889634, kWhole);
+    const double r = fma(t - kWhole, -0.6931471805599453, d);
+    double y = 2.4876178959085513e-05;
+    y = fma(y, r, 0.00019915881871396035);
+    y = fma(y, r, 0.001388882165071769);
+    y = fma(y, r, 0.008333266071022454);
+    y = fma(y, r, 0.0416666668910917);
+    y = fma(y, r, 0.16666666891180545);
+    y = fma(y, r, 0.49999999999797773);
+    y = fma(y, r, 0.999999999979769);
     y = fma(y, r, 1.0);
-    y = fma(y, r, 1.0);
-    return d < -700.0 ? 0.0 : ldexp(y, static_cast<int>(n));
+    return ldexp(y, static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, t))));
+}
+
+// The r-th largest of the wave's values, r from 1 to 64 (the order of their bits, bit by bit).
+__device__ __forceinline__ uint32_t wave_rth_largest(uint32_t v, int r) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | 1u << bit;
+        t = __builtin_popcountll(__ballot(v >= c)) >= r ? c : t;
+    }
+    return t;
 }
 
 template <int E>
-__global__ __launch_bounds__(kThreads) void beam_part_kernel(BeamCall c, int parts) {
-    __shared__ unsigned long long key[kThreads];
-    __shared__ unsigned long long list[kBeamMostKeep * E];
+__global__ __launch_bounds__(kThreads, 4) void beam_part_kernel(BeamCall c, int parts) {
+    constexpr int kMost = kBeamMostKeep * E;
+    __shared__ unsigned long long list[kMost];
     __shared__ float top_of[kWaves];
+    __shared__ uint32_t bar_of[kWaves];
     __shared__ int bad_of[kWaves];
     __shared__ double sum_of[kWaves];
-    __shared__ unsigned long long bar;
     __shared__ int found;
-    const int tid = threadIdx.x, wave = tid / 64;
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const long long total = static_cast<long long>(c.groups) * c.beams * parts;
     for (long long w = blockIdx.x; w < total; w += gridDim.x) {
-        const int part = static_cast<int>(w % parts);
-        const long long row = w / parts;
-        const int lo = static_cast<int>(static_cast<long long>(c.vocab) * part / parts);
-        const int n = static_cast<int>(static_cast<long long>(c.vocab) * (part + 1) / parts) - lo;  // E * kThreads at the most
-        const float* const from = c.logits + static_cast<size_t>(row) * c.vocab + lo;
+        const int lo = static_cast<int>(w % parts) * (E * kThreads), n = min(c.vocab - lo, E * kThreads);
+        const float* const from = c.logits + static_cast<size_t>(w / parts) * c.vocab + lo;
         float x[E];
+        if (n == E * kThreads) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = e * kThreads + tid;
-            x[e] = i < n ? from[i] : -__builtin_inff();
+            for (int e = 0; e < E; ++e) x[e] = from[e * kThreads + tid];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = e * kThreads + tid < n ? from[e * kThreads + tid] : -__builtin_inff();
         }
-        float top = -__builtin_inff();
+        float mine = -__builtin_inff();
         bool bad = false;
-        unsigned long long mine = kNoKey;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             bad = bad || !(x[e] < __builtin_inff());
-            top = fmaxf(top, x[e]);
-            const int i = e * kThreads + tid;
-            if (i < n) {
-                const unsigned long long k = key_of(x[e], static_cast<uint32_t>(lo + i));
-                mine = k > mine ? k : mine;
-            }
+            mine = fmaxf(mine, x[e]);
         }
+        // Enough of the wave's threads have a logit from here on.
+        const uint32_t wave_bar = wave_rth_largest(order_of(mine), (c.keep + kWaves - 1) / kWaves);
+        float top = mine;
 #pragma unroll
         for (int s = 32; s > 0; s /= 2) top = fmaxf(top, __shfl_xor(top, s));
         const bool wave_bad = __any(bad);
         __syncthreads();  // the last part's readers are done
-        key[tid] = mine;
-        if (tid % 64 == 0) top_of[wave] = top, bad_of[wave] = wave_bad;
+        if (lane == 0) top_of[wave] = top, bad_of[wave] = wave_bad, bar_of[wave] = wave_bar;
         if (tid == 0) found = 0;
         __syncthreads();
+        uint32_t lowest = bar_of[0];
         bad = false;
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) top = fmaxf(top, top_of[k]), bad = bad || bad_of[k] != 0;
-        // The sum, and where this thread's largest stands among the threads'.
+        for (int k = 0; k < kWaves; ++k) {
+            top = fmaxf(top, top_of[k]);
+            bad = bad || bad_of[k] != 0;
+            lowest = min(lowest, bar_of[k]);
+        }
+        // The keys of what passes the bar.
+        const float bar = fmaxf(value_of(lowest), -3.402823466e38f);  // (-Inf is no continuation)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const unsigned long long who = __ballot(x[e] >= bar);
+            if (who == 0) continue;
+            int base = 0;
+            if (lane == 0) base = atomicAdd(&found, __builtin_popcountll(who));
+            base = __builtin_amdgcn_readfirstlane(base);
+            const int at = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32),
+                                                            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+            if (x[e] >= bar && at < kMost) list[at] = key_of(x[e], static_cast<uint32_t>(lo + e * kThreads + tid));
+        }
         double sum = 0.0;
         if (top > -__builtin_inff()) {
+            const double top64 = top;
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += x[e] > -__builtin_inff() ? exp64(static_cast<double>(x[e]) - static_cast<double>(top)) : 0.0;
+            for (int e = 0; e < E; ++e) {
+                sum += exp64(static_cast<double>(x[e]) - top64);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few of them at a time: registers)
+            }
         }
 #pragma unroll
         for (int s = 32; s > 0; s /= 2) sum += __shfl_xor(sum, s);
-        if (tid % 64 == 0) sum_of[wave] = sum;
-        int rank = 0;
-        for (int k = 0; k < kThreads; ++k) rank += key[k] > mine || (key[k] == mine && k < tid) ? 1 : 0;
-        if (rank == c.keep - 1) bar = mine;
+        if (lane == 0) sum_of[wave] = sum;
         __syncthreads();
-        // (a thread without logits has kNoKey; with a bar of that all logits pass, which are then fewer than keep * E)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = e * kThreads + tid;
-            if (i < n) {
-                const unsigned long long k = key_of(x[e], static_cast<uint32_t>(lo + i));
-                if (k >= bar) list[atomicAdd(&found, 1)] = k;
+        int m = found;
+        if (__builtin_expect(m > kMost, 0)) {
+            // As many equal logits: the bar is that of the threads' best keys, which differ.
+            __shared__ unsigned long long key[kThreads], key_bar;
+            unsigned long long best = kNoKey;
+#pragma unroll 1
+            for (int i = tid; i < n; i += kThreads) {
+                const float v = from[i];
+                const unsigned long long k = key_of(v, static_cast<uint32_t>(lo + i));
+                if (v > -__builtin_inff() && k > best) best = k;
             }
+            key[tid] = best;
+            __syncthreads();
+            int rank = 0;
+            for (int k = 0; k < kThreads; ++k) rank += key[k] > best || (key[k] == best && k < tid) ? 1 : 0;
+            if (rank == c.keep - 1) key_bar = best;
+            if (tid == 0) found = 0;
+            __syncthreads();
+            // (of keep threads: at most all their logits)
+#pragma unroll 1
+            for (int i = tid; i < n; i += kThreads) {
+                const float v = from[i];
+                const unsigned long long k = key_of(v, static_cast<uint32_t>(lo + i));
+                if (v > -__builtin_inff() && k >= key_bar) list[atomicAdd(&found, 1)] = k;
+            }
+            __syncthreads();
+            m = found;
         }
-        __syncthreads();
-        const int m = found;
         unsigned long long* const best = c.best + static_cast<size_t>(w) * c.keep;
         for (int i = tid; i < m; i += kThreads) {
             const unsigned long long k = list[i];
             int at = 0;
+#pragma unroll 8
             for (int j = 0; j < m; ++j) at += list[j] > k ? 1 : 0;
             if (at < c.keep) best[at] = k;
         }
@@ -152,42 +199,69 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
     return a.value != b.value ? a.value > b.value : a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
 }
 
+constexpr int kGroupEach = 8;  // candidates a thread and round
+constexpr int kLanes = 16;     // that take a beam's parts
+
 __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int parts) {
-    constexpr int E = 4;  // candidates a thread and round
+    constexpr int E = kGroupEach, kMost = kBeamMostKeep * E;
     __shared__ double sums[kBeamMostBeams], score[kBeamMostBeams];
     __shared__ int state[kBeamMostBeams];  // 0: no continuations, 1: of the logits, 2: ended
-    __shared__ Candidate of_thread[kThreads], bar, list[kBeamMostKeep * (E + 1)], best[kBeamMostKeep];
-    __shared__ int found, have, bad;
-    const int tid = threadIdx.x, keep = c.keep;
+    __shared__ Candidate list[kMost + kBeamMostKeep], best[kBeamMostKeep];
+    __shared__ double value[kMost + kBeamMostKeep];  // of the list
+    __shared__ uint32_t bar_of[kWaves];
+    __shared__ int found, bad;
+    const int tid = threadIdx.x, wave = tid / 64, keep = c.keep;
     const double none = -__builtin_inf();
     for (int group = blockIdx.x; group < c.groups; group += gridDim.x) {
+        const int per = parts * keep, n = c.beams * per;
+        const unsigned long long* const keys = c.best + static_cast<size_t>(group) * n;
+        // (neighbours go to the waves in turn, so that each has its part of few candidates)
+        const int turn = tid % 64 * kWaves + wave;
+        unsigned long long key[E];
+        auto load = [&](int first) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = first + e * kThreads + turn;
+                key[e] = i < n ? keys[i] : kNoKey;
+            }
+        };
+        load(0);
+        __syncthreads();  // the last group's readers are done
+        if (tid == 0) bad = 0;
         __syncthreads();
-        if (tid == 0) have = 0, bad = 0;
-        __syncthreads();
-        for (int b = tid; b < c.beams; b += kThreads) {
-            const size_t row = static_cast<size_t>(group) * c.beams + b;
+        // The beams' sums: the parts' over their largest logit, lanes and then pairs of lanes in order.
+        for (int b = tid / kLanes; b < (c.beams + 3) / 4 * 4; b += kThreads / kLanes) {  // (whole waves)
+            const bool there = b < c.beams;
+            const size_t row = static_cast<size_t>(group) * c.beams + min(b, c.beams - 1);
             const float s = c.scores[row];
             int what = !(s < __builtin_inff()) ? -1 : s == -__builtin_inff() ? 0 : c.ended != nullptr && c.ended[row] != 0 ? 2 : 1;
-            sums[b] = 0.0;
-            if (what == 1) {
-                const BeamPart* const p = c.parts + row * parts;
-                float top = -__builtin_inff();
-                bool wrong = false;
-                for (int k = 0; k < parts; ++k) {
-                    const float x = p[k].largest;
-                    wrong = wrong || x != x;
-                    top = fmaxf(top, x);
-                }
-                double sum = 0.0;
-                for (int k = 0; k < parts; ++k) {
-                    if (p[k].largest > -__builtin_inff()) sum += p[k].sum * exp64(static_cast<double>(p[k].largest) - static_cast<double>(top));
-                }
-                sums[b] = static_cast<double>(top) + log(sum);
-                what = wrong ? -1 : top == -__builtin_inff() ? 0 : 1;
+            const BeamPart* const p = c.parts + row * parts;
+            float top = -__builtin_inff();
+            int wrong = 0;
+            for (int k = tid % kLanes; k < parts; k += kLanes) {
+                const float x = p[k].largest;
+                wrong |= x != x ? 1 : 0;
+                top = fmaxf(top, x);
             }
-            score[b] = static_cast<double>(s);
-            state[b] = what;
-            if (what < 0) bad = 1;
+#pragma unroll
+            for (int k = kLanes / 2; k > 0; k /= 2) {
+                top = fmaxf(top, __shfl_xor(top, k));
+                wrong |= __shfl_xor(wrong, k);
+            }
+            double sum = 0.0;
+            for (int k = tid % kLanes; k < parts; k += kLanes) {
+                const BeamPart x = p[k];
+                if (x.largest > -__builtin_inff()) sum += x.sum * exp64(static_cast<double>(x.largest) - static_cast<double>(top));
+            }
+#pragma unroll
+            for (int k = kLanes / 2; k > 0; k /= 2) sum += __shfl_xor(sum, k);
+            if (there && tid % kLanes == 0) {
+                if (what == 1) what = wrong != 0 ? -1 : top == -__builtin_inff() ? 0 : 1;
+                sums[b] = what == 1 ? static_cast<double>(top) + log(sum) : 0.0;
+                score[b] = static_cast<double>(s);
+                state[b] = what;
+                if (what < 0) bad = 1;
+            }
         }
         __syncthreads();
         const size_t out = static_cast<size_t>(group) * keep;
@@ -199,54 +273,92 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
             continue;
         }
         // Rounds: what is best so far, and the next candidates.
-        const int per = parts * keep, n = c.beams * per;
-        const unsigned long long* const keys = c.best + static_cast<size_t>(group) * n;
+        int have = 0;
         for (int first = 0; first < n; first += E * kThreads) {
-            Candidate mine{none, kNoKey, c.beams}, x[E];
+            Candidate x[E];
+            float mine = -__builtin_inff();  // of the thread's, rounded down
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int i = first + e * kThreads + tid;
-                x[e] = Candidate{none, kNoKey, c.beams};
+                const int i = first + e * kThreads + turn, b = min(i / per, c.beams - 1);
+                x[e] = Candidate{none, key[e], b};
                 if (i < n) {
-                    const int b = i / per;
-                    if (state[b] == 1) {
-                        const unsigned long long k = keys[i];
-                        const float logit = logit_of(k);
-                        if (k != kNoKey && logit > -__builtin_inff()) {
-                            x[e] = Candidate{score[b] + (static_cast<double>(logit) - sums[b]), k, b};
-                        }
+                    const float logit = logit_of(key[e]);
+                    if (state[b] == 1 && key[e] != kNoKey) {
+                        x[e].value = score[b] + (static_cast<double>(logit) - sums[b]);
                     } else if (state[b] == 2 && i % per == 0) {
-                        x[e] = Candidate{score[b], key_of(0.0f, static_cast<uint32_t>(c.end_token)), b};
+                        x[e].value = score[b];
+                        x[e].key = key_of(0.0f, static_cast<uint32_t>(c.end_token));
                     }
                 }
-                if (before(x[e], mine)) mine = x[e];
+                mine = fmaxf(mine, __double2float_rd(x[e].value));
             }
-            of_thread[tid] = mine;
+            if (first + E * kThreads < n) load(first + E * kThreads);
+            const uint32_t wave_bar = wave_rth_largest(order_of(mine), (keep + kWaves - 1) / kWaves);
+            if (tid % 64 == 0) bar_of[wave] = wave_bar;
             if (tid == 0) found = 0;
             __syncthreads();
-            int rank = 0;
-            for (int k = 0; k < kThreads; ++k) {
-                const Candidate other = of_thread[k];
-                rank += before(other, mine) || (k < tid && !before(mine, other)) ? 1 : 0;
-            }
-            if (rank == keep - 1) bar = mine;
-            __syncthreads();
-            const Candidate least = bar;
+            uint32_t lowest = bar_of[0];
+#pragma unroll
+            for (int k = 1; k < kWaves; ++k) lowest = min(lowest, bar_of[k]);
+            double bar = static_cast<double>(value_of(lowest));
+            if (have == keep) bar = fmax(bar, best[keep - 1].value);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                if (x[e].beam < c.beams && !before(least, x[e])) list[atomicAdd(&found, 1)] = x[e];
-            }
-            for (int i = tid; i < have; i += kThreads) list[atomicAdd(&found, 1)] = best[i];
-            __syncthreads();
-            const int m = found;
-            for (int i = tid; i < m; i += kThreads) {
-                const Candidate k = list[i];
-                int at = 0;
-                for (int j = 0; j < m; ++j) at += before(list[j], k) ? 1 : 0;
-                if (at < keep) best[at] = k;
+                if (x[e].value >= bar && x[e].value > none) {
+                    const int at = atomicAdd(&found, 1);
+                    if (at < kMost) list[at] = x[e];
+                }
             }
             __syncthreads();
-            if (tid == 0) have = min(m, keep);
+            int m = found;
+            if (__builtin_expect(m > kMost, 0)) {
+                // As many values that f32 does not tell apart: the bar is that of the threads' best, which differ.
+                __shared__ Candidate of_thread[kThreads], exact_bar;
+                Candidate top{none, kNoKey, c.beams};
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (x[e].value > none && before(x[e], top)) top = x[e];
+                }
+                of_thread[tid] = top;
+                __syncthreads();
+                int rank = 0;
+                for (int k = 0; k < kThreads; ++k) {
+                    const Candidate other = of_thread[k];
+                    rank += before(other, top) || (k < tid && !before(top, other)) ? 1 : 0;
+                }
+                if (rank == keep - 1) exact_bar = top;
+                if (tid == 0) found = 0;
+                __syncthreads();
+                const Candidate least = exact_bar;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (x[e].value > none && !before(least, x[e])) list[atomicAdd(&found, 1)] = x[e];
+                }
+                __syncthreads();
+                m = found;
+            }
+            if (m > 0) {
+                for (int i = tid; i < have; i += kThreads) list[m + i] = best[i];
+                m += have;
+                __syncthreads();
+                for (int i = tid; i < m; i += kThreads) value[i] = list[i].value;
+                __syncthreads();
+                for (int i = tid; i < m; i += kThreads) {
+                    const Candidate k = list[i];
+                    int at = 0, equal = 0;
+#pragma unroll 8
+                    for (int j = 0; j < m; ++j) {
+                        const double v = value[j];
+                        at += v > k.value ? 1 : 0;
+                        equal += v == k.value ? 1 : 0;
+                    }
+                    if (equal > 1) {
+                        for (int j = 0; j < m; ++j) at += value[j] == k.value && before(list[j], k) ? 1 : 0;
+                    }
+                    if (at < keep) best[at] = k;
+                }
+                have = min(m, keep);
+            }
             __syncthreads();
         }
         for (int i = tid; i < keep; i += kThreads) {
@@ -261,9 +373,11 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
 }  // namespace
 
 hipError_t launch_beam_select(const BeamCall& c, hipStream_t s) {
-    const int parts = beam_parts(c.vocab);
+    const int each = beam_part(static_cast<long long>(c.groups) * c.beams, c.vocab), parts = (c.vocab + each - 1) / each;
     const long long groups = static_cast<long long>(c.groups) * c.beams * parts;
-    beam_part_kernel<kBeamPart / kThreads><<<static_cast<unsigned>(std::min<long long>(groups, 1 << 20)), kThreads, 0, s>>>(c, parts);
+    const unsigned grid = static_cast<unsigned>(std::min<long long>(groups, 1 << 20));
+    if (each == kBeamPart) beam_part_kernel<kBeamPart / kThreads><<<grid, kThreads, 0, s>>>(c, parts);
+    else beam_part_kernel<kBeamSmallPart / kThreads><<<grid, kThreads, 0, s>>>(c, parts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     beam_group_kernel<<<std::min(c.groups, 1 << 20), kThreads, 0, s>>>(c, parts);

@@ -40,7 +40,7 @@ int entry(const char* caller, F&& body) {
 }
 
 size_t part_count(const mlq_beam_s& h) {
-    return static_cast<size_t>(h.max_groups) * h.max_beams * mlq::beam_parts(h.max_vocab);
+    return mlq::beam_parts(static_cast<long long>(h.max_groups) * h.max_beams, h.max_vocab);
 }
 
 struct Buffer {
@@ -67,7 +67,7 @@ int mlq_hip_beam_create(int device, int max_groups, int max_beams, int max_vocab
         }
         auto h = std::make_unique<mlq_beam_s>();
         h->device = device, h->max_groups = max_groups, h->max_beams = max_beams, h->max_vocab = max_vocab, h->max_keep = max_keep;
-        if (static_cast<double>(max_groups) * max_beams * mlq::beam_parts(max_vocab) > 0x1p28) {
+        if (static_cast<double>(max_groups) * max_beams * (max_vocab / mlq::kBeamPart + 1) > 0x1p28) {
             return abi_fail(MLQ_ERR_LIMIT, who + ": more than 2^28 parts of rows of logits");
         }
         const int rc = mlq::abi_device(device);
