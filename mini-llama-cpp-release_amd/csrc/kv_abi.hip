@@ -201,7 +201,7 @@ int create_plan(const char* caller, mlq_kv_cache_t cache, int n_heads, int windo
         p->scale = scale != 0.0f ? scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(kv.head_dim)));
         p->shape = mlq::KvPlanShape{kv.page_size, kv.n_pages, kv.n_kv, n_heads / kv.n_kv, mlq::kv_wide_rows(kv.nb),
                                     window, sinks, max_seqs, max_tokens, max_pages, max_nodes,
-                                    mlq::kv_tree_rows(kv.nb)};
+                                    mlq::kv_tree_cost(kv.qtype, kv.nb)};
         const mlq::KvPlanLimits lim = mlq::kv_plan_limits(p->shape);
         if (lim.masks > kMost) return abi_fail(MLQ_ERR_LIMIT, who + ": more than 2^30 words of who sees whom");
         const bool trees = max_nodes > 0;
@@ -232,8 +232,7 @@ int create_plan(const char* caller, mlq_kv_cache_t cache, int n_heads, int windo
         size_t floats[2], words[2];
         for (int i = 0; i < 2; ++i) {
             words[i] = (static_cast<size_t>(lim.slots[i]) * kv.n_kv + 63) / 64 * 64;
-            floats[i] = static_cast<size_t>(lim.slots[i]) * kv.n_kv *
-                        (trees ? mlq::kv_tree_partial_floats(kv.nb, i) : mlq::kv_partial_floats(kv.nb, i));
+            floats[i] = static_cast<size_t>(lim.slots[i]) * kv.n_kv * mlq::kv_partial_floats(kv.nb, i);
         }
         const size_t keys = trees ? std::max(max_tokens, mlq::kKvPickParts) : 0;
         MLQ_KV_HIP(hipMalloc(&p->work, (words[0] + words[1] + floats[0] + floats[1]) * 4 + keys * 8));
@@ -498,7 +497,6 @@ int mlq_hip_kv_attention(mlq_kv_plan_t p, int layer, const float* q, float* out,
         for (int kind = 0; kind < 2; ++kind) {
             const int count = p->counts[mlq::kKvCountNarrow + kind];
             if (count == 0 && !recorded) continue;
-            if (kind == 1 && p->trees() && p->shape.tree_rows == mlq::kKvTreeRows) continue;  // (all are in the first list)
             const float to_base_2 = static_cast<float>(p->scale * 1.4426950408889634);
             if (p->trees()) {
                 const mlq::KvTreeAttention a{p->view(layer), p->tree_lists(), p->shape.group, p->shape.window, p->shape.sinks,

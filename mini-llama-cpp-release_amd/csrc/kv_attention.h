@@ -76,14 +76,15 @@ __device__ __forceinline__ T bits(uint32_t v) { return __builtin_bit_cast(T, v);
 
 // Reads of the work lists, through the scalar cache: uniform, constant for the launch.
 __device__ __forceinline__ int uniform(const int* p) { return *(const __attribute__((address_space(4))) int*)(p); }
-__device__ __forceinline__ KvAttnItem uniform(const KvAttnItem* p) {
-    constexpr int N = sizeof(KvAttnItem) / sizeof(int);
+template <typename Item>
+__device__ __forceinline__ Item uniform(const Item* p) {
+    constexpr int N = sizeof(Item) / sizeof(int);
     struct Words {
         int v[N];
     } w;
 #pragma unroll
     for (int i = 0; i < N; ++i) w.v[i] = uniform(reinterpret_cast<const int*>(p) + i);
-    return __builtin_bit_cast(KvAttnItem, w);
+    return __builtin_bit_cast(Item, w);
 }
 
 __device__ __forceinline__ float max_quarters(float v) {  // over the lanes of equal lane % 16

@@ -42,6 +42,23 @@
 namespace mlq {
 namespace kv {
 
+// What a call takes and its items are, of plain sequences and of trees: there a token's place in the sequence is its
+// slot, and who sees whom among the nodes is a bit a slot.
+template <bool TREE>
+using Attention = typename std::conditional<TREE, KvTreeAttention, KvAttention>::type;
+template <bool TREE>
+using AttentionItem = typename std::conditional<TREE, KvTreeItem, KvAttnItem>::type;
+
+// Of a tree: the bits of tile `tile`, one of the nodes', that the token in slot `slot` sees.
+__device__ __forceinline__ uint32_t node_bits(const KvTreeAttention& a, const KvTreeItem& it, int slot, int tile) {
+    const int start = it.len - it.new_tokens;
+    return a.lists.masks[it.mask0 + (slot - start) * it.words + tile - start / kKvTile];
+}
+// And its position.
+__device__ __forceinline__ int node_position(const KvTreeAttention& a, const KvTreeItem& it, int slot) {
+    return a.lists.pos[it.token0 + slot - (it.len - it.new_tokens)];
+}
+
 // Scales of a tile in LDS: what a code (f32: an element) is multiplied by, and, for f32
 // arithmetic on quantized codes, what is added then.
 template <int QT, int NB>
@@ -76,8 +93,8 @@ __device__ __forceinline__ float element(uint32_t w, int i, float d, float add) 
 // attention_rows_kernel does where blocks of a position that the row sees or of its query differ too much in size for
 // its operands.  Four rows at a time; a lane takes one position's half of every block for the scores, every 64th dimension for
 // the values.  In few registers: the kernel's own are not touched by it.  lds: the wave's, 4 (32 NB + 32) floats.
-template <int QT, int NB, int NQ>
-__device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnItem& it, int head, int row_base, uint32_t which, int wave,
+template <int QT, int NB, int NQ, bool TREE>
+__device__ __forceinline__ void plain_rows(const Attention<TREE>& a, const AttentionItem<TREE>& it, int head, int row_base, uint32_t which, int wave,
                                            int lane, const float* __restrict__ q, float* __restrict__ out, float* lds) {
     using F = KvForm<QT>;
     constexpr int KL = F::key_lane(NB), VL = F::value_lane(NB), HD = 32 * NB, DIMS = (HD + 63) / 64;
@@ -187,7 +204,13 @@ __device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnIte
             for (int k = 0; k < 4; ++k) {
                 float x = (s[k] + __shfl_xor(s[k], 32)) * to_t[k];
                 x = fmaf(x, 0.0f, x);  // an infinite scale: NaN
-                const bool seen = key <= pos[k] && (a.window == 0 || key > pos[k] - a.window || key < a.sinks);
+                bool seen;
+                if constexpr (TREE) {
+                    seen = t >= start / kKvTile ? (node_bits(a, it, pos[k], t) >> slot & 1u) != 0
+                                                : a.window == 0 || key > node_position(a, it, pos[k]) - a.window || key < a.sinks;
+                } else {
+                    seen = key <= pos[k] && (a.window == 0 || key > pos[k] - a.window || key < a.sinks);
+                }
                 x = seen ? x : -INFINITY;
                 const float to = fmaxf(m[k], over_lanes(x, larger)), c = __builtin_amdgcn_exp2f(m[k] - to);
                 m[k] = to;
@@ -258,8 +281,8 @@ __device__ __forceinline__ void plain_rows(const KvAttention& a, const KvAttnIte
     }
 }
 
-template <int QT, int NB, int NQ>
-__global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention a, int count, const float* __restrict__ q,
+template <int QT, int NB, int NQ, bool TREE = false>
+__global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(Attention<TREE> a, int count, const float* __restrict__ q,
                                                                       float* __restrict__ out) {
     using F = KvForm<QT>;
     using Scales = TileScales<QT, NB>;
@@ -311,7 +334,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 
     for (int w = blockIdx.x; w < total; w += gridDim.x) {
         const int head = w % n_kv;
-        const KvAttnItem it = uniform(a.lists.items[1] + w / n_kv);
+        const AttentionItem<TREE> it = uniform(a.lists.items[1] + w / n_kv);
         const int rows = it.new_tokens * a.group, start = it.len - it.new_tokens;
         const int row0 = it.row0 + wave * ROWS, row1 = min(rows, row0 + ROWS);
         const bool idle = row0 >= rows;
@@ -602,7 +625,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 
         // Fill the pipeline: scales of tiles 0 and 1 (counted from the item's first), keys of 0.
         if (threadIdx.x == 0) {
-            item_range[0] = start + it.row0 / a.group;
+            if constexpr (TREE) item_range[0] = it.near;
+            else item_range[0] = start + it.row0 / a.group;
             item_range[1] = start + (min(rows, it.row0 + kKvWaves * ROWS) - 1) / a.group;
         }
         __syncthreads();  // the last item's readers are done
@@ -711,8 +735,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x_[u][j] = sc[u][j >> 2][j & 3];
             const int first = tile_of(i) * kKvTile;
-            const bool full = first + kKvTile - 1 <= pos_lo &&
-                              (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
+            bool full;
+            if constexpr (TREE) {
+                full = tile_of(i) < start / kKvTile && (a.window == 0 || first > it.far - a.window || first + kKvTile <= a.sinks);
+            } else {
+                full = first + kKvTile - 1 <= pos_lo && (a.window == 0 || first > pos_hi - a.window || first + kKvTile <= a.sinks);
+            }
             const u4_t all = *reinterpret_cast<const u4_t*>(s->flags);
             const uint32_t flags = __builtin_amdgcn_readfirstlane(all.x | all.y | all.z | all.w);
             // (a lane's positions are 4 g .. and 16 + 4 g ..)
@@ -731,14 +759,34 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
                 }
             }
             if (!full) {
+                if constexpr (TREE) {
 #pragma unroll
-                for (int u = 0; u < NQ; ++u)
+                    for (int u = 0; u < NQ; ++u) {
+                        if (tile_of(i) >= start / kKvTile) {
+                            const uint32_t word = node_bits(a, it, pos[u], tile_of(i));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
-                        const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
-                        x_[u][j] = seen ? x_[u][j] : -INFINITY;
+                            for (int j = 0; j < 8; ++j) {
+                                x_[u][j] = (word >> ((j >> 2) * 16 + 4 * g + (j & 3)) & 1u) != 0 ? x_[u][j] : -INFINITY;
+                            }
+                        } else {
+                            const int since = node_position(a, it, pos[u]) - a.window;  // (there is a window, or the tile were full)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                                x_[u][j] = k > since || k < a.sinks ? x_[u][j] : -INFINITY;
+                            }
+                        }
                     }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int k = first + (j >> 2) * 16 + 4 * g + (j & 3);
+                            const bool seen = k <= pos[u] && (a.window == 0 || k > pos[u] - a.window || k < a.sinks);
+                            x_[u][j] = seen ? x_[u][j] : -INFINITY;
+                        }
+                }
             }
             // The maximum moves when it is passed by kSlack.
             float top[NQ];
@@ -856,7 +904,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
         }
         auto plain = [&] {
             // (in the LDS of the first keys' operands, which no wave reads any more)
-            plain_rows<QT, NB, NQ>(a, it, head, row0, again, wave, lane, q, out, reinterpret_cast<float*>(lds) + wave * 4 * (32 * NB + 32));
+            plain_rows<QT, NB, NQ, TREE>(a, it, head, row0, again, wave, lane, q, out, reinterpret_cast<float*>(lds) + wave * 4 * (32 * NB + 32));
         };
 
         if (it.nsplit > 1) {
@@ -903,24 +951,29 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(KvAttention
 constexpr unsigned kRecorded = 1024;
 constexpr long long kMostGroups = 1 << 20;
 
+// (a launch holds less than 2^32 threads; the kernels walk their lists whatever the grid)
+inline unsigned grid_of(const KvView& kv, int count) {
+    return count > 0 ? static_cast<unsigned>(std::min<long long>(static_cast<long long>(count) * kv.n_kv, kMostGroups)) : kRecorded;
+}
+
+template <int QT, int NB, bool TREE>
+hipError_t launch_rows(const Attention<TREE>& a, int count, const float* q, float* out, hipStream_t s) {
+    constexpr int NQ = NB <= 4 ? 2 : 1;
+    constexpr int lds = rows_lds_bytes<QT, NB>();
+    const auto kernel = attention_rows_kernel<QT, NB, NQ, TREE>;
+    if (lds > 64 << 10) {
+        const hipError_t e =
+            hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    kernel<<<grid_of(a.kv, count), kThreads, lds, s>>>(a, count, q, out);
+    return hipGetLastError();
+}
+
 template <int QT, int NB>
 hipError_t launch_blocks(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
-    // (a launch holds less than 2^32 threads; the kernels walk their lists whatever the grid)
-    const unsigned grid =
-        count > 0 ? static_cast<unsigned>(std::min<long long>(static_cast<long long>(count) * a.kv.n_kv, kMostGroups)) : kRecorded;
-    if (kind == 0) {
-        attention_kernel<QT, NB><<<grid, kThreads, 0, s>>>(a, count, q, out);
-    } else {
-        constexpr int NQ = NB <= 4 ? 2 : 1;
-        constexpr int lds = rows_lds_bytes<QT, NB>();
-        const auto kernel = attention_rows_kernel<QT, NB, NQ>;
-        if (lds > 64 << 10) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            if (e != hipSuccess) return e;
-        }
-        kernel<<<grid, kThreads, lds, s>>>(a, count, q, out);
-    }
+    if (kind != 0) return launch_rows<QT, NB, false>(a, count, q, out, s);
+    attention_kernel<QT, NB><<<grid_of(a.kv, count), kThreads, 0, s>>>(a, count, q, out);
     return hipGetLastError();
 }
 

@@ -11,35 +11,24 @@
 // lie, queries split in two fp16 parts over their block's largest, value scales in the weights, which are split over a
 // power of two of every row and block that keeps its largest at 2^9 .. 2^15.  There eight rows stand beside their own
 // low parts in an operand's sixteen columns; a tree has more rows than that, so here the sixteen columns are sixteen
-// rows, a block takes two products (f32: three, as low parts times low parts, 2^-22 of an element, are left out), and a
-// wave has NQ such groups for one decoding of a tile.
+// rows and a block takes two products (f32: three, as low parts times low parts, 2^-22 of an element, are left out).
 #pragma once
 
-#include "kv_attention.h"
+#include "kv_attention_rows.h"
 
 #include <algorithm>
 
 namespace mlq {
 namespace kv {
 
-__device__ __forceinline__ KvTreeItem uniform(const KvTreeItem* p) {
-    constexpr int N = sizeof(KvTreeItem) / sizeof(int);
-    struct Words {
-        int v[N];
-    } w;
-#pragma unroll
-    for (int i = 0; i < N; ++i) w.v[i] = uniform(reinterpret_cast<const int*>(p) + i);
-    return __builtin_bit_cast(KvTreeItem, w);
-}
-
-// (Two waves a SIMD where the registers allow it.)
-template <int QT, int NB, int NQ>
+// Waves a SIMD: two where 256 registers are enough, else one with all 512 (the compiler would rather have two that spill).
+template <int QT, int NB>
 constexpr int tree_waves() {
-    return (QT == 0 ? NB * NQ <= 2 : NB * NQ <= 4) ? 2 : 1;
+    return (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1;
 }
 
-template <int QT, int NB, int NQ>
-__global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attention_tree_kernel(
+template <int QT, int NB>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(tree_waves<QT, NB>(), NB <= 4 ? 8 : 1))) void attention_tree_kernel(
     KvTreeAttention a, int count, const float* __restrict__ q, float* __restrict__ out) {
     using F = KvForm<QT>;
     constexpr int SB = F::kScaleBytes;
@@ -54,52 +43,41 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
     const int i16 = lane & 15, g = lane >> 4;
     const int n_kv = a.kv.n_kv, hd = a.kv.head_dim, heads = n_kv * a.group;
     const int page_tiles = a.kv.page_tiles, tile_shift = __builtin_ctz(page_tiles);
-    const int total = (count > 0 ? count : uniform(a.lists.counts + kKvCountNarrow + NQ - 1)) * n_kv;
+    const int total = (count > 0 ? count : uniform(a.lists.counts + kKvCountNarrow)) * n_kv;
 
     for (int w = blockIdx.x; w < total; w += gridDim.x) {
         const int head = w % n_kv;
-        const KvTreeItem it = uniform(a.lists.items[NQ - 1] + w / n_kv);
+        const KvTreeItem it = uniform(a.lists.items[0] + w / n_kv);
         const int rows = it.new_tokens * a.group, start = it.len - it.new_tokens;
         const int first_node_tile = start / kKvTile;
 
-        // Lane's row u: its token, its position (only a window asks for it), where its bits and elements start.
-        auto row_of = [&](int u) { return min(it.row0 + 16 * u + i16, rows - 1); };
-        auto element_of = [&](int u) {
-            const int row = row_of(u);
-            return (static_cast<size_t>(it.token0 + row / a.group) * heads + head * a.group + row % a.group) * hd;
-        };
-        int pos[NQ];
-        const uint32_t* mask[NQ];
-        h8_t qh[NQ][NB], ql[NQ][NB];
-        float qsum[NQ][NB], to_t[NQ][NB];
-#pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            const int token = row_of(u) / a.group;
-            pos[u] = a.window > 0 ? a.lists.pos[it.token0 + token] : 0;
-            mask[u] = a.lists.masks + (it.mask0 + token * it.words - first_node_tile);
+        // The lane's row: its token's position (only a window asks for it), where its bits and its elements start.
+        const int row = min(it.row0 + i16, rows - 1), token = row / a.group;
+        const int pos = a.window > 0 ? a.lists.pos[it.token0 + token] : 0;
+        const uint32_t* const mask = a.lists.masks + (it.mask0 + token * it.words - first_node_tile);
+        const size_t out_row = (static_cast<size_t>(it.token0 + token) * heads + head * a.group + row % a.group) * hd;
+        h8_t qh[NB], ql[NB];
+        float qsum[NB], to_t[NB];
+        {
             float v[NB][8];
-            load_query<NB, true>(q + element_of(u), hd, g, a.scale * (QT == 0 ? 1.0f / kElementLift : 1.0f), v, qsum[u], to_t[u]);
+            load_query<NB, true>(q + out_row, hd, g, a.scale * (QT == 0 ? 1.0f / kElementLift : 1.0f), v, qsum, to_t);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                split8(v[b], &qh[u][b], &ql[u][b]);
-                if (QT == 3) qsum[u][b] = sum_quarters(qsum[u][b]) * to_t[u][b];
+                split8(v[b], &qh[b], &ql[b]);
+                if (QT == 3) qsum[b] = sum_quarters(qsum[b]) * to_t[b];
             }
         }
 
         const f4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        f4_t o[NQ][2 * NB];
-        float om[NQ][NB];   // Q4_1: this lane's part of the sum of weights times minima
-        int frame[NQ][NB];  // log2 f_b
-        uint32_t spoilt[NQ];  // bit b: this lane's part of the row sees a block that is not finite with a weight of 0
-        float m[NQ], l[NQ];
+        f4_t o[2 * NB];
+        float om[NB];   // Q4_1: this lane's part of the sum of weights times minima
+        int frame[NB];  // log2 f_b
+        uint32_t spoilt = 0;  // bit b: this lane's part of the row sees a block that is not finite with a weight of 0
+        float m = -3.402823466e38f, l = 0.0f;
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            m[u] = -3.402823466e38f, l[u] = 0.0f, spoilt[u] = 0;
+        for (int t = 0; t < 2 * NB; ++t) o[t] = zero;
 #pragma unroll
-            for (int t = 0; t < 2 * NB; ++t) o[u][t] = zero;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) om[u][b] = 0.0f, frame[u][b] = kMostFrame - kFirstUp;
-        }
+        for (int b = 0; b < NB; ++b) om[b] = 0.0f, frame[b] = kMostFrame - kFirstUp;
 
         // This wave's tiles: every fourth of the item's.
         const int end = it.first + it.count;
@@ -139,7 +117,7 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
         };
 
         // The next tile's loads are under way during this one's work, unless its registers are not enough for both.
-        constexpr bool AHEAD = QT == 0 ? NB * NQ <= 4 : QT != 3 || NB * NQ <= 6;
+        constexpr bool AHEAD = QT == 0 ? NB <= 4 : QT != 3 || NB <= 6;
         int at = it.first + wave;
         int next_page = 0;
         if (AHEAD && at < end) {
@@ -157,19 +135,14 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
             if (!AHEAD) load_keys(next);
             const bool nodes = tile_index >= first_node_tile;
             const bool full = !nodes && (a.window == 0 || first > it.far - a.window || first + kKvTile <= a.sinks);
-            uint32_t word[NQ];  // the tile's bits of the rows: of the nodes' tiles alone
-            if (nodes) {
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) word[u] = mask[u][tile_index];
-            }
+            uint32_t word = 0;  // a tile of nodes: the row's bits
+            if (nodes) word = mask[tile_index];
 
             // Scores.
-            float t[NQ][8];
+            float t[8];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                f4_t s[NQ];
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) s[u] = zero;
+                f4_t s = zero;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     h8_t hi, lo;
@@ -185,108 +158,100 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
                         const uint32_t x = kw[h][b];
                         hi = codes8(x & 0x0f0f0f0fu, (x >> 4) & 0x0f0f0f0fu, static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f));
                     }
+                    f4_t acc = mfma(hi, ql[b], mfma(hi, qh[b], zero));
+                    if (QT == 0) acc = mfma(lo, qh[b], acc);  // (times kElementLift, which to_t takes back)
+                    acc *= to_t[b];
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u) {
-                        f4_t acc = mfma(hi, ql[u][b], mfma(hi, qh[u][b], zero));
-                        if (QT == 0) acc = mfma(lo, qh[u][b], acc);  // (times kElementLift, which to_t takes back)
-                        acc *= to_t[u][b];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[u][i] = fmaf(scale_at(ks[h], 4 * b + i), acc[i], s[u][i]);
-                            if (QT == 3) s[u][i] = fmaf(scale_at(km[h], 4 * b + i), qsum[u][b], s[u][i]);
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        s[i] = fmaf(scale_at(ks[h], 4 * b + i), acc[i], s[i]);
+                        if (QT == 3) s[i] = fmaf(scale_at(km[h], 4 * b + i), qsum[b], s[i]);
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < NQ; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) t[u][4 * h + i] = s[u][i];
+                for (int i = 0; i < 4; ++i) t[4 * h + i] = s[i];
             }
             if (more) load_keys(next);
             if (!AHEAD) load_values(next);
 
             // Weights.
             auto key_in_tile = [&](int j) { return (j >> 2) * 16 + 4 * g + (j & 3); };
-            float p[NQ][8];
+            float p[8];
+            auto seen = [&](int j) -> bool {
+                const int k = key_in_tile(j), key = first + k;
+                return nodes ? (word >> k & 1u) != 0 : (a.window == 0) | (key > pos - a.window) | (key < a.sinks);
+            };
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                auto seen = [&](int j) -> bool {
-                    const int k = key_in_tile(j), key = first + k;
-                    return nodes ? (word[u] >> k & 1u) != 0 : (a.window == 0) | (key > pos[u] - a.window) | (key < a.sinks);
-                };
+            for (int j = 0; j < 8; ++j) {
+                // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
+                if (QT >= 2) t[j] = fmaf(t[j], 0.0f, t[j]);
+            }
+            if (!full) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    // an infinite scale (minimum) with codes that are not 0: NaN like the sum of its elements
-                    if (QT >= 2) t[u][j] = fmaf(t[u][j], 0.0f, t[u][j]);
+                for (int j = 0; j < 8; ++j) t[j] = seen(j) ? t[j] : -INFINITY;
+            }
+            float top = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])),
+                              fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+            top = max_quarters(top);
+            if (__any(top > m + kSlack)) {
+                const bool moves = top > m + kSlack;
+                const float to = ceilf(top);
+                const int up = moves ? static_cast<int>(fminf(to - m, static_cast<float>(kFirstUp))) : 0;
+                m = moves ? to : m;
+                l = ldexpf(l, -up);
+                int over = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    frame[b] += up;
+                    over = max(over, frame[b] - kMostFrame);
+                    if (QT == 3) om[b] = ldexpf(om[b], -up);
                 }
-                if (!full) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) t[u][j] = seen(j) ? t[u][j] : -INFINITY;
-                }
-                float top = fmaxf(fmaxf(fmaxf(t[u][0], t[u][1]), fmaxf(t[u][2], t[u][3])),
-                                  fmaxf(fmaxf(t[u][4], t[u][5]), fmaxf(t[u][6], t[u][7])));
-                top = max_quarters(top);
-                if (__any(top > m[u] + kSlack)) {
-                    const bool moves = top > m[u] + kSlack;
-                    const float to = ceilf(top);
-                    const int up = moves ? static_cast<int>(fminf(to - m[u], static_cast<float>(kFirstUp))) : 0;
-                    m[u] = moves ? to : m[u];
-                    l[u] = ldexpf(l[u], -up);
-                    int over = 0;
+                if (__builtin_expect(__any(over > 0), 0)) {
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        frame[u][b] += up;
-                        over = max(over, frame[u][b] - kMostFrame);
-                        if (QT == 3) om[u][b] = ldexpf(om[u][b], -up);
+                        const int less = max(frame[b] - kMostFrame, 0);
+                        frame[b] -= less;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[2 * b + x][i] = ldexpf(o[2 * b + x][i], -less);
                     }
-                    if (__builtin_expect(__any(over > 0), 0)) {
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = __builtin_amdgcn_exp2f(t[j] - m);
+                l += p[j];
+            }
+            const float least = fminf(fminf(fminf(p[0], p[1]), fminf(p[2], p[3])),
+                                      fminf(fminf(p[4], p[5]), fminf(p[6], p[7])));
+            if (__builtin_expect(__any(least == 0.0f), 0)) {
+                // (the largest of all scales and minima tells whether there is anything to look for)
+                uint32_t any_bad;
+                if (QT == 0) {
+                    uint32_t x = vs[0];
+#pragma unroll
+                    for (int i = 1; i < VS; ++i) x = max(x, vs[i]);
+                    any_bad = x >= 0x7f800000u;
+                } else {
+                    us2_t x{0, 0};
+#pragma unroll
+                    for (int i = 0; i < VS; ++i) {
+                        x = __builtin_elementwise_max(x, bits<us2_t>(vs[i]));
+                        if (QT == 3) x = __builtin_elementwise_max(x, bits<us2_t>(vm[QT == 3 ? i : 0] & 0x7fff7fffu));
+                    }
+                    any_bad = max(x.x, x.y) >= 0x7c00;
+                }
+                if (__builtin_expect(__any(any_bad != 0), 0)) {
+                    auto bad_at = [&](const uint32_t* s, int i) {
+                        return QT == 0 ? s[i] >= 0x7f800000u : ((s[i / 2] >> (i % 2 * 16)) & 0x7fffu) >= 0x7c00u;
+                    };
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bool lost = p[j] == 0.0f && seen(j);
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
-                            const int less = max(frame[u][b] - kMostFrame, 0);
-                            frame[u][b] -= less;
-#pragma unroll
-                            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], -less);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    p[u][j] = __builtin_amdgcn_exp2f(t[u][j] - m[u]);
-                    l[u] += p[u][j];
-                }
-                const float least = fminf(fminf(fminf(p[u][0], p[u][1]), fminf(p[u][2], p[u][3])),
-                                          fminf(fminf(p[u][4], p[u][5]), fminf(p[u][6], p[u][7])));
-                if (__builtin_expect(__any(least == 0.0f), 0)) {
-                    // (the largest of all scales and minima tells whether there is anything to look for)
-                    uint32_t any_bad;
-                    if (QT == 0) {
-                        uint32_t x = vs[0];
-#pragma unroll
-                        for (int i = 1; i < VS; ++i) x = max(x, vs[i]);
-                        any_bad = x >= 0x7f800000u;
-                    } else {
-                        us2_t x{0, 0};
-#pragma unroll
-                        for (int i = 0; i < VS; ++i) {
-                            x = __builtin_elementwise_max(x, bits<us2_t>(vs[i]));
-                            if (QT == 3) x = __builtin_elementwise_max(x, bits<us2_t>(vm[QT == 3 ? i : 0] & 0x7fff7fffu));
-                        }
-                        any_bad = max(x.x, x.y) >= 0x7c00;
-                    }
-                    if (__builtin_expect(__any(any_bad != 0), 0)) {
-                        auto bad_at = [&](const uint32_t* s, int i) {
-                            return QT == 0 ? s[i] >= 0x7f800000u : ((s[i / 2] >> (i % 2 * 16)) & 0x7fffu) >= 0x7c00u;
-                        };
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const bool lost = p[u][j] == 0.0f && seen(j);
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                const bool bad = bad_at(vs, 8 * b + j) || (QT == 3 && bad_at(vm, QT == 3 ? 8 * b + j : 0));
-                                spoilt[u] |= (lost && bad ? 1u : 0u) << b;
-                            }
+                            const bool bad = bad_at(vs, 8 * b + j) || (QT == 3 && bad_at(vm, QT == 3 ? 8 * b + j : 0));
+                            spoilt |= (lost && bad ? 1u : 0u) << b;
                         }
                     }
                 }
@@ -313,85 +278,76 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
                                        static_cast<_Float16>(QT == 2 ? 8.0f : 0.0f));
                     }
                 }
+                float v[8];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    float v[8];
+                for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[j], scale_at(vs, 8 * b + j));
+                float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+                if (__builtin_expect(__any(ldexpf(most, frame[b]) > 0x1p15f), 0)) {
+                    most = max_quarters(most);
+                    const int to = ldexpf(most, frame[b]) > 0x1p15f ? 9 - exponent(most) : frame[b];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = mul_or_zero(p[u][j], scale_at(vs, 8 * b + j));
-                    float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
-                    if (__builtin_expect(__any(ldexpf(most, frame[u][b]) > 0x1p15f), 0)) {
-                        most = max_quarters(most);
-                        const int to = ldexpf(most, frame[u][b]) > 0x1p15f ? 9 - exponent(most) : frame[u][b];
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
+                        for (int i = 0; i < 4; ++i) o[2 * b + x][i] = ldexpf(o[2 * b + x][i], to - frame[b]);
+                    frame[b] = to;
+                }
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], to - frame[u][b]);
-                        frame[u][b] = to;
-                    }
+                for (int j = 0; j < 8; ++j) v[j] = ldexpf(v[j], frame[b]);
+                if (QT == 3) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = ldexpf(v[j], frame[u][b]);
-                    if (QT == 3) {
+                    for (int j = 0; j < 8; ++j) om[b] += mul_or_zero(p[j], scale_at(vm, 8 * b + j));
+                }
+                h8_t ph, pl;
+                split8(v, &ph, &pl);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) om[u][b] += mul_or_zero(p[u][j], scale_at(vm, 8 * b + j));
-                    }
-                    h8_t ph, pl;
-                    split8(v, &ph, &pl);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        f4_t& acc = o[u][2 * b + x];
-                        acc = mfma(vh[x], pl, mfma(vh[x], ph, acc));
-                        if (QT == 0) acc = mfma(vl[x], ph, acc);
-                    }
+                for (int x = 0; x < 2; ++x) {
+                    f4_t& acc = o[2 * b + x];
+                    acc = mfma(vh[x], pl, mfma(vh[x], ph, acc));
+                    if (QT == 0) acc = mfma(vl[x], ph, acc);
                 }
             }
             if (more) load_values(next);
         }
 
         // The lanes' sums and the minima's part, out of the blocks' frames.
+        l = sum_quarters(l);
+        const bool any_spoilt = __any(spoilt != 0);
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) {
-            l[u] = sum_quarters(l[u]);
-            const bool any_spoilt = __any(spoilt[u] != 0);
+        for (int b = 0; b < NB; ++b) {
+            float add = QT == 3 ? sum_quarters(om[b]) : 0.0f;
+            add = fmaf(add, 0.0f, add);  // an infinite minimum: NaN
+            if (__builtin_expect(any_spoilt, 0)) add += sum_quarters((spoilt >> b) & 1u ? NAN : 0.0f);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float add = QT == 3 ? sum_quarters(om[u][b]) : 0.0f;
-                add = fmaf(add, 0.0f, add);  // an infinite minimum: NaN
-                if (__builtin_expect(any_spoilt, 0)) add += sum_quarters((spoilt[u] >> b) & 1u ? NAN : 0.0f);
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[u][2 * b + x][i] = ldexpf(o[u][2 * b + x][i], -frame[u][b] - (QT == 0 ? 13 : 0)) + add;
-                    }
-            }
+                for (int i = 0; i < 4; ++i) {
+                    o[2 * b + x][i] = ldexpf(o[2 * b + x][i], -frame[b] - (QT == 0 ? 13 : 0)) + add;
+                }
         }
-        // The four waves' states into wave 0, in a fixed order, sixteen rows at a time.
-        auto leave = [&](int u, float* to) {
+        // The four waves' states into wave 0, in a fixed order.
+        auto leave = [&](float* to) {
 #pragma unroll
-            for (int x = 0; x < 2 * NB; ++x) *reinterpret_cast<f4_t*>(to + (x * 64 + lane) * 4) = o[u][x];
-            to[2 * NB * 256 + lane] = m[u];
-            to[2 * NB * 256 + 64 + lane] = l[u];
+            for (int x = 0; x < 2 * NB; ++x) *reinterpret_cast<f4_t*>(to + (x * 64 + lane) * 4) = o[x];
+            to[2 * NB * 256 + lane] = m;
+            to[2 * NB * 256 + 64 + lane] = l;
         };
-        auto take = [&](int u, const float* from) {
+        auto take = [&](const float* from) {
             float w0, w1;
-            fold(m[u], l[u], from[2 * NB * 256 + lane], from[2 * NB * 256 + 64 + lane], &w0, &w1);
+            fold(m, l, from[2 * NB * 256 + lane], from[2 * NB * 256 + 64 + lane], &w0, &w1);
 #pragma unroll
             for (int x = 0; x < 2 * NB; ++x) {
-                o[u][x] = o[u][x] * w0 + *reinterpret_cast<const f4_t*>(from + (x * 64 + lane) * 4) * w1;
+                o[x] = o[x] * w0 + *reinterpret_cast<const f4_t*>(from + (x * 64 + lane) * 4) * w1;
             }
         };
         auto merge_waves = [&] {
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                __syncthreads();
-                if (wave >= 2) leave(u, merge + (wave - 2) * STATE);
-                __syncthreads();
-                if (wave < 2) take(u, merge + wave * STATE);
-                __syncthreads();
-                if (wave == 1) leave(u, merge);
-                __syncthreads();
-                if (wave == 0) take(u, merge);
-            }
+            __syncthreads();
+            if (wave >= 2) leave(merge + (wave - 2) * STATE);
+            __syncthreads();
+            if (wave < 2) take(merge + wave * STATE);
+            __syncthreads();
+            if (wave == 1) leave(merge);
+            __syncthreads();
+            if (wave == 0) take(merge);
         };
         merge_waves();
 
@@ -399,10 +355,10 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
             // This part's state to memory; the workgroup that arrives last merges all parts, wave w
             // taking w, w + 4, ...
             auto rsrc_of = [&](int split) {
-                return state_rsrc(a.partial, static_cast<size_t>(it.slot + split) * n_kv + head, NQ * STATE);
+                return state_rsrc(a.partial, static_cast<size_t>(it.slot + split) * n_kv + head, STATE);
             };
             if (wave == 0) {
-                leave_state<NQ, NB>(rsrc_of(it.split), lane, o, m, l);
+                leave_state<1, NB>(rsrc_of(it.split), lane, &o, &m, &l);
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the state is in memory
                 if (lane == 0) last = arrive(a.arrived + static_cast<size_t>(it.slot) * n_kv + head, it.nsplit);
             }
@@ -410,36 +366,22 @@ __global__ __launch_bounds__(kThreads, (tree_waves<QT, NB, NQ>())) void attentio
             const bool mine = last != 0u;
             __syncthreads();
             if (!mine) continue;
+            m = -3.402823466e38f;
+            l = 0.0f;
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                m[u] = -3.402823466e38f;
-                l[u] = 0.0f;
-#pragma unroll
-                for (int x = 0; x < 2 * NB; ++x) o[u][x] = zero;
-            }
-            for (int part = wave; part < it.nsplit; part += kKvWaves) take_state<NQ, NB>(rsrc_of(part), lane, o, m, l);
+            for (int x = 0; x < 2 * NB; ++x) o[x] = zero;
+            for (int part = wave; part < it.nsplit; part += kKvWaves) take_state<1, NB>(rsrc_of(part), lane, &o, &m, &l);
             merge_waves();
         }
 
-        if (wave == 0) {
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                if (it.row0 + 16 * u + i16 < rows) store_row<NB>(out + element_of(u), hd, g, o[u], 1.0f / l[u]);
-            }
-        }
+        if (wave == 0 && it.row0 + i16 < rows) store_row<NB>(out + out_row, hd, g, o, 1.0f / l);
     }
 }
 
-// Workgroups of a recorded launch, which walks whatever list is set by then.
-constexpr unsigned kTreeRecorded = 1024;
-
 template <int QT, int NB>
 hipError_t launch_tree_blocks(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {
-    // (a launch holds less than 2^32 threads; the kernel walks its list whatever the grid)
-    const unsigned grid =
-        count > 0 ? static_cast<unsigned>(std::min<long long>(static_cast<long long>(count) * a.kv.n_kv, 1 << 20)) : kTreeRecorded;
-    if (kind == 0) attention_tree_kernel<QT, NB, 1><<<grid, kThreads, 0, s>>>(a, count, q, out);
-    else if constexpr (NB <= 4) attention_tree_kernel<QT, NB, 2><<<grid, kThreads, 0, s>>>(a, count, q, out);
+    if (kind != 0) return launch_rows<QT, NB, true>(a, count, q, out, s);
+    attention_tree_kernel<QT, NB><<<grid_of(a.kv, count), kThreads, 0, s>>>(a, count, q, out);
     return hipGetLastError();
 }
 

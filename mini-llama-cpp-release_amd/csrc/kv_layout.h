@@ -147,9 +147,8 @@ struct KvTreeAttention {
     float* partial;
     unsigned* arrived;
 };
-// Query rows of a workgroup of the second list.
-int kv_tree_rows(int nb);
-size_t kv_tree_partial_floats(int nb, int kind);
+// (A part's floats in `partial` are those of kv_partial_floats.)
+KvTreeCost kv_tree_cost(int qtype, int nb);
 hipError_t launch_kv_tree_attention(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
 
 // Positions and pages moved within a cache, in all layers (kv_moves.hip).

@@ -121,9 +121,8 @@ KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     int whole[2] = {static_cast<int>(narrow) + s.max_seqs, static_cast<int>(rows / s.wide_rows) + s.max_seqs};
     KvPlanLimits l;
     if (s.max_nodes > 0) {
+        whole[0] = static_cast<int>(rows / kKvTreeRows) + s.max_seqs;
         // (a node's bits begin inside a tile at the most)
-        whole[0] = static_cast<int>(s.tree_rows > kKvTreeRows ? 0 : rows / kKvTreeRows) + s.max_seqs;
-        whole[1] = static_cast<int>(rows / s.tree_rows) + s.max_seqs;
         l.masks = static_cast<int64_t>(s.max_tokens) * (s.max_nodes / kKvTile + 2);
     }
     // a sequence's new tokens begin and end inside a tile at the most
@@ -185,10 +184,18 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     std::vector<KvAttnItem> base[2];
     std::vector<KvTreeItem> of_trees[2];
     int token0 = 0, row0 = 0, page0 = 0;
+    // Trees: the kernel that takes less for all of them (two launches would follow each other).
+    double few = 0.0, many = s.tree_cost.fill;
+    for (int i = 0; i < n_seqs && s.max_nodes > 0; ++i) {
+        const int rows = new_tokens[i] * s.group, tiles = ceil_div(kv_len[i], kKvTile);
+        few += static_cast<double>(ceil_div(rows, kKvTreeRows)) * tiles * s.n_kv_heads * s.tree_cost.few;
+        many += static_cast<double>(ceil_div(rows, s.wide_rows)) * tiles * s.n_kv_heads * s.tree_cost.many;
+    }
+    const int tree_kind = few <= many ? 0 : 1;
     // The row groups of sequence i's tree.
     auto add_item = [&](int i, int token, int page) -> std::string {
         const int n = new_tokens[i], start = kv_len[i] - n, rows = n * s.group;
-        const int kind = rows <= kKvTreeRows || s.tree_rows <= kKvTreeRows ? 0 : 1, step = kind == 0 ? kKvTreeRows : s.tree_rows;
+        const int step = tree_kind == 0 ? kKvTreeRows : s.wide_rows;
         const int mask0 = static_cast<int>(b.masks.size()), words = (kv_len[i] - 1) / kKvTile - start / kKvTile + 1;
         const std::string wrong =
             add_tree(s, "sequence " + std::to_string(i), n, start, parents != nullptr ? parents + token : nullptr, b);
@@ -202,7 +209,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
             }
             // (from the tree's first tile at the latest: a node may be seen as a sink wherever it lies)
             const Seen t = seen_tiles(s, near, start + last, start);
-            of_trees[kind].push_back(KvTreeItem{token, n, kv_len[i], page, r, 0, t.count, t.sinks, t.shift, 0, 1, 0, mask0, words, far, 0});
+            of_trees[tree_kind].push_back(KvTreeItem{token, n, kv_len[i], page, r, 0, t.count, t.sinks, t.shift, 0, 1, 0, mask0, words, near, far});
         }
         return "";
     };

@@ -49,8 +49,7 @@ struct KvTreeItem {
     int sinks, shift;
     int split, nsplit, slot;
     int mask0, words;
-    int far;  // the largest position of the item's rows
-    int pad;
+    int near, far;  // the smallest and the largest position of the item's rows
 };
 
 // A sequence of a batch of trees: its first row in the token buffers, and its nodes.
@@ -62,6 +61,13 @@ struct KvTreeSeq {
 constexpr int kKvTreeRows = 16;
 constexpr int kKvMostNodes = 1024;
 
+// What the trees' two kernels take, in ns: for a tile by a workgroup of the one for few rows (16 at a time) and of the one
+// for many (wide_rows at a time), and what the second takes longer for filling its pipeline and merging.  A batch runs
+// the one that takes less.
+struct KvTreeCost {
+    float few = 1.0f, many = 5.0f, fill = 30000.0f;
+};
+
 struct KvPlanShape {
     int page_size, n_pages, n_kv_heads;
     int group;      // query heads per KV head
@@ -69,7 +75,7 @@ struct KvPlanShape {
     int window, sinks;
     int max_seqs, max_tokens, max_pages;
     int max_nodes = 0;  // of a sequence's tree; 0: batches of plain sequences
-    int tree_rows = 2 * kKvTreeRows;  // query rows of a workgroup of the trees' second list
+    KvTreeCost tree_cost = {};
 };
 
 

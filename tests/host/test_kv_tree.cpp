@@ -67,7 +67,7 @@ void one(std::mt19937& rng, int trial) {
     s.wide_rows = 128;
     s.window = pick(rng, {0, 0, 1, 3, 20, 33, 100, 2147483647});
     s.sinks = s.window ? pick(rng, {0, 1, 4, 40, 2147483647}) : 0;
-    s.tree_rows = pick(rng, {16, 32});
+    s.tree_cost.fill = static_cast<float>(pick(rng, {0, 100, 30000, 1000000}));
     const int n_seqs = rng() % 5;
     std::vector<int> nodes(n_seqs), len(n_seqs), parents, pages;
     std::vector<Tree> trees;
@@ -103,7 +103,7 @@ void one(std::mt19937& rng, int trial) {
     std::map<int, std::set<int>> parts;
     for (int kind = 0; kind < 2; ++kind) {
         CHECK(static_cast<int>(b.trees[kind].size()) <= lim.items[kind], "trial %d: %d items", trial, static_cast<int>(b.trees[kind].size()));
-        const int step = kind == 0 ? mlq::kKvTreeRows : s.tree_rows;
+        const int step = kind == 0 ? mlq::kKvTreeRows : s.wide_rows;
         for (const KvTreeItem& it : b.trees[kind]) {
             CHECK(it.count > 0 && it.first >= 0 && it.split < it.nsplit, "trial %d", trial);
             if (it.nsplit > 1) {
@@ -207,8 +207,7 @@ void not_kept(const KvPlanShape& s, std::vector<int> n_kept, std::vector<int> ke
 int main() {
     std::mt19937 rng(11);
     for (int t = 0; t < 300; ++t) one(rng, t);
-    KvPlanShape s{64, 10, 2, 4, 256, 0, 0, 3, 100, 6};
-    s.max_nodes = 8;
+    KvPlanShape s{64, 10, 2, 4, 256, 0, 0, 3, 100, 6, 8, {}};
     refused(s, {9}, {9}, {-1, 0, 1, 2, 3, 4, 5, 6, 7}, "sequence 0: 9 nodes, the plan's trees hold 8");
     refused(s, {2}, {5}, {-1, 1}, "sequence 0: node 1 has parent 1");
     refused(s, {1, 3}, {5, 3}, {-1, -1, 0, 5}, "sequence 1: node 2 has parent 5");
