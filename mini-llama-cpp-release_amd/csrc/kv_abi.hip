@@ -60,8 +60,9 @@ struct mlq_kv_plan_s {
     float* partial[2] = {nullptr, nullptr};
     unsigned* arrived[2] = {nullptr, nullptr};
     void* work = nullptr;
-    // Of trees: keys of the picks' parts.
+    // Of trees: keys of the picks' parts, and their arrival counters.
     unsigned long long* keys = nullptr;
+    unsigned* picked = nullptr;
     // The batch; of trees also its sequences, parents and pages (for what is kept of it).
     bool set = false;
     int n_tokens = 0, n_positions = 0;
@@ -90,6 +91,7 @@ struct mlq_kv_plan_s {
         l.pos = reinterpret_cast<const int*>(lists + at[6]);
         l.parents = reinterpret_cast<const int*>(lists + at[7]);
         l.masks = reinterpret_cast<const uint32_t*>(lists + at[8]);
+        l.seq_of = reinterpret_cast<const int*>(lists + at[9]);
         return l;
     }
     bool trees() const { return shape.max_nodes > 0; }
@@ -211,7 +213,7 @@ int create_plan(const char* caller, mlq_kv_cache_t cache, int n_heads, int windo
             static_cast<size_t>(max_pages) * sizeof(mlq::KvPage), static_cast<size_t>(lim.items[0]) * item,
             static_cast<size_t>(lim.items[1]) * item, of_trees * max_seqs * sizeof(mlq::KvTreeSeq),
             of_trees * max_tokens * sizeof(int), of_trees * max_tokens * sizeof(int),
-            static_cast<size_t>(lim.masks) * sizeof(uint32_t)};
+            static_cast<size_t>(lim.masks) * sizeof(uint32_t), of_trees * max_tokens * sizeof(int)};
         for (int i = 0; i < mlq::kKvParts; ++i) {
             p->at[i] = p->list_bytes;
             p->list_bytes += (sizes[i] + 255) / 256 * 256;
@@ -234,14 +236,15 @@ int create_plan(const char* caller, mlq_kv_cache_t cache, int n_heads, int windo
             words[i] = (static_cast<size_t>(lim.slots[i]) * kv.n_kv + 63) / 64 * 64;
             floats[i] = static_cast<size_t>(lim.slots[i]) * kv.n_kv * mlq::kv_partial_floats(kv.nb, i);
         }
-        const size_t keys = trees ? std::max(max_tokens, mlq::kKvPickParts) : 0;
-        MLQ_KV_HIP(hipMalloc(&p->work, (words[0] + words[1] + floats[0] + floats[1]) * 4 + keys * 8));
+        const size_t keys = trees ? std::max(max_tokens, mlq::kKvPickParts) : 0, picked = of_trees * max_seqs * mlq::kKvPickApart;
+        MLQ_KV_HIP(hipMalloc(&p->work, (words[0] + words[1] + picked + floats[0] + floats[1]) * 4 + keys * 8));
         p->arrived[0] = static_cast<unsigned*>(p->work);
         p->arrived[1] = p->arrived[0] + words[0];
-        p->partial[0] = reinterpret_cast<float*>(p->arrived[1] + words[1]);
+        p->picked = p->arrived[1] + words[1];
+        p->partial[0] = reinterpret_cast<float*>(p->picked + picked);
         p->partial[1] = p->partial[0] + floats[0];
         p->keys = reinterpret_cast<unsigned long long*>(p->partial[1] + floats[1]);
-        MLQ_KV_HIP(hipMemsetAsync(p->work, 0, (words[0] + words[1]) * 4, s));
+        MLQ_KV_HIP(hipMemsetAsync(p->work, 0, (words[0] + words[1] + picked) * 4, s));
         MLQ_KV_HIP(hipStreamSynchronize(s));
         *out = p.release();
         return MLQ_OK;
@@ -276,7 +279,7 @@ int set_plan(const char* caller, mlq_kv_plan_t p, int n_seqs, const int* new_tok
             item_bytes[i] = trees ? b.trees[i].size() * sizeof b.trees[i][0] : b.items[i].size() * sizeof b.items[i][0];
         }
         const void* from[mlq::kKvParts] = {counts,   b.fresh.data(), b.pages.data(),   items[0],      items[1], b.seqs.data(),
-                                           b.pos.data(), b.parents.data(), b.masks.data()};
+                                           b.pos.data(), b.parents.data(), b.masks.data(), b.seq_of.data()};
         const size_t bytes[mlq::kKvParts] = {sizeof counts,
                                              b.fresh.size() * sizeof b.fresh[0],
                                              b.pages.size() * sizeof b.pages[0],
@@ -285,7 +288,8 @@ int set_plan(const char* caller, mlq_kv_plan_t p, int n_seqs, const int* new_tok
                                              b.seqs.size() * sizeof b.seqs[0],
                                              b.pos.size() * sizeof b.pos[0],
                                              b.parents.size() * sizeof b.parents[0],
-                                             b.masks.size() * sizeof b.masks[0]};
+                                             b.masks.size() * sizeof b.masks[0],
+                                             b.seq_of.size() * sizeof b.seq_of[0]};
         const int t = p->turn;
         MLQ_KV_HIP(hipEventSynchronize(p->uploaded[t]));  // the block's last upload (none yet: done)
         mlq::KvParts parts;
@@ -548,7 +552,7 @@ int mlq_hip_kv_tree_pick(mlq_kv_plan_t p, const float* logits, int vocab, const 
                 }
             }
         }
-        const mlq::KvPick k{p->tree_lists(), logits, vocab, tokens, picks, n_kept, kept, next, p->keys};
+        const mlq::KvPick k{p->tree_lists(), logits, vocab, tokens, picks, n_kept, kept, next, p->keys, p->picked};
         const hipError_t e = mlq::launch_kv_pick(k, recorded ? -1 : static_cast<int>(rows), recorded ? -1 : static_cast<int>(seqs), s);
         return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
     });

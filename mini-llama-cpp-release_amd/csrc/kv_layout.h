@@ -97,6 +97,7 @@ struct KvTreeLists {
     const KvTreeSeq* seqs;
     const int* pos;      // of each token
     const int* parents;  // of each token, among its sequence's
+    const int* seq_of;   // of each token
     const uint32_t* masks;
 };
 
@@ -107,7 +108,7 @@ struct KvRope {
 };
 
 // Copies `n` parts of pinned host memory to the lists (one launch, any stream).
-constexpr int kKvParts = 9;
+constexpr int kKvParts = 10;
 struct KvParts {
     const uint32_t* src[kKvParts];
     uint32_t* dst[kKvParts];
@@ -160,8 +161,10 @@ hipError_t launch_kv_moves(const KvView& kv, int n_layers, size_t layer_bytes, c
                            hipStream_t s);
 
 // Picks of a batch of trees and the paths they confirm (kv_pick.hip).  keys: a word a row and part, as many as rows,
-// kKvPickParts at the least.  tokens and seqs: of the batch, or -1: as many as the device says.
+// kKvPickParts at the least; arrived: kKvPickApart words a sequence, zero between launches.  tokens and seqs: of the
+// batch, or -1: as many as the device says.
 constexpr int kKvPickParts = 1024;
+constexpr int kKvPickApart = 16;
 struct KvPick {
     KvTreeLists lists;
     const float* logits;
@@ -169,6 +172,7 @@ struct KvPick {
     const int* tokens;
     int *picks, *n_kept, *kept, *next;
     unsigned long long* keys;
+    unsigned* arrived;
 };
 hipError_t launch_kv_pick(const KvPick& p, int tokens, int seqs, hipStream_t s);
 

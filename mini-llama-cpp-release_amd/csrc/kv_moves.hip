@@ -10,11 +10,12 @@ namespace mlq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCopies = 240, kMoves = 240;  // of a launch: its arguments stay below 4 KB
+constexpr int kCopies = 360, kMoves = 240;  // of a launch: its arguments stay below 4 KB
 constexpr int kTogether = 8;                // moves of a path that are read before one is written
 
 struct CopyArgs {
-    KvCopy copy[kCopies];
+    int from[kCopies], to[kCopies];
+    uint16_t tiles[kCopies];
 };
 struct MoveArgs {
     KvMove move[kMoves];
@@ -28,7 +29,8 @@ __global__ __launch_bounds__(kThreads) void kv_copy_kernel(KvView kv, int n_laye
     for (long long w = blockIdx.x; w < total; w += gridDim.x) {
         const int head = static_cast<int>(w % kv.n_kv);
         const long long rest = w / kv.n_kv;
-        const KvCopy c = args.copy[rest % n];
+        const int i_copy = static_cast<int>(rest % n);
+        const KvCopy c{args.from[i_copy], args.to[i_copy], args.tiles[i_copy]};
         uint8_t* const layer = kv.base + layer_bytes * (rest / n);
         const size_t page_bytes = static_cast<size_t>(kv.page_tiles) * tile_bytes;
         const uint4* const from = reinterpret_cast<const uint4*>(layer + (static_cast<size_t>(c.from) * kv.n_kv + head) * page_bytes);
@@ -168,7 +170,11 @@ hipError_t launch_kv_copy(const KvView& kv, int n_layers, size_t layer_bytes, co
     for (int at = 0; at < n; at += kCopies) {
         CopyArgs args;
         const int now = std::min(kCopies, n - at);
-        std::copy(copies + at, copies + at + now, args.copy);
+        for (int i = 0; i < now; ++i) {
+            args.from[i] = copies[at + i].from;
+            args.to[i] = copies[at + i].to;
+            args.tiles[i] = static_cast<uint16_t>(copies[at + i].tiles);
+        }
         const long long groups = static_cast<long long>(now) * n_layers * kv.n_kv;
         kv_copy_kernel<<<static_cast<unsigned>(std::min<long long>(groups, 1 << 20)), kThreads, 0, s>>>(kv, n_layers, layer_bytes,
                                                                                                       tile_bytes, args, now);

@@ -235,6 +235,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
                 if (!wrong.empty()) return wrong;
             }
             b.seqs.push_back(KvTreeSeq{token0, n});
+            b.seq_of.insert(b.seq_of.end(), n, i);
             b.starts.push_back(start);
             b.first_page.push_back(page0);
         } else if (n > 0) {

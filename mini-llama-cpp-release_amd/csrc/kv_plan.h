@@ -97,7 +97,7 @@ struct KvBatch {
     std::vector<KvTreeItem> trees[2];
     std::vector<KvTreeSeq> seqs;
     std::vector<int> starts, first_page;  // of each sequence: positions before its tree, first entry in `pages`
-    std::vector<int> pos, parents;  // of each token: its position, the parent among its sequence's nodes
+    std::vector<int> pos, parents, seq_of;  // of each token: its position, the parent among its sequence's nodes, the sequence
     std::vector<uint32_t> masks;
 };
 

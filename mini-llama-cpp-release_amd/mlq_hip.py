@@ -11,6 +11,7 @@ memory, streams and events, so a process never carries two HIP runtimes.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 
@@ -642,6 +643,16 @@ def _ints(x, what: str) -> np.ndarray:
     return np.ascontiguousarray(a, np.int32)
 
 
+def _int_list(x, what: str) -> array.array:
+    """The same as an array, in a few hundred ns where x is a list of Python's integers."""
+    if type(x) is list and set(map(type, x)) <= {int}:
+        try:
+            return array.array("i", x)
+        except OverflowError:
+            raise ValueError(f"{what}: not a list of 32-bit integers") from None
+    return array.array("i", _ints(x, what).tobytes())
+
+
 class KvCache:
     """Pages of keys and values that several sequences share (mlq_hip_kv_cache_*)."""
 
@@ -660,12 +671,12 @@ class KvCache:
 
     def copy_pages(self, src, dst, positions=None, stream=None) -> None:
         """The first positions of each page (all by default) into another page, in every layer."""
-        a, b = _ints(src, "src"), _ints(dst, "dst")
-        n = _ints(positions, "positions") if positions is not None else None
-        if a.size != b.size or (n is not None and n.size != a.size):
+        a, b = _int_list(src, "src"), _int_list(dst, "dst")
+        n = None if positions is None else _int_list(positions, "positions")
+        if len(a) != len(b) or (n is not None and len(n) != len(a)):
             raise ValueError("one destination, and one count of positions, per page")
-        _check(_LIB.mlq_hip_kv_copy_pages(self.h, a.size, a.ctypes.data, b.ctypes.data,
-                                          n.ctypes.data if n is not None else None, stream))
+        _check(_LIB.mlq_hip_kv_copy_pages(self.h, len(a), a.buffer_info()[0], b.buffer_info()[0],
+                                          None if n is None else n.buffer_info()[0], stream))
 
     def destroy(self) -> None:
         if getattr(self, "h", None):
@@ -736,12 +747,13 @@ class KvPlan:
     def keep(self, n_kept, kept, stream=None) -> None:
         """Moves the kept nodes of each sequence's tree (host lists, one sequence's after the other's) to its first
         slots, in every layer."""
-        n, k = _ints(n_kept, "n_kept"), _ints(kept, "kept")
-        if n.size != self._n_seqs:
+        n, k = _int_list(n_kept, "n_kept"), _int_list(kept, "kept")
+        if len(n) != self._n_seqs:
             raise ValueError("one count per sequence of the batch")
-        if k.size != sum(int(x) for x in n if x > 0):
-            raise ValueError(f"{k.size} kept nodes, the counts need {sum(int(x) for x in n if x > 0)}")
-        _check(_LIB.mlq_hip_kv_keep(self.h, n.ctypes.data, k.ctypes.data, stream))
+        need = sum(x for x in n if x > 0)
+        if len(k) != need:
+            raise ValueError(f"{len(k)} kept nodes, the counts need {need}")
+        _check(_LIB.mlq_hip_kv_keep(self.h, n.buffer_info()[0], k.buffer_info()[0], stream))
 
     def destroy(self) -> None:
         if getattr(self, "h", None):
