@@ -38,7 +38,7 @@ struct BeamCall {
     int end_token, groups, beams, vocab, keep;
     int *parents, *tokens;  // [groups][keep]
     float* out_scores;      // [groups][keep]
-    // Workspace: of every part its BeamPart and the keys of its best `keep` logits, best first.
+    // Workspace: of every part its BeamPart and the keys of its best `keep` logits, [groups][keep][parts of the group].
     BeamPart* parts;
     unsigned long long* best;
 };

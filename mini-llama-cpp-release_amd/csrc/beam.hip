@@ -40,11 +40,10 @@ __device__ __forceinline__ uint32_t index_of(unsigned long long key) { return ~s
 constexpr unsigned long long kNoKey = 0;  // below every logit's key, -Inf's too
 
 // exp(d) for d <= 0 in 64 bits, 2^-39 of it off at the most: 2^n times a polynomial of the rest, at most 0.3466 (of
-// degree 8, through exp at the Chebyshev points; 1.1e-12 off, the series to degree 9 6.9e-12).  0 below -800.  n is
-// rounded by a sum whose last places are whole numbers: its low word is n.
+// degree 8, through exp at the Chebyshev points; 1.1e-12 off, the series to degree 9 6.9e-12).  n is rounded by a sum
+// whose last places are whole numbers: its low word is n.  d is far above -2^31.
 __device__ __forceinline__ double exp64(double d) {
     constexpr double kWhole = 6755399441055744.0;  // 1.5 x 2^52
-    d = fmax(d, -800.0);
     const double t = fma(d, 1.4426950408889634, kWhole);
     const double r = fma(t - kWhole, -0.6931471805599453, d);
     double y = 2.4876178959085513e-05;
@@ -59,6 +58,34 @@ __device__ __forceinline__ double exp64(double d) {
     return ldexp(y, static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, t))));
 }
 
+// Over a wave, by lane permutations of the vector unit: rows of sixteen turned by 8, 4, 2 and 1, then the rows.
+template <int ROR>
+__device__ __forceinline__ float turned(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x120 + ROR, 0xf, 0xf, true));
+}
+template <int ROR>
+__device__ __forceinline__ double turned(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2(__builtin_amdgcn_mov_dpp(static_cast<int>(w.x), 0x120 + ROR, 0xf, 0xf, true),
+                                                 __builtin_amdgcn_mov_dpp(static_cast<int>(w.y), 0x120 + ROR, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, turned<8>(v));
+    v = fmaxf(v, turned<4>(v));
+    v = fmaxf(v, turned<2>(v));
+    v = fmaxf(v, turned<1>(v));
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v += turned<8>(v);
+    v += turned<4>(v);
+    v += turned<2>(v);
+    v += turned<1>(v);
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
 // The r-th largest of the wave's values, r from 1 to 64 (the order of their bits, bit by bit).
 __device__ __forceinline__ uint32_t wave_rth_largest(uint32_t v, int r) {
     uint32_t t = 0;
@@ -71,12 +98,11 @@ __device__ __forceinline__ uint32_t wave_rth_largest(uint32_t v, int r) {
 }
 
 template <int E>
-__global__ __launch_bounds__(kThreads, 4) void beam_part_kernel(BeamCall c, int parts) {
+__global__ __launch_bounds__(kThreads, 5) void beam_part_kernel(BeamCall c, int parts) {
     constexpr int kMost = kBeamMostKeep * E;
     __shared__ unsigned long long list[kMost];
     __shared__ float top_of[kWaves];
     __shared__ uint32_t bar_of[kWaves];
-    __shared__ int bad_of[kWaves];
     __shared__ double sum_of[kWaves];
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
@@ -93,54 +119,58 @@ __global__ __launch_bounds__(kThreads, 4) void beam_part_kernel(BeamCall c, int 
             for (int e = 0; e < E; ++e) x[e] = e * kThreads + tid < n ? from[e * kThreads + tid] : -__builtin_inff();
         }
         float mine = -__builtin_inff();
-        bool bad = false;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            bad = bad || !(x[e] < __builtin_inff());
-            mine = fmaxf(mine, x[e]);
-        }
+        for (int e = 0; e < E; ++e) mine = fmaxf(mine, x[e]);
         // Enough of the wave's threads have a logit from here on.
         const uint32_t wave_bar = wave_rth_largest(order_of(mine), (c.keep + kWaves - 1) / kWaves);
-        float top = mine;
-#pragma unroll
-        for (int s = 32; s > 0; s /= 2) top = fmaxf(top, __shfl_xor(top, s));
-        const bool wave_bad = __any(bad);
+        float top = wave_max(mine);
         __syncthreads();  // the last part's readers are done
-        if (lane == 0) top_of[wave] = top, bad_of[wave] = wave_bad, bar_of[wave] = wave_bar;
+        if (lane == 0) top_of[wave] = top, bar_of[wave] = wave_bar;
         if (tid == 0) found = 0;
         __syncthreads();
         uint32_t lowest = bar_of[0];
-        bad = false;
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
             top = fmaxf(top, top_of[k]);
-            bad = bad || bad_of[k] != 0;
             lowest = min(lowest, bar_of[k]);
         }
         // The keys of what passes the bar.
         const float bar = fmaxf(value_of(lowest), -3.402823466e38f);  // (-Inf is no continuation)
+        int index = lo + tid;
+        asm("" : "+v"(index));  // (or all of them would be computed ahead)
+        unsigned long long who[E];
+        int passing = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const unsigned long long who = __ballot(x[e] >= bar);
-            if (who == 0) continue;
-            int base = 0;
-            if (lane == 0) base = atomicAdd(&found, __builtin_popcountll(who));
-            base = __builtin_amdgcn_readfirstlane(base);
-            const int at = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32),
-                                                            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
-            if (x[e] >= bar && at < kMost) list[at] = key_of(x[e], static_cast<uint32_t>(lo + e * kThreads + tid));
+            who[e] = __ballot(x[e] >= bar);
+            passing += __builtin_popcountll(who[e]);
         }
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&found, passing);
+        base = __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (who[e] == 0) continue;
+            const int at = base + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who[e] >> 32),
+                                                            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who[e]), 0));
+            if (x[e] >= bar && at < kMost) list[at] = key_of(x[e], static_cast<uint32_t>(index + e * kThreads));
+            base += __builtin_popcountll(who[e]);
+        }
+        // (a logit that is NaN, or +Inf and so minus itself, makes the sum NaN)
         double sum = 0.0;
         if (top > -__builtin_inff()) {
             const double top64 = top;
+            const float least = top - 800.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                sum += exp64(static_cast<double>(x[e]) - top64);
+                sum += exp64(static_cast<double>(__builtin_elementwise_maximum(x[e], least)) - top64);
                 if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few of them at a time: registers)
             }
-        }
+        } else {
 #pragma unroll
-        for (int s = 32; s > 0; s /= 2) sum += __shfl_xor(sum, s);
+            for (int e = 0; e < E; ++e) sum += x[e] != x[e] ? static_cast<double>(x[e]) : 0.0;
+        }
+        sum = wave_sum(sum);
         if (lane == 0) sum_of[wave] = sum;
         __syncthreads();
         int m = found;
@@ -171,20 +201,22 @@ __global__ __launch_bounds__(kThreads, 4) void beam_part_kernel(BeamCall c, int 
             __syncthreads();
             m = found;
         }
-        unsigned long long* const best = c.best + static_cast<size_t>(w) * c.keep;
+        // (a group's lists lie side by side, best ones first)
+        const int lists = c.beams * parts;
+        unsigned long long* const best = c.best + static_cast<size_t>(w / lists) * lists * c.keep + w % lists;
         for (int i = tid; i < m; i += kThreads) {
             const unsigned long long k = list[i];
             int at = 0;
 #pragma unroll 8
             for (int j = 0; j < m; ++j) at += list[j] > k ? 1 : 0;
-            if (at < c.keep) best[at] = k;
+            if (at < c.keep) best[static_cast<size_t>(at) * lists] = k;
         }
-        for (int i = m + tid; i < c.keep; i += kThreads) best[i] = kNoKey;
+        for (int i = m + tid; i < c.keep; i += kThreads) best[static_cast<size_t>(i) * lists] = kNoKey;
         if (tid == 0) {
             double all = sum_of[0];
 #pragma unroll
             for (int k = 1; k < kWaves; ++k) all += sum_of[k];
-            c.parts[w] = BeamPart{all, bad ? __builtin_nanf("") : top, 0};
+            c.parts[w] = BeamPart{all, all != all ? __builtin_nanf("") : top, 0};
         }
     }
 }
@@ -213,15 +245,21 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
     const int tid = threadIdx.x, wave = tid / 64, keep = c.keep;
     const double none = -__builtin_inf();
     for (int group = blockIdx.x; group < c.groups; group += gridDim.x) {
-        const int per = parts * keep, n = c.beams * per;
+        // Candidates as they lie: the best of every part, the second best of every part ...
+        const int lists = c.beams * parts, n = lists * keep;
         const unsigned long long* const keys = c.best + static_cast<size_t>(group) * n;
-        // (neighbours go to the waves in turn, so that each has its part of few candidates)
-        const int turn = tid % 64 * kWaves + wave;
+        // Four neighbours go to the four waves, from place to place in another order, so that each has its part of few
+        // candidates and of every list: the waves' bars are then alike, whatever the beams' scores.
+        const int shift = 31 - __builtin_clz(lists);  // (a place is about as many candidates)
+        auto candidate = [&](int first, int e) {
+            const int four = first + e * kThreads + tid % 64 * kWaves;
+            return four + (wave + (four >> shift)) % kWaves;
+        };
         unsigned long long key[E];
         auto load = [&](int first) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int i = first + e * kThreads + turn;
+                const int i = candidate(first, e);
                 key[e] = i < n ? keys[i] : kNoKey;
             }
         };
@@ -251,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
             double sum = 0.0;
             for (int k = tid % kLanes; k < parts; k += kLanes) {
                 const BeamPart x = p[k];
-                if (x.largest > -__builtin_inff()) sum += x.sum * exp64(static_cast<double>(x.largest) - static_cast<double>(top));
+                if (x.largest > -__builtin_inff()) sum += x.sum * exp64(static_cast<double>(fmaxf(x.largest, top - 800.0f)) - static_cast<double>(top));
             }
 #pragma unroll
             for (int k = kLanes / 2; k > 0; k /= 2) sum += __shfl_xor(sum, k);
@@ -272,20 +310,20 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
             }
             continue;
         }
-        // Rounds: what is best so far, and the next candidates.
-        int have = 0;
-        for (int first = 0; first < n; first += E * kThreads) {
+        // Rounds: what is best so far, and the next candidates, until a candidate of every list has been too small.
+        int have = 0, small = 0;
+        for (int first = 0; first < n && small < lists; first += E * kThreads) {
             Candidate x[E];
             float mine = -__builtin_inff();  // of the thread's, rounded down
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int i = first + e * kThreads + turn, b = min(i / per, c.beams - 1);
+                const int i = candidate(first, e), list_of = i % lists, b = list_of / parts;
                 x[e] = Candidate{none, key[e], b};
                 if (i < n) {
                     const float logit = logit_of(key[e]);
                     if (state[b] == 1 && key[e] != kNoKey) {
                         x[e].value = score[b] + (static_cast<double>(logit) - sums[b]);
-                    } else if (state[b] == 2 && i % per == 0) {
+                    } else if (state[b] == 2 && i < lists && list_of % parts == 0) {
                         x[e].value = score[b];
                         x[e].key = key_of(0.0f, static_cast<uint32_t>(c.end_token));
                     }
@@ -293,24 +331,44 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
                 mine = fmaxf(mine, __double2float_rd(x[e].value));
             }
             if (first + E * kThreads < n) load(first + E * kThreads);
-            const uint32_t wave_bar = wave_rth_largest(order_of(mine), (keep + kWaves - 1) / kWaves);
-            if (tid % 64 == 0) bar_of[wave] = wave_bar;
-            if (tid == 0) found = 0;
-            __syncthreads();
-            uint32_t lowest = bar_of[0];
+            const int each = (keep + kWaves - 1) / kWaves;
+            // To the list goes what passes the waves' bars, as many as have to and more.
+            auto gather = [&](uint32_t wave_bar) {
+                if (tid % 64 == 0) bar_of[wave] = wave_bar;
+                if (tid == 0) found = 0;
+                __syncthreads();
+                uint32_t lowest = bar_of[0];
 #pragma unroll
-            for (int k = 1; k < kWaves; ++k) lowest = min(lowest, bar_of[k]);
-            double bar = static_cast<double>(value_of(lowest));
-            if (have == keep) bar = fmax(bar, best[keep - 1].value);
+                for (int k = 1; k < kWaves; ++k) lowest = min(lowest, bar_of[k]);
+                double bar = static_cast<double>(value_of(lowest));
+                if (have == keep) bar = fmax(bar, best[keep - 1].value);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (x[e].value >= bar && x[e].value > none) {
-                    const int at = atomicAdd(&found, 1);
-                    if (at < kMost) list[at] = x[e];
+                for (int e = 0; e < E; ++e) {
+                    if (x[e].value >= bar && x[e].value > none) {
+                        const int at = atomicAdd(&found, 1);
+                        if (at < kMost) list[at] = x[e];
+                    }
                 }
+                __syncthreads();
+                return found;
+            };
+            int m = gather(wave_rth_largest(order_of(mine), each));
+            if (m > kThreads) {
+                // (many of a thread's: the bar is that of all the wave's)
+                uint32_t order[E], t = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) order[e] = order_of(__double2float_rd(x[e].value));
+#pragma unroll 1
+                for (int bit = 31; bit >= 0; --bit) {
+                    const uint32_t c = t | 1u << bit;
+                    int above = 0;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) above += __builtin_popcountll(__ballot(order[e] >= c));
+                    t = above >= each ? c : t;
+                }
+                __syncthreads();  // (all have read what was found)
+                m = gather(t);
             }
-            __syncthreads();
-            int m = found;
             if (__builtin_expect(m > kMost, 0)) {
                 // As many values that f32 does not tell apart: the bar is that of the threads' best, which differ.
                 __shared__ Candidate of_thread[kThreads], exact_bar;
@@ -337,6 +395,7 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
                 __syncthreads();
                 m = found;
             }
+            small = m > 0 ? 0 : small + E * kThreads;
             if (m > 0) {
                 for (int i = tid; i < have; i += kThreads) list[m + i] = best[i];
                 m += have;
