@@ -175,10 +175,10 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 // max_nodes 0: a plan of plain sequences.
 int create_plan(const char* caller, mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
                 int max_tokens, int max_pages, int max_nodes, mlq_kv_plan_t* out) {
-    if (out == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null output handle");
-    *out = nullptr;
     return entry(caller, [&]() -> int {
         const std::string who(caller);
+        if (out == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null output handle");
+        *out = nullptr;
         if (cache == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null cache");
         const KvMemory& kv = *cache->kv;
         if (n_heads <= 0 || n_heads % kv.n_kv != 0) {
@@ -392,12 +392,14 @@ int mlq_hip_kv_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int si
 int mlq_hip_kv_tree_plan_create(mlq_kv_cache_t cache, int n_heads, int window, int sinks, float scale, int max_seqs,
                                 int max_tokens, int max_pages, int max_nodes, mlq_kv_plan_t* out) {
     const char* caller = "hip_kv_tree_plan_create";
-    if (max_nodes < 1 || max_nodes > mlq::kKvMostNodes) {
-        if (out != nullptr) *out = nullptr;
-        return abi_fail(MLQ_ERR_LIMIT, std::string(caller) + ": trees of " + std::to_string(max_nodes) + " nodes, not 1 to " +
-                                           std::to_string(mlq::kKvMostNodes));
-    }
-    return create_plan(caller, cache, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages, max_nodes, out);
+    return entry(caller, [&]() -> int {
+        if (max_nodes < 1 || max_nodes > mlq::kKvMostNodes) {
+            if (out != nullptr) *out = nullptr;
+            return abi_fail(MLQ_ERR_LIMIT, std::string(caller) + ": trees of " + std::to_string(max_nodes) + " nodes, not 1 to " +
+                                               std::to_string(mlq::kKvMostNodes));
+        }
+        return create_plan(caller, cache, n_heads, window, sinks, scale, max_seqs, max_tokens, max_pages, max_nodes, out);
+    });
 }
 
 int mlq_hip_kv_plan_set(mlq_kv_plan_t p, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
@@ -408,9 +410,11 @@ int mlq_hip_kv_plan_set(mlq_kv_plan_t p, int n_seqs, const int* new_tokens, cons
 int mlq_hip_kv_plan_set_tree(mlq_kv_plan_t p, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
                              const int* parents, void* stream) {
     const char* caller = "hip_kv_plan_set_tree";
-    if (p == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null plan");
-    if (!p->trees()) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": the plan holds no trees");
-    return set_plan(caller, p, n_seqs, new_tokens, kv_len, pages, parents, stream);
+    return entry(caller, [&]() -> int {
+        if (p == nullptr) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": null plan");
+        if (!p->trees()) return abi_fail(MLQ_ERR_INVALID, std::string(caller) + ": the plan holds no trees");
+        return set_plan(caller, p, n_seqs, new_tokens, kv_len, pages, parents, stream);
+    });
 }
 
 int mlq_hip_kv_plan_destroy(mlq_kv_plan_t p) {

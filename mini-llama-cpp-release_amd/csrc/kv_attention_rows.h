@@ -466,6 +466,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_rows_kernel(Attention<T
         };
         auto seen_by_some = [&](int i, int key) {
             const int at = tile_of(i) * kKvTile + key;
+            // (a node may be seen as one of the first positions wherever it lies)
+            if (TREE && at >= start) return at <= item_range[1];
             return at <= item_range[1] && (a.window == 0 || at > item_range[0] - a.window || at < a.sinks);
         };
         // Scales to LDS.  Operands lie there times 2^8 and over a power of two per position, so that what they lose,

@@ -75,6 +75,17 @@ def test_counts(hip, beams, keep):
     Beams(hip, *random(rng, 3, beams, 9001 if beams < 20 else 1500), keep).check()
 
 
+def test_wide_searches(hip):
+    """Many beams whose scores lie far apart, so that a few of them hold all continuations, and many kept."""
+    rng = np.random.default_rng(11)
+    for groups, beams, vocab in ((5, 64, 8000), (1, 64, 33000), (3, 61, 700)):
+        x, s = random(rng, groups, beams, vocab)
+        Beams(hip, x, s, 64).check()
+        Beams(hip, x, (s * 20).astype(np.float32), 64).check()
+        s[:] = np.where(np.arange(beams) % 4 == 1, s, s - 50)
+        Beams(hip, x, s, 64).check()
+
+
 def test_many_groups(hip):
     Beams(hip, *random(np.random.default_rng(1), 300, 3, 777), 6).check()
 
