@@ -11,6 +11,9 @@
 // largest of the threads' own largest, so few pass that bar, and those few are ranked by counting.  Then a
 // workgroup a group: the rows' sums, and the best of the parts' best by the same bar.  Sums are taken in a fixed
 // order: equal rows have equal sums, and the same call gives the same bits.
+//
+// Measured: 32 groups of 8 beams over 128011 tokens, 16 kept, 47 us (40 + 9 of kernels, 3.3 TB/s of logits in the first);
+// 4 beams over 32000 tokens 11 us.  In one launch, the last part of a group to arrive selecting, 55 and 11.
 
 #include "beam.h"
 
@@ -97,6 +100,8 @@ __device__ __forceinline__ uint32_t wave_rth_largest(uint32_t v, int r) {
     return t;
 }
 
+// Bound: issue, half of it the exponentials (16 instructions in 64 bits a logit, which run at about the rate of 32; a logit
+// takes 29 in all), then memory.  Five waves a SIMD (four: 42 us for the 256 rows above); parts of 4096 logits 47 us.
 template <int E>
 __global__ __launch_bounds__(kThreads, 5) void beam_part_kernel(BeamCall c, int parts) {
     constexpr int kMost = kBeamMostKeep * E;

@@ -65,6 +65,7 @@ int mlq_hip_beam_create(int device, int max_groups, int max_beams, int max_vocab
         if (max_beams > mlq::kBeamMostBeams || max_keep > mlq::kBeamMostKeep) {
             return abi_fail(MLQ_ERR_LIMIT, who + ": more than 64 beams of a group, or 64 continuations");
         }
+        if (max_vocab > mlq::kBeamMostVocab) return abi_fail(MLQ_ERR_LIMIT, who + ": more than 2^30 tokens");
         auto h = std::make_unique<mlq_beam_s>();
         h->device = device, h->max_groups = max_groups, h->max_beams = max_beams, h->max_vocab = max_vocab, h->max_keep = max_keep;
         if (static_cast<double>(max_groups) * max_beams * (max_vocab / mlq::kBeamPart + 1) > 0x1p28) {

@@ -528,7 +528,9 @@ int mlq_hip_kv_tree_pick(mlq_kv_plan_t p, const float* logits, int vocab, const 
     return entry(caller, [&]() -> int {
         int rc = check_trees(p, caller);
         if (rc != MLQ_OK) return rc;
-        if (vocab <= 0) return abi_fail(MLQ_ERR_SHAPE, std::string(caller) + ": vocabulary of " + std::to_string(vocab));
+        if (vocab <= 0 || vocab > kMost) {
+            return abi_fail(MLQ_ERR_SHAPE, std::string(caller) + ": vocabulary of " + std::to_string(vocab) + ", not 1 to 2^30");
+        }
         const hipStream_t s = mlq::abi_stream(p->kv->device, stream);
         const bool recorded = mlq::abi_capturing(s);
         const size_t rows = recorded ? p->shape.max_tokens : p->n_tokens;

@@ -12,6 +12,17 @@
 // power of two of every row and block that keeps its largest at 2^9 .. 2^15.  There eight rows stand beside their own
 // low parts in an operand's sixteen columns; a tree has more rows than that, so here the sixteen columns are sixteen
 // rows and a block takes two products (f32: three, as low parts times low parts, 2^-22 of an element, are left out).
+// Batches with rows enough to fill its workgroups many times over run the kernel of kv_attention_rows.h instead, in
+// its form for trees (kv_tree_cost says which; a batch runs one of them, as two launches would follow each other).
+//
+// Bound: issue.  A tile takes a wave 470 vector instructions and 32 products, some 2800 cycles at two waves a SIMD
+// (64 nodes after 4000 positions, Q8_0, 32 heads over 8 KV heads of 128: 32 us, 20 of them tiles; the cache is read
+// 16 times, from L2); small batches by the launch, four dependent trips to memory and the merge (8 nodes after 700
+// positions, 14 heads over 2 of 64: 8.9 us).  24 nodes of 16 sequences, Q4_1, 80 elements, a window of 1024: 40 us.
+// Measured and no faster: 32 rows a wave (one wave a SIMD: 46 us for the 64 nodes, 57 for the 16 sequences), weights
+// times scales as one mixed-precision instruction each (33 us), with one look at a tile's frames as well (33),
+// s_setprio around the products, 256 and 1024 workgroups (34 and 36); one power of two for a row's queries in place of one
+// a block saves 2 % but needs a second form for queries whose blocks lie far apart.
 #pragma once
 
 #include "kv_attention_rows.h"

@@ -22,7 +22,9 @@ struct MoveArgs {
     uint16_t end[kMoves];  // of each path, in moves
 };
 
-// Bound: memory.  A workgroup copies the tiles of one page, head and layer, which lie together.
+// Bound: memory.  A workgroup copies the tiles of one page, head and layer, which lie together (256 pages of 64 positions,
+// 8 KV heads of 128 in Q8_0, 4 layers: 75 us, 3.8 TB/s read and written; three pages of a small model 5 us).  Eight
+// 16-byte loads in flight a thread are no faster than four.
 __global__ __launch_bounds__(kThreads) void kv_copy_kernel(KvView kv, int n_layers, size_t layer_bytes, int tile_bytes, CopyArgs args,
                                                            int n) {
     const long long total = static_cast<long long>(n) * n_layers * kv.n_kv;
@@ -95,7 +97,9 @@ __device__ __forceinline__ void move_piece(uint8_t* to, const uint8_t* from, int
     }
 }
 
-// Bound: latency.  A workgroup takes one path in one head and layer: reads up to kTogether slots into LDS, then
+// Bound: the lines of memory that a slot's pieces lie in, some ten of 128 bytes for the 150 bytes of a Q4_0 head of 128,
+// read and written back (paths of four nodes of 64 sequences, 16 layers, 8 heads: 19 us); few paths by latency (4 us).
+// A path a wave, without barriers, takes 17 and 6.  A workgroup takes one path in one head and layer: reads up to kTogether slots into LDS, then
 // writes them where they go, piece by piece, so that what else lies in their tiles is never rewritten.  A path's
 // sources ascend and lie at or behind their destinations: none is one of an earlier move, so it is read before
 // anything has been written there.

@@ -77,7 +77,7 @@ __device__ __forceinline__ void walk(const KvPick& p, int seq, const KvTreeSeq& 
     }
 }
 
-// Bound: memory (the logits once); of few rows, launch, a trip for the logits, one for the arrival, one for the keys and
+// Bound: memory (the logits once: 315 rows of 152000, 32 us, 6 TB/s, part of it from the last-level cache); of few rows, launch, a trip for the logits, one for the arrival, one for the keys and
 // the walk.
 __global__ __launch_bounds__(kThreads) void kv_pick_kernel(KvPick p, int tokens, int seqs) {
     __shared__ unsigned long long of_wave[kThreads / 64];

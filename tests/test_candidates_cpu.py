@@ -52,7 +52,8 @@ def test_beam_create_refusals():
         assert h.value is None
     for a in ((1, 65, 1, 1), (1, 1, 1, 65)):
         refused(lib.mlq_hip_beam_create(0, *a, ctypes.byref(h)), 6, "more than 64")
-    refused(lib.mlq_hip_beam_create(0, 2 ** 31 - 1, 64, 2 ** 31 - 1, 64, ctypes.byref(h)), 6, "2^28")
+    refused(lib.mlq_hip_beam_create(0, 2 ** 31 - 1, 64, 2 ** 30, 64, ctypes.byref(h)), 6, "2^28")
+    refused(lib.mlq_hip_beam_create(0, 1, 1, 2 ** 30 + 1, 1, ctypes.byref(h)), 6, "2^30")
     refused(lib.mlq_hip_beam_create(0, 1, 1, 1, 1, None), 1, "null output handle")
 
 

@@ -727,7 +727,7 @@ def test_refusals(hip):
             bad()
     for call, what in ((lambda: p.keep([2, 0], [0, 3]), "kept node 3"), (lambda: p.keep([3, 0], [0, 1, 2]), "not a child of node 1"),
                        (lambda: p.keep([4, 0], [0, 1, 2, 2]), "4 of 3"), (lambda: p.keep([0, 1], [1]), "not a child of what came before"),
-                       (lambda: p.pick(logits, 0, *ints), "vocabulary"), (lambda: p.pick(logits, 100, *ints), "too small"),
+                       (lambda: p.pick(logits, 0, *ints), "vocabulary"), (lambda: p.pick(logits, 2 ** 30 + 1, *ints), "vocabulary"), (lambda: p.pick(logits, 100, *ints), "too small"),
                        (lambda: p.pick(None, 10, *ints), "null"), (lambda: p.pick(logits, 10, None, *ints[1:]), "null"),
                        (lambda: p.pick(logits, 10, *ints[:4], None), "null"),
                        (lambda: p.pick(logits.ptr + 2, 10, *ints), "aligned"),
