@@ -495,7 +495,9 @@ int mlq_hip_kv_tree_plan_create(mlq_kv_cache_t cache, int n_heads, int window, i
  * sequence and has position kv_len - new_tokens + its depth: mlq_hip_kv_write
  * rotates by that, and in mlq_hip_kv_attention it sees what came before the tree,
  * its ancestors and itself, as far as the window (of positions) and the first
- * tokens go. */
+ * tokens go.  (All sequences of a batch take the attention's form for many rows a
+ * KV head, with its slow cases, or none: trees of more than 32 rows may over long
+ * contexts, over short ones only batches of hundreds.) */
 int mlq_hip_kv_plan_set_tree(mlq_kv_plan_t plan, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
                              const int* parents, void* stream);
 /* Checks drafted trees greedily.  logits [tokens][vocab]: what the model says
@@ -516,8 +518,9 @@ int mlq_hip_kv_tree_pick(mlq_kv_plan_t plan, const float* logits, int vocab, con
  * indexes, one sequence's after the other's (host arrays).  Their keys and values
  * move, in every layer, to the first slots of the tree, so that the sequence goes
  * on with kv_len - new_tokens + n_kept[s] positions; what the tree's other slots
- * hold is then undefined.  The batch stays set.  Asynchronous on `stream`; not
- * under graph capture. */
+ * hold is then undefined.  The batch stays set, but a node that another one has
+ * been moved over is not kept any more until the next set (a refusal).
+ * Asynchronous on `stream`; not under graph capture. */
 int mlq_hip_kv_keep(mlq_kv_plan_t plan, const int* n_kept, const int* kept, void* stream);
 /* Copies the first positions[i] positions (NULL: all) of page from[i] to page
  * to[i], in every layer: a sequence that forks keeps its full pages in common and

@@ -580,7 +580,9 @@ int mlq_hip_kv_keep(mlq_kv_plan_t p, const int* n_kept, const int* kept, void* s
         if (moves.empty()) return MLQ_OK;
         const hipError_t e = mlq::launch_kv_moves(p->view(0), p->kv->n_layers, p->kv->layer_bytes, moves.data(), ends.data(),
                                                   static_cast<int>(ends.size()), s);
-        return e == hipSuccess ? MLQ_OK : abi_hip_fail(e, caller);
+        if (e != hipSuccess) return abi_hip_fail(e, caller);
+        mlq::kv_keep_done(n_kept, kept, &p->batch);
+        return MLQ_OK;
     });
 }
 

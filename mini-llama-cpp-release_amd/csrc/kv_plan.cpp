@@ -89,6 +89,7 @@ std::string add_tree(const KvPlanShape& s, const std::string& who, int n, int st
             return who + ": node " + std::to_string(i) + " has parent " + std::to_string(parent) + ", not -1 or an earlier node";
         }
         b.parents.push_back(parent);
+        b.holds.push_back(i);
         const int pos = parent < 0 ? start : b.pos[pos0 + parent] + 1;
         b.pos.push_back(pos);
         uint32_t* const mask = &b.masks[first + static_cast<size_t>(i) * words];
@@ -300,6 +301,10 @@ std::string kv_keep_build(const KvPlanShape& s, const KvBatch& b, const int* n_k
                 return "sequence " + std::to_string(i) + ": kept node " + std::to_string(node) + " is not a child of " +
                        (j > 0 ? "node " + std::to_string(before) : "what came before the tree");
             }
+            if (b.holds[q.token0 + node] != node) {
+                return "sequence " + std::to_string(i) + ": kept node " + std::to_string(node) + " has been moved over by node " +
+                       std::to_string(b.holds[q.token0 + node]);
+            }
             // A path's nodes ascend, so node j lies at slot j or later.
             if (node != j) {
                 const int from = b.starts[i] + node, to = b.starts[i] + j;
@@ -313,6 +318,13 @@ std::string kv_keep_build(const KvPlanShape& s, const KvBatch& b, const int* n_k
         }
     }
     return "";
+}
+
+void kv_keep_done(const int* n_kept, const int* kept, KvBatch* b) {
+    for (size_t i = 0; i < b->seqs.size(); ++i) {
+        std::copy(kept, kept + n_kept[i], b->holds.begin() + b->seqs[i].token0);
+        kept += n_kept[i];
+    }
 }
 
 }  // namespace mlq

@@ -99,6 +99,7 @@ struct KvBatch {
     std::vector<int> starts, first_page;  // of each sequence: positions before its tree, first entry in `pages`
     std::vector<int> pos, parents, seq_of;  // of each token: its position, the parent among its sequence's nodes, the sequence
     std::vector<uint32_t> masks;
+    std::vector<int> holds;  // which of its tree's nodes lies in each token's slot (moves change it)
 };
 
 // Checks a batch and builds its lists.  Returns "" or what is wrong with it;
@@ -120,5 +121,7 @@ struct KvMove {
 // and lists the moves, one sequence's after the other's, `ends` the list's length after each sequence that has some.
 std::string kv_keep_build(const KvPlanShape& s, const KvBatch& b, const int* n_kept, const int* kept, std::vector<KvMove>* moves,
                           std::vector<int>* ends);
+// Notes what its moves have left in the slots.
+void kv_keep_done(const int* n_kept, const int* kept, KvBatch* b);
 
 }  // namespace mlq

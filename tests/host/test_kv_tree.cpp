@@ -230,6 +230,17 @@ int main() {
     const int some[2] = {0, 1}, none[2] = {0, 0};
     CHECK(mlq::kv_keep_build(s, batch, some, nullptr, &moves, &ends) == "null list", "null list");
     CHECK(mlq::kv_keep_build(s, batch, none, nullptr, &moves, &ends) == "" && moves.empty() && ends.empty(), "nothing kept");
+    // What has been moved over is not kept any more; what lies in place, or has not been moved over, is.
+    const int path_n[2] = {3, 2}, path[5] = {0, 2, 3, 0, 2};
+    CHECK(mlq::kv_plan_build(s, 2, n2, l2, p2, up, &batch) == "", "two trees");
+    CHECK(mlq::kv_keep_build(s, batch, path_n, path, &moves, &ends) == "" && moves.size() == 3, "a path");
+    mlq::kv_keep_done(path_n, path, &batch);
+    CHECK(batch.holds == std::vector<int>({0, 2, 3, 3, 0, 2, 2}), "what the slots hold");
+    not_kept(s, {3, 2}, {0, 2, 3, 0, 2}, "sequence 0: kept node 2 has been moved over by node 3");
+    not_kept(s, {1, 0}, {1}, "sequence 0: kept node 1 has been moved over by node 2");
+    not_kept(s, {0, 2}, {0, 1}, "sequence 1: kept node 1 has been moved over by node 2");
+    const int again_n[2] = {1, 2}, again[3] = {0, 0, 2};
+    CHECK(mlq::kv_keep_build(s, batch, again_n, again, &moves, &ends) == "" && moves.size() == 1, "a path that can be moved again");
     std::printf("PASS kv_tree\n");
     return 0;
 }

@@ -376,6 +376,31 @@ def test_keep(hip, kind, case):
     assert np.array_equal(got[:, :, ~free], want[:, :, ~free])
 
 
+def test_keep_twice(hip):
+    """A path that lies apart from where it moves may be moved again; a node that another one has been moved over is
+    refused until the next set."""
+    rng = np.random.default_rng(3)
+    parents = [-1, 0, 0, 2, 3, 4, 4]
+    b = Batch(rng, [(7, 40)], 32)
+    f = Filled(hip, "q8_0", b.n_pages, 32, 1, 64, 2)
+    plan = hip.KvPlan(f.cache, 1, max_seqs=1, max_tokens=7, max_pages=b.entries, max_nodes=7)
+    plan.set(b.new, b.kv_len, b.pages, parents=parents)
+    plan.keep([2], [0, 2])
+    once = f.read()
+    plan.keep([2], [0, 2])
+    assert np.array_equal(f.read(), once)
+    with pytest.raises(hip.MlqError, match="kept node 1 has been moved over by node 2"):
+        plan.keep([2], [0, 1])
+    plan.keep([4], [0, 2, 3, 4])
+    moved = f.read()
+    with pytest.raises(hip.MlqError, match="kept node 2 has been moved over by node 3"):
+        plan.keep([4], [0, 2, 3, 4])
+    assert np.array_equal(f.read(), moved)
+    plan.set(b.new, b.kv_len, b.pages, parents=parents)
+    plan.keep([2], [0, 1])
+    assert np.array_equal(f.read(), moved)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_keep_many_paths(hip, kind):
     """More moves than a launch's arguments hold, paths cut between launches."""
