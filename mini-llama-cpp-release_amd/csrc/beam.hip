@@ -41,6 +41,9 @@ __device__ __forceinline__ unsigned long long key_of(float v, uint32_t index) {
 __device__ __forceinline__ float logit_of(unsigned long long key) { return value_of(static_cast<uint32_t>(key >> 32)); }
 __device__ __forceinline__ uint32_t index_of(unsigned long long key) { return ~static_cast<uint32_t>(key); }
 constexpr unsigned long long kNoKey = 0;  // below every logit's key, -Inf's too
+// From this magnitude on the neighbours of a row's largest logit are 512 and more away, so that exp(logit - largest) is
+// nothing beside 1 for all but its equals; below, largest - 800 is at least 288 smaller in f32 too.
+constexpr float kFarTop = 0x1p33f;
 
 // exp(d) for d <= 0 in 64 bits, 2^-39 of it off at the most: 2^n times a polynomial of the rest, at most 0.3466 (of
 // degree 8, through exp at the Chebyshev points; 1.1e-12 off, the series to degree 9 6.9e-12).  n is rounded by a sum
@@ -175,6 +178,16 @@ __global__ __launch_bounds__(kThreads, 5) void beam_part_kernel(BeamCall c, int 
 #pragma unroll
             for (int e = 0; e < E; ++e) sum += x[e] != x[e] ? static_cast<double>(x[e]) : 0.0;
         }
+        if (__builtin_expect(fabsf(top) >= kFarTop && top > -__builtin_inff(), 0)) {
+            sum = 0.0;
+            int first = tid;
+            asm("" : "+v"(first));  // (as above: no addresses ahead)
+#pragma unroll 1
+            for (int i = first; i < n; i += kThreads) {  // (read again: rare, and the registers are the others')
+                const float v = from[i];
+                sum += v != v || v == __builtin_inff() ? __builtin_nan("") : v == top ? 1.0 : 0.0;
+            }
+        }
         sum = wave_sum(sum);
         if (lane == 0) sum_of[wave] = sum;
         __syncthreads();
@@ -241,7 +254,7 @@ constexpr int kLanes = 16;     // that take a beam's parts
 
 __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int parts) {
     constexpr int E = kGroupEach, kMost = kBeamMostKeep * E;
-    __shared__ double sums[kBeamMostBeams], score[kBeamMostBeams];
+    __shared__ double largest[kBeamMostBeams], sums[kBeamMostBeams], score[kBeamMostBeams];  // (the sums' logarithms)
     __shared__ int state[kBeamMostBeams];  // 0: no continuations, 1: of the logits, 2: ended
     __shared__ Candidate list[kMost + kBeamMostKeep], best[kBeamMostKeep];
     __shared__ double value[kMost + kBeamMostKeep];  // of the list
@@ -294,13 +307,18 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
             double sum = 0.0;
             for (int k = tid % kLanes; k < parts; k += kLanes) {
                 const BeamPart x = p[k];
-                if (x.largest > -__builtin_inff()) sum += x.sum * exp64(static_cast<double>(fmaxf(x.largest, top - 800.0f)) - static_cast<double>(top));
+                if (x.largest == top) {
+                    sum += x.sum;
+                } else if (x.largest > -__builtin_inff() && fabsf(top) < kFarTop) {
+                    sum += x.sum * exp64(static_cast<double>(fmaxf(x.largest, top - 800.0f)) - static_cast<double>(top));
+                }
             }
 #pragma unroll
             for (int k = kLanes / 2; k > 0; k /= 2) sum += __shfl_xor(sum, k);
             if (there && tid % kLanes == 0) {
                 if (what == 1) what = wrong != 0 ? -1 : top == -__builtin_inff() ? 0 : 1;
-                sums[b] = what == 1 ? static_cast<double>(top) + log(sum) : 0.0;
+                largest[b] = what == 1 ? static_cast<double>(top) : 0.0;
+                sums[b] = what == 1 ? log(sum) : 0.0;
                 score[b] = static_cast<double>(s);
                 state[b] = what;
                 if (what < 0) bad = 1;
@@ -327,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void beam_group_kernel(BeamCall c, int pa
                 if (i < n) {
                     const float logit = logit_of(key[e]);
                     if (state[b] == 1 && key[e] != kNoKey) {
-                        x[e].value = score[b] + (static_cast<double>(logit) - sums[b]);
+                        x[e].value = score[b] + (static_cast<double>(logit) - largest[b] - sums[b]);
                     } else if (state[b] == 2 && i < lists && list_of % parts == 0) {
                         x[e].value = score[b];
                         x[e].key = key_of(0.0f, static_cast<uint32_t>(c.end_token));

@@ -117,6 +117,32 @@ def test_values_far_apart(hip):
     Beams(hip, x, s, 64).check()
 
 
+@pytest.mark.parametrize("vocab", [40, 3000, 40000])
+@pytest.mark.parametrize("top", [2.0 ** 32, 2.0 ** 33, 1e10, -1e10, 1e12, -1e12, 3e38, -3e38])
+def test_large_logits(hip, vocab, top):
+    """Logits whose neighbours in f32 are hundreds apart and more: only the largest have a part in the sum, and a value
+    keeps the logarithm of their number."""
+    rng = np.random.default_rng(6)
+    top = np.float32(top)
+    x = np.full((1, 3, vocab), np.nextafter(top, np.float32(-np.inf)))
+    x[0, 0, vocab // 2:] = -3.4e38
+    x[0, 1, ::3] = -3.4e38
+    x[0, 2, rng.permutation(vocab)[:vocab // 4]] = top / 2 if top > 0 else top * 1.125
+    x[0, 0, [3, vocab - 1]] = top
+    x[0, 1, [vocab - 2, vocab - 3, 1]] = top
+    x[0, 2, vocab - 7] = top
+    s = np.array([[-1.0, -0.25, -2.0]], np.float32)
+    b = Beams(hip, x, s, 6)
+    b.call()
+    parents, tokens, values = (y[0] for y in b.result())
+    want = [(s[0, 2], 2, vocab - 7)] + [(s[0, 1] - np.log(3.0), 1, t) for t in (1, vocab - 3, vocab - 2)] + \
+        [(s[0, 0] - np.log(2.0), 0, t) for t in (3, vocab - 1)]
+    want.sort(key=lambda w: (-w[0], w[1], w[2]))
+    assert parents.tolist() == [w[1] for w in want] and tokens.tolist() == [w[2] for w in want]
+    v = np.array([w[0] for w in want])
+    assert (np.abs(values - v) <= np.abs(v) * 2.0 ** -24 + 2.0 ** -35).all()
+
+
 def test_masked_dead_and_ended(hip):
     rng = np.random.default_rng(4)
     x, s = random(rng, 7, 8, 9000)
