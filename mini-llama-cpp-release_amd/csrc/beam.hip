@@ -12,8 +12,8 @@
 // workgroup a group: the rows' sums, and the best of the parts' best by the same bar.  Sums are taken in a fixed
 // order: equal rows have equal sums, and the same call gives the same bits.
 //
-// Measured: 32 groups of 8 beams over 128011 tokens, 16 kept, 47 us (40 + 9 of kernels, 3.3 TB/s of logits in the first);
-// 4 beams over 32000 tokens 11 us.  In one launch, the last part of a group to arrive selecting, 55 and 11.
+// Measured: 32 groups of 8 beams over 128011 tokens, 16 kept, 48 us (40 + 9 of kernels, 3.3 TB/s of logits in the first), with a
+// quarter of the beams ended 44 (48 while their rows were read); 4 beams over 32000 tokens 11 us.  In one launch, the last part of a group to arrive selecting, 55 and 11.
 
 #include "beam.h"
 
@@ -117,7 +117,11 @@ __global__ __launch_bounds__(kThreads, 5) void beam_part_kernel(BeamCall c, int 
     const long long total = static_cast<long long>(c.groups) * c.beams * parts;
     for (long long w = blockIdx.x; w < total; w += gridDim.x) {
         const int lo = static_cast<int>(w % parts) * (E * kThreads), n = min(c.vocab - lo, E * kThreads);
-        const float* const from = c.logits + static_cast<size_t>(w / parts) * c.vocab + lo;
+        const size_t row = static_cast<size_t>(w / parts);
+        // (rows without continuations of their own, and those of groups that come out as NaN: nothing is read of them here)
+        const float score = c.scores[row];
+        if (!(fabsf(score) < __builtin_inff()) || (c.ended != nullptr && c.ended[row] != 0)) continue;
+        const float* const from = c.logits + row * c.vocab + lo;
         float x[E];
         if (n == E * kThreads) {
 #pragma unroll
