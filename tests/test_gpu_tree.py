@@ -654,6 +654,36 @@ def test_recorded_step(hip, orc):
     hip.stream_destroy(s)
 
 
+@pytest.mark.parametrize("kind", ["f32", "q8_0", "q4_1"])
+def test_recorded_attention_of_large_and_small_batches(hip, orc, kind):
+    """One recorded call runs whichever kernel the batch that is set takes: many rows, few, many again."""
+    rng = np.random.default_rng(21)
+    s = hip.stream_create()
+    large = Step(hip, orc, kind, [(ragged(rng, 256 - i), 900 + 9 * i) for i in range(16)], 8, 8, 64, 64, stream=s).write()
+    b, n = large.batch, large.batch.tokens
+    q = dev(hip, large.turned)
+    out, eager = (dev(hip, np.full(large.turned.shape, 7.25)) for _ in range(2))
+    parents = [list(t) for t, _ in large.forest]
+    first = [-(-t // 64) for t in b.kv_len]
+    g = hip.Graph.record(lambda: large.plan.attention(0, q, out, stream=s), stream=s)
+    for some in (range(16), [3], range(16), [], [0, 5], range(16)):
+        pages = sum((b.pages[sum(first[:i]):sum(first[:i + 1])] for i in some), [])
+        rows = sum(b.new[i] for i in some)
+        large.plan.set([b.new[i] for i in some], [b.kv_len[i] for i in some], pages, parents=sum((parents[i] for i in some), []),
+                       stream=s)
+        for x in (out, eager):
+            x.upload(np.full(large.turned.size, 7.25, np.float32))
+        for _ in range(3):
+            g.launch(s)
+        large.plan.attention(0, q, eager, stream=s)
+        got, want = (back(hip, x, large.turned.shape, stream=s) for x in (out, eager))
+        assert np.array_equal(got, want) and (got[rows:] == 7.25).all()
+        if rows == n:
+            large.check(got)
+    g.destroy()
+    hip.stream_destroy(s)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_drafted_decoding_is_decoding(hip, orc, kind):
     """Two steps of drafted trees on a stream of their own: the kept path of the first is a prefix of the second, which then
