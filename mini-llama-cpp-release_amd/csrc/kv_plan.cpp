@@ -16,6 +16,11 @@ constexpr int kTargetGroups = 512;
 // 4000 positions, at least 4 / 8 / 16 tiles: 14.9 / 12.8 / 13.8 us; over 700 9.6 / 10.3 / 11.6; 128 rows
 // over 4000 53 / 46 / 54.
 constexpr int kLeastTiles = 8;
+// Few rows of trees: a tile a wave where that makes no more workgroups than there are CUs and a merge of a few parts.
+// At least 8 and 4 tiles, us with the write: 16 nodes after 700 positions (Q4_0, 32 heads over 8 of 128, 192
+// workgroups) 17.5 and 16.5, after 1500 (384) 18.2 and 19.5; 4 nodes after 1500 (Q8_0, 14 heads over 2 of 64, 12
+// parts) 13.6 and 13.3, after 4000 (32) 14.5 and 15.4; 4 x 8 nodes after 300 (f32, 32 heads of 128) 19.2 and 17.0.
+constexpr int kFewTiles = 4, kFewParts = 16, kFewGroups = 256;
 
 int ceil_div(int a, int b) { return a / b + (a % b != 0); }  // (sinks go up to the largest int)
 
@@ -39,8 +44,9 @@ Seen seen_tiles(const KvPlanShape& s, int lo, int hi, int most) {
 // Where there is a round without splits, only items of twice the average are split if `lone` (64 ragged
 // sequences of up to 4000: 79 us, 85 with those over the average split).
 // (Not a prompt's row groups, whose lengths are spread: 2048 tokens, 32 heads: 167 us, 193 unsplit.)
+// few: the items are few rows of trees.
 template <typename Item>
-void split_items(const std::vector<Item>& whole, int n_kv_heads, bool lone, std::vector<Item>& list) {
+void split_items(const std::vector<Item>& whole, int n_kv_heads, bool lone, bool few, std::vector<Item>& list) {
     int64_t tiles = 0;
     for (const Item& w : whole) tiles += w.count;
     const int target = std::max(1, kTargetGroups / n_kv_heads);
@@ -50,8 +56,11 @@ void split_items(const std::vector<Item>& whole, int n_kv_heads, bool lone, std:
         return n;
     };
     const bool enough = static_cast<int>(whole.size()) >= target;
-    int64_t lo = std::max<int64_t>(kLeastTiles, (enough && lone ? 2 : 1) * ((tiles + target - 1) / target)), hi = lo;
-    for (const Item& w : whole) hi = std::max<int64_t>(hi, w.count);
+    int longest = 0;
+    for (const Item& w : whole) longest = std::max(longest, w.count);
+    few = few && longest <= kFewParts * kFewTiles && items_of(kFewTiles) * n_kv_heads <= kFewGroups;
+    int64_t lo = std::max<int64_t>(few ? kFewTiles : kLeastTiles, (enough && lone ? 2 : 1) * ((tiles + target - 1) / target)), hi = lo;
+    hi = std::max<int64_t>(hi, longest);
     while (lo < hi && !enough) {
         const int64_t mid = (lo + hi) / 2;
         if (items_of(mid) <= target) hi = mid;
@@ -258,7 +267,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     }
 
     for (int kind = 0; kind < 2; ++kind) {
-        split_items(of_trees[kind], s.n_kv_heads, true, b.trees[kind]);
+        split_items(of_trees[kind], s.n_kv_heads, true, kind == 0, b.trees[kind]);
         const int step = kind == 0 ? kKvNarrowRows : s.wide_rows;
         std::vector<KvAttnItem> whole;
         for (const KvAttnItem& q : base[kind]) {
@@ -273,7 +282,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
                 whole.push_back(it);
             }
         }
-        split_items(whole, s.n_kv_heads, kind == 0, b.items[kind]);
+        split_items(whole, s.n_kv_heads, kind == 0, false, b.items[kind]);
     }
     return "";
 }
