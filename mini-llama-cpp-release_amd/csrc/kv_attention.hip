@@ -37,8 +37,11 @@ hipError_t launch_kv_attention(const KvAttention& a, int kind, int count, const 
 // 446 and 171.  Per tile that is about as much a block of 32 elements.
 KvTreeCost kv_tree_cost(int qtype, int nb) {
     constexpr float kFew[4] = {0.74f, 0.33f, 0.32f, 0.40f}, kMany[4] = {2.0f, 1.3f, 1.25f, 1.5f};
-    // (above 128 elements a SIMD has one wave of the kernel for few rows, and a workgroup of the other half the rows)
-    return KvTreeCost{kFew[qtype] * nb * (nb > 4 ? 1.3f : 1.0f), kMany[qtype] * nb, 14000.0f + 4000.0f * nb};
+    // Above 128 elements (f32: 64) a SIMD has one wave of the kernel for few rows, so more workgroups than CUs are two rounds:
+    // 4 x 8 nodes after 1500 positions of f32, 32 heads over 8 of 128, in 512 33 us, in 256 24; 16 after 4000 of Q4_1 of
+    // 192 elements 41 and 32.  (A workgroup of the other has half the rows above 128.)
+    return KvTreeCost{kFew[qtype] * nb * (nb > 4 ? 1.3f : 1.0f), kMany[qtype] * nb, 14000.0f + 4000.0f * nb,
+                      nb > (qtype == 0 ? 2 : 4) ? 256 : 512};
 }
 
 hipError_t launch_kv_tree_attention(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s) {

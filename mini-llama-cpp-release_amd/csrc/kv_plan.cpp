@@ -46,10 +46,10 @@ Seen seen_tiles(const KvPlanShape& s, int lo, int hi, int most) {
 // (Not a prompt's row groups, whose lengths are spread: 2048 tokens, 32 heads: 167 us, 193 unsplit.)
 // few: the items are few rows of trees.
 template <typename Item>
-void split_items(const std::vector<Item>& whole, int n_kv_heads, bool lone, bool few, std::vector<Item>& list) {
+void split_items(const std::vector<Item>& whole, int n_kv_heads, bool lone, bool few, int groups, std::vector<Item>& list) {
     int64_t tiles = 0;
     for (const Item& w : whole) tiles += w.count;
-    const int target = std::max(1, kTargetGroups / n_kv_heads);
+    const int target = std::max(1, groups / n_kv_heads);
     auto items_of = [&](int64_t most) {
         int64_t n = 0;
         for (const Item& w : whole) n += (w.count + most - 1) / most;
@@ -140,7 +140,8 @@ KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     for (int kind = 0; kind < 2; ++kind) {
         // Only an item of n parts adds to the list, n - 1 items, and all parts take slots: at
         // most twice what is added.
-        const int extra = ceil_div(kTargetGroups, s.n_kv_heads);
+        const int groups = s.max_nodes > 0 ? std::max(kTargetGroups, s.tree_cost.groups) : kTargetGroups;
+        const int extra = ceil_div(groups, s.n_kv_heads);
         l.items[kind] = whole[kind] + extra;
         l.slots[kind] = 2 * extra;
     }
@@ -267,7 +268,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     }
 
     for (int kind = 0; kind < 2; ++kind) {
-        split_items(of_trees[kind], s.n_kv_heads, true, kind == 0, b.trees[kind]);
+        split_items(of_trees[kind], s.n_kv_heads, true, kind == 0, kind == 0 ? s.tree_cost.groups : kTargetGroups, b.trees[kind]);
         const int step = kind == 0 ? kKvNarrowRows : s.wide_rows;
         std::vector<KvAttnItem> whole;
         for (const KvAttnItem& q : base[kind]) {
@@ -282,7 +283,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
                 whole.push_back(it);
             }
         }
-        split_items(whole, s.n_kv_heads, kind == 0, false, b.items[kind]);
+        split_items(whole, s.n_kv_heads, kind == 0, false, kTargetGroups, b.items[kind]);
     }
     return "";
 }

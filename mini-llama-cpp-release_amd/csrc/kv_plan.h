@@ -66,6 +66,7 @@ constexpr int kKvMostNodes = 1024;
 // the one that takes less.
 struct KvTreeCost {
     float few = 1.0f, many = 5.0f, fill = 30000.0f;
+    int groups = 512;  // workgroups of the first that the chip holds at once
 };
 
 struct KvPlanShape {
