@@ -15,10 +15,10 @@
 // Batches with rows enough to fill its workgroups many times over run the kernel of kv_attention_rows.h instead, in
 // its form for trees (kv_tree_cost says which; a batch runs one of them, as two launches would follow each other).
 //
-// Bound: issue.  A tile takes a wave 470 vector instructions and 32 products, some 2800 cycles at two waves a SIMD
-// (64 nodes after 4000 positions, Q8_0, 32 heads over 8 KV heads of 128: 32 us, 20 of them tiles; the cache is read
-// 16 times, from L2); small batches by the launch, four dependent trips to memory and the merge (8 nodes after 700
-// positions, 14 heads over 2 of 64: 8.9 us).  24 nodes of 16 sequences, Q4_1, 80 elements, a window of 1024: 40 us.
+// Bound: issue.  A tile takes a wave 500 vector instructions and 32 products, and the two waves of a SIMD issue vector
+// instructions 78 % of their time (64 nodes after 4000 positions, Q8_0, 32 heads over 8 KV heads of 128: 32 us, 20 of them
+// tiles; the cache is read 16 times, from L2); small batches by the launch, four dependent trips to memory and the merge
+// (8 nodes after 700 positions, 14 heads over 2 of 64: 8.3 us).  24 nodes of 16 sequences, Q4_1, 80 elements, a window of 1024: 40 us.
 // Measured and no faster: 32 rows a wave (one wave a SIMD: 46 us for the 64 nodes, 57 for the 16 sequences), weights
 // times scales as one mixed-precision instruction each (33 us), with one look at a tile's frames as well (33),
 // s_setprio around the products, 256 and 1024 workgroups (34 and 36); one power of two for a row's queries in place of one
