@@ -99,9 +99,10 @@ __device__ __forceinline__ void move_piece(uint8_t* to, const uint8_t* from, int
 
 // Bound: the lines of memory that a slot's pieces lie in, some ten of 128 bytes for the 150 bytes of a Q4_0 head of 128,
 // read and written back (paths of four nodes of 64 sequences, 16 layers, 8 heads: 19 us); few paths by latency (4 us).
-// A path a wave, without barriers, takes 17 and 6.  A workgroup takes one path in one head and layer: reads up to kTogether slots into LDS, then
-// writes them where they go, piece by piece, so that what else lies in their tiles is never rewritten.  A path's
-// sources ascend and lie at or behind their destinations: none is one of an earlier move, so it is read before
+// A path a wave, without barriers, takes 17 and 6, pieces in registers 27, a move by whole waves 22 (its addresses are
+// then the waves', not the lanes').  A workgroup takes one path in one head and layer: reads up to kTogether slots into
+// LDS, then writes them where they go, piece by piece, so that what else lies in their tiles is never rewritten.  A
+// path's sources ascend and lie at or behind their destinations: none is one of an earlier move, so it is read before
 // anything has been written there.
 template <int QT>
 __global__ __launch_bounds__(kThreads) void kv_moves_kernel(KvView kv, int n_layers, size_t layer_bytes, MoveArgs args, int n_ends) {
