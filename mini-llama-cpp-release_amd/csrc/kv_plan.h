@@ -79,7 +79,6 @@ struct KvPlanShape {
     KvTreeCost tree_cost = {};
 };
 
-
 // What a set of a plan of this shape can need at the most.
 struct KvPlanLimits {
     int fresh;     // tiles with new tokens
