@@ -132,8 +132,7 @@ struct KvAttention {
     float* partial;     // [slot][KV head][kv_partial_floats]
     unsigned* arrived;  // [first slot of a split][KV head], zero between launches
 };
-// Query rows of a workgroup of the kernel for many rows, and a part's floats in `partial` by list (0 narrow, 1 wide).
-int kv_wide_rows(int nb);
+// A part's floats in `partial` by list (0 narrow, 1 wide).
 size_t kv_partial_floats(int nb, int kind);
 // count: items of the narrow (kind 0) or wide list, 0 as above.
 hipError_t launch_kv_attention(const KvAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
@@ -149,7 +148,6 @@ struct KvTreeAttention {
     unsigned* arrived;
 };
 // (A part's floats in `partial` are those of kv_partial_floats.)
-KvTreeCost kv_tree_cost(int qtype, int nb);
 hipError_t launch_kv_tree_attention(const KvTreeAttention& a, int kind, int count, const float* q, float* out, hipStream_t s);
 
 // Positions and pages moved within a cache, in all layers (kv_moves.hip).

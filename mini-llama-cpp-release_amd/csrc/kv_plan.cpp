@@ -125,6 +125,25 @@ std::string add_tree(const KvPlanShape& s, const std::string& who, int n, int st
 
 }  // namespace
 
+int kv_wide_rows(int nb) { return nb <= 4 ? 128 : 64; }
+
+// Measured, us by the kernel for few rows and the one for many (8 KV heads of 128, rows a KV head and sequence x
+// sequences x positions): Q8_0 64 x 1 x 4000 17 and 45, 256 x 1 x 4000 31 and 49, 32 x 32 x 2000 48 and 121, 96 x 16 x 3000
+// 106 and 105, 256 x 16 x 2000 182 and 127; Q4_1 96 x 16 x 3000 134 and 113; f32 128 x 4 x 3000 93 and 62, 256 x 16 x 2000
+// 446 and 171.  Per tile that is about as much a block of 32 elements.  Beside its tiles, which a window may leave few of,
+// a workgroup of the first holds its place for 3 us (launch, trips to memory, the waves' merge), for 8 where it has its CU
+// to itself.  Of 1400 random batches of all types, 32 to 256 elements, with and without windows, the chosen kernel takes
+// 1.0 % longer than the better one on average, 3.9 % without those, 5.4 % where tiles outside the windows count as well.
+KvTreeCost kv_tree_cost(int qtype, int nb) {
+    constexpr float kFew[4] = {0.74f, 0.33f, 0.32f, 0.40f}, kMany[4] = {2.0f, 1.3f, 1.25f, 1.5f};
+    // Above 128 elements (f32: 64) a SIMD has one wave of the kernel for few rows, so more workgroups than CUs are two rounds:
+    // 4 x 8 nodes after 1500 positions of f32, 32 heads over 8 of 128, in 512 33 us, in 256 24; 16 after 4000 of Q4_1 of
+    // 192 elements 41 and 32.  (A workgroup of the other has half the rows above 128.)
+    const int groups = nb > (qtype == 0 ? 2 : 4) ? 256 : 512;
+    return KvTreeCost{kFew[qtype] * nb * (nb > 4 ? 1.3f : 1.0f), kMany[qtype] * nb, 14000.0f + 4000.0f * nb, groups,
+                      groups == 256 ? 30.0f : 6.0f};
+}
+
 KvPlanLimits kv_plan_limits(const KvPlanShape& s) {
     const int64_t rows = static_cast<int64_t>(s.max_tokens) * s.group;
     const int64_t narrow = std::min(rows / kKvNarrowRows, static_cast<int64_t>(s.max_seqs) * (kKvNarrowMost / kKvNarrowRows - 1));
@@ -195,35 +214,7 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
     std::vector<KvAttnItem> base[2];
     std::vector<KvTreeItem> of_trees[2];
     int token0 = 0, row0 = 0, page0 = 0;
-    // Trees: the kernel that takes less for all of them (two launches would follow each other).
-    double few = 0.0, many = s.tree_cost.fill;
-    for (int i = 0; i < n_seqs && s.max_nodes > 0; ++i) {
-        const int rows = new_tokens[i] * s.group, tiles = ceil_div(kv_len[i], kKvTile);
-        few += static_cast<double>(ceil_div(rows, kKvTreeRows)) * tiles * s.n_kv_heads * s.tree_cost.few;
-        many += static_cast<double>(ceil_div(rows, s.wide_rows)) * tiles * s.n_kv_heads * s.tree_cost.many;
-    }
-    const int tree_kind = few <= many ? 0 : 1;
-    // The row groups of sequence i's tree.
-    auto add_item = [&](int i, int token, int page) -> std::string {
-        const int n = new_tokens[i], start = kv_len[i] - n, rows = n * s.group;
-        const int step = tree_kind == 0 ? kKvTreeRows : s.wide_rows;
-        const int mask0 = static_cast<int>(b.masks.size()), words = (kv_len[i] - 1) / kKvTile - start / kKvTile + 1;
-        const std::string wrong =
-            add_tree(s, "sequence " + std::to_string(i), n, start, parents != nullptr ? parents + token : nullptr, b);
-        if (!wrong.empty()) return wrong;
-        for (int r = 0; r < rows; r += step) {
-            const int last = (std::min(rows, r + step) - 1) / s.group;
-            int near = b.pos[token + r / s.group], far = near;
-            for (int t = r / s.group; t <= last; ++t) {
-                near = std::min(near, b.pos[token + t]);
-                far = std::max(far, b.pos[token + t]);
-            }
-            // (from the tree's first tile at the latest: a node may be seen as a sink wherever it lies)
-            const Seen t = seen_tiles(s, near, start + last, start);
-            of_trees[tree_kind].push_back(KvTreeItem{token, n, kv_len[i], page, r, 0, t.count, t.sinks, t.shift, 0, 1, 0, mask0, words, near, far});
-        }
-        return "";
-    };
+    std::vector<int> mask0;  // of each sequence's tree
     for (int i = 0; i < n_seqs; ++i) {
         const int len = kv_len[i], n = new_tokens[i], start = len - n;
         for (int p = 0; p < len; p += s.page_size) {
@@ -241,8 +232,10 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
             p = end;
         }
         if (s.max_nodes > 0) {
+            mask0.push_back(static_cast<int>(b.masks.size()));
             if (n > 0) {
-                const std::string wrong = add_item(i, token0, page0);
+                const std::string wrong =
+                    add_tree(s, "sequence " + std::to_string(i), n, start, parents != nullptr ? parents + token0 : nullptr, b);
                 if (!wrong.empty()) return wrong;
             }
             b.seqs.push_back(KvTreeSeq{token0, n});
@@ -267,6 +260,36 @@ std::string kv_plan_build(const KvPlanShape& s, int n_seqs, const int* new_token
         }
     }
 
+    if (s.max_nodes > 0) {
+        // The row groups of either kernel, and the kernel that takes less for all of them, by the tiles that they visit (two
+        // launches would follow each other).  256 nodes after 8000 positions with a window of 64 (Q8_0, 32 heads over 8 of
+        // 128): 13 us by the kernel for few rows, 32 by the other, which takes less where all positions are seen.
+        double cost[2] = {0.0, s.tree_cost.fill};
+        for (int kind = 0; kind < 2; ++kind) {
+            if (cost[0] <= cost[1] && kind == 1) break;  // (whatever the second visits)
+            const int step = kind == 0 ? kKvTreeRows : s.wide_rows;
+            of_trees[kind].reserve(static_cast<size_t>(b.n_tokens) * s.group / step + n_seqs);
+            for (int i = 0; i < n_seqs; ++i) {
+                const int n = new_tokens[i], start = kv_len[i] - n, rows = n * s.group, token = b.seqs[i].token0;
+                const int words = n > 0 ? (kv_len[i] - 1) / kKvTile - start / kKvTile + 1 : 0;
+                for (int r = 0; r < rows; r += step) {
+                    const int last = (std::min(rows, r + step) - 1) / s.group;
+                    int near = b.pos[token + r / s.group], far = near;
+                    for (int t = r / s.group; t <= last; ++t) {
+                        near = std::min(near, b.pos[token + t]);
+                        far = std::max(far, b.pos[token + t]);
+                    }
+                    // (from the tree's first tile at the latest: a node may be seen as a sink wherever it lies)
+                    const Seen t = seen_tiles(s, near, start + last, start);
+                    of_trees[kind].push_back(KvTreeItem{token, n, kv_len[i], b.first_page[i], r, 0, t.count, t.sinks, t.shift, 0, 1, 0,
+                                                        mask0[i], words, near, far});
+                    cost[kind] += s.n_kv_heads * (kind == 0 ? s.tree_cost.few * static_cast<double>(t.count) + s.tree_cost.each
+                                                            : s.tree_cost.many * static_cast<double>(t.count));
+                }
+            }
+        }
+        of_trees[cost[0] <= cost[1] ? 1 : 0].clear();
+    }
     for (int kind = 0; kind < 2; ++kind) {
         split_items(of_trees[kind], s.n_kv_heads, true, kind == 0, kind == 0 ? s.tree_cost.groups : kTargetGroups, b.trees[kind]);
         const int step = kind == 0 ? kKvNarrowRows : s.wide_rows;

@@ -62,12 +62,16 @@ constexpr int kKvTreeRows = 16;
 constexpr int kKvMostNodes = 1024;
 
 // What the trees' two kernels take, in ns: for a tile by a workgroup of the one for few rows (16 at a time) and of the one
-// for many (wide_rows at a time), and what the second takes longer for filling its pipeline and merging.  A batch runs
-// the one that takes less.
+// for many (wide_rows at a time), what the second takes longer for filling its pipeline and merging, and what a workgroup
+// of the first takes beside its tiles.  A batch runs the one that takes less.
 struct KvTreeCost {
     float few = 1.0f, many = 5.0f, fill = 30000.0f;
     int groups = 512;  // workgroups of the first that the chip holds at once
+    float each = 0.0f;
 };
+KvTreeCost kv_tree_cost(int qtype, int nb);  // of heads of nb blocks of 32 elements
+// Query rows of a workgroup of the kernel for many rows.
+int kv_wide_rows(int nb);
 
 struct KvPlanShape {
     int page_size, n_pages, n_kv_heads;
