@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 import test_gpu_tree
+import test_gpu_tree_rows
 from kv_reference import QT
 from tree_reference import ragged
 
@@ -57,3 +58,16 @@ def test_recorded_batches(qtype):
     forest = [(ragged(rng, 256 - i), 900 + 9 * i) for i in range(16)]
     assert kind(qtype, 64, 8, 8, 0, 0, forest) == "many"
     assert kind(qtype, 64, 8, 8, 0, 0, forest[3:4]) == "few"
+
+
+@pytest.mark.parametrize("case", range(len(test_gpu_tree_rows.WINDOWED)))
+def test_windowed_batches(case):
+    qtype, hd, heads, kv, _, _, _, window, sinks = test_gpu_tree_rows.WINDOWED[case]
+    assert kind(qtype, hd, heads, kv, window, sinks, test_gpu_tree_rows.windowed(case)) == "many"
+
+
+@pytest.mark.parametrize("qtype", list(QT))
+def test_batches_with_values_that_are_not_finite(qtype):
+    t = test_gpu_tree_rows
+    for window, sinks in t.WINDOWS:
+        assert kind(qtype, t.HD, t.HEADS, t.KV, window, sinks, t.apart()) == "many"
