@@ -525,9 +525,9 @@ int mlq_hip_kv_keep(mlq_kv_plan_t plan, const int* n_kept, const int* kept, void
 /* Copies the first positions[i] positions (NULL: all) of page from[i] to page
  * to[i], in every layer: a sequence that forks keeps its full pages in common and
  * takes a copy of its last one.  No page may be written twice, or read and
- * written.  Positions up to the next multiple of 32 are copied with them.  Host
- * arrays, copied before the call returns.  Asynchronous on `stream`; a recorded
- * call copies the same pages at every replay. */
+ * written (a copy of 0 positions does neither).  Positions up to the next multiple
+ * of 32 are copied with them.  Host arrays, copied before the call returns.
+ * Asynchronous on `stream`; a recorded call copies the same pages at every replay. */
 int mlq_hip_kv_copy_pages(mlq_kv_cache_t cache, int n, const int* from, const int* to, const int* positions, void* stream);
 
 /* Beam search's selection.  Each of `groups` sequences has `beams` beams: their

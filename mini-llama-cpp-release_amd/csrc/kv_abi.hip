@@ -596,7 +596,8 @@ int mlq_hip_kv_copy_pages(mlq_kv_cache_t cache, int n, const int* from, const in
         if (n == 0) return MLQ_OK;
         if (from == nullptr || to == nullptr) return abi_fail(MLQ_ERR_INVALID, who + ": null page list");
         std::vector<mlq::KvCopy> copies;
-        std::vector<int> sources(from, from + n), targets(to, to + n);
+        std::vector<int> sources, targets;
+        sources.reserve(n), targets.reserve(n), copies.reserve(n);
         for (int i = 0; i < n; ++i) {
             const int used = positions != nullptr ? positions[i] : kv.page_size;
             if (from[i] < 0 || from[i] >= kv.n_pages || to[i] < 0 || to[i] >= kv.n_pages) {
@@ -607,12 +608,15 @@ int mlq_hip_kv_copy_pages(mlq_kv_cache_t cache, int n, const int* from, const in
                 return abi_fail(MLQ_ERR_SHAPE, who + ": copy " + std::to_string(i) + ": " + std::to_string(used) +
                                                    " positions of a page of " + std::to_string(kv.page_size));
             }
-            if (used > 0) copies.push_back(mlq::KvCopy{from[i], to[i], (used + mlq::kKvTile - 1) / mlq::kKvTile});
+            if (used == 0) continue;
+            copies.push_back(mlq::KvCopy{from[i], to[i], (used + mlq::kKvTile - 1) / mlq::kKvTile});
+            sources.push_back(from[i]);
+            targets.push_back(to[i]);
         }
         // Copies run side by side: no page is written twice, or both read and written.
         std::sort(sources.begin(), sources.end());
         std::sort(targets.begin(), targets.end());
-        for (int i = 0; i < n; ++i) {
+        for (size_t i = 0; i < targets.size(); ++i) {
             if (i > 0 && targets[i] == targets[i - 1]) {
                 return abi_fail(MLQ_ERR_SHAPE, who + ": page " + std::to_string(targets[i]) + " is written twice");
             }
