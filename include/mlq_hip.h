@@ -503,7 +503,8 @@ int mlq_hip_kv_plan_set_tree(mlq_kv_plan_t plan, int n_seqs, const int* new_toke
 /* Checks drafted trees greedily.  logits [tokens][vocab]: what the model says
  * after each node; tokens: the nodes' tokens.  picks [tokens] is the first index
  * of each row's largest logit, -1 where one is infinite or NaN (as
- * mlq_hip_quant_linear_argmax).  A sequence's first node is its last token, which
+ * mlq_hip_quant_linear_argmax; tokens that are not allowed get a finite logit far
+ * below the others, not -Inf).  A sequence's first node is its last token, which
  * is certain; from there its path goes on to the lowest child whose token is the
  * last node's pick.  n_kept [sequences]: the path's nodes (0 of an empty tree);
  * kept [tokens]: at the sequence's rows, the path's node indexes, then -1; next

@@ -103,8 +103,11 @@ __device__ __forceinline__ uint32_t wave_rth_largest(uint32_t v, int r) {
     return t;
 }
 
-// Bound: issue, half of it the exponentials (16 instructions in 64 bits a logit, which run at about the rate of 32; a logit
-// takes 29 in all), then memory.  Five waves a SIMD (four: 42 us for the 256 rows above); parts of 4096 logits 47 us.
+// Bound: issue and what it waits for, in turn.  Of the 36 us over the 192 live of the 256 rows above the vector units issue
+// for 20 (by counters: 32 instructions a logit, 16 of them the exponential in 64 bits, which run at about the rate of 32);
+// a wave spends 36 % of its life waiting for memory or at barriers and 37 % for its turn to issue.  3072 live workgroups
+// share 1280 places, and each loads its part, then computes, then ranks, so that only other workgroups' work hides its loads.
+// Five waves a SIMD (four: 42 us for the 256 rows); parts of 4096 logits 47 us.
 template <int E>
 __global__ __launch_bounds__(kThreads, 5) void beam_part_kernel(BeamCall c, int parts) {
     constexpr int kMost = kBeamMostKeep * E;

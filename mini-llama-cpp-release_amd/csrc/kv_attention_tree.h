@@ -18,7 +18,8 @@
 // Bound: issue.  A tile takes a wave 500 vector instructions and 32 products, and the two waves of a SIMD issue vector
 // instructions 78 % of their time (64 nodes after 4000 positions, Q8_0, 32 heads over 8 KV heads of 128: 32 us, 20 of them
 // tiles; the cache is read 16 times, from L2); small batches by the launch, four dependent trips to memory and the merge
-// (8 nodes after 700 positions, 14 heads over 2 of 64: 8.3 us).  24 nodes of 16 sequences, Q4_1, 80 elements, a window of 1024: 40 us.
+// (8 nodes after 700 positions, 14 heads over 2 of 64: 8.3 us).  24 nodes of 16 sequences, Q4_1, 80 elements, a window of 1024:
+// 40 us, in two rounds, as its 528 workgroups are more than the 512 that the chip holds and whole items are not split then.
 // Measured and no faster: 32 rows a wave (one wave a SIMD: 46 us for the 64 nodes, 57 for the 16 sequences), weights
 // times scales as one mixed-precision instruction each (33 us), with one look at a tile's frames as well (33),
 // s_setprio around the products, 256 and 1024 workgroups (34 and 36); one power of two for a row's queries in place of one
@@ -32,7 +33,8 @@
 namespace mlq {
 namespace kv {
 
-// Waves a SIMD: two where 256 registers are enough, else one with all 512 (the compiler would rather have two that spill).
+// Waves a SIMD: two at the least up to 128 elements (f32: 64), where 256 registers are enough but for Q4_1 of four blocks,
+// which keeps 76 bytes a lane in scratch; above, one with all 512 (the compiler would rather have two that spill).
 template <int QT, int NB>
 constexpr int tree_waves() {
     return (QT == 0 ? NB <= 2 : NB <= 4) ? 2 : 1;
