@@ -497,7 +497,7 @@ int mlq_hip_kv_tree_plan_create(mlq_kv_cache_t cache, int n_heads, int window, i
  * its ancestors and itself, as far as the window (of positions) and the first
  * tokens go.  (All sequences of a batch take the attention's form for many rows a
  * KV head, with its slow cases, or none: trees of more than 32 rows may over long
- * contexts, over short ones only batches of hundreds.) */
+ * contexts, over short ones or within short windows only batches of hundreds.) */
 int mlq_hip_kv_plan_set_tree(mlq_kv_plan_t plan, int n_seqs, const int* new_tokens, const int* kv_len, const int* pages,
                              const int* parents, void* stream);
 /* Checks drafted trees greedily.  logits [tokens][vocab]: what the model says
